@@ -325,7 +325,9 @@ SNN_HIP_API int snn_hip_conv2d_workspace_size(
  * uses.  SNN_HIP_DTYPE_F32 answers as snn_hip_conv2d_workspace_size. */
 typedef enum snn_hip_dtype {
   SNN_HIP_DTYPE_F32 = 0,
-  SNN_HIP_DTYPE_F16 = 1
+  SNN_HIP_DTYPE_F16 = 1,
+  /* bfloat16: the operators of a residual block over sequences only */
+  SNN_HIP_DTYPE_BF16 = 2
 } snn_hip_dtype;
 SNN_HIP_API int snn_hip_conv2d_workspace_size_for(
     const snn_hip_conv2d_params* params, int direction, int algorithm,
@@ -450,7 +452,12 @@ SNN_HIP_API int snn_hip_matmul_f16(const void* lhs, const void* rhs,
  * snn_hip_activation.  Everything else as snn_hip_conv2d_forward_f32. */
 typedef enum snn_hip_activation {
   SNN_HIP_ACTIVATION_NONE = 0,
-  SNN_HIP_ACTIVATION_RELU = 1
+  SNN_HIP_ACTIVATION_RELU = 1,
+  /* snn_hip_matmul_bias_act_* only: z Phi(z), its approximation through
+   * tanh(sqrt(2 / pi) (z + 0.044715 z^3)), and z sigmoid(z). */
+  SNN_HIP_ACTIVATION_GELU = 2,
+  SNN_HIP_ACTIVATION_GELU_TANH = 3,
+  SNN_HIP_ACTIVATION_SILU = 4
 } snn_hip_activation;
 SNN_HIP_API int snn_hip_conv2d_forward_bias_act_f32(
     const float* input, const float* filter, const float* bias, float* output,
@@ -527,6 +534,269 @@ SNN_HIP_API int snn_hip_binaryop_f16(const void* lhs, const void* rhs,
                                      void* output, const int* lhs_dims,
                                      int n_lhs_dims, const int* rhs_dims,
                                      int n_rhs_dims, int op, void* stream);
+
+/* ---- a residual block over sequences ---------------------------------------
+ * Operators of language models that portDNN has no counterpart of: a matrix
+ * product with its epilogue, the norms around a block and a gated linear
+ * recurrence.  Tensors are row-major with the channels innermost, so that a
+ * [batch, steps, channels] tensor is the NHWC tensor of one row of `steps`
+ * columns.  Data types: float, IEEE binary16 (_f16) and bfloat16 (_bf16);
+ * sums, statistics and states are fp32, and an output is rounded to its type
+ * once.  A stride is the number of elements from one row to the next, at least
+ * the row's length; 0 stands for rows that follow one another. */
+
+/* output = act(op(lhs) op(rhs) + bias) + residual.
+ *
+ * op(lhs) is m x k: stored m x k, or k x m when transpose_lhs; op(rhs) is
+ * k x n: stored k x n, or n x k when transpose_rhs.  bias holds n values,
+ * residual and output are m x n.  bias, residual and pre_activation may be
+ * NULL; pre_activation, m x n without a stride, receives the value in front of
+ * the activation, which the gradient takes.  residual may be output (the sum
+ * in place); no other operand may overlap an output.
+ *
+ * Every dimension is positive and every row shorter than 2^30 bytes; tensors
+ * may be of any size beyond that.  A workspace of the recommended size lets products with few output tiles share
+ * their reduction between work-groups (the parts are added in a fixed order:
+ * two calls with the same arguments, workspace included, return the same
+ * bits); without it they run on fewer work-groups. */
+typedef struct snn_hip_matmul_bias_act_params {
+  int m;
+  int k;
+  int n;
+  int transpose_lhs;
+  int transpose_rhs;
+  int activation; /* a snn_hip_activation */
+  int lhs_stride;
+  int rhs_stride;
+  int residual_stride;
+  int output_stride;
+} snn_hip_matmul_bias_act_params;
+SNN_HIP_API int snn_hip_matmul_bias_act_f32(
+    const void* lhs, const void* rhs, const void* bias, const void* residual,
+    void* output, void* pre_activation,
+    const snn_hip_matmul_bias_act_params* params, void* workspace,
+    size_t workspace_elems, void* stream);
+SNN_HIP_API int snn_hip_matmul_bias_act_f16(
+    const void* lhs, const void* rhs, const void* bias, const void* residual,
+    void* output, void* pre_activation,
+    const snn_hip_matmul_bias_act_params* params, void* workspace,
+    size_t workspace_elems, void* stream);
+SNN_HIP_API int snn_hip_matmul_bias_act_bf16(
+    const void* lhs, const void* rhs, const void* bias, const void* residual,
+    void* output, void* pre_activation,
+    const snn_hip_matmul_bias_act_params* params, void* workspace,
+    size_t workspace_elems, void* stream);
+/* The gradients.  grad_output is m x n with the stride output_stride (it is
+ * the residual's gradient as it stands), pre_activation what the forward call
+ * wrote (not read where activation is none).  grad_lhs and grad_rhs are stored
+ * as lhs and rhs are, transposed or not, without a stride; grad_bias holds n
+ * values.  Any of the three may be NULL and is then not computed; lhs is needed
+ * for grad_rhs and rhs for grad_lhs only.  grad_bias and, where there is an
+ * activation, the products (which need the gradient with respect to
+ * pre_activation, rounded to the data type) take workspace:
+ * SNN_HIP_INSUFFICIENT_WORKSPACE without the required size. */
+SNN_HIP_API int snn_hip_matmul_bias_act_grad_f32(
+    const void* grad_output, const void* lhs, const void* rhs,
+    const void* pre_activation, void* grad_lhs, void* grad_rhs,
+    void* grad_bias, const snn_hip_matmul_bias_act_params* params,
+    void* workspace, size_t workspace_elems, void* stream);
+SNN_HIP_API int snn_hip_matmul_bias_act_grad_f16(
+    const void* grad_output, const void* lhs, const void* rhs,
+    const void* pre_activation, void* grad_lhs, void* grad_rhs,
+    void* grad_bias, const snn_hip_matmul_bias_act_params* params,
+    void* workspace, size_t workspace_elems, void* stream);
+SNN_HIP_API int snn_hip_matmul_bias_act_grad_bf16(
+    const void* grad_output, const void* lhs, const void* rhs,
+    const void* pre_activation, void* grad_lhs, void* grad_rhs,
+    void* grad_bias, const snn_hip_matmul_bias_act_params* params,
+    void* workspace, size_t workspace_elems, void* stream);
+/* Workspace of the forward call (grad == 0) or of the gradients, in elements
+ * of `dtype`; the pointer is aligned to 16 bytes, as all workspaces of this
+ * section are. */
+SNN_HIP_API int snn_hip_matmul_bias_act_workspace_size(
+    const snn_hip_matmul_bias_act_params* params, int grad, int dtype,
+    size_t* required_elems, size_t* recommended_elems);
+
+/* The norms before and after a block, with its gate and residual scale, in
+ * one pass over the rows:
+ *
+ *   n = post_norm(x) * post_weight + post_bias     the block's output
+ *   sum = residual + scale * gate * n              the residual stream
+ *   normed = pre_norm(sum) * pre_weight + pre_bias the next block's input
+ *
+ * x, residual, sum and normed are rows x channels; scale and the norms'
+ * weights and biases hold one value per channel; the gate has one row for
+ * `gate_rows` consecutive rows of x (1: one for each) and enters as it is,
+ * through a sigmoid, or as gate * sigmoid(gate).  A norm divides by
+ * sqrt(mean(v^2) + epsilon) (RMS) or takes the mean out first (LAYER).
+ * residual, gate, scale, the weights and biases, sum, normed and stats may be
+ * NULL; weights and biases of an absent norm have to be, normed has to be
+ * where there is no pre_norm, and sum or normed has to be there.  `gate` and
+ * the operand are both there or both not.  stats (rows x 4 floats) receives
+ * mean and reciprocal deviation of the two norms, zeros for what a row has
+ * not, for the gradients.  sum may be x or residual (with the stride of x
+ * that sum has); no other output may overlap an input.  At most 16384
+ * channels. */
+typedef enum snn_hip_norm {
+  SNN_HIP_NORM_NONE = 0,
+  SNN_HIP_NORM_RMS = 1,
+  SNN_HIP_NORM_LAYER = 2
+} snn_hip_norm;
+typedef enum snn_hip_gate {
+  SNN_HIP_GATE_NONE = 0,
+  SNN_HIP_GATE_VALUE = 1,
+  SNN_HIP_GATE_SIGMOID = 2,
+  SNN_HIP_GATE_SILU = 3
+} snn_hip_gate;
+typedef struct snn_hip_residual_norm_params {
+  int rows;
+  int channels;
+  int post_norm; /* a snn_hip_norm */
+  int pre_norm;  /* a snn_hip_norm */
+  int gate;      /* a snn_hip_gate */
+  int gate_rows;
+  int x_stride;    /* of x */
+  int gate_stride; /* of the gate */
+  float epsilon;
+} snn_hip_residual_norm_params;
+typedef struct snn_hip_residual_norm_tensors {
+  const void* x;
+  const void* residual;
+  const void* gate;
+  const void* scale;
+  const void* post_weight;
+  const void* post_bias;
+  const void* pre_weight;
+  const void* pre_bias;
+  void* sum;
+  void* normed;
+  float* stats;
+} snn_hip_residual_norm_tensors;
+SNN_HIP_API int snn_hip_residual_norm_f32(
+    const snn_hip_residual_norm_tensors* tensors,
+    const snn_hip_residual_norm_params* params, void* stream);
+SNN_HIP_API int snn_hip_residual_norm_f16(
+    const snn_hip_residual_norm_tensors* tensors,
+    const snn_hip_residual_norm_params* params, void* stream);
+SNN_HIP_API int snn_hip_residual_norm_bf16(
+    const snn_hip_residual_norm_tensors* tensors,
+    const snn_hip_residual_norm_params* params, void* stream);
+/* The gradients.  `tensors` holds the forward call's operands and its sum and
+ * stats (residual and normed are not read, sum is read where there is a
+ * pre_norm, stats where there is any norm).  grad_sum and grad_normed are the
+ * gradients of the two outputs (either may be NULL; grad_normed has to be
+ * where there is no pre_norm); the others are outputs without strides, NULL
+ * where they are not wanted.  The weights', biases', scale's and a shared
+ * gate's gradients are sums over rows, added in a fixed order; their partial
+ * sums take the required workspace. */
+typedef struct snn_hip_residual_norm_gradients {
+  const void* grad_sum;
+  const void* grad_normed;
+  void* grad_x;
+  void* grad_residual;
+  void* grad_gate;
+  void* grad_scale;
+  void* grad_post_weight;
+  void* grad_post_bias;
+  void* grad_pre_weight;
+  void* grad_pre_bias;
+} snn_hip_residual_norm_gradients;
+SNN_HIP_API int snn_hip_residual_norm_grad_f32(
+    const snn_hip_residual_norm_tensors* tensors,
+    const snn_hip_residual_norm_gradients* gradients,
+    const snn_hip_residual_norm_params* params, void* workspace,
+    size_t workspace_elems, void* stream);
+SNN_HIP_API int snn_hip_residual_norm_grad_f16(
+    const snn_hip_residual_norm_tensors* tensors,
+    const snn_hip_residual_norm_gradients* gradients,
+    const snn_hip_residual_norm_params* params, void* workspace,
+    size_t workspace_elems, void* stream);
+SNN_HIP_API int snn_hip_residual_norm_grad_bf16(
+    const snn_hip_residual_norm_tensors* tensors,
+    const snn_hip_residual_norm_gradients* gradients,
+    const snn_hip_residual_norm_params* params, void* workspace,
+    size_t workspace_elems, void* stream);
+/* Workspace of the gradients in elements of `dtype`, enough for all of them;
+ * the sums over rows need the required size, the others none. */
+SNN_HIP_API int snn_hip_residual_norm_grad_workspace_size(
+    const snn_hip_residual_norm_params* params, int dtype,
+    size_t* required_elems, size_t* recommended_elems);
+
+/* A gated linear recurrence over the steps of a sequence, channel by channel:
+ *
+ *   a_t = sigmoid(forget_t)
+ *   b_t = w_t x_t,  w_t = sigmoid(input_gate_t), or 1 - a_t without that gate
+ *   h_t = a_t h_{t-1} + b_t
+ *
+ * x, forget and input_gate are [batch][steps][channels] with row_stride
+ * elements from step to step (steps * row_stride from sequence to sequence),
+ * so that they may be slices of one projection's output; h is
+ * [batch][steps][channels] without a stride.  initial_state and final_state
+ * are [batch][channels] floats (NULL: zero, not wanted) and may be one buffer:
+ * a single token is a call with one step that updates the state in place.
+ * resets ([batch][steps] bytes, NULL: none): where it is not zero a_t h_{t-1}
+ * is left out, whatever it is, so that a sequence may hold several documents.
+ * lengths ([batch] ints, NULL: all steps; clamped to 0 ... steps): steps from
+ * there on are not read, their h is zero, and final_state is the state behind
+ * the last step that counts (the initial state for a length of zero).
+ *
+ * Long sequences are divided into pieces that run beside one another, given a
+ * workspace of the recommended size; without one a sequence is one piece.  The
+ * order of operations is fixed by the sizes and the workspace. */
+typedef struct snn_hip_linear_recurrence_params {
+  int batch;
+  int steps;
+  int channels;
+  int row_stride;      /* of x, forget and input_gate */
+  int grad_row_stride; /* of their gradients */
+} snn_hip_linear_recurrence_params;
+SNN_HIP_API int snn_hip_linear_recurrence_f32(
+    const void* x, const void* forget, const void* input_gate,
+    const unsigned char* resets, const int* lengths,
+    const float* initial_state, void* h, float* final_state,
+    const snn_hip_linear_recurrence_params* params, void* workspace,
+    size_t workspace_elems, void* stream);
+SNN_HIP_API int snn_hip_linear_recurrence_f16(
+    const void* x, const void* forget, const void* input_gate,
+    const unsigned char* resets, const int* lengths,
+    const float* initial_state, void* h, float* final_state,
+    const snn_hip_linear_recurrence_params* params, void* workspace,
+    size_t workspace_elems, void* stream);
+SNN_HIP_API int snn_hip_linear_recurrence_bf16(
+    const void* x, const void* forget, const void* input_gate,
+    const unsigned char* resets, const int* lengths,
+    const float* initial_state, void* h, float* final_state,
+    const snn_hip_linear_recurrence_params* params, void* workspace,
+    size_t workspace_elems, void* stream);
+/* The gradients: `h` is what the forward call wrote, grad_final_state may be
+ * NULL.  grad_x, grad_forget and grad_input_gate (which is there exactly where
+ * input_gate is) have grad_row_stride and are zero from a sequence's length
+ * on; grad_initial_state may be NULL or grad_final_state. */
+SNN_HIP_API int snn_hip_linear_recurrence_grad_f32(
+    const void* grad_h, const float* grad_final_state, const void* x,
+    const void* forget, const void* input_gate, const unsigned char* resets,
+    const int* lengths, const float* initial_state, const void* h,
+    void* grad_x, void* grad_forget, void* grad_input_gate,
+    float* grad_initial_state, const snn_hip_linear_recurrence_params* params,
+    void* workspace, size_t workspace_elems, void* stream);
+SNN_HIP_API int snn_hip_linear_recurrence_grad_f16(
+    const void* grad_h, const float* grad_final_state, const void* x,
+    const void* forget, const void* input_gate, const unsigned char* resets,
+    const int* lengths, const float* initial_state, const void* h,
+    void* grad_x, void* grad_forget, void* grad_input_gate,
+    float* grad_initial_state, const snn_hip_linear_recurrence_params* params,
+    void* workspace, size_t workspace_elems, void* stream);
+SNN_HIP_API int snn_hip_linear_recurrence_grad_bf16(
+    const void* grad_h, const float* grad_final_state, const void* x,
+    const void* forget, const void* input_gate, const unsigned char* resets,
+    const int* lengths, const float* initial_state, const void* h,
+    void* grad_x, void* grad_forget, void* grad_input_gate,
+    float* grad_initial_state, const snn_hip_linear_recurrence_params* params,
+    void* workspace, size_t workspace_elems, void* stream);
+/* Workspace of either call, in elements of `dtype`; none is required. */
+SNN_HIP_API int snn_hip_linear_recurrence_workspace_size(
+    const snn_hip_linear_recurrence_params* params, int dtype,
+    size_t* required_elems, size_t* recommended_elems);
 
 #ifdef __cplusplus
 }

@@ -43,6 +43,28 @@ class DIRECTION:
 class DTYPE:
     F32 = 0
     F16 = 1
+    BF16 = 2
+
+
+class ACTIVATION:
+    NONE = 0
+    RELU = 1
+    GELU = 2
+    GELU_TANH = 3
+    SILU = 4
+
+
+class NORM:
+    NONE = 0
+    RMS = 1
+    LAYER = 2
+
+
+class GATE:
+    NONE = 0
+    VALUE = 1
+    SIGMOID = 2
+    SILU = 3
 
 
 class POOL_OP:
@@ -67,9 +89,9 @@ class BINARY_OP:
     DIV = 3
 
 
-def _struct(name, fields, defaults):
+def _struct(name, fields, defaults, types={}):
     class S(ctypes.Structure):
-        _fields_ = [(f, ctypes.c_int) for f in fields]
+        _fields_ = [(f, types.get(f, ctypes.c_int)) for f in fields]
 
         def __init__(self, **kw):
             super().__init__()
@@ -80,7 +102,7 @@ def _struct(name, fields, defaults):
 
         def __repr__(self):
             return name + "(" + ", ".join(
-                "%s=%d" % (f, getattr(self, f)) for f in fields) + ")"
+                "%s=%s" % (f, getattr(self, f)) for f in fields) + ")"
     S.__name__ = name
     return S
 
@@ -104,6 +126,35 @@ PoolParams = _struct(
     ["in_rows", "in_cols", "out_rows", "out_cols", "window_rows",
      "window_cols", "stride_rows", "stride_cols", "batch", "channels",
      "pad_rows", "pad_cols", "input_format"], {})
+
+MatmulBiasActParams = _struct(
+    "MatmulBiasActParams",
+    ["m", "k", "n", "transpose_lhs", "transpose_rhs", "activation",
+     "lhs_stride", "rhs_stride", "residual_stride", "output_stride"], {})
+
+ResidualNormParams = _struct(
+    "ResidualNormParams",
+    ["rows", "channels", "post_norm", "pre_norm", "gate", "gate_rows",
+     "x_stride", "gate_stride", "epsilon"],
+    {"gate_rows": 1}, {"epsilon": ctypes.c_float})
+
+_NORM_TENSORS = ["x", "residual", "gate", "scale", "post_weight", "post_bias",
+                 "pre_weight", "pre_bias", "sum", "normed", "stats"]
+ResidualNormTensors = _struct(
+    "ResidualNormTensors", _NORM_TENSORS, {f: None for f in _NORM_TENSORS},
+    {f: ctypes.c_void_p for f in _NORM_TENSORS})
+
+_NORM_GRADIENTS = ["grad_sum", "grad_normed", "grad_x", "grad_residual",
+                   "grad_gate", "grad_scale", "grad_post_weight",
+                   "grad_post_bias", "grad_pre_weight", "grad_pre_bias"]
+ResidualNormGradients = _struct(
+    "ResidualNormGradients", _NORM_GRADIENTS,
+    {f: None for f in _NORM_GRADIENTS},
+    {f: ctypes.c_void_p for f in _NORM_GRADIENTS})
+
+LinearRecurrenceParams = _struct(
+    "LinearRecurrenceParams",
+    ["batch", "steps", "channels", "row_stride", "grad_row_stride"], {})
 
 _P = ctypes.c_void_p
 _SZ = ctypes.c_size_t
@@ -172,7 +223,21 @@ SIGNATURES = {
                              ctypes.POINTER(_I), _I, _I, _P],
     "snn_hip_binaryop_f16": [_P, _P, _P, ctypes.POINTER(_I), _I,
                              ctypes.POINTER(_I), _I, _I, _P],
+    "snn_hip_matmul_bias_act_workspace_size": [
+        _P, _I, _I, ctypes.POINTER(_SZ), ctypes.POINTER(_SZ)],
+    "snn_hip_residual_norm_grad_workspace_size": [
+        _P, _I, ctypes.POINTER(_SZ), ctypes.POINTER(_SZ)],
+    "snn_hip_linear_recurrence_workspace_size": [
+        _P, _I, ctypes.POINTER(_SZ), ctypes.POINTER(_SZ)],
 }
+for _type in ("f32", "f16", "bf16"):
+    SIGNATURES["snn_hip_matmul_bias_act_" + _type] = [_P] * 8 + [_SZ, _P]
+    SIGNATURES["snn_hip_matmul_bias_act_grad_" + _type] = [_P] * 9 + [_SZ, _P]
+    SIGNATURES["snn_hip_residual_norm_" + _type] = [_P] * 3
+    SIGNATURES["snn_hip_residual_norm_grad_" + _type] = [_P] * 4 + [_SZ, _P]
+    SIGNATURES["snn_hip_linear_recurrence_" + _type] = [_P] * 10 + [_SZ, _P]
+    SIGNATURES["snn_hip_linear_recurrence_grad_" + _type] = (
+        [_P] * 15 + [_SZ, _P])
 
 _lib = None
 

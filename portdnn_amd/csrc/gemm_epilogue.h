@@ -1,0 +1,655 @@
+// Matrix product with its epilogue, and the product of its gradients:
+//
+//   C[m][n] = act(sum over r of P[m][r] Q[n][r] + bias[n]) + residual[m][n]
+//
+// on the matrix instructions of gfx950: v_mfma_f32_16x16x32_{f16,bf16} for the
+// 16-bit types, v_mfma_f32_16x16x4_f32 for fp32, sums in fp32.  Both operands
+// come in either order in memory, the reduction contiguous ("K inner") or the
+// row, so that the forward product of any transposition and the two products of
+// its gradients, whose operands are the forward ones read the other way, run on
+// the same kernel without a copy.
+//
+// A work-group owns a BM x BN tile of C and a range of the reduction, which it
+// walks in chunks of 128 bytes (64 16-bit values, 32 floats).  A chunk of P and Q
+// goes to LDS, STAGES chunks in a ring:
+//
+//   K inner    [BM rows][128 bytes]; a fragment is one 16-byte read per lane
+//   row inner  [64 or 32 reductions][BM values]; 16-bit fragments are two
+//              transposing reads (ds_read_b64_tr_b16: within 16 lanes, lane
+//              4 j + i supplies the address of four values of reduction j and
+//              lane t receives column t of reductions 0 ... 3), floats four
+//              4-byte reads
+//
+// 16-byte pieces are XOR-swizzled so that lanes that read together fall into
+// different banks (swizzle() below).  Where rows start at multiples of 16 bytes
+// the loads go from memory straight to LDS and the swizzle is applied to their
+// source; elsewhere they pass through registers, so that odd sizes cost no copy.
+//
+// Q is the instruction's A operand, so a lane ends up with four neighbouring
+// columns of a row.  The tile leaves through LDS, each wave's part in its own
+// place: there a lane picks up eight neighbouring columns, for which the bias, the
+// residual, the activation and the rounding are one piece of code, and stores
+// whole rows.
+#ifndef PORTDNN_AMD_CSRC_GEMM_EPILOGUE_H_
+#define PORTDNN_AMD_CSRC_GEMM_EPILOGUE_H_
+
+#include "gemm_tile.h"
+#include "sequence.h"
+
+namespace snn {
+namespace epi {
+
+typedef float float4v __attribute__((ext_vector_type(4)));
+typedef unsigned int uint4v __attribute__((ext_vector_type(4)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef short short8v __attribute__((ext_vector_type(8)));
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) void* lds_ptr;
+typedef __attribute__((address_space(3))) short4v* lds_short4_ptr;
+
+// One product with its epilogue.  Sizes and strides in elements.
+struct Product {
+  const void *p, *q;
+  long p_stride, q_stride;
+  int m, n, k;  // k: the reduction
+  bool p_k_inner, q_k_inner;
+  const void *bias, *residual;
+  void *out, *pre;
+  long residual_stride, out_stride, pre_stride;
+  int activation;
+  bool wide;  // the epilogue's rows start at multiples of 16 bytes, n % 8 == 0
+  // division of the work
+  int tiles_m, tiles_n, splits, split_chunks;  // chunks of a share
+  float* partial;                              // [splits][m][n]
+};
+
+int run_f32(Product& g, void* workspace, size_t bytes, hipStream_t stream);
+int run_f16(Product& g, void* workspace, size_t bytes, hipStream_t stream);
+int run_bf16(Product& g, void* workspace, size_t bytes, hipStream_t stream);
+// Bytes of workspace that a product of m x n over k shares its reduction with.
+size_t split_bytes(int m, int n, int k, int elem_size);
+
+__device__ __forceinline__ float activate(float z, int kind) {
+  switch (kind) {
+    case SNN_HIP_ACTIVATION_RELU:
+      return z < 0.f ? 0.f : z;  // (a NaN stays)
+    case SNN_HIP_ACTIVATION_GELU:
+      return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+    case SNN_HIP_ACTIVATION_GELU_TANH: {
+      // (1 + tanh(u)) / 2 = sigmoid(2 u)
+      float s, rest;
+      seq::sigmoid<float>(
+          1.5957691216057308f * (z + 0.044715f * z * z * z), &s, &rest);
+      return z * s;
+    }
+    case SNN_HIP_ACTIVATION_SILU: {
+      float s, rest;
+      seq::sigmoid<float>(z, &s, &rest);
+      return z * s;
+    }
+    default:
+      return z;
+  }
+}
+
+__device__ __forceinline__ float activation_slope(float z, int kind) {
+  switch (kind) {
+    case SNN_HIP_ACTIVATION_RELU:
+      return z > 0.f ? 1.f : 0.f;
+    case SNN_HIP_ACTIVATION_GELU:
+      return 0.5f * (1.f + erff(z * 0.70710678118654752f)) +
+             z * 0.39894228040143268f * expf(-0.5f * z * z);
+    case SNN_HIP_ACTIVATION_GELU_TANH: {
+      float s, rest;
+      seq::sigmoid<float>(
+          1.5957691216057308f * (z + 0.044715f * z * z * z), &s, &rest);
+      return s + z * s * rest * 1.5957691216057308f *
+                     (1.f + 0.134145f * z * z);
+    }
+    case SNN_HIP_ACTIVATION_SILU: {
+      float s, rest;
+      seq::sigmoid<float>(z, &s, &rest);
+      return s + z * s * rest;
+    }
+    default:
+      return 1.f;
+  }
+}
+
+// Eight neighbouring columns of a row: bias, activation, residual, one rounding.
+template <typename T>
+__device__ __forceinline__ void finish8(const Product& g, int row, int col,
+                                        float (&v)[8]) {
+  constexpr int VEC = 16 / sizeof(T);
+  typedef typename seq::Pack<T, VEC>::type V;
+  const T* const bias = static_cast<const T*>(g.bias);
+  const T* const residual =
+      g.residual == nullptr
+          ? nullptr
+          : static_cast<const T*>(g.residual) + row * g.residual_stride;
+  T* const pre =
+      g.pre == nullptr ? nullptr : static_cast<T*>(g.pre) + row * g.pre_stride;
+  T* const out = static_cast<T*>(g.out) + row * g.out_stride;
+  if (g.wide) {
+    auto load = [&](const T* from, float (&to)[8]) {
+#pragma unroll
+      for (int j = 0; j < 8; j += VEC) {
+        float part[VEC];
+        seq::unpack<T, VEC>(*reinterpret_cast<const V*>(from + col + j), part);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) to[j + i] = part[i];
+      }
+    };
+    auto store = [&](T* to, const float (&from)[8]) {
+#pragma unroll
+      for (int j = 0; j < 8; j += VEC) {
+        float part[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) part[i] = from[j + i];
+        *reinterpret_cast<V*>(to + col + j) = seq::pack<T, VEC>(part);
+      }
+    };
+    float add[8];
+    if (bias != nullptr) {
+      load(bias, add);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] += add[i];
+    }
+    if (pre != nullptr) store(pre, v);
+    if (residual != nullptr) load(residual, add);
+    if (g.activation != SNN_HIP_ACTIVATION_NONE) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = activate(v[i], g.activation);
+    }
+    if (residual != nullptr) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] += add[i];
+    }
+    store(out, v);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (col + i >= g.n) break;
+    float z = v[i];
+    if (bias != nullptr) z += static_cast<float>(bias[col + i]);
+    if (pre != nullptr) pre[col + i] = static_cast<T>(z);
+    z = activate(z, g.activation);
+    if (residual != nullptr) z += static_cast<float>(residual[col + i]);
+    out[col + i] = static_cast<T>(z);
+  }
+}
+
+constexpr int kChunkBytes = 128;
+constexpr unsigned kOob = 0x80000000u;  // beyond every buffer's range
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* p) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, 0x7FFFFFF0,
+                                           0x00020000);
+}
+
+constexpr int vmcnt_imm(int n) { return 0x0F70 | (n & 15) | ((n >> 4) << 14); }
+constexpr int kLgkm0 = ~0x0F00;  // ... and all LDS reads, by &
+
+// Which 16-byte position of its row holds piece c: c ^ swizzle(row).
+//   K inner: the 16 rows of a fragment, two of which fill the 64 banks.
+//   row inner, 16-bit: the four reductions of a transposing read by the two
+//   blocks of eight, 32 bytes each.
+//   row inner, floats: four blocks of four reductions, 64 bytes each.
+template <int E, bool K_INNER, int ROWS>
+__device__ __forceinline__ constexpr unsigned swizzle(unsigned row) {
+  if (K_INNER) return (row >> 1) & 7u;
+  constexpr int kPitch = ROWS * E;
+  if (E == 2) {
+    if (kPitch >= 256) return 2u * ((row & 3u) | (((row >> 3) & 1u) << 2));
+    if (kPitch == 128)
+      return 2u * (((row >> 1) & 1u) | (((row >> 3) & 1u) << 1));
+    return 0;
+  }
+  if (kPitch >= 256) return 4u * ((row >> 2) & 3u);
+  if (kPitch == 128) return 4u * ((row >> 2) & 1u);
+  return 0;
+}
+
+// One operand's tile: ROWS rows of the result's dimension by a chunk of the
+// reduction, ROWS * 128 bytes either way.
+template <typename T, bool K_INNER, int ROWS>
+struct Operand {
+  static constexpr int E = sizeof(T);
+  static constexpr int kBlocks = ROWS * kChunkBytes / 1024;  // of 1 KiB
+  static constexpr int kPitch = K_INNER ? kChunkBytes : ROWS * E;
+  static constexpr int kPiece = 16 / E;  // values
+  static constexpr int kChunk = kChunkBytes / E;
+
+  // Row and column (in values) of the tile's memory that LDS position `pos`
+  // holds.
+  static __device__ __forceinline__ void source(unsigned pos, int* row,
+                                                int* col) {
+    const unsigned r = pos / kPitch;
+    const unsigned piece = (pos % kPitch) >> 4;
+    *row = static_cast<int>(r);
+    *col = static_cast<int>((piece ^ swizzle<E, K_INNER, ROWS>(r)) * kPiece);
+  }
+  // The tile's values at memory row / column, of which `rows_left` rows of the
+  // result and `k_left` reductions exist.
+  static __device__ __forceinline__ bool inside(int row, int col, int rows_left,
+                                                int k_left) {
+    return K_INNER ? row < rows_left && col < k_left
+                   : row < k_left && col < rows_left;
+  }
+  static __device__ __forceinline__ const T* at(const void* p, long stride,
+                                                int row0, int k0) {
+    return static_cast<const T*>(p) +
+           (K_INNER ? row0 * stride + k0 : k0 * stride + row0);
+  }
+
+  // LDS address of the lane's part of the fragment of rows row0 ... row0 + 15
+  // (step 0); K inner: step s is at the address ^ 64 s, row inner:
+  // at + s * kStep.
+  static __device__ __forceinline__ unsigned fragment(int row0, int lane) {
+    if (K_INNER) {
+      const unsigned row = row0 + (lane & 15);
+      return row * kChunkBytes +
+             (((lane >> 4) ^ swizzle<E, true, ROWS>(row)) << 4);
+    }
+    if (E == 2) {
+      const unsigned k = 8 * (lane >> 4) + ((lane >> 2) & 3);
+      const unsigned piece = row0 / 8 + ((lane & 3) >> 1);
+      return k * kPitch + ((piece ^ swizzle<E, false, ROWS>(k)) << 4) +
+             ((lane & 1) << 3);
+    }
+    const unsigned k = 4 * (lane >> 4);
+    const unsigned piece = row0 / 4 + ((lane & 15) >> 2);
+    return k * kPitch + ((piece ^ swizzle<E, false, ROWS>(k)) << 4) +
+           ((lane & 3) << 2);
+  }
+  static __device__ __forceinline__ uint4v read(const char* tile, unsigned at,
+                                                int s) {
+    if constexpr (K_INNER) {
+      return *reinterpret_cast<const uint4v*>(tile + (at ^ (s << 6)));
+    } else if constexpr (E == 2) {
+      const char* const from = tile + at + s * (32 * kPitch);
+      const short4v lo =
+          __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_ptr)(from));
+      const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (lds_short4_ptr)(from + 4 * kPitch));
+      return __builtin_bit_cast(
+          uint4v, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
+      const char* const from = tile + at + s * (16 * kPitch);
+      uint4v v;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+        v[t] = *reinterpret_cast<const unsigned*>(from + t * kPitch);
+      return v;
+    }
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ float4v multiply(uint4v q, uint4v p, float4v acc);
+template <>
+__device__ __forceinline__ float4v multiply<_Float16>(uint4v q, uint4v p,
+                                                      float4v acc) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(
+      __builtin_bit_cast(half8, q), __builtin_bit_cast(half8, p), acc, 0, 0, 0);
+}
+template <>
+__device__ __forceinline__ float4v multiply<__bf16>(uint4v q, uint4v p,
+                                                    float4v acc) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+      __builtin_bit_cast(bf16x8, q), __builtin_bit_cast(bf16x8, p), acc, 0, 0,
+      0);
+}
+// (four instructions over four reductions each: lane group g holds reductions
+// 4 g ... 4 g + 3 of the step's 16, instruction t takes the t-th of each)
+template <>
+__device__ __forceinline__ float4v multiply<float>(uint4v q, uint4v p,
+                                                   float4v acc) {
+  const float4v a = __builtin_bit_cast(float4v, q);
+  const float4v b = __builtin_bit_cast(float4v, p);
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+    acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[t], b[t], acc, 0, 0, 0);
+  return acc;
+}
+
+// LDS of a work-group: the ring of chunks, rounded up so that every wave issues
+// the same number of loads, or the tile on its way out.
+template <int BM, int BN, int WAVES, int STAGES>
+struct Space {
+  static constexpr int kBlocks = (BM + BN) * kChunkBytes / 1024;
+  static constexpr int kLoads = (kBlocks + WAVES - 1) / WAVES;  // per wave
+  static constexpr int kStage = kLoads * WAVES * 1024;
+};
+
+template <typename T, bool PK, bool QK, int BM, int BN, int WM, int WN,
+          int STAGES, bool DIRECT>
+__device__ __forceinline__ void gemm_body(const Product& g, char* r0, char* r1,
+                                          char* r2, char* r3) {
+  typedef Operand<T, PK, BM> OP;
+  typedef Operand<T, QK, BN> OQ;
+  constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
+  typedef Space<BM, BN, WAVES, STAGES> S;
+  constexpr int TM = BM / WM, TN = BN / WN, IM = TM / 16, IN = TN / 16;
+  constexpr int kPBytes = BM * kChunkBytes;
+  constexpr int kChunk = OP::kChunk;
+  auto ring = [&](int u) { return u == 0 ? r0 : u == 1 ? r1 : u == 2 ? r2 : r3; };
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave % WM, wn = wave / WM;
+
+  // Every XCD takes a run of tiles, in bands of eight tiles of rows, so that the
+  // tiles it works on at a time share both operands in its L2.
+  const unsigned tiles = static_cast<unsigned>(g.tiles_m) * g.tiles_n;
+  const unsigned lin = gemm::xcd_remap(blockIdx.x, tiles * g.splits);
+  const unsigned split = lin / tiles, tile = lin - split * tiles;
+  constexpr unsigned kBand = 8;
+  const unsigned band = tile / (kBand * g.tiles_n);
+  const unsigned in_band = tile - band * kBand * g.tiles_n;
+  const unsigned height = min(kBand, g.tiles_m - band * kBand);
+  const int row0 = static_cast<int>(band * kBand + in_band % height) * BM;
+  const int col0 = static_cast<int>(in_band / height) * BN;
+  const int k_begin = static_cast<int>(split) * g.split_chunks * kChunk;
+  const int k_end = min(g.k, k_begin + g.split_chunks * kChunk);
+  const int chunks = (k_end - k_begin + kChunk - 1) / kChunk;
+  const int rows_left = g.m - row0, cols_left = g.n - col0;
+
+  unsigned at_p[IM], at_q[IN];
+#pragma unroll
+  for (int i = 0; i < IM; ++i)
+    at_p[i] = OP::fragment(wm * TM + 16 * i, lane);
+#pragma unroll
+  for (int j = 0; j < IN; ++j)
+    at_q[j] = kPBytes + OQ::fragment(wn * TN + 16 * j, lane);
+
+  float4v acc[IM][IN];
+#pragma unroll
+  for (int i = 0; i < IM; ++i)
+#pragma unroll
+    for (int j = 0; j < IN; ++j) acc[i][j] = float4v{0.f, 0.f, 0.f, 0.f};
+
+  auto compute = [&](const char* tile_at) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      uint4v p[IM], q[IN];
+#pragma unroll
+      for (int j = 0; j < IN; ++j) q[j] = OQ::read(tile_at, at_q[j], s);
+#pragma unroll
+      for (int i = 0; i < IM; ++i) p[i] = OP::read(tile_at, at_p[i], s);
+#pragma unroll
+      for (int i = 0; i < IM; ++i)
+#pragma unroll
+        for (int j = 0; j < IN; ++j) acc[i][j] = multiply<T>(q[j], p[i], acc[i][j]);
+    }
+  };
+
+  if constexpr (DIRECT) {
+    // Offsets of the lane's loads within a chunk; the chunk's own place is in
+    // the buffer's base, so that operands may be of any size.
+    unsigned offset[S::kLoads];
+    int order[S::kLoads];  // its reduction index
+#pragma unroll
+    for (int l = 0; l < S::kLoads; ++l) {
+      const int block = wave + l * WAVES;
+      int row, col;
+      bool in;
+      long stride;
+      if (block < OP::kBlocks) {
+        OP::source(block * 1024 + lane * 16, &row, &col);
+        in = PK ? row < rows_left : col < rows_left;
+        stride = g.p_stride;
+        order[l] = PK ? col : row;
+      } else {
+        OQ::source((block - OP::kBlocks) * 1024 + lane * 16, &row, &col);
+        in = block < S::kBlocks && (QK ? row < cols_left : col < cols_left);
+        stride = g.q_stride;
+        order[l] = QK ? col : row;
+      }
+      offset[l] = in ? static_cast<unsigned>((row * stride + col) * sizeof(T))
+                     : kOob;
+    }
+    const char* from_p =
+        reinterpret_cast<const char*>(OP::at(g.p, g.p_stride, row0, k_begin));
+    const char* from_q =
+        reinterpret_cast<const char*>(OQ::at(g.q, g.q_stride, col0, k_begin));
+    const long step_p = PK ? kChunkBytes : kChunkBytes * g.p_stride;
+    const long step_q = QK ? kChunkBytes : kChunkBytes * g.q_stride;
+    int k_left = k_end - k_begin;
+    auto issue = [&](char* to) {  // the next chunk
+      const __amdgpu_buffer_rsrc_t p = make_rsrc(from_p), q = make_rsrc(from_q);
+#pragma unroll
+      for (int l = 0; l < S::kLoads; ++l) {
+        const int block = wave + l * WAVES;
+        const unsigned from = order[l] < k_left ? offset[l] : kOob;
+        if (block < OP::kBlocks)
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(
+              p, (lds_ptr)(to + block * 1024), 16, from, 0, 0, 0);
+        else
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(
+              q, (lds_ptr)(to + block * 1024), 16, from, 0, 0, 0);
+      }
+      from_p += step_p;
+      from_q += step_q;
+      k_left -= kChunk;
+    };
+    // STAGES - 1 chunks are under way while one is multiplied; behind the last
+    // one the loads are out of range, so that there is always the same number.  A
+    // chunk's place is loaded again behind the barrier that every wave reaches
+    // when it has read it.  (The places are arrays of their own: the compiler
+    // waits for all loads into an array before it reads from it.)
+#pragma unroll
+    for (int c = 0; c < STAGES - 1; ++c) issue(ring(c));
+    int left = chunks;
+    while (left > 0) {
+#pragma unroll
+      for (int u = 0; u < STAGES; ++u) {
+        if (left == 0) break;
+        // the chunk is here, and the reads of the one before have returned
+        __builtin_amdgcn_s_waitcnt(kLgkm0 &
+                                   vmcnt_imm((STAGES - 2) * S::kLoads));
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        issue(ring((u + STAGES - 1) % STAGES));
+        compute(ring(u));
+        --left;
+      }
+    }
+    __builtin_amdgcn_s_waitcnt(kLgkm0 & vmcnt_imm(0));
+  } else {
+    // Through registers: the loads of a chunk are under way while the one before
+    // it is multiplied, two places in turn.
+    constexpr int kPieces = (BM + BN) * kChunkBytes / 16;
+    constexpr int kEach = (kPieces + THREADS - 1) / THREADS;
+    uint4v held[kEach];
+    auto load_piece = [&](auto operand, const void* base, long stride,
+                          int left, int first, unsigned pos, int k0) {
+      typedef decltype(operand) O;
+      int row, col;
+      O::source(pos, &row, &col);
+      const int k_left = k_end - k0;
+      const T* const from =
+          O::at(base, stride, first, k0) + row * stride + col;
+      uint4v v = {0u, 0u, 0u, 0u};
+      if (O::inside(row, col + O::kPiece - 1, left, k_left)) {
+        __builtin_memcpy(&v, from, 16);
+      } else if (O::inside(row, col, left, k_left)) {
+        T part[O::kPiece] = {};
+#pragma unroll
+        for (int i = 0; i < O::kPiece; ++i)
+          if (O::inside(row, col + i, left, k_left)) part[i] = from[i];
+        __builtin_memcpy(&v, part, 16);
+      }
+      return v;
+    };
+    auto load = [&](int chunk) {
+      const int k0 = k_begin + chunk * kChunk;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        const unsigned pos = (tid + e * THREADS) * 16;
+        if (pos < static_cast<unsigned>(kPBytes))
+          held[e] = load_piece(OP(), g.p, g.p_stride, rows_left, row0, pos, k0);
+        else if (pos < static_cast<unsigned>(kPieces) * 16)
+          held[e] = load_piece(OQ(), g.q, g.q_stride, cols_left, col0,
+                               pos - kPBytes, k0);
+      }
+    };
+    auto put = [&](char* to) {
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        const unsigned pos = (tid + e * THREADS) * 16;
+        if (pos < static_cast<unsigned>(kPieces) * 16)
+          *reinterpret_cast<uint4v*>(to + pos) = held[e];
+      }
+    };
+    load(0);
+    int c = 0;
+    while (c < chunks) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if (c == chunks) break;
+        put(ring(u));
+        __syncthreads();
+        if (c + 1 < chunks) load(c + 1);
+        compute(ring(u));
+        ++c;
+      }
+    }
+  }
+
+  // The way out.  A wave's part of the tile in passes of kRows rows, a 16-byte
+  // piece c of row r at c ^ (r & 15) (& 7 for rows of 32 columns).
+  __syncthreads();
+  constexpr int kSharers = (WAVES + STAGES - 1) / STAGES;  // of a chunk's place
+  constexpr int kSpace = S::kStage / kSharers / 1024 * 1024;
+  constexpr int kFit = kSpace / (TN * 4) / 16 * 16;
+  constexpr int kRows = TM <= kFit ? TM : kFit;
+  static_assert(kRows >= 16 && TM % kRows == 0, "no room for the way out");
+  constexpr unsigned kMask = TN / 4 - 1 < 15 ? TN / 4 - 1 : 15;
+  char* own = ring(0);
+#pragma unroll
+  for (int u = 1; u < STAGES; ++u)
+    if (wave / kSharers == u) own = ring(u);
+  own += wave % kSharers * kSpace;
+  constexpr int kLanes = TN / 8;          // of a row
+  constexpr int kTurnRows = 64 / kLanes;  // rows at a time
+#pragma unroll
+  for (int pass = 0; pass < TM / kRows; ++pass) {
+#pragma unroll
+    for (int i = 0; i < kRows / 16; ++i) {
+      const unsigned r = 16 * i + (lane & 15);
+#pragma unroll
+      for (int j = 0; j < IN; ++j) {
+        const unsigned piece = (4 * j + (lane >> 4)) ^ (r & kMask);
+        *reinterpret_cast<float4v*>(own + r * (TN * 4) + piece * 16) =
+            acc[pass * (kRows / 16) + i][j];
+      }
+    }
+    const int col = col0 + wn * TN + (lane % kLanes) * 8;
+#pragma unroll 1
+    for (int t = 0; t < kRows; t += kTurnRows) {
+      const unsigned r = t + lane / kLanes;
+      const int row = row0 + wm * TM + pass * kRows + static_cast<int>(r);
+      if (row >= g.m || col >= g.n) continue;
+      float v[8];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const unsigned piece = (2 * (lane % kLanes) + h) ^ (r & kMask);
+        const float4v f =
+            *reinterpret_cast<const float4v*>(own + r * (TN * 4) + piece * 16);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[4 * h + i] = f[i];
+      }
+      if (g.splits == 1) {
+        finish8<T>(g, row, col, v);
+      } else {
+        float* const to =
+            g.partial + (static_cast<long>(split) * g.m + row) * g.n + col;
+        if (g.n % 8 == 0) {
+          *reinterpret_cast<float4v*>(to) = float4v{v[0], v[1], v[2], v[3]};
+          *reinterpret_cast<float4v*>(to + 4) = float4v{v[4], v[5], v[6], v[7]};
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (col + i < g.n) to[i] = v[i];
+        }
+      }
+    }
+  }
+}
+
+// Adds the shares of a divided reduction in their order and finishes.
+template <typename T>
+__global__ void __launch_bounds__(256) gemm_join_kernel(Product g) {
+  const int groups = (g.n + 7) / 8;
+  const long at = static_cast<long>(blockIdx.x) * 256 + threadIdx.x;
+  const int row = static_cast<int>(at / groups);
+  const int col = static_cast<int>(at - static_cast<long>(row) * groups) * 8;
+  if (row >= g.m) return;
+  const long size = static_cast<long>(g.m) * g.n;
+  const float* from = g.partial + static_cast<long>(row) * g.n + col;
+  float v[8] = {};
+  if (g.n % 8 == 0) {
+#pragma unroll 4
+    for (int s = 0; s < g.splits; ++s) {
+      const float4v a = *reinterpret_cast<const float4v*>(from + s * size);
+      const float4v b = *reinterpret_cast<const float4v*>(from + s * size + 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] += a[i];
+        v[4 + i] += b[i];
+      }
+    }
+  } else {
+    for (int s = 0; s < g.splits; ++s)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (col + i < g.n) v[i] += from[s * size + i];
+  }
+  finish8<T>(g, row, col, v);
+}
+
+// How a product is divided: the tile's shape and the shares of the reduction.
+struct Plan {
+  int bm, bn, tiles_m, tiles_n, splits, split_chunks;
+};
+
+inline Plan make_plan(int m, int n, int k, int elem_size, bool direct,
+                      size_t bytes) {
+  Plan p;
+  const int chunk = kChunkBytes / elem_size;
+  const int chunks = ceil_div(k, chunk);
+  if (m <= 16) {
+    p.bm = 16;
+    p.bn = 128;
+  } else if (m <= 64) {
+    p.bm = 64;
+    p.bn = 128;
+  } else if (elem_size == 2 && direct &&
+             static_cast<long>(ceil_div(m, 256)) * ceil_div(n, 256) >= 192) {
+    p.bm = p.bn = 256;
+  } else {
+    p.bm = p.bn = 128;
+  }
+  p.tiles_m = ceil_div(m, p.bm);
+  p.tiles_n = ceil_div(n, p.bn);
+  // As many shares as fill the CUs, of four chunks at least.
+  const long tiles = static_cast<long>(p.tiles_m) * p.tiles_n;
+  long want = tiles >= 256 ? 1 : 512 / tiles;
+  want = want > chunks / 4 ? chunks / 4 : want;
+  const size_t share = static_cast<size_t>(m) * n * sizeof(float);
+  if (static_cast<size_t>(want) * share > bytes)
+    want = static_cast<long>(bytes / share);
+  if (want < 2) want = 1;
+  p.split_chunks = ceil_div(chunks, static_cast<int>(want));
+  p.splits = ceil_div(chunks, p.split_chunks);
+  return p;
+}
+
+}  // namespace epi
+}  // namespace snn
+
+#endif  // PORTDNN_AMD_CSRC_GEMM_EPILOGUE_H_

@@ -52,6 +52,13 @@ class Args {
     if (v == -1 && PyErr_Occurred()) ok = false;
     return static_cast<int>(v);
   }
+  double real() {
+    PyObject* const o = args_[next_++];
+    if (!ok) return 0.0;
+    const double v = PyFloat_AsDouble(o);
+    if (v == -1.0 && PyErr_Occurred()) ok = false;
+    return v;
+  }
   template <typename T>
   T params() {
     PyObject* const o = args_[next_++];
@@ -302,6 +309,201 @@ PyObject* binaryop(PyObject*, PyObject* const* args, Py_ssize_t n) {
   });
 }
 
+// The operators of a residual block take their parameter records as plain
+// numbers: they have many optional operands, and a record built in Python for
+// every call would cost as much as the call.
+void read_params(Args& a, snn_hip_matmul_bias_act_params* p) {
+  p->m = a.integer();
+  p->k = a.integer();
+  p->n = a.integer();
+  p->transpose_lhs = a.integer();
+  p->transpose_rhs = a.integer();
+  p->activation = a.integer();
+  p->lhs_stride = a.integer();
+  p->rhs_stride = a.integer();
+  p->residual_stride = a.integer();
+  p->output_stride = a.integer();
+}
+
+// (fn, lhs, rhs, bias, residual, output, pre_activation, <10 numbers>,
+//  workspace, elements, stream)
+PyObject* matmul_bias_act(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 20);
+  if (!a.ok) return nullptr;
+  using Fn = int (*)(const void*, const void*, const void*, const void*, void*,
+                     void*, const snn_hip_matmul_bias_act_params*, void*,
+                     size_t, void*);
+  const Fn fn = reinterpret_cast<Fn>(a.pointer());
+  void* t[6];
+  for (void*& p : t) p = a.pointer();
+  snn_hip_matmul_bias_act_params params;
+  read_params(a, &params);
+  void* const workspace = a.pointer();
+  const size_t elems = a.size();
+  void* const stream = a.pointer();
+  return launch(a, [&] {
+    return fn(t[0], t[1], t[2], t[3], t[4], t[5], &params, workspace, elems,
+              stream);
+  });
+}
+
+// (fn, grad_output, lhs, rhs, pre_activation, grad_lhs, grad_rhs, grad_bias,
+//  <10 numbers>, workspace, elements, stream)
+PyObject* matmul_bias_act_grad(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 21);
+  if (!a.ok) return nullptr;
+  using Fn = int (*)(const void*, const void*, const void*, const void*, void*,
+                     void*, void*, const snn_hip_matmul_bias_act_params*, void*,
+                     size_t, void*);
+  const Fn fn = reinterpret_cast<Fn>(a.pointer());
+  void* t[7];
+  for (void*& p : t) p = a.pointer();
+  snn_hip_matmul_bias_act_params params;
+  read_params(a, &params);
+  void* const workspace = a.pointer();
+  const size_t elems = a.size();
+  void* const stream = a.pointer();
+  return launch(a, [&] {
+    return fn(t[0], t[1], t[2], t[3], t[4], t[5], t[6], &params, workspace,
+              elems, stream);
+  });
+}
+
+void read_tensors(Args& a, snn_hip_residual_norm_tensors* t) {
+  t->x = a.pointer();
+  t->residual = a.pointer();
+  t->gate = a.pointer();
+  t->scale = a.pointer();
+  t->post_weight = a.pointer();
+  t->post_bias = a.pointer();
+  t->pre_weight = a.pointer();
+  t->pre_bias = a.pointer();
+  t->sum = a.pointer();
+  t->normed = a.pointer();
+  t->stats = static_cast<float*>(a.pointer());
+}
+
+void read_params(Args& a, snn_hip_residual_norm_params* p) {
+  p->rows = a.integer();
+  p->channels = a.integer();
+  p->post_norm = a.integer();
+  p->pre_norm = a.integer();
+  p->gate = a.integer();
+  p->gate_rows = a.integer();
+  p->x_stride = a.integer();
+  p->gate_stride = a.integer();
+  p->epsilon = static_cast<float>(a.real());
+}
+
+// (fn, <11 tensors>, <8 numbers>, epsilon, stream)
+PyObject* residual_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 22);
+  if (!a.ok) return nullptr;
+  using Fn = int (*)(const snn_hip_residual_norm_tensors*,
+                     const snn_hip_residual_norm_params*, void*);
+  const Fn fn = reinterpret_cast<Fn>(a.pointer());
+  snn_hip_residual_norm_tensors t;
+  read_tensors(a, &t);
+  snn_hip_residual_norm_params params;
+  read_params(a, &params);
+  void* const stream = a.pointer();
+  return launch(a, [&] { return fn(&t, &params, stream); });
+}
+
+// (fn, <11 tensors>, <10 gradients>, <8 numbers>, epsilon, workspace, elements,
+//  stream)
+PyObject* residual_norm_grad(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 34);
+  if (!a.ok) return nullptr;
+  using Fn = int (*)(const snn_hip_residual_norm_tensors*,
+                     const snn_hip_residual_norm_gradients*,
+                     const snn_hip_residual_norm_params*, void*, size_t, void*);
+  const Fn fn = reinterpret_cast<Fn>(a.pointer());
+  snn_hip_residual_norm_tensors t;
+  read_tensors(a, &t);
+  snn_hip_residual_norm_gradients g;
+  g.grad_sum = a.pointer();
+  g.grad_normed = a.pointer();
+  g.grad_x = a.pointer();
+  g.grad_residual = a.pointer();
+  g.grad_gate = a.pointer();
+  g.grad_scale = a.pointer();
+  g.grad_post_weight = a.pointer();
+  g.grad_post_bias = a.pointer();
+  g.grad_pre_weight = a.pointer();
+  g.grad_pre_bias = a.pointer();
+  snn_hip_residual_norm_params params;
+  read_params(a, &params);
+  void* const workspace = a.pointer();
+  const size_t elems = a.size();
+  void* const stream = a.pointer();
+  return launch(a, [&] {
+    return fn(&t, &g, &params, workspace, elems, stream);
+  });
+}
+
+void read_params(Args& a, snn_hip_linear_recurrence_params* p) {
+  p->batch = a.integer();
+  p->steps = a.integer();
+  p->channels = a.integer();
+  p->row_stride = a.integer();
+  p->grad_row_stride = a.integer();
+}
+
+// (fn, x, forget, input_gate, resets, lengths, initial_state, h, final_state,
+//  <5 numbers>, workspace, elements, stream)
+PyObject* linear_recurrence(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 17);
+  if (!a.ok) return nullptr;
+  using Fn = int (*)(const void*, const void*, const void*,
+                     const unsigned char*, const int*, const float*, void*,
+                     float*, const snn_hip_linear_recurrence_params*, void*,
+                     size_t, void*);
+  const Fn fn = reinterpret_cast<Fn>(a.pointer());
+  void* t[8];
+  for (void*& p : t) p = a.pointer();
+  snn_hip_linear_recurrence_params params;
+  read_params(a, &params);
+  void* const workspace = a.pointer();
+  const size_t elems = a.size();
+  void* const stream = a.pointer();
+  return launch(a, [&] {
+    return fn(t[0], t[1], t[2], static_cast<const unsigned char*>(t[3]),
+              static_cast<const int*>(t[4]), static_cast<const float*>(t[5]),
+              t[6], static_cast<float*>(t[7]), &params, workspace, elems,
+              stream);
+  });
+}
+
+// (fn, grad_h, grad_final_state, x, forget, input_gate, resets, lengths,
+//  initial_state, h, grad_x, grad_forget, grad_input_gate, grad_initial_state,
+//  <5 numbers>, workspace, elements, stream)
+PyObject* linear_recurrence_grad(PyObject*, PyObject* const* args,
+                                 Py_ssize_t n) {
+  Args a(args, n, 22);
+  if (!a.ok) return nullptr;
+  using Fn = int (*)(const void*, const float*, const void*, const void*,
+                     const void*, const unsigned char*, const int*,
+                     const float*, const void*, void*, void*, void*, float*,
+                     const snn_hip_linear_recurrence_params*, void*, size_t,
+                     void*);
+  const Fn fn = reinterpret_cast<Fn>(a.pointer());
+  void* t[13];
+  for (void*& p : t) p = a.pointer();
+  snn_hip_linear_recurrence_params params;
+  read_params(a, &params);
+  void* const workspace = a.pointer();
+  const size_t elems = a.size();
+  void* const stream = a.pointer();
+  return launch(a, [&] {
+    return fn(t[0], static_cast<const float*>(t[1]), t[2], t[3], t[4],
+              static_cast<const unsigned char*>(t[5]),
+              static_cast<const int*>(t[6]), static_cast<const float*>(t[7]),
+              t[8], t[9], t[10], t[11], static_cast<float*>(t[12]), &params,
+              workspace, elems, stream);
+  });
+}
+
 #define SNN_PY_METHOD(name)                                              \
   {                                                                      \
     #name,                                                               \
@@ -316,6 +518,12 @@ PyMethodDef methods[] = {SNN_PY_METHOD(conv2d),
                          SNN_PY_METHOD(pooling_avg_grad),
                          SNN_PY_METHOD(pointwise_forward),
                          SNN_PY_METHOD(binaryop),
+                         SNN_PY_METHOD(matmul_bias_act),
+                         SNN_PY_METHOD(matmul_bias_act_grad),
+                         SNN_PY_METHOD(residual_norm),
+                         SNN_PY_METHOD(residual_norm_grad),
+                         SNN_PY_METHOD(linear_recurrence),
+                         SNN_PY_METHOD(linear_recurrence_grad),
                          {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods,

@@ -1,0 +1,181 @@
+// What the kernels of residual_norm.hip and residual_norm_grad.hip share.
+#ifndef PORTDNN_AMD_CSRC_RESIDUAL_NORM_H_
+#define PORTDNN_AMD_CSRC_RESIDUAL_NORM_H_
+
+#include "sequence.h"
+
+namespace snn {
+namespace norm {
+
+// Rows of up to kMaxChannels values stay in registers: PT of them per lane.
+constexpr int kMaxChannels = 16384;
+
+// The operands as a kernel takes them: strides filled in.
+struct Rows {
+  snn_hip_residual_norm_tensors t;
+  int rows, channels, post, pre, gate, gate_rows;
+  long x_stride, gate_stride;
+  float epsilon;
+};
+
+inline Rows rows_of(const snn_hip_residual_norm_tensors& t,
+                    const snn_hip_residual_norm_params& p) {
+  Rows r = {};
+  r.t = t;
+  r.rows = p.rows;
+  r.channels = p.channels;
+  r.post = p.post_norm;
+  r.pre = p.pre_norm;
+  r.gate = p.gate;
+  r.gate_rows = p.gate_rows;
+  r.x_stride = p.x_stride == 0 ? p.channels : p.x_stride;
+  r.gate_stride = p.gate_stride == 0 ? p.channels : p.gate_stride;
+  r.epsilon = p.epsilon;
+  return r;
+}
+
+inline int check_params(const snn_hip_residual_norm_params* p) {
+  if (p == nullptr) return SNN_HIP_INVALID_PARAMETER;
+  SNN_REQUIRE(p->rows > 0 && p->channels > 0 && p->channels <= kMaxChannels);
+  SNN_REQUIRE(p->post_norm >= SNN_HIP_NORM_NONE &&
+              p->post_norm <= SNN_HIP_NORM_LAYER);
+  SNN_REQUIRE(p->pre_norm >= SNN_HIP_NORM_NONE &&
+              p->pre_norm <= SNN_HIP_NORM_LAYER);
+  SNN_REQUIRE(p->gate >= SNN_HIP_GATE_NONE && p->gate <= SNN_HIP_GATE_SILU);
+  SNN_REQUIRE(p->gate == SNN_HIP_GATE_NONE || p->gate_rows > 0);
+  SNN_REQUIRE(p->x_stride == 0 || p->x_stride >= p->channels);
+  SNN_REQUIRE(p->gate_stride == 0 || p->gate_stride >= p->channels);
+  SNN_REQUIRE(p->epsilon >= 0.f);  // (a NaN is not)
+  return SNN_HIP_OK;
+}
+
+inline int check_operands(const snn_hip_residual_norm_tensors* t,
+                          const snn_hip_residual_norm_params& p) {
+  if (t == nullptr) return SNN_HIP_INVALID_PARAMETER;
+  SNN_REQUIRE(t->x != nullptr);
+  SNN_REQUIRE((t->gate != nullptr) == (p.gate != SNN_HIP_GATE_NONE));
+  SNN_REQUIRE(p.post_norm != SNN_HIP_NORM_NONE ||
+              (t->post_weight == nullptr && t->post_bias == nullptr));
+  SNN_REQUIRE(p.pre_norm != SNN_HIP_NORM_NONE ||
+              (t->pre_weight == nullptr && t->pre_bias == nullptr));
+  return SNN_HIP_OK;
+}
+
+// The gate's factor and its derivative.
+template <typename T>
+__device__ __forceinline__ void gate_of(int kind, float g, float* value,
+                                        float* slope) {
+  if (kind == SNN_HIP_GATE_VALUE) {
+    *value = g;
+    *slope = 1.f;
+    return;
+  }
+  float s, rest;
+  seq::sigmoid<T>(g, &s, &rest);
+  if (kind == SNN_HIP_GATE_SIGMOID) {
+    *value = s;
+    *slope = s * rest;
+  } else {
+    *value = g * s;
+    *slope = s + g * s * rest;
+  }
+}
+
+// Sums over the lanes that share a row: a wave, or all waves of the work-group
+// through LDS.  Two slots in turn, so that one barrier a sum is enough: a wave
+// is past the reads of a slot when it has passed the next sum's barrier.
+template <int WAVES, int N>
+__device__ __forceinline__ void row_sums(float (&v)[N], float* lds, int* turn) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = seq::wave_sum(v[i]);
+  if constexpr (WAVES > 1) {
+    float* const slot = lds + *turn * (2 * WAVES);
+    *turn ^= 1;
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) slot[i * WAVES + wave] = v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float s = 0.f;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) s += slot[i * WAVES + w];
+      v[i] = s;
+    }
+  }
+}
+
+// PT values of a row per lane, as PT / VEC accesses: access j of lane l holds
+// the channels (j * lanes + l) * VEC ... + VEC - 1.  Beyond the row's end the
+// values are zero and nothing is stored.
+template <typename T, int VEC, int PT, int WAVES>
+struct Slice {
+  static constexpr int kLanes = 64 * WAVES;
+  typedef typename seq::Pack<T, VEC>::type V;
+
+  static __device__ __forceinline__ int lane() {
+    return WAVES == 1 ? static_cast<int>(threadIdx.x & 63)
+                      : static_cast<int>(threadIdx.x);
+  }
+  static __device__ __forceinline__ int channel(int j) {
+    return (j * kLanes + lane()) * VEC;
+  }
+  static __device__ __forceinline__ void load(const void* row, int channels,
+                                              float (&out)[PT]) {
+    V raw[PT / VEC];
+#pragma unroll
+    for (int j = 0; j < PT / VEC; ++j) {
+      raw[j] = V{};
+      if (channel(j) < channels)
+        raw[j] = *reinterpret_cast<const V*>(static_cast<const T*>(row) +
+                                             channel(j));
+    }
+#pragma unroll
+    for (int j = 0; j < PT / VEC; ++j) {
+      float part[VEC];
+      seq::unpack<T, VEC>(raw[j], part);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) out[j * VEC + k] = part[k];
+    }
+  }
+  static __device__ __forceinline__ void store(void* row, int channels,
+                                               const float (&in)[PT]) {
+#pragma unroll
+    for (int j = 0; j < PT / VEC; ++j) {
+      float part[VEC];
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) part[k] = in[j * VEC + k];
+      if (channel(j) < channels)
+        *reinterpret_cast<V*>(static_cast<T*>(row) + channel(j)) =
+            seq::pack<T, VEC>(part);
+    }
+  }
+  static __device__ __forceinline__ bool inside(int i, int channels) {
+    return channel(i / VEC) < channels;  // (channels is a multiple of VEC)
+  }
+};
+
+// Calls `go` with the waves that share a row: at most PT = 8 values per lane up
+// to 8192 channels, 16 beyond.
+template <typename Go>
+int by_channels(int channels, Go go) {
+  using std::integral_constant;
+  if (channels <= 512)
+    return go(integral_constant<int, 1>(), integral_constant<int, 8>());
+  if (channels <= 1024)
+    return go(integral_constant<int, 2>(), integral_constant<int, 8>());
+  if (channels <= 2048)
+    return go(integral_constant<int, 4>(), integral_constant<int, 8>());
+  if (channels <= 4096)
+    return go(integral_constant<int, 8>(), integral_constant<int, 8>());
+  if (channels <= 8192)
+    return go(integral_constant<int, 16>(), integral_constant<int, 8>());
+  return go(integral_constant<int, 16>(), integral_constant<int, 16>());
+}
+
+}  // namespace norm
+}  // namespace snn
+
+#endif  // PORTDNN_AMD_CSRC_RESIDUAL_NORM_H_

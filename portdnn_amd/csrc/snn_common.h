@@ -106,6 +106,19 @@ struct Elem<_Float16> {
   }
 };
 
+template <>
+struct Elem<__bf16> {
+  __host__ __device__ static float load(const __bf16* p) {
+    return static_cast<float>(*p);
+  }
+  __host__ __device__ static float to_float(__bf16 v) {
+    return static_cast<float>(v);
+  }
+  __host__ __device__ static __bf16 from_float(float v) {
+    return static_cast<__bf16>(v);  // to nearest, ties to even
+  }
+};
+
 // Stream-ordered temporaries (partial results, re-laid-out filters) for calls
 // that bring no workspace.  They come from a memory pool of the library's own,
 // one per device, that keeps up to 512 MiB of freed blocks instead of handing

@@ -8,8 +8,9 @@ import ctypes
 import torch
 
 from . import _native, capi
-from .capi import ALGO, BINARY_OP, DIRECTION, POINTWISE_OP, POOL_OP, STATUS, \
-    ConvParams, DepthwiseParams, PoolParams
+from .capi import ACTIVATION, ALGO, BINARY_OP, DIRECTION, DTYPE, GATE, NORM, \
+    POINTWISE_OP, POOL_OP, STATUS, ConvParams, DepthwiseParams, \
+    LinearRecurrenceParams, MatmulBiasActParams, PoolParams, ResidualNormParams
 
 
 def calculate_padding(inp, window, stride, same):
@@ -484,17 +485,372 @@ def binaryop(lhs, rhs, lhs_dims, rhs_dims, op, out=None):
     return out
 
 
+# ---- a residual block over sequences -----------------------------------------
+# The operators below take their sizes and strides from the tensors: a matrix is
+# a 2-D tensor, a sequence a [batch, steps, channels] one, whose rows may be
+# slices of wider ones.
+
+_TYPES = {torch.float32: ("_f32", DTYPE.F32), torch.float16: ("_f16", DTYPE.F16),
+          torch.bfloat16: ("_bf16", DTYPE.BF16)}
+
+
+def _row_stride(t):
+    """Elements from row to row of a matrix whose rows are contiguous."""
+    rows, cols = t.shape
+    if rows == 1:
+        assert cols == 1 or t.stride(1) == 1
+        return cols
+    step, unit = t.stride()
+    assert (unit == 1 or cols == 1) and step >= cols, "rows are not contiguous"
+    return step
+
+
+def _step_stride(t):
+    """Elements from step to step of a [batch, steps, channels] tensor."""
+    batch, steps, channels = t.shape
+    outer, step, unit = t.stride()
+    assert unit == 1 or channels == 1, "channels are not contiguous"
+    if steps == 1:
+        step = outer if batch > 1 else channels
+    else:
+        assert batch == 1 or outer == steps * step, \
+            "sequences do not follow one another"
+    assert step >= channels
+    return step
+
+
+def _vector(t, n, dtype):
+    """The address of an optional vector of n values."""
+    if t is None:
+        return None
+    assert t.numel() == n and t.dtype == dtype and t.is_contiguous()
+    return t.data_ptr()
+
+
+def _like(t, shape, dtype):
+    """The address of an optional contiguous tensor."""
+    if t is None:
+        return None
+    assert t.shape == shape and t.dtype == dtype and t.is_contiguous()
+    return t.data_ptr()
+
+
+_sizes = {}
+
+
+def _workspace(entry, params, *args):
+    """(required, recommended) elements of a workspace query; the answer goes
+    by the sizes alone."""
+    key = (entry, bytes(params)) + args
+    got = _sizes.get(key)
+    if got is None:
+        req, rec = ctypes.c_size_t(), ctypes.c_size_t()
+        capi.check(getattr(capi.lib(), entry)(
+            ctypes.byref(params), *args, ctypes.byref(req), ctypes.byref(rec)))
+        got = _sizes[key] = (req.value, rec.value)
+    return got
+
+
+_matmul_sizes = {}
+
+
+def _matmul_workspace(m, k, n, trans_a, trans_b, activation, grad, t):
+    key = (m, k, n, trans_a, trans_b, activation, grad, t.dtype)
+    elems = _matmul_sizes.get(key)
+    if elems is None:
+        elems = _matmul_sizes[key] = _workspace(
+            "snn_hip_matmul_bias_act_workspace_size",
+            MatmulBiasActParams(m=m, k=k, n=n, transpose_lhs=int(trans_a),
+                                transpose_rhs=int(trans_b),
+                                activation=activation),
+            int(grad), _TYPES[t.dtype][1])[1]
+    return torch.empty(elems, dtype=t.dtype, device=t.device) if elems else None
+
+
+def matmul_bias_act(a, b, bias=None, residual=None,
+                    activation=ACTIVATION.NONE, trans_a=False, trans_b=False,
+                    keep_pre_activation=False, out=None, workspace=None):
+    """snn_hip_matmul_bias_act: act(op(a) op(b) + bias) + residual.  With
+    keep_pre_activation returns (output, op(a) op(b) + bias), of which the
+    gradient takes the second.  `out` may be the residual."""
+    dtype = a.dtype
+    m, k = (a.shape[1], a.shape[0]) if trans_a else a.shape
+    n = b.shape[0] if trans_b else b.shape[1]
+    assert (b.shape[1] if trans_b else b.shape[0]) == k and b.dtype == dtype
+    if out is None:
+        out = torch.empty((m, n), dtype=dtype, device=a.device)
+    else:
+        assert out.shape == (m, n) and out.dtype == dtype
+    add, add_stride = None, 0
+    if residual is not None:
+        assert residual.shape == (m, n) and residual.dtype == dtype
+        add, add_stride = residual.data_ptr(), _row_stride(residual)
+    z = (torch.empty((m, n), dtype=dtype, device=a.device)
+         if keep_pre_activation else None)
+    if workspace is None:
+        workspace = _matmul_workspace(m, k, n, trans_a, trans_b, activation,
+                                      False, a)
+    code = _native.matmul_bias_act(
+        _address("snn_hip_matmul_bias_act" + _TYPES[dtype][0]), a.data_ptr(),
+        b.data_ptr(), _vector(bias, n, dtype), add, out.data_ptr(), _at(z),
+        m, k, n, trans_a, trans_b, activation, _row_stride(a), _row_stride(b),
+        add_stride, _row_stride(out), _at(workspace),
+        0 if workspace is None else workspace.numel(), _stream())
+    if code:
+        capi.check(code)
+    return (out, z) if keep_pre_activation else out
+
+
+def matmul_bias_act_grad(grad, a, b, pre_activation=None,
+                         activation=ACTIVATION.NONE, trans_a=False,
+                         trans_b=False, bias=True, need_a=True, need_b=True,
+                         workspace=None):
+    """snn_hip_matmul_bias_act_grad: the gradients of a, b and the bias, None
+    for those that are not wanted (the residual's is `grad` itself)."""
+    dtype = a.dtype
+    m, k = (a.shape[1], a.shape[0]) if trans_a else a.shape
+    n = b.shape[0] if trans_b else b.shape[1]
+    assert (b.shape[1] if trans_b else b.shape[0]) == k and b.dtype == dtype
+    assert grad.shape == (m, n) and grad.dtype == dtype
+    a_stride, b_stride = _row_stride(a), _row_stride(b)
+
+    grad_a = (torch.empty(a.shape, dtype=dtype, device=a.device) if need_a
+              else None)
+    grad_b = (torch.empty(b.shape, dtype=dtype, device=b.device) if need_b
+              else None)
+    grad_bias = (torch.empty(n, dtype=dtype, device=a.device) if bias else None)
+    if workspace is None:
+        workspace = _matmul_workspace(m, k, n, trans_a, trans_b, activation,
+                                      True, a)
+    code = _native.matmul_bias_act_grad(
+        _address("snn_hip_matmul_bias_act_grad" + _TYPES[dtype][0]),
+        grad.data_ptr(), a.data_ptr(), b.data_ptr(),
+        _like(pre_activation, (m, n), dtype), _at(grad_a), _at(grad_b),
+        _at(grad_bias), m, k, n, trans_a, trans_b, activation, a_stride,
+        b_stride, 0, _row_stride(grad), _at(workspace),
+        0 if workspace is None else workspace.numel(), _stream())
+    if code:
+        capi.check(code)
+    return grad_a, grad_b, grad_bias
+
+
+def _gate_operand(gate, gate_op, gate_rows, rows, channels, dtype):
+    if gate is None:
+        assert gate_op == GATE.NONE, "an operation without a gate"
+        return None, 0
+    assert gate.shape == (-(-rows // gate_rows), channels) and \
+        gate.dtype == dtype
+    return gate.data_ptr(), _row_stride(gate)
+
+
+def residual_norm(x, residual=None, gate=None, scale=None, post=NORM.NONE,
+                  post_weight=None, post_bias=None, pre=NORM.NONE,
+                  pre_weight=None, pre_bias=None, gate_op=None, gate_rows=1,
+                  eps=1e-6, keep_sum=True, keep_stats=False, out=None):
+    """snn_hip_residual_norm: sum = residual + scale * gate * post_norm(x) and
+    normed = pre_norm(sum).  Returns (sum, normed, stats), None for what is not
+    wanted or not there; `out` takes the sum and may be x or the residual."""
+    rows, channels = x.shape
+    dtype = x.dtype
+    if gate_op is None:
+        gate_op = GATE.NONE if gate is None else GATE.VALUE
+    gate_at, gate_stride = _gate_operand(gate, gate_op, gate_rows, rows,
+                                         channels, dtype)
+    shape = x.shape
+    if out is None:
+        if keep_sum:
+            out = torch.empty(shape, dtype=dtype, device=x.device)
+    else:
+        _like(out, shape, dtype)
+    normed = (torch.empty(shape, dtype=dtype, device=x.device)
+              if pre != NORM.NONE else None)
+    stats = (torch.empty((rows, 4), dtype=torch.float32, device=x.device)
+             if keep_stats else None)
+    code = _native.residual_norm(
+        _address("snn_hip_residual_norm" + _TYPES[dtype][0]), x.data_ptr(),
+        _like(residual, shape, dtype), gate_at, _vector(scale, channels, dtype),
+        _vector(post_weight, channels, dtype),
+        _vector(post_bias, channels, dtype),
+        _vector(pre_weight, channels, dtype),
+        _vector(pre_bias, channels, dtype), _at(out), _at(normed), _at(stats),
+        rows, channels, post, pre, gate_op, gate_rows, _row_stride(x),
+        gate_stride, eps, _stream())
+    if code:
+        capi.check(code)
+    return out, normed, stats
+
+
+_norm_sizes = {}
+
+
+def residual_norm_grad(x, sum, stats, grad_sum=None, grad_normed=None,
+                       gate=None, scale=None, post=NORM.NONE, post_weight=None,
+                       post_bias=None, pre=NORM.NONE, pre_weight=None,
+                       pre_bias=None, gate_op=None, gate_rows=1, eps=1e-6,
+                       workspace=None):
+    """snn_hip_residual_norm_grad: a dict of the gradients of x, residual and
+    of those of gate, scale, post_weight, post_bias, pre_weight and pre_bias
+    that are given."""
+    rows, channels = x.shape
+    dtype, shape, device = x.dtype, x.shape, x.device
+    if gate_op is None:
+        gate_op = GATE.NONE if gate is None else GATE.VALUE
+    gate_at, gate_stride = _gate_operand(gate, gate_op, gate_rows, rows,
+                                         channels, dtype)
+    got = {"x": torch.empty(shape, dtype=dtype, device=device),
+           "residual": torch.empty(shape, dtype=dtype, device=device)}
+    addresses = {}
+    for name, t in (("scale", scale), ("post_weight", post_weight),
+                    ("post_bias", post_bias), ("pre_weight", pre_weight),
+                    ("pre_bias", pre_bias)):
+        addresses[name] = _vector(t, channels, dtype)
+        if t is not None and (grad_normed is not None or
+                              not name.startswith("pre")):
+            got[name] = torch.empty(channels, dtype=dtype, device=device)
+    if gate is not None:
+        got["gate"] = torch.empty(gate.shape, dtype=dtype, device=device)
+    if workspace is None:
+        key = (rows, channels, gate_op, gate_rows, dtype)
+        elems = _norm_sizes.get(key)
+        if elems is None:
+            elems = _norm_sizes[key] = _workspace(
+                "snn_hip_residual_norm_grad_workspace_size",
+                ResidualNormParams(rows=rows, channels=channels, gate=gate_op,
+                                   gate_rows=gate_rows),
+                _TYPES[dtype][1])[1]
+        workspace = torch.empty(elems, dtype=dtype, device=device)
+    code = _native.residual_norm_grad(
+        _address("snn_hip_residual_norm_grad" + _TYPES[dtype][0]),
+        x.data_ptr(), None, gate_at, addresses["scale"],
+        addresses["post_weight"], addresses["post_bias"],
+        addresses["pre_weight"], addresses["pre_bias"],
+        _like(sum, shape, dtype), None,
+        _like(stats, (rows, 4), torch.float32), _like(grad_sum, shape, dtype),
+        _like(grad_normed, shape, dtype), got["x"].data_ptr(),
+        got["residual"].data_ptr(), _at(got.get("gate")),
+        _at(got.get("scale")), _at(got.get("post_weight")),
+        _at(got.get("post_bias")), _at(got.get("pre_weight")),
+        _at(got.get("pre_bias")), rows, channels, post, pre, gate_op, gate_rows,
+        _row_stride(x), gate_stride, eps, workspace.data_ptr(),
+        workspace.numel(), _stream())
+    if code:
+        capi.check(code)
+    return got
+
+
+_recurrence_sizes = {}
+
+
+def _recurrence_workspace(t):
+    key = (t.shape, t.dtype)
+    elems = _recurrence_sizes.get(key)
+    if elems is None:
+        batch, steps, channels = t.shape
+        elems = _recurrence_sizes[key] = _workspace(
+            "snn_hip_linear_recurrence_workspace_size",
+            LinearRecurrenceParams(batch=batch, steps=steps,
+                                   channels=channels),
+            _TYPES[t.dtype][1])[1]
+    return torch.empty(elems, dtype=t.dtype, device=t.device) if elems else None
+
+
+def _recurrence_operands(x, forget, input_gate, resets, lengths):
+    """The common row stride and the optional operands' addresses."""
+    batch, steps, channels = shape = x.shape
+    stride = _step_stride(x)
+    for t in (forget, input_gate):
+        assert t is None or (t.shape == shape and t.dtype == x.dtype and
+                             _step_stride(t) == stride)
+    return stride, _like(resets, (batch, steps), torch.uint8), \
+        _vector(lengths, batch, torch.int32)
+
+
+def linear_recurrence(x, forget, input_gate=None, resets=None, lengths=None,
+                      initial_state=None, out=None, final_state=None,
+                      workspace=None):
+    """snn_hip_linear_recurrence over [batch, steps, channels] tensors; resets
+    is a uint8 [batch, steps] tensor, lengths an int32 [batch] one, states are
+    fp32 [batch, channels].  Returns (h, final state); final_state may be
+    initial_state, which is then updated in place."""
+    batch, steps, channels = shape = x.shape
+    dtype = x.dtype
+    stride, resets_at, lengths_at = _recurrence_operands(x, forget, input_gate,
+                                                         resets, lengths)
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=x.device)
+    if final_state is None:
+        final_state = torch.empty((batch, channels), dtype=torch.float32,
+                                  device=x.device)
+    if workspace is None:
+        workspace = _recurrence_workspace(x)
+    state = (batch, channels)
+    code = _native.linear_recurrence(
+        _address("snn_hip_linear_recurrence" + _TYPES[dtype][0]), x.data_ptr(),
+        forget.data_ptr(), _at(input_gate), resets_at, lengths_at,
+        _like(initial_state, state, torch.float32), _like(out, shape, dtype),
+        _like(final_state, state, torch.float32), batch, steps, channels,
+        stride, 0, _at(workspace),
+        0 if workspace is None else workspace.numel(), _stream())
+    if code:
+        capi.check(code)
+    return out, final_state
+
+
+def linear_recurrence_grad(grad, x, forget, h, input_gate=None, resets=None,
+                           lengths=None, initial_state=None,
+                           grad_final_state=None, out=None, workspace=None):
+    """snn_hip_linear_recurrence_grad: a dict of the gradients of x, forget,
+    input_gate (where it is given) and initial_state.  `out` is a [batch, steps,
+    channels * n] tensor that takes those of x, forget and input_gate side by
+    side, the gradient of a projection that they are slices of."""
+    batch, steps, channels = shape = x.shape
+    dtype, device = x.dtype, x.device
+    stride, resets_at, lengths_at = _recurrence_operands(x, forget, input_gate,
+                                                         resets, lengths)
+    names = ["x", "forget"] + (["input_gate"] if input_gate is not None else [])
+    if out is None:
+        got = {name: torch.empty(shape, dtype=dtype, device=device)
+               for name in names}
+        grad_stride = channels
+    else:
+        _like(out, (batch, steps, channels * len(names)), dtype)
+        got = {name: out[..., i * channels:(i + 1) * channels]
+               for i, name in enumerate(names)}
+        grad_stride = channels * len(names)
+    got["initial_state"] = torch.empty((batch, channels), dtype=torch.float32,
+                                       device=device)
+    if workspace is None:
+        workspace = _recurrence_workspace(x)
+    state = (batch, channels)
+    code = _native.linear_recurrence_grad(
+        _address("snn_hip_linear_recurrence_grad" + _TYPES[dtype][0]),
+        _like(grad, shape, dtype),
+        _like(grad_final_state, state, torch.float32), x.data_ptr(),
+        forget.data_ptr(), _at(input_gate), resets_at, lengths_at,
+        _like(initial_state, state, torch.float32), _like(h, shape, dtype),
+        got["x"].data_ptr(), got["forget"].data_ptr(),
+        _at(got.get("input_gate")), got["initial_state"].data_ptr(), batch,
+        steps, channels, stride, grad_stride, _at(workspace),
+        0 if workspace is None else workspace.numel(), _stream())
+    if code:
+        capi.check(code)
+    return got
+
+
 __all__ = [
-    "ALGO", "BINARY_OP", "DIRECTION", "POINTWISE_OP", "POOL_OP", "STATUS",
+    "ACTIVATION", "ALGO", "BINARY_OP", "DIRECTION", "GATE", "NORM",
+    "POINTWISE_OP", "POOL_OP", "STATUS",
     "ConvParams", "DepthwiseParams", "PoolParams", "add_padding_to",
     "binaryop", "binaryop_raw", "calculate_padding", "conv2d",
     "conv2d_bias_act", "conv2d_prepare_filter", "conv2d_prepared",
     "conv2d_raw", "conv_flops", "conv_params", "conv_sizes",
     "default_algorithm",
-    "depthwise_conv2d", "depthwise_params", "depthwise_sizes", "matmul",
+    "depthwise_conv2d", "depthwise_params", "depthwise_sizes",
+    "linear_recurrence", "linear_recurrence_grad", "matmul", "matmul_bias_act",
+    "matmul_bias_act_grad",
     "pointwise_forward", "pointwise_grad", "pool_params", "pooling_avg_grad",
-    "pooling_forward", "pooling_max_grad",
-    "workspace_size",
+    "pooling_forward", "pooling_max_grad", "residual_norm",
+    "residual_norm_grad", "workspace_size",
 ]
 
 
