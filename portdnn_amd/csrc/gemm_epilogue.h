@@ -10,11 +10,11 @@
 // the same kernel without a copy.
 //
 // A work-group owns a BM x BN tile of C and a range of the reduction, which it
-// walks in chunks of 128 bytes (64 16-bit values, 32 floats).  A chunk of P and Q
+// walks in chunks of CB = 128 or 64 bytes (64 or 32 16-bit values).  A chunk of P and Q
 // goes to LDS, STAGES chunks in a ring:
 //
-//   K inner    [BM rows][128 bytes]; a fragment is one 16-byte read per lane
-//   row inner  [64 or 32 reductions][BM values]; 16-bit fragments are two
+//   K inner    [BM rows][CB bytes]; a fragment is one 16-byte read per lane
+//   row inner  [reductions][BM values]; 16-bit fragments are two
 //              transposing reads (ds_read_b64_tr_b16: within 16 lanes, lane
 //              4 j + i supplies the address of four values of reduction j and
 //              lane t receives column t of reductions 0 ... 3), floats four
@@ -32,6 +32,9 @@
 // whole rows.
 #ifndef PORTDNN_AMD_CSRC_GEMM_EPILOGUE_H_
 #define PORTDNN_AMD_CSRC_GEMM_EPILOGUE_H_
+
+#include <algorithm>
+#include <cmath>
 
 #include "gemm_tile.h"
 #include "sequence.h"
@@ -67,8 +70,9 @@ struct Product {
 int run_f32(Product& g, void* workspace, size_t bytes, hipStream_t stream);
 int run_f16(Product& g, void* workspace, size_t bytes, hipStream_t stream);
 int run_bf16(Product& g, void* workspace, size_t bytes, hipStream_t stream);
-// Bytes of workspace that a product of m x n over k shares its reduction with.
-size_t split_bytes(int m, int n, int k, int elem_size);
+// Bytes of workspace that a product makes use of; goes by its sizes, strides and
+// orders alone.
+size_t workspace_bytes(const Product& g, int elem_size);
 
 __device__ __forceinline__ float activate(float z, int kind) {
   switch (kind) {
@@ -181,6 +185,7 @@ __device__ __forceinline__ void finish8(const Product& g, int row, int col,
   }
 }
 
+// Shares of a reduction are multiples of this many bytes of a row.
 constexpr int kChunkBytes = 128;
 constexpr unsigned kOob = 0x80000000u;  // beyond every buffer's range
 
@@ -192,14 +197,34 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* p) {
 constexpr int vmcnt_imm(int n) { return 0x0F70 | (n & 15) | ((n >> 4) << 14); }
 constexpr int kLgkm0 = ~0x0F00;  // ... and all LDS reads, by &
 
+// Eight neighbouring columns of a tile: the result, or a share of its sums.
+template <typename T>
+__device__ __forceinline__ void leave(const Product& g, unsigned split, int row,
+                                      int col, float (&v)[8]) {
+  if (g.splits == 1) {
+    finish8<T>(g, row, col, v);
+    return;
+  }
+  float* const to =
+      g.partial + (static_cast<long>(split) * g.m + row) * g.n + col;
+  if (g.n % 8 == 0) {
+    *reinterpret_cast<float4v*>(to) = float4v{v[0], v[1], v[2], v[3]};
+    *reinterpret_cast<float4v*>(to + 4) = float4v{v[4], v[5], v[6], v[7]};
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (col + i < g.n) to[i] = v[i];
+  }
+}
+
 // Which 16-byte position of its row holds piece c: c ^ swizzle(row).
-//   K inner: the 16 rows of a fragment, two of which fill the 64 banks.
+//   K inner: the 16 rows of a fragment, two (four) of which fill the 64 banks.
 //   row inner, 16-bit: the four reductions of a transposing read by the two
 //   blocks of eight, 32 bytes each.
 //   row inner, floats: four blocks of four reductions, 64 bytes each.
-template <int E, bool K_INNER, int ROWS>
+template <int E, bool K_INNER, int ROWS, int CB>
 __device__ __forceinline__ constexpr unsigned swizzle(unsigned row) {
-  if (K_INNER) return (row >> 1) & 7u;
+  if (K_INNER) return CB == 128 ? (row >> 1) & 7u : (row >> 2) & 3u;
   constexpr int kPitch = ROWS * E;
   if (E == 2) {
     if (kPitch >= 256) return 2u * ((row & 3u) | (((row >> 3) & 1u) << 2));
@@ -212,15 +237,17 @@ __device__ __forceinline__ constexpr unsigned swizzle(unsigned row) {
   return 0;
 }
 
-// One operand's tile: ROWS rows of the result's dimension by a chunk of the
-// reduction, ROWS * 128 bytes either way.
-template <typename T, bool K_INNER, int ROWS>
+// One operand's tile: ROWS rows of the result's dimension by a chunk of CB bytes
+// of the reduction.
+template <typename T, bool K_INNER, int ROWS, int CB>
 struct Operand {
   static constexpr int E = sizeof(T);
-  static constexpr int kBlocks = ROWS * kChunkBytes / 1024;  // of 1 KiB
-  static constexpr int kPitch = K_INNER ? kChunkBytes : ROWS * E;
+  static constexpr bool kInner = K_INNER;
+  static constexpr int kRows = ROWS;
+  static constexpr int kBlocks = ROWS * CB / 1024;  // of 1 KiB
+  static constexpr int kPitch = K_INNER ? CB : ROWS * E;
   static constexpr int kPiece = 16 / E;  // values
-  static constexpr int kChunk = kChunkBytes / E;
+  static constexpr int kChunk = CB / E;
 
   // Row and column (in values) of the tile's memory that LDS position `pos`
   // holds.
@@ -229,14 +256,7 @@ struct Operand {
     const unsigned r = pos / kPitch;
     const unsigned piece = (pos % kPitch) >> 4;
     *row = static_cast<int>(r);
-    *col = static_cast<int>((piece ^ swizzle<E, K_INNER, ROWS>(r)) * kPiece);
-  }
-  // The tile's values at memory row / column, of which `rows_left` rows of the
-  // result and `k_left` reductions exist.
-  static __device__ __forceinline__ bool inside(int row, int col, int rows_left,
-                                                int k_left) {
-    return K_INNER ? row < rows_left && col < k_left
-                   : row < k_left && col < rows_left;
+    *col = static_cast<int>((piece ^ swizzle<E, K_INNER, ROWS, CB>(r)) * kPiece);
   }
   static __device__ __forceinline__ const T* at(const void* p, long stride,
                                                 int row0, int k0) {
@@ -250,18 +270,18 @@ struct Operand {
   static __device__ __forceinline__ unsigned fragment(int row0, int lane) {
     if (K_INNER) {
       const unsigned row = row0 + (lane & 15);
-      return row * kChunkBytes +
-             (((lane >> 4) ^ swizzle<E, true, ROWS>(row)) << 4);
+      return row * CB +
+             (((lane >> 4) ^ swizzle<E, true, ROWS, CB>(row)) << 4);
     }
     if (E == 2) {
       const unsigned k = 8 * (lane >> 4) + ((lane >> 2) & 3);
       const unsigned piece = row0 / 8 + ((lane & 3) >> 1);
-      return k * kPitch + ((piece ^ swizzle<E, false, ROWS>(k)) << 4) +
+      return k * kPitch + ((piece ^ swizzle<E, false, ROWS, CB>(k)) << 4) +
              ((lane & 1) << 3);
     }
     const unsigned k = 4 * (lane >> 4);
     const unsigned piece = row0 / 4 + ((lane & 15) >> 2);
-    return k * kPitch + ((piece ^ swizzle<E, false, ROWS>(k)) << 4) +
+    return k * kPitch + ((piece ^ swizzle<E, false, ROWS, CB>(k)) << 4) +
            ((lane & 3) << 2);
   }
   static __device__ __forceinline__ uint4v read(const char* tile, unsigned at,
@@ -317,25 +337,27 @@ __device__ __forceinline__ float4v multiply<float>(uint4v q, uint4v p,
 
 // LDS of a work-group: the ring of chunks, rounded up so that every wave issues
 // the same number of loads, or the tile on its way out.
-template <int BM, int BN, int WAVES, int STAGES>
+template <int BM, int BN, int WAVES, int CB>
 struct Space {
-  static constexpr int kBlocks = (BM + BN) * kChunkBytes / 1024;
+  static constexpr int kBlocks = (BM + BN) * CB / 1024;
   static constexpr int kLoads = (kBlocks + WAVES - 1) / WAVES;  // per wave
   static constexpr int kStage = kLoads * WAVES * 1024;
 };
 
 template <typename T, bool PK, bool QK, int BM, int BN, int WM, int WN,
-          int STAGES, bool DIRECT>
+          int CB, int STAGES>
 __device__ __forceinline__ void gemm_body(const Product& g, char* r0, char* r1,
-                                          char* r2, char* r3) {
-  typedef Operand<T, PK, BM> OP;
-  typedef Operand<T, QK, BN> OQ;
-  constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
-  typedef Space<BM, BN, WAVES, STAGES> S;
+                                          char* r2, char* r3, char* r4) {
+  typedef Operand<T, PK, BM, CB> OP;
+  typedef Operand<T, QK, BN, CB> OQ;
+  constexpr int WAVES = WM * WN;
+  typedef Space<BM, BN, WAVES, CB> S;
   constexpr int TM = BM / WM, TN = BN / WN, IM = TM / 16, IN = TN / 16;
-  constexpr int kPBytes = BM * kChunkBytes;
+  constexpr int kPBytes = BM * CB;
   constexpr int kChunk = OP::kChunk;
-  auto ring = [&](int u) { return u == 0 ? r0 : u == 1 ? r1 : u == 2 ? r2 : r3; };
+  auto ring = [&](int u) {
+    return u == 0 ? r0 : u == 1 ? r1 : u == 2 ? r2 : u == 3 ? r3 : r4;
+  };
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave % WM, wn = wave / WM;
@@ -351,8 +373,9 @@ __device__ __forceinline__ void gemm_body(const Product& g, char* r0, char* r1,
   const unsigned height = min(kBand, g.tiles_m - band * kBand);
   const int row0 = static_cast<int>(band * kBand + in_band % height) * BM;
   const int col0 = static_cast<int>(in_band / height) * BN;
-  const int k_begin = static_cast<int>(split) * g.split_chunks * kChunk;
-  const int k_end = min(g.k, k_begin + g.split_chunks * kChunk);
+  const int share = g.split_chunks * (kChunkBytes / static_cast<int>(sizeof(T)));
+  const int k_begin = static_cast<int>(split) * share;
+  const int k_end = min(g.k, k_begin + share);
   const int chunks = (k_end - k_begin + kChunk - 1) / kChunk;
   const int rows_left = g.m - row0, cols_left = g.n - col0;
 
@@ -372,7 +395,7 @@ __device__ __forceinline__ void gemm_body(const Product& g, char* r0, char* r1,
 
   auto compute = [&](const char* tile_at) {
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < CB / 64; ++s) {
       uint4v p[IM], q[IN];
 #pragma unroll
       for (int j = 0; j < IN; ++j) q[j] = OQ::read(tile_at, at_q[j], s);
@@ -385,140 +408,80 @@ __device__ __forceinline__ void gemm_body(const Product& g, char* r0, char* r1,
     }
   };
 
-  if constexpr (DIRECT) {
-    // Offsets of the lane's loads within a chunk; the chunk's own place is in
-    // the buffer's base, so that operands may be of any size.
-    unsigned offset[S::kLoads];
-    int order[S::kLoads];  // its reduction index
+  // Offsets of the lane's loads within a chunk; the chunk's own place is in
+  // the buffer's base, so that operands may be of any size.
+  unsigned offset[S::kLoads];
+  int order[S::kLoads];  // its reduction index
+#pragma unroll
+  for (int l = 0; l < S::kLoads; ++l) {
+    const int block = wave + l * WAVES;
+    int row, col;
+    bool in;
+    long stride;
+    if (block < OP::kBlocks) {
+      OP::source(block * 1024 + lane * 16, &row, &col);
+      in = PK ? row < rows_left : col < rows_left;
+      stride = g.p_stride;
+      order[l] = PK ? col : row;
+    } else {
+      OQ::source((block - OP::kBlocks) * 1024 + lane * 16, &row, &col);
+      in = block < S::kBlocks && (QK ? row < cols_left : col < cols_left);
+      stride = g.q_stride;
+      order[l] = QK ? col : row;
+    }
+    offset[l] = in ? static_cast<unsigned>((row * stride + col) * sizeof(T))
+                   : kOob;
+  }
+  const char* from_p =
+      reinterpret_cast<const char*>(OP::at(g.p, g.p_stride, row0, k_begin));
+  const char* from_q =
+      reinterpret_cast<const char*>(OQ::at(g.q, g.q_stride, col0, k_begin));
+  const long step_p = PK ? CB : CB * g.p_stride;
+  const long step_q = QK ? CB : CB * g.q_stride;
+  int k_left = k_end - k_begin;
+  auto issue = [&](char* to) {  // the next chunk
+    const __amdgpu_buffer_rsrc_t p = make_rsrc(from_p), q = make_rsrc(from_q);
 #pragma unroll
     for (int l = 0; l < S::kLoads; ++l) {
       const int block = wave + l * WAVES;
-      int row, col;
-      bool in;
-      long stride;
-      if (block < OP::kBlocks) {
-        OP::source(block * 1024 + lane * 16, &row, &col);
-        in = PK ? row < rows_left : col < rows_left;
-        stride = g.p_stride;
-        order[l] = PK ? col : row;
-      } else {
-        OQ::source((block - OP::kBlocks) * 1024 + lane * 16, &row, &col);
-        in = block < S::kBlocks && (QK ? row < cols_left : col < cols_left);
-        stride = g.q_stride;
-        order[l] = QK ? col : row;
-      }
-      offset[l] = in ? static_cast<unsigned>((row * stride + col) * sizeof(T))
-                     : kOob;
+      const unsigned from = order[l] < k_left ? offset[l] : kOob;
+      if (block < OP::kBlocks)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            p, (lds_ptr)(to + block * 1024), 16, from, 0, 0, 0);
+      else
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            q, (lds_ptr)(to + block * 1024), 16, from, 0, 0, 0);
     }
-    const char* from_p =
-        reinterpret_cast<const char*>(OP::at(g.p, g.p_stride, row0, k_begin));
-    const char* from_q =
-        reinterpret_cast<const char*>(OQ::at(g.q, g.q_stride, col0, k_begin));
-    const long step_p = PK ? kChunkBytes : kChunkBytes * g.p_stride;
-    const long step_q = QK ? kChunkBytes : kChunkBytes * g.q_stride;
-    int k_left = k_end - k_begin;
-    auto issue = [&](char* to) {  // the next chunk
-      const __amdgpu_buffer_rsrc_t p = make_rsrc(from_p), q = make_rsrc(from_q);
+    from_p += step_p;
+    from_q += step_q;
+    k_left -= kChunk;
+  };
+  // STAGES - 1 chunks are under way while one is multiplied; behind the last
+  // one the loads are out of range, so that there is always the same number.  A
+  // chunk's place is loaded again behind the barrier that every wave reaches
+  // when it has read it.  (The places are arrays of their own: the compiler
+  // waits for all loads into an array before it reads from it.)
 #pragma unroll
-      for (int l = 0; l < S::kLoads; ++l) {
-        const int block = wave + l * WAVES;
-        const unsigned from = order[l] < k_left ? offset[l] : kOob;
-        if (block < OP::kBlocks)
-          __builtin_amdgcn_raw_ptr_buffer_load_lds(
-              p, (lds_ptr)(to + block * 1024), 16, from, 0, 0, 0);
-        else
-          __builtin_amdgcn_raw_ptr_buffer_load_lds(
-              q, (lds_ptr)(to + block * 1024), 16, from, 0, 0, 0);
-      }
-      from_p += step_p;
-      from_q += step_q;
-      k_left -= kChunk;
-    };
-    // STAGES - 1 chunks are under way while one is multiplied; behind the last
-    // one the loads are out of range, so that there is always the same number.  A
-    // chunk's place is loaded again behind the barrier that every wave reaches
-    // when it has read it.  (The places are arrays of their own: the compiler
-    // waits for all loads into an array before it reads from it.)
+  for (int c = 0; c < STAGES - 1; ++c) issue(ring(c));
+  auto step = [&](int u) {
+    // the chunk is here, and the reads of the one before have returned
+    __builtin_amdgcn_s_waitcnt(kLgkm0 & vmcnt_imm((STAGES - 2) * S::kLoads));
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    issue(ring((u + STAGES - 1) % STAGES));
+    compute(ring(u));
+  };
+  int left = chunks;
+  for (; left >= STAGES; left -= STAGES) {
 #pragma unroll
-    for (int c = 0; c < STAGES - 1; ++c) issue(ring(c));
-    int left = chunks;
-    while (left > 0) {
-#pragma unroll
-      for (int u = 0; u < STAGES; ++u) {
-        if (left == 0) break;
-        // the chunk is here, and the reads of the one before have returned
-        __builtin_amdgcn_s_waitcnt(kLgkm0 &
-                                   vmcnt_imm((STAGES - 2) * S::kLoads));
-        asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        __builtin_amdgcn_sched_barrier(0);
-        issue(ring((u + STAGES - 1) % STAGES));
-        compute(ring(u));
-        --left;
-      }
-    }
-    __builtin_amdgcn_s_waitcnt(kLgkm0 & vmcnt_imm(0));
-  } else {
-    // Through registers: the loads of a chunk are under way while the one before
-    // it is multiplied, two places in turn.
-    constexpr int kPieces = (BM + BN) * kChunkBytes / 16;
-    constexpr int kEach = (kPieces + THREADS - 1) / THREADS;
-    uint4v held[kEach];
-    auto load_piece = [&](auto operand, const void* base, long stride,
-                          int left, int first, unsigned pos, int k0) {
-      typedef decltype(operand) O;
-      int row, col;
-      O::source(pos, &row, &col);
-      const int k_left = k_end - k0;
-      const T* const from =
-          O::at(base, stride, first, k0) + row * stride + col;
-      uint4v v = {0u, 0u, 0u, 0u};
-      if (O::inside(row, col + O::kPiece - 1, left, k_left)) {
-        __builtin_memcpy(&v, from, 16);
-      } else if (O::inside(row, col, left, k_left)) {
-        T part[O::kPiece] = {};
-#pragma unroll
-        for (int i = 0; i < O::kPiece; ++i)
-          if (O::inside(row, col + i, left, k_left)) part[i] = from[i];
-        __builtin_memcpy(&v, part, 16);
-      }
-      return v;
-    };
-    auto load = [&](int chunk) {
-      const int k0 = k_begin + chunk * kChunk;
-#pragma unroll
-      for (int e = 0; e < kEach; ++e) {
-        const unsigned pos = (tid + e * THREADS) * 16;
-        if (pos < static_cast<unsigned>(kPBytes))
-          held[e] = load_piece(OP(), g.p, g.p_stride, rows_left, row0, pos, k0);
-        else if (pos < static_cast<unsigned>(kPieces) * 16)
-          held[e] = load_piece(OQ(), g.q, g.q_stride, cols_left, col0,
-                               pos - kPBytes, k0);
-      }
-    };
-    auto put = [&](char* to) {
-#pragma unroll
-      for (int e = 0; e < kEach; ++e) {
-        const unsigned pos = (tid + e * THREADS) * 16;
-        if (pos < static_cast<unsigned>(kPieces) * 16)
-          *reinterpret_cast<uint4v*>(to + pos) = held[e];
-      }
-    };
-    load(0);
-    int c = 0;
-    while (c < chunks) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        if (c == chunks) break;
-        put(ring(u));
-        __syncthreads();
-        if (c + 1 < chunks) load(c + 1);
-        compute(ring(u));
-        ++c;
-      }
-    }
+    for (int u = 0; u < STAGES; ++u) step(u);
   }
+#pragma unroll
+  for (int u = 0; u < STAGES - 1; ++u)
+    if (u < left) step(u);
+  __builtin_amdgcn_s_waitcnt(kLgkm0 & vmcnt_imm(0));
 
   // The way out.  A wave's part of the tile in passes of kRows rows, a 16-byte
   // piece c of row r at c ^ (r & 15) (& 7 for rows of 32 columns).
@@ -526,8 +489,10 @@ __device__ __forceinline__ void gemm_body(const Product& g, char* r0, char* r1,
   constexpr int kSharers = (WAVES + STAGES - 1) / STAGES;  // of a chunk's place
   constexpr int kSpace = S::kStage / kSharers / 1024 * 1024;
   constexpr int kFit = kSpace / (TN * 4) / 16 * 16;
-  constexpr int kRows = TM <= kFit ? TM : kFit;
-  static_assert(kRows >= 16 && TM % kRows == 0, "no room for the way out");
+  constexpr int kRows = TM <= kFit       ? TM
+                        : TM / 2 <= kFit ? TM / 2
+                                         : TM / 4;
+  static_assert(kRows <= kFit && kRows % 16 == 0, "no room for the way out");
   constexpr unsigned kMask = TN / 4 - 1 < 15 ? TN / 4 - 1 : 15;
   char* own = ring(0);
 #pragma unroll
@@ -563,21 +528,233 @@ __device__ __forceinline__ void gemm_body(const Product& g, char* r0, char* r1,
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[4 * h + i] = f[i];
       }
-      if (g.splits == 1) {
-        finish8<T>(g, row, col, v);
-      } else {
-        float* const to =
-            g.partial + (static_cast<long>(split) * g.m + row) * g.n + col;
-        if (g.n % 8 == 0) {
-          *reinterpret_cast<float4v*>(to) = float4v{v[0], v[1], v[2], v[3]};
-          *reinterpret_cast<float4v*>(to + 4) = float4v{v[4], v[5], v[6], v[7]};
-        } else {
+      leave<T>(g, split, row, col, v);
+    }
+  }
+}
+
+// A 16-byte piece of an operand's tile from any address, by way of registers.
+// Rows (or columns) beyond the operand are others of its rows, whose results are
+// not kept; reductions beyond `k_end` are zero.  Where the piece does not exist
+// as a whole it is put together from single values, all of them loads of
+// existing ones, so that no load waits for another.
+template <typename O, typename T>
+__device__ __forceinline__ uint4v load_piece(const void* base, long stride,
+                                             int left, int first, int k0,
+                                             int k_end, unsigned pos) {
+  int row, col;
+  O::source(pos, &row, &col);
+  const int k_left = k_end - k0;
+  const T* const from = O::at(base, stride, first, k0);
+  uint4v v = {0u, 0u, 0u, 0u};
+  if (k_left <= 0) return v;
+  // what exists of the tile, rows and columns of memory
+  const int rows = O::kInner ? left : k_left;
+  const int cols = O::kInner ? k_left : left;
+  const T* const line = from + min(row, rows - 1) * stride;
+  if (k_left >= O::kChunk && (O::kInner || left >= O::kRows)) {
+    __builtin_memcpy(&v, line + col, 16);
+    return v;
+  }
+  T part[O::kPiece];
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (col + i < g.n) to[i] = v[i];
-        }
+  for (int i = 0; i < O::kPiece; ++i) part[i] = line[min(col + i, cols - 1)];
+#pragma unroll
+  for (int i = 0; i < O::kPiece; ++i)
+    if ((O::kInner ? col + i : row) >= k_left) part[i] = T(0);
+  __builtin_memcpy(&v, part, 16);
+  return v;
+}
+
+// Products of a few rows, which are bound by the bytes of Q.  The work-group's
+// waves share the reduction of a BM x BN tile, chunk by chunk in turn, and every
+// wave has a ring of its own, so that nothing but its own loads holds it up:
+// STAGES chunks of each wave are under way.  Their sums meet in LDS at the end.
+template <typename T, bool PK, bool QK, int BM, int BN, int WAVES, int STAGES,
+          bool DIRECT>
+__device__ __forceinline__ void gemm_few_body(const Product& g, char* r0,
+                                              char* r1, char* r2, char* r3) {
+  constexpr int CB = kChunkBytes;
+  typedef Operand<T, PK, BM, CB> OP;
+  typedef Operand<T, QK, BN, CB> OQ;
+  constexpr int IM = BM / 16, IN = BN / 16;
+  constexpr int kPBytes = BM * CB, kOwn = (BM + BN) * CB;
+  constexpr int kLoads = kOwn / 1024, kChunk = OP::kChunk;
+  auto ring = [&](int u) { return u == 0 ? r0 : u == 1 ? r1 : u == 2 ? r2 : r3; };
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const unsigned tiles = static_cast<unsigned>(g.tiles_m) * g.tiles_n;
+  const unsigned lin = gemm::xcd_remap(blockIdx.x, tiles * g.splits);
+  const unsigned split = lin / tiles, tile = lin - split * tiles;
+  const int row0 = static_cast<int>(tile % g.tiles_m) * BM;
+  const int col0 = static_cast<int>(tile / g.tiles_m) * BN;
+  const int share = g.split_chunks * kChunk;
+  const int k_begin = static_cast<int>(split) * share + wave * kChunk;
+  const int k_end = min(g.k, static_cast<int>(split) * share + share);
+  const int rows_left = g.m - row0, cols_left = g.n - col0;
+
+  unsigned at_p[IM], at_q[IN];
+#pragma unroll
+  for (int i = 0; i < IM; ++i)
+    at_p[i] = wave * kOwn + OP::fragment(16 * i, lane);
+#pragma unroll
+  for (int j = 0; j < IN; ++j)
+    at_q[j] = wave * kOwn + kPBytes + OQ::fragment(16 * j, lane);
+  float4v acc[IM][IN];
+#pragma unroll
+  for (int i = 0; i < IM; ++i)
+#pragma unroll
+    for (int j = 0; j < IN; ++j) acc[i][j] = float4v{0.f, 0.f, 0.f, 0.f};
+
+  // The fragments of a chunk, and what becomes of them.
+  uint4v p[2][IM], q[2][IN];
+  auto fetch = [&](const char* place) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+      for (int j = 0; j < IN; ++j) q[s][j] = OQ::read(place, at_q[j], s);
+#pragma unroll
+      for (int i = 0; i < IM; ++i) p[s][i] = OP::read(place, at_p[i], s);
+    }
+  };
+  auto multiply_all = [&]() {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int i = 0; i < IM; ++i)
+#pragma unroll
+        for (int j = 0; j < IN; ++j)
+          acc[i][j] = multiply<T>(q[s][j], p[s][i], acc[i][j]);
+  };
+  int k_left = k_end - k_begin;  // at the chunk that is loaded next
+  int left = (k_left + WAVES * kChunk - 1) / (WAVES * kChunk);
+
+  if constexpr (DIRECT) {
+    unsigned offset[kLoads];
+    int order[kLoads];
+#pragma unroll
+    for (int l = 0; l < kLoads; ++l) {
+      int row, col;
+      bool in;
+      long stride;
+      if (l < OP::kBlocks) {
+        OP::source(l * 1024 + lane * 16, &row, &col);
+        in = PK ? row < rows_left : col < rows_left;
+        stride = g.p_stride;
+        order[l] = PK ? col : row;
+      } else {
+        OQ::source((l - OP::kBlocks) * 1024 + lane * 16, &row, &col);
+        in = QK ? row < cols_left : col < cols_left;
+        stride = g.q_stride;
+        order[l] = QK ? col : row;
+      }
+      offset[l] =
+          in ? static_cast<unsigned>((row * stride + col) * sizeof(T)) : kOob;
+    }
+    const char* from_p =
+        reinterpret_cast<const char*>(OP::at(g.p, g.p_stride, row0, k_begin));
+    const char* from_q =
+        reinterpret_cast<const char*>(OQ::at(g.q, g.q_stride, col0, k_begin));
+    const long step_p = WAVES * (PK ? CB : CB * g.p_stride);
+    const long step_q = WAVES * (QK ? CB : CB * g.q_stride);
+    auto issue = [&](char* to) {
+      const __amdgpu_buffer_rsrc_t p = make_rsrc(from_p), q = make_rsrc(from_q);
+#pragma unroll
+      for (int l = 0; l < kLoads; ++l) {
+        const unsigned from = order[l] < k_left ? offset[l] : kOob;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            l < OP::kBlocks ? p : q, (lds_ptr)(to + wave * kOwn + l * 1024), 16,
+            from, 0, 0, 0);
+      }
+      from_p += step_p;
+      from_q += step_q;
+      k_left -= WAVES * kChunk;
+    };
+    auto step = [&](char* place) {
+      __builtin_amdgcn_s_waitcnt(vmcnt_imm((STAGES - 1) * kLoads));
+      asm volatile("" ::: "memory");
+      fetch(place);
+      // the chunk is in registers before its place is loaded again
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_waitcnt(kLgkm0 & vmcnt_imm(63));
+      asm volatile("" ::: "memory");
+      issue(place);
+      multiply_all();
+    };
+#pragma unroll
+    for (int u = 0; u < STAGES; ++u) issue(ring(u));
+    for (; left >= STAGES; left -= STAGES) {
+#pragma unroll
+      for (int u = 0; u < STAGES; ++u) step(ring(u));
+    }
+#pragma unroll
+    for (int u = 0; u < STAGES - 1; ++u)
+      if (u < left) step(ring(u));
+  } else {
+    // Through registers, STAGES chunks of which are under way; LDS holds one.
+    uint4v held[STAGES][kLoads];
+    int k0 = k_begin;
+    auto load = [&](uint4v (&to)[kLoads]) {
+#pragma unroll
+      for (int l = 0; l < kLoads; ++l) {
+        if (l < OP::kBlocks)
+          to[l] = load_piece<OP, T>(g.p, g.p_stride, rows_left, row0, k0, k_end,
+                                    l * 1024 + lane * 16);
+        else
+          to[l] = load_piece<OQ, T>(g.q, g.q_stride, cols_left, col0, k0, k_end,
+                                    (l - OP::kBlocks) * 1024 + lane * 16);
+      }
+      k0 += WAVES * kChunk;
+    };
+    auto step = [&](uint4v (&from)[kLoads]) {
+#pragma unroll
+      for (int l = 0; l < kLoads; ++l)
+        *reinterpret_cast<uint4v*>(r0 + wave * kOwn + l * 1024 + lane * 16) =
+            from[l];
+      fetch(r0);
+      load(from);
+      multiply_all();
+    };
+#pragma unroll
+    for (int u = 0; u < STAGES; ++u) load(held[u]);
+    for (; left >= STAGES; left -= STAGES) {
+#pragma unroll
+      for (int u = 0; u < STAGES; ++u) step(held[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < STAGES - 1; ++u)
+      if (u < left) step(held[u]);
+  }
+  __builtin_amdgcn_s_waitcnt(kLgkm0 & vmcnt_imm(0));
+
+  // The waves' tiles, [wave][BM][BN], over the first ring; their sums eight
+  // columns at a time.
+  __syncthreads();
+  static_assert(BM * BN * 4 <= kOwn, "no room for the sums");
+#pragma unroll
+  for (int i = 0; i < IM; ++i)
+#pragma unroll
+    for (int j = 0; j < IN; ++j)
+      *reinterpret_cast<float4v*>(r0 + ((wave * BM + 16 * i + (lane & 15)) * BN +
+                                        16 * j + 4 * (lane >> 4)) *
+                                           4) = acc[i][j];
+  __syncthreads();
+  for (int e = tid; e < BM * BN / 8; e += 64 * WAVES) {
+    const int r = e / (BN / 8), c = e % (BN / 8) * 8;
+    const int row = row0 + r, col = col0 + c;
+    if (row >= g.m || col >= g.n) continue;
+    float v[8] = {};
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      const float4v* const f = reinterpret_cast<const float4v*>(
+          r0 + ((w * BM + r) * BN + c) * 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] += f[0][i];
+        v[4 + i] += f[1][i];
       }
     }
+    leave<T>(g, split, row, col, v);
   }
 }
 
@@ -612,41 +789,163 @@ __global__ void __launch_bounds__(256) gemm_join_kernel(Product g) {
   finish8<T>(g, row, col, v);
 }
 
-// How a product is divided: the tile's shape and the shares of the reduction.
-struct Plan {
-  int bm, bn, tiles_m, tiles_n, splits, split_chunks;
+// The kernels of a product: tiles of work-groups that walk the reduction
+// together, tiles whose waves share it (for few rows), and those of the latter
+// that take rows at any address.
+enum Kernel {
+  kFew16x16,
+  kFew16x32,
+  kFew32x32,
+  kFew64x32,
+  kTile64x128,
+  kTile128,
+  kTile128Pair,  // two work-groups of a CU
+  kTile256,
+  kAny16x16,
+  kAny32x32,
+  kAny64x32,
+  kKernels
 };
 
-inline Plan make_plan(int m, int n, int k, int elem_size, bool direct,
-                      size_t bytes) {
-  Plan p;
-  const int chunk = kChunkBytes / elem_size;
-  const int chunks = ceil_div(k, chunk);
-  if (m <= 16) {
-    p.bm = 16;
-    p.bn = 128;
-  } else if (m <= 64) {
-    p.bm = 64;
-    p.bn = 128;
-  } else if (elem_size == 2 && direct &&
-             static_cast<long>(ceil_div(m, 256)) * ceil_div(n, 256) >= 192) {
-    p.bm = p.bn = 256;
-  } else {
-    p.bm = p.bn = 128;
+// What the choice goes by, measured: microseconds of a round of `slots`
+// work-groups that does not go into its steps, and of a step (`chunks` 128-byte
+// chunks of the reduction) with Q K inner and row inner; 0: not for this type.
+struct Shape {
+  int bm, bn, chunks, slots;
+  float fixed, step_k, step_row;
+};
+constexpr Shape kShapes16[kKernels] = {
+    {16, 16, 4, 384, 2.3f, 0.43f, 0.6f},   {16, 32, 4, 256, 2.5f, 0.49f, 0.62f},
+    {32, 32, 4, 256, 2.5f, 0.42f, 0.7f},   {64, 32, 4, 256, 2.8f, 0.55f, 0.88f},
+    {64, 128, 1, 256, 4.3f, 0.24f, 0.24f}, {128, 128, 1, 256, 5.2f, 0.42f, 0.42f},
+    {128, 128, 1, 512, 5.0f, 0.92f, 0.92f}, {256, 256, 1, 256, 8.0f, 1.5f, 1.5f},
+    {16, 16, 4, 768, 3.0f, 0.6f, 1.2f},    {32, 32, 8, 256, 3.0f, 1.8f, 5.5f},
+    {64, 32, 4, 256, 3.0f, 1.55f, 3.6f}};
+constexpr Shape kShapes32[kKernels] = {
+    {16, 16, 4, 384, 2.3f, 0.33f, 0.5f},   {16, 32, 4, 256, 2.5f, 0.45f, 0.72f},
+    {32, 32, 4, 256, 2.5f, 0.6f, 0.8f},    {64, 32, 4, 256, 0.f, 0.f, 0.f},
+    {64, 128, 1, 256, 4.3f, 1.0f, 1.0f},   {128, 128, 1, 256, 5.0f, 1.9f, 1.9f},
+    {128, 128, 1, 512, 0.f, 0.f, 0.f},     {256, 256, 1, 256, 0.f, 0.f, 0.f},
+    {16, 16, 4, 768, 3.0f, 0.9f, 1.2f},    {32, 32, 8, 256, 3.0f, 2.0f, 5.5f},
+    {64, 32, 4, 256, 3.0f, 2.0f, 4.0f}};
+
+// How a product is run: the kernel, which operands are copied to rows that start
+// at multiples of 16 bytes, the shares of the reduction.
+struct Plan {
+  int kernel;
+  bool copy_p, copy_q;
+  size_t p_bytes, q_bytes;  // of the copies
+  int tiles_m, tiles_n, splits, split_chunks;
+};
+
+// Rows of an operand in memory, and their length.
+inline int memory_rows(bool k_inner, int rows, int k) { return k_inner ? rows : k; }
+inline int memory_cols(bool k_inner, int rows, int k) { return k_inner ? k : rows; }
+inline long copied_stride(int cols, int elem_size) {
+  const int piece = 16 / elem_size;
+  return (cols + piece - 1) / piece * piece;
+}
+
+// The kernel and the shares with the least time by the table above; the shares'
+// sums cost a launch and their bytes.  `direct`: whole 16-byte pieces at aligned
+// addresses.  `bytes`: the workspace that is left for the shares.
+inline float choose(const Product& g, int elem_size, bool direct, size_t bytes,
+                    Plan* p) {
+  const Shape* const shapes = elem_size == 2 ? kShapes16 : kShapes32;
+  const int chunks = ceil_div(g.k, kChunkBytes / elem_size);
+  // (operands that an L2 holds)
+  const bool cached = (static_cast<double>(g.m) + g.n) * g.k * elem_size < 4e6;
+  const float share_mb = static_cast<float>(g.m) * g.n * 4e-6f;
+  float best = -1.f;
+  for (int kernel = direct ? 0 : kAny16x16;
+       kernel < (direct ? kAny16x16 : kKernels); ++kernel) {
+    const Shape& s = shapes[kernel];
+    if (s.fixed == 0.f) continue;
+#ifdef SNN_HIP_TUNING
+    if (const char* only = std::getenv("SNN_HIP_EPI_KERNEL"))
+      if (std::atoi(only) % kAny16x16 != kernel % kAny16x16) continue;
+#endif
+    const int tiles_m = ceil_div(g.m, s.bm), tiles_n = ceil_div(g.n, s.bn);
+    const double tiles = static_cast<double>(tiles_m) * tiles_n;
+    for (int want = 1; want <= 32; want *= 2) {
+#ifdef SNN_HIP_TUNING
+      if (const char* only = std::getenv("SNN_HIP_EPI_SPLITS"))
+        if (std::atoi(only) != want) continue;
+#endif
+      if (want > 1 && (want > chunks / s.chunks || tiles * want > 1024 ||
+                       static_cast<size_t>(g.m) * g.n * 4 * want > bytes))
+        break;
+      const int split_chunks = ceil_div(chunks, want);
+      const int splits = ceil_div(chunks, split_chunks);
+      double rounds = std::ceil(tiles * splits / s.slots);
+      if (s.slots == 512)  // work-groups that are alone on their CU are faster
+        rounds += std::max(0.55, std::min(1.0, tiles * splits / 512 -
+                                                   (rounds - 1.0))) -
+                  1.0;
+      const float steps =
+          static_cast<float>(ceil_div(split_chunks, s.chunks));
+      float step = g.q_k_inner ? s.step_k : s.step_row;
+      if (s.chunks > 1 && cached) step *= 0.6f;
+      const float time =
+          static_cast<float>(std::ceil(rounds)) * s.fixed +
+          static_cast<float>(rounds) * steps * step +
+          (splits > 1 ? 2.f + 0.55f * share_mb * splits : 0.f);
+      if (best < 0.f || time < best) {
+        best = time;
+        p->kernel = kernel;
+        p->tiles_m = tiles_m;
+        p->tiles_n = tiles_n;
+        p->splits = splits;
+        p->split_chunks = split_chunks;
+      }
+    }
   }
-  p.tiles_m = ceil_div(m, p.bm);
-  p.tiles_n = ceil_div(n, p.bn);
-  // As many shares as fill the CUs, of four chunks at least.
-  const long tiles = static_cast<long>(p.tiles_m) * p.tiles_n;
-  long want = tiles >= 256 ? 1 : 512 / tiles;
-  want = want > chunks / 4 ? chunks / 4 : want;
-  const size_t share = static_cast<size_t>(m) * n * sizeof(float);
-  if (static_cast<size_t>(want) * share > bytes)
-    want = static_cast<long>(bytes / share);
-  if (want < 2) want = 1;
-  p.split_chunks = ceil_div(chunks, static_cast<int>(want));
-  p.splits = ceil_div(chunks, p.split_chunks);
-  return p;
+  return best;
+}
+
+// `bytes`: the workspace.  `p_aligned`, `q_aligned`: of the pointers.
+inline Plan make_plan(const Product& g, int elem_size, size_t bytes,
+                      bool p_aligned, bool q_aligned) {
+  Plan p = {};
+  const int m = g.m, n = g.n, k = g.k;
+  // Straight to LDS go whole 16-byte pieces, and tiles within 31 bits.
+  const int chunk = kChunkBytes / elem_size;
+  auto direct = [&](bool k_inner, bool aligned, int rows, long stride) {
+    return aligned && stride * elem_size % 16 == 0 &&
+           memory_cols(k_inner, rows, k) * static_cast<long>(elem_size) % 16 ==
+               0 &&
+           (k_inner ? 256 : chunk) * stride * elem_size < 0x7FFF0000l;
+  };
+  const bool p_direct = direct(g.p_k_inner, p_aligned, m, g.p_stride);
+  const bool q_direct = direct(g.q_k_inner, q_aligned, n, g.q_stride);
+  if (p_direct && q_direct) {
+    choose(g, elem_size, true, bytes, &p);
+    return p;
+  }
+  const float any = choose(g, elem_size, false, bytes, &p);
+  auto copy_bytes = [&](bool k_inner, int rows) {
+    return static_cast<size_t>(memory_rows(k_inner, rows, k)) *
+           copied_stride(memory_cols(k_inner, rows, k), elem_size) * elem_size;
+  };
+  const size_t p_bytes = p_direct ? 0 : copy_bytes(g.p_k_inner, m);
+  const size_t q_bytes = q_direct ? 0 : copy_bytes(g.q_k_inner, n);
+  const int reach = 0x7FFF0000 / 256 / elem_size;
+  if (p_bytes + q_bytes > bytes || m >= reach || n >= reach || k >= reach)
+    return p;
+  Plan copied = {};
+  copied.copy_p = !p_direct;
+  copied.copy_q = !q_direct;
+  copied.p_bytes = p_bytes;
+  copied.q_bytes = q_bytes;
+  // (a launch, and the operands read and written)
+  const float with_copies =
+      choose(g, elem_size, true, bytes - p_bytes - q_bytes, &copied) + 3.f +
+      static_cast<float>(p_bytes + q_bytes) * 0.5e-6f;
+#ifdef SNN_HIP_TUNING
+  if (const char* copy = std::getenv("SNN_HIP_EPI_COPY"))
+    return std::atoi(copy) != 0 ? copied : p;
+#endif
+  return with_copies < any ? copied : p;
 }
 
 }  // namespace epi

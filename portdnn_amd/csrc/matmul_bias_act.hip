@@ -114,22 +114,81 @@ long or_else(int stride, int row) { return stride == 0 ? row : stride; }
 
 size_t round16(size_t bytes) { return (bytes + 15) / 16 * 16; }
 
-// Where the gradients' workspace has what: dz, the bias's partial sums, the
-// shares of the two products' reductions in turn.
+// The forward product and those of the gradients, but for the addresses.
+Product forward_product(const snn_hip_matmul_bias_act_params& p) {
+  Product g = {};
+  g.p_stride = or_else(p.lhs_stride, p.transpose_lhs ? p.m : p.k);
+  g.p_k_inner = !p.transpose_lhs;
+  g.q_stride = or_else(p.rhs_stride, p.transpose_rhs ? p.k : p.n);
+  g.q_k_inner = p.transpose_rhs != 0;
+  g.m = p.m;
+  g.n = p.n;
+  g.k = p.k;
+  g.residual_stride = or_else(p.residual_stride, p.n);
+  g.out_stride = or_else(p.output_stride, p.n);
+  g.pre_stride = p.n;
+  g.activation = p.activation;
+  return g;
+}
+
+// An operand of the gradients' products: the address, its values with the
+// result's dimension first, and whether the reduction is contiguous.
+struct Side {
+  const void* at;
+  long stride;
+  bool k_inner;
+  int rows;
+};
+Product grad_product(const Side& a, const Side& b, int k) {
+  Product g = {};
+  g.p = a.at;
+  g.p_stride = a.stride;
+  g.p_k_inner = a.k_inner;
+  g.m = a.rows;
+  g.q = b.at;
+  g.q_stride = b.stride;
+  g.q_k_inner = b.k_inner;
+  g.n = b.rows;
+  g.k = k;
+  g.out_stride = b.rows;
+  return g;
+}
+// over n: dz (m x n) and op(rhs) (k x n)
+Product lhs_product(const snn_hip_matmul_bias_act_params& p, const void* d,
+                    long d_stride, const void* rhs) {
+  const Side of_d = {d, d_stride, true, p.m};
+  const Side of_r = {rhs, or_else(p.rhs_stride, p.transpose_rhs ? p.k : p.n),
+                     !p.transpose_rhs, p.k};
+  return p.transpose_lhs ? grad_product(of_r, of_d, p.n)
+                         : grad_product(of_d, of_r, p.n);
+}
+// over m: op(lhs)^T (k x m) and dz^T (n x m)
+Product rhs_product(const snn_hip_matmul_bias_act_params& p, const void* d,
+                    long d_stride, const void* lhs) {
+  const Side of_l = {lhs, or_else(p.lhs_stride, p.transpose_lhs ? p.m : p.k),
+                     p.transpose_lhs != 0, p.k};
+  const Side of_d = {d, d_stride, false, p.n};
+  return p.transpose_rhs ? grad_product(of_d, of_l, p.m)
+                         : grad_product(of_l, of_d, p.m);
+}
+
+// Where the gradients' workspace has what: dz, the bias's partial sums, and
+// what the two products take in turn.
 struct GradSpace {
-  size_t dz, sums, shares;
+  size_t dz, sums, products;
 };
 GradSpace grad_space(const snn_hip_matmul_bias_act_params& p, int size) {
   GradSpace s = {};
-  if (p.activation != SNN_HIP_ACTIVATION_NONE)
-    s.dz = round16(static_cast<size_t>(p.m) * p.n * size);
+  const bool act = p.activation != SNN_HIP_ACTIVATION_NONE;
+  if (act) s.dz = round16(static_cast<size_t>(p.m) * p.n * size);
   s.sums = round16(static_cast<size_t>(ceil_div(p.m, rows_per_group(p.m, p.n))) *
                    p.n * sizeof(float));
-  const size_t lhs = p.transpose_lhs ? epi::split_bytes(p.k, p.m, p.n, size)
-                                     : epi::split_bytes(p.m, p.k, p.n, size);
-  const size_t rhs = p.transpose_rhs ? epi::split_bytes(p.n, p.k, p.m, size)
-                                     : epi::split_bytes(p.k, p.n, p.m, size);
-  s.shares = std::max(lhs, rhs);
+  const long stride = act ? p.n : or_else(p.output_stride, p.n);
+  s.products =
+      std::max(epi::workspace_bytes(lhs_product(p, nullptr, stride, nullptr),
+                                    size),
+               epi::workspace_bytes(rhs_product(p, nullptr, stride, nullptr),
+                                    size));
   return s;
 }
 
@@ -141,25 +200,13 @@ int forward(int dtype, const void* lhs, const void* rhs, const void* bias,
   const int v = check(params, sizeof(T), workspace);
   if (v != SNN_HIP_OK) return v;
   SNN_REQUIRE(lhs != nullptr && rhs != nullptr && output != nullptr);
-  const snn_hip_matmul_bias_act_params& p = *params;
-  Product g = {};
+  Product g = forward_product(*params);
   g.p = lhs;
-  g.p_stride = or_else(p.lhs_stride, p.transpose_lhs ? p.m : p.k);
-  g.p_k_inner = !p.transpose_lhs;
   g.q = rhs;
-  g.q_stride = or_else(p.rhs_stride, p.transpose_rhs ? p.k : p.n);
-  g.q_k_inner = p.transpose_rhs;
-  g.m = p.m;
-  g.n = p.n;
-  g.k = p.k;
   g.bias = bias;
   g.residual = residual;
-  g.residual_stride = or_else(p.residual_stride, p.n);
   g.out = output;
-  g.out_stride = or_else(p.output_stride, p.n);
   g.pre = pre;
-  g.pre_stride = p.n;
-  g.activation = p.activation;
   KernelTimer timer(as_stream(stream));
   return run(dtype, g, workspace, workspace == nullptr ? 0 : elems * sizeof(T),
              as_stream(stream));
@@ -207,8 +254,8 @@ int backward(int dtype, const void* grad, const void* lhs, const void* rhs,
   T* const dz = space.dz > 0 ? reinterpret_cast<T*>(at) : nullptr;
   float* const sums =
       space.sums > 0 ? reinterpret_cast<float*>(at + space.dz) : nullptr;
-  void* const shares = bytes > 0 ? at + space.dz + space.sums : nullptr;
-  const size_t share_bytes = bytes - space.dz - space.sums;
+  void* const rest = bytes > 0 ? at + space.dz + space.sums : nullptr;
+  const size_t rest_bytes = bytes - space.dz - space.sums;
 
   KernelTimer timer(stream);
   const long grad_stride = or_else(p.output_stride, p.n);
@@ -232,45 +279,18 @@ int backward(int dtype, const void* grad, const void* lhs, const void* rhs,
     SNN_HIP_CHECK_LAUNCH();
   }
 
-  // An operand of the products: its values with the result's dimension first,
-  // and whether the reduction is contiguous.
-  struct Side {
-    const void* at;
-    long stride;
-    bool k_inner;
-    int rows;
-  };
   const void* const d = dz != nullptr ? static_cast<const void*>(dz) : grad;
   const long d_stride = dz != nullptr ? p.n : grad_stride;
-  const long lhs_stride = or_else(p.lhs_stride, p.transpose_lhs ? p.m : p.k);
-  const long rhs_stride = or_else(p.rhs_stride, p.transpose_rhs ? p.k : p.n);
-  auto product = [&](const Side& a, const Side& b, int k, void* out) {
-    Product g = {};
-    g.p = a.at;
-    g.p_stride = a.stride;
-    g.p_k_inner = a.k_inner;
-    g.m = a.rows;
-    g.q = b.at;
-    g.q_stride = b.stride;
-    g.q_k_inner = b.k_inner;
-    g.n = b.rows;
-    g.k = k;
-    g.out = out;
-    g.out_stride = b.rows;
-    return run(dtype, g, shares, share_bytes, stream);
-  };
-  if (grad_lhs != nullptr) {  // over n: dz (m x n) and op(rhs) (k x n)
-    const Side of_d = {d, d_stride, true, p.m};
-    const Side of_r = {rhs, rhs_stride, !p.transpose_rhs, p.k};
-    const int s = p.transpose_lhs ? product(of_r, of_d, p.n, grad_lhs)
-                                  : product(of_d, of_r, p.n, grad_lhs);
+  if (grad_lhs != nullptr) {
+    Product g = lhs_product(p, d, d_stride, rhs);
+    g.out = grad_lhs;
+    const int s = run(dtype, g, rest, rest_bytes, stream);
     if (s != SNN_HIP_OK) return s;
   }
-  if (grad_rhs != nullptr) {  // over m: op(lhs)^T (k x m) and dz^T (n x m)
-    const Side of_l = {lhs, lhs_stride, p.transpose_lhs != 0, p.k};
-    const Side of_d = {d, d_stride, false, p.n};
-    const int s = p.transpose_rhs ? product(of_d, of_l, p.m, grad_rhs)
-                                  : product(of_l, of_d, p.m, grad_rhs);
+  if (grad_rhs != nullptr) {
+    Product g = rhs_product(p, d, d_stride, lhs);
+    g.out = grad_rhs;
+    const int s = run(dtype, g, rest, rest_bytes, stream);
     if (s != SNN_HIP_OK) return s;
   }
   return SNN_HIP_OK;
@@ -280,14 +300,16 @@ int backward(int dtype, const void* grad, const void* lhs, const void* rhs,
 
 namespace epi {
 
-size_t split_bytes(int m, int n, int k, int elem_size) {
-  // (the division by the larger tiles of aligned operands and by the others)
+size_t workspace_bytes(const Product& g, int elem_size) {
+  // (with aligned addresses and without: other tiles, other shares)
   size_t most = 0;
-  for (const bool direct : {false, true}) {
-    const Plan p = make_plan(m, n, k, elem_size, direct, ~size_t{0});
-    if (p.splits > 1)
-      most = std::max(most, static_cast<size_t>(m) * n * p.splits *
-                                sizeof(float));
+  for (const bool aligned : {false, true}) {
+    const Plan p = make_plan(g, elem_size, ~size_t{0}, aligned, aligned);
+    const size_t shares = p.splits > 1 ? static_cast<size_t>(g.m) * g.n *
+                                             p.splits * sizeof(float)
+                                       : 0;
+    // (copies only for what the sizes and strides ask for)
+    most = std::max(most, shares + (aligned ? p.p_bytes + p.q_bytes : 0));
   }
   return round16(most);
 }
@@ -333,11 +355,11 @@ int snn_hip_matmul_bias_act_workspace_size(
   if (grad != 0) {
     const snn::GradSpace s = snn::grad_space(*params, size);
     *required_elems = (s.dz + s.sums) / size;
-    *recommended_elems = (s.dz + s.sums + s.shares) / size;
+    *recommended_elems = (s.dz + s.sums + s.products) / size;
   } else {
     *required_elems = 0;
     *recommended_elems =
-        snn::epi::split_bytes(params->m, params->n, params->k, size) / size;
+        snn::epi::workspace_bytes(snn::forward_product(*params), size) / size;
   }
   return SNN_HIP_OK;
 }

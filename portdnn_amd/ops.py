@@ -523,7 +523,7 @@ def _vector(t, n, dtype):
     """The address of an optional vector of n values."""
     if t is None:
         return None
-    assert t.numel() == n and t.dtype == dtype and t.is_contiguous()
+    assert t.dtype is dtype and t.numel() == n and t.is_contiguous()
     return t.data_ptr()
 
 
@@ -535,36 +535,46 @@ def _like(t, shape, dtype):
     return t.data_ptr()
 
 
-_sizes = {}
+# What a call derives from its operands' sizes, strides and types (and from
+# nothing else): settled once, as small calls are bound by the interpreter.
+_plans = {}
+_MOST_PLANS = 4096
+
+
+def _keep(key, plan):
+    if len(_plans) >= _MOST_PLANS:  # (lengths that never come again)
+        _plans.clear()
+    _plans[key] = plan
+    return plan
 
 
 def _workspace(entry, params, *args):
-    """(required, recommended) elements of a workspace query; the answer goes
-    by the sizes alone."""
-    key = (entry, bytes(params)) + args
-    got = _sizes.get(key)
-    if got is None:
-        req, rec = ctypes.c_size_t(), ctypes.c_size_t()
-        capi.check(getattr(capi.lib(), entry)(
-            ctypes.byref(params), *args, ctypes.byref(req), ctypes.byref(rec)))
-        got = _sizes[key] = (req.value, rec.value)
-    return got
+    """The recommended elements of a workspace."""
+    req, rec = ctypes.c_size_t(), ctypes.c_size_t()
+    capi.check(getattr(capi.lib(), entry)(
+        ctypes.byref(params), *args, ctypes.byref(req), ctypes.byref(rec)))
+    return rec.value
 
 
-_matmul_sizes = {}
-
-
-def _matmul_workspace(m, k, n, trans_a, trans_b, activation, grad, t):
-    key = (m, k, n, trans_a, trans_b, activation, grad, t.dtype)
-    elems = _matmul_sizes.get(key)
-    if elems is None:
-        elems = _matmul_sizes[key] = _workspace(
-            "snn_hip_matmul_bias_act_workspace_size",
-            MatmulBiasActParams(m=m, k=k, n=n, transpose_lhs=int(trans_a),
-                                transpose_rhs=int(trans_b),
-                                activation=activation),
-            int(grad), _TYPES[t.dtype][1])[1]
-    return torch.empty(elems, dtype=t.dtype, device=t.device) if elems else None
+def _matmul_plan(key, a, b, grad, activation, trans_a, trans_b):
+    dtype = a.dtype
+    m, k = (a.shape[1], a.shape[0]) if trans_a else a.shape
+    n = b.shape[0] if trans_b else b.shape[1]
+    assert (b.shape[1] if trans_b else b.shape[0]) == k and b.dtype == dtype
+    suffix, code = _TYPES[dtype]
+    out_stride = 0
+    if grad is not None:
+        assert grad.shape == (m, n) and grad.dtype == dtype
+        out_stride = _row_stride(grad)
+    p = MatmulBiasActParams(
+        m=m, k=k, n=n, transpose_lhs=int(trans_a), transpose_rhs=int(trans_b),
+        activation=activation, lhs_stride=_row_stride(a),
+        rhs_stride=_row_stride(b), output_stride=out_stride)
+    elems = _workspace("snn_hip_matmul_bias_act_workspace_size", p,
+                       int(grad is not None), code)
+    name = "snn_hip_matmul_bias_act" + ("_grad" if grad is not None else "")
+    return _keep(key, (_address(name + suffix), m, k, n, p.lhs_stride,
+                       p.rhs_stride, out_stride, elems))
 
 
 def matmul_bias_act(a, b, bias=None, residual=None,
@@ -574,28 +584,32 @@ def matmul_bias_act(a, b, bias=None, residual=None,
     keep_pre_activation returns (output, op(a) op(b) + bias), of which the
     gradient takes the second.  `out` may be the residual."""
     dtype = a.dtype
-    m, k = (a.shape[1], a.shape[0]) if trans_a else a.shape
-    n = b.shape[0] if trans_b else b.shape[1]
-    assert (b.shape[1] if trans_b else b.shape[0]) == k and b.dtype == dtype
+    key = (a.shape, a.stride(), b.shape, b.stride(), dtype, b.dtype, activation,
+           trans_a, trans_b)
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _matmul_plan(key, a, b, None, activation, trans_a, trans_b)
+    fn, m, k, n, a_stride, b_stride, _, elems = plan
     if out is None:
-        out = torch.empty((m, n), dtype=dtype, device=a.device)
+        out = a.new_empty((m, n))
+        out_stride = n
     else:
         assert out.shape == (m, n) and out.dtype == dtype
+        out_stride = _row_stride(out)
     add, add_stride = None, 0
     if residual is not None:
         assert residual.shape == (m, n) and residual.dtype == dtype
         add, add_stride = residual.data_ptr(), _row_stride(residual)
-    z = (torch.empty((m, n), dtype=dtype, device=a.device)
-         if keep_pre_activation else None)
+    z = a.new_empty((m, n)) if keep_pre_activation else None
     if workspace is None:
-        workspace = _matmul_workspace(m, k, n, trans_a, trans_b, activation,
-                                      False, a)
+        if elems:
+            workspace = a.new_empty(elems)
+    else:
+        elems = workspace.numel()
     code = _native.matmul_bias_act(
-        _address("snn_hip_matmul_bias_act" + _TYPES[dtype][0]), a.data_ptr(),
-        b.data_ptr(), _vector(bias, n, dtype), add, out.data_ptr(), _at(z),
-        m, k, n, trans_a, trans_b, activation, _row_stride(a), _row_stride(b),
-        add_stride, _row_stride(out), _at(workspace),
-        0 if workspace is None else workspace.numel(), _stream())
+        fn, a.data_ptr(), b.data_ptr(), _vector(bias, n, dtype), add,
+        out.data_ptr(), _at(z), m, k, n, trans_a, trans_b, activation, a_stride,
+        b_stride, add_stride, out_stride, _at(workspace), elems, _stream())
     if code:
         capi.check(code)
     return (out, z) if keep_pre_activation else out
@@ -608,36 +622,31 @@ def matmul_bias_act_grad(grad, a, b, pre_activation=None,
     """snn_hip_matmul_bias_act_grad: the gradients of a, b and the bias, None
     for those that are not wanted (the residual's is `grad` itself)."""
     dtype = a.dtype
-    m, k = (a.shape[1], a.shape[0]) if trans_a else a.shape
-    n = b.shape[0] if trans_b else b.shape[1]
-    assert (b.shape[1] if trans_b else b.shape[0]) == k and b.dtype == dtype
-    assert grad.shape == (m, n) and grad.dtype == dtype
-    a_stride, b_stride = _row_stride(a), _row_stride(b)
-
-    grad_a = (torch.empty(a.shape, dtype=dtype, device=a.device) if need_a
-              else None)
-    grad_b = (torch.empty(b.shape, dtype=dtype, device=b.device) if need_b
-              else None)
-    grad_bias = (torch.empty(n, dtype=dtype, device=a.device) if bias else None)
+    key = (a.shape, a.stride(), b.shape, b.stride(), grad.shape, grad.stride(),
+           dtype, b.dtype, grad.dtype, activation, trans_a, trans_b)
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _matmul_plan(key, a, b, grad, activation, trans_a, trans_b)
+    fn, m, k, n, a_stride, b_stride, grad_stride, elems = plan
+    grad_a = a.new_empty(a.shape) if need_a else None
+    grad_b = a.new_empty(b.shape) if need_b else None
+    grad_bias = a.new_empty(n) if bias else None
     if workspace is None:
-        workspace = _matmul_workspace(m, k, n, trans_a, trans_b, activation,
-                                      True, a)
+        if elems:
+            workspace = a.new_empty(elems)
+    else:
+        elems = workspace.numel()
     code = _native.matmul_bias_act_grad(
-        _address("snn_hip_matmul_bias_act_grad" + _TYPES[dtype][0]),
-        grad.data_ptr(), a.data_ptr(), b.data_ptr(),
+        fn, grad.data_ptr(), a.data_ptr(), b.data_ptr(),
         _like(pre_activation, (m, n), dtype), _at(grad_a), _at(grad_b),
         _at(grad_bias), m, k, n, trans_a, trans_b, activation, a_stride,
-        b_stride, 0, _row_stride(grad), _at(workspace),
-        0 if workspace is None else workspace.numel(), _stream())
+        b_stride, 0, grad_stride, _at(workspace), elems, _stream())
     if code:
         capi.check(code)
     return grad_a, grad_b, grad_bias
 
 
-def _gate_operand(gate, gate_op, gate_rows, rows, channels, dtype):
-    if gate is None:
-        assert gate_op == GATE.NONE, "an operation without a gate"
-        return None, 0
+def _gate_operand(gate, gate_rows, rows, channels, dtype):
     assert gate.shape == (-(-rows // gate_rows), channels) and \
         gate.dtype == dtype
     return gate.data_ptr(), _row_stride(gate)
@@ -650,37 +659,38 @@ def residual_norm(x, residual=None, gate=None, scale=None, post=NORM.NONE,
     """snn_hip_residual_norm: sum = residual + scale * gate * post_norm(x) and
     normed = pre_norm(sum).  Returns (sum, normed, stats), None for what is not
     wanted or not there; `out` takes the sum and may be x or the residual."""
-    rows, channels = x.shape
+    rows, channels = shape = x.shape
     dtype = x.dtype
-    if gate_op is None:
-        gate_op = GATE.NONE if gate is None else GATE.VALUE
-    gate_at, gate_stride = _gate_operand(gate, gate_op, gate_rows, rows,
-                                         channels, dtype)
-    shape = x.shape
+    gate_at, gate_stride = None, 0
+    if gate is None:
+        assert not gate_op, "an operation without a gate"
+        gate_op = GATE.NONE
+    else:
+        if gate_op is None:
+            gate_op = GATE.VALUE
+        gate_at, gate_stride = _gate_operand(gate, gate_rows, rows, channels,
+                                             dtype)
     if out is None:
         if keep_sum:
-            out = torch.empty(shape, dtype=dtype, device=x.device)
+            out = x.new_empty(shape)
+        sum_at = _at(out)
     else:
-        _like(out, shape, dtype)
-    normed = (torch.empty(shape, dtype=dtype, device=x.device)
-              if pre != NORM.NONE else None)
-    stats = (torch.empty((rows, 4), dtype=torch.float32, device=x.device)
-             if keep_stats else None)
+        sum_at = _like(out, shape, dtype)
+    normed = x.new_empty(shape) if pre != NORM.NONE else None
+    stats = (x.new_empty((rows, 4), dtype=torch.float32) if keep_stats
+             else None)
     code = _native.residual_norm(
         _address("snn_hip_residual_norm" + _TYPES[dtype][0]), x.data_ptr(),
         _like(residual, shape, dtype), gate_at, _vector(scale, channels, dtype),
         _vector(post_weight, channels, dtype),
         _vector(post_bias, channels, dtype),
         _vector(pre_weight, channels, dtype),
-        _vector(pre_bias, channels, dtype), _at(out), _at(normed), _at(stats),
+        _vector(pre_bias, channels, dtype), sum_at, _at(normed), _at(stats),
         rows, channels, post, pre, gate_op, gate_rows, _row_stride(x),
         gate_stride, eps, _stream())
     if code:
         capi.check(code)
     return out, normed, stats
-
-
-_norm_sizes = {}
 
 
 def residual_norm_grad(x, sum, stats, grad_sum=None, grad_normed=None,
@@ -691,14 +701,19 @@ def residual_norm_grad(x, sum, stats, grad_sum=None, grad_normed=None,
     """snn_hip_residual_norm_grad: a dict of the gradients of x, residual and
     of those of gate, scale, post_weight, post_bias, pre_weight and pre_bias
     that are given."""
-    rows, channels = x.shape
-    dtype, shape, device = x.dtype, x.shape, x.device
-    if gate_op is None:
-        gate_op = GATE.NONE if gate is None else GATE.VALUE
-    gate_at, gate_stride = _gate_operand(gate, gate_op, gate_rows, rows,
-                                         channels, dtype)
-    got = {"x": torch.empty(shape, dtype=dtype, device=device),
-           "residual": torch.empty(shape, dtype=dtype, device=device)}
+    rows, channels = shape = x.shape
+    dtype = x.dtype
+    got = {"x": x.new_empty(shape), "residual": x.new_empty(shape)}
+    gate_at, gate_stride = None, 0
+    if gate is None:
+        assert not gate_op, "an operation without a gate"
+        gate_op = GATE.NONE
+    else:
+        if gate_op is None:
+            gate_op = GATE.VALUE
+        gate_at, gate_stride = _gate_operand(gate, gate_rows, rows, channels,
+                                             dtype)
+        got["gate"] = x.new_empty(gate.shape)
     addresses = {}
     for name, t in (("scale", scale), ("post_weight", post_weight),
                     ("post_bias", post_bias), ("pre_weight", pre_weight),
@@ -706,19 +721,16 @@ def residual_norm_grad(x, sum, stats, grad_sum=None, grad_normed=None,
         addresses[name] = _vector(t, channels, dtype)
         if t is not None and (grad_normed is not None or
                               not name.startswith("pre")):
-            got[name] = torch.empty(channels, dtype=dtype, device=device)
-    if gate is not None:
-        got["gate"] = torch.empty(gate.shape, dtype=dtype, device=device)
+            got[name] = x.new_empty(channels)
     if workspace is None:
         key = (rows, channels, gate_op, gate_rows, dtype)
-        elems = _norm_sizes.get(key)
+        elems = _plans.get(key)
         if elems is None:
-            elems = _norm_sizes[key] = _workspace(
+            elems = _keep(key, _workspace(
                 "snn_hip_residual_norm_grad_workspace_size",
                 ResidualNormParams(rows=rows, channels=channels, gate=gate_op,
-                                   gate_rows=gate_rows),
-                _TYPES[dtype][1])[1]
-        workspace = torch.empty(elems, dtype=dtype, device=device)
+                                   gate_rows=gate_rows), _TYPES[dtype][1]))
+        workspace = x.new_empty(elems)
     code = _native.residual_norm_grad(
         _address("snn_hip_residual_norm_grad" + _TYPES[dtype][0]),
         x.data_ptr(), None, gate_at, addresses["scale"],
@@ -738,31 +750,24 @@ def residual_norm_grad(x, sum, stats, grad_sum=None, grad_normed=None,
     return got
 
 
-_recurrence_sizes = {}
-
-
-def _recurrence_workspace(t):
-    key = (t.shape, t.dtype)
-    elems = _recurrence_sizes.get(key)
-    if elems is None:
-        batch, steps, channels = t.shape
-        elems = _recurrence_sizes[key] = _workspace(
+def _recurrence_operands(x, forget, input_gate, resets, lengths):
+    """The common row stride, the workspace's elements and the optional
+    operands' addresses."""
+    shape, stride, dtype = x.shape, x.stride(), x.dtype
+    key = (shape, stride, dtype)
+    plan = _plans.get(key)
+    if plan is None:
+        batch, steps, channels = shape
+        plan = _keep(key, (_step_stride(x), _workspace(
             "snn_hip_linear_recurrence_workspace_size",
             LinearRecurrenceParams(batch=batch, steps=steps,
-                                   channels=channels),
-            _TYPES[t.dtype][1])[1]
-    return torch.empty(elems, dtype=t.dtype, device=t.device) if elems else None
-
-
-def _recurrence_operands(x, forget, input_gate, resets, lengths):
-    """The common row stride and the optional operands' addresses."""
-    batch, steps, channels = shape = x.shape
-    stride = _step_stride(x)
+                                   channels=channels), _TYPES[dtype][1])))
     for t in (forget, input_gate):
-        assert t is None or (t.shape == shape and t.dtype == x.dtype and
-                             _step_stride(t) == stride)
-    return stride, _like(resets, (batch, steps), torch.uint8), \
-        _vector(lengths, batch, torch.int32)
+        assert t is None or (t.shape == shape and t.dtype == dtype and
+                             (t.stride() == stride or
+                              _step_stride(t) == plan[0]))
+    return plan[0], plan[1], _like(resets, shape[:2], torch.uint8), \
+        _vector(lengths, shape[0], torch.int32)
 
 
 def linear_recurrence(x, forget, input_gate=None, resets=None, lengths=None,
@@ -774,23 +779,24 @@ def linear_recurrence(x, forget, input_gate=None, resets=None, lengths=None,
     initial_state, which is then updated in place."""
     batch, steps, channels = shape = x.shape
     dtype = x.dtype
-    stride, resets_at, lengths_at = _recurrence_operands(x, forget, input_gate,
-                                                         resets, lengths)
+    stride, elems, resets_at, lengths_at = _recurrence_operands(
+        x, forget, input_gate, resets, lengths)
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=x.device)
+        out = x.new_empty(shape)
     if final_state is None:
-        final_state = torch.empty((batch, channels), dtype=torch.float32,
-                                  device=x.device)
+        final_state = x.new_empty((batch, channels), dtype=torch.float32)
     if workspace is None:
-        workspace = _recurrence_workspace(x)
+        if elems:
+            workspace = x.new_empty(elems)
+    else:
+        elems = workspace.numel()
     state = (batch, channels)
     code = _native.linear_recurrence(
         _address("snn_hip_linear_recurrence" + _TYPES[dtype][0]), x.data_ptr(),
         forget.data_ptr(), _at(input_gate), resets_at, lengths_at,
         _like(initial_state, state, torch.float32), _like(out, shape, dtype),
         _like(final_state, state, torch.float32), batch, steps, channels,
-        stride, 0, _at(workspace),
-        0 if workspace is None else workspace.numel(), _stream())
+        stride, 0, _at(workspace), elems, _stream())
     if code:
         capi.check(code)
     return out, final_state
@@ -804,23 +810,24 @@ def linear_recurrence_grad(grad, x, forget, h, input_gate=None, resets=None,
     channels * n] tensor that takes those of x, forget and input_gate side by
     side, the gradient of a projection that they are slices of."""
     batch, steps, channels = shape = x.shape
-    dtype, device = x.dtype, x.device
-    stride, resets_at, lengths_at = _recurrence_operands(x, forget, input_gate,
-                                                         resets, lengths)
+    dtype = x.dtype
+    stride, elems, resets_at, lengths_at = _recurrence_operands(
+        x, forget, input_gate, resets, lengths)
     names = ["x", "forget"] + (["input_gate"] if input_gate is not None else [])
     if out is None:
-        got = {name: torch.empty(shape, dtype=dtype, device=device)
-               for name in names}
+        got = {name: x.new_empty(shape) for name in names}
         grad_stride = channels
     else:
         _like(out, (batch, steps, channels * len(names)), dtype)
         got = {name: out[..., i * channels:(i + 1) * channels]
                for i, name in enumerate(names)}
         grad_stride = channels * len(names)
-    got["initial_state"] = torch.empty((batch, channels), dtype=torch.float32,
-                                       device=device)
+    got["initial_state"] = x.new_empty((batch, channels), dtype=torch.float32)
     if workspace is None:
-        workspace = _recurrence_workspace(x)
+        if elems:
+            workspace = x.new_empty(elems)
+    else:
+        elems = workspace.numel()
     state = (batch, channels)
     code = _native.linear_recurrence_grad(
         _address("snn_hip_linear_recurrence_grad" + _TYPES[dtype][0]),
@@ -830,8 +837,7 @@ def linear_recurrence_grad(grad, x, forget, h, input_gate=None, resets=None,
         _like(initial_state, state, torch.float32), _like(h, shape, dtype),
         got["x"].data_ptr(), got["forget"].data_ptr(),
         _at(got.get("input_gate")), got["initial_state"].data_ptr(), batch,
-        steps, channels, stride, grad_stride, _at(workspace),
-        0 if workspace is None else workspace.numel(), _stream())
+        steps, channels, stride, grad_stride, _at(workspace), elems, _stream())
     if code:
         capi.check(code)
     return got
