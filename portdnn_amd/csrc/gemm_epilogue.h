@@ -61,7 +61,6 @@ struct Product {
   void *out, *pre;
   long residual_stride, out_stride, pre_stride;
   int activation;
-  bool wide;  // the epilogue's rows start at multiples of 16 bytes, n % 8 == 0
   // division of the work
   int tiles_m, tiles_n, splits, split_chunks;  // chunks of a share
   float* partial;                              // [splits][m][n]
@@ -122,6 +121,7 @@ __device__ __forceinline__ float activation_slope(float z, int kind) {
 }
 
 // Eight neighbouring columns of a row: bias, activation, residual, one rounding.
+// Rows may start anywhere (see Pack).
 template <typename T>
 __device__ __forceinline__ void finish8(const Product& g, int row, int col,
                                         float (&v)[8]) {
@@ -135,7 +135,7 @@ __device__ __forceinline__ void finish8(const Product& g, int row, int col,
   T* const pre =
       g.pre == nullptr ? nullptr : static_cast<T*>(g.pre) + row * g.pre_stride;
   T* const out = static_cast<T*>(g.out) + row * g.out_stride;
-  if (g.wide) {
+  if (col + 8 <= g.n) {
     auto load = [&](const T* from, float (&to)[8]) {
 #pragma unroll
       for (int j = 0; j < 8; j += VEC) {
@@ -173,10 +173,11 @@ __device__ __forceinline__ void finish8(const Product& g, int row, int col,
     store(out, v);
     return;
   }
+#pragma unroll 1
+  for (int i = 0; col + i < g.n; ++i) {
+    float z = v[0];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if (col + i >= g.n) break;
-    float z = v[i];
+    for (int k = 1; k < 8; ++k) z = i == k ? v[k] : z;
     if (bias != nullptr) z += static_cast<float>(bias[col + i]);
     if (pre != nullptr) pre[col + i] = static_cast<T>(z);
     z = activate(z, g.activation);
@@ -219,12 +220,18 @@ __device__ __forceinline__ void leave(const Product& g, unsigned split, int row,
 
 // Which 16-byte position of its row holds piece c: c ^ swizzle(row).
 //   K inner: the 16 rows of a fragment, two (four) of which fill the 64 banks.
+//   Lanes that read together are rows 0 ... 3 and 12 ... 15 of one piece and 4 ...
+//   11 of the next; with four rows a bank row that takes the order 0, 2, 3, 1.
 //   row inner, 16-bit: the four reductions of a transposing read by the two
 //   blocks of eight, 32 bytes each.
 //   row inner, floats: four blocks of four reductions, 64 bytes each.
 template <int E, bool K_INNER, int ROWS, int CB>
 __device__ __forceinline__ constexpr unsigned swizzle(unsigned row) {
-  if (K_INNER) return CB == 128 ? (row >> 1) & 7u : (row >> 2) & 3u;
+  if (K_INNER) {
+    if (CB == 128) return (row >> 1) & 7u;
+    const unsigned four = (row >> 2) & 3u;
+    return (((four ^ (four >> 1)) & 1u) << 1) | (four >> 1);
+  }
   constexpr int kPitch = ROWS * E;
   if (E == 2) {
     if (kPitch >= 256) return 2u * ((row & 3u) | (((row >> 3) & 1u) << 2));

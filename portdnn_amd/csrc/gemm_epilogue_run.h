@@ -107,6 +107,11 @@ int launch_tile(const Product& g, int kernel, hipStream_t stream) {
       case kTile128Pair:
         return launch_as<T, PK, QK, 128, 128, 2, 4, 128, 2>(g, stream);
       case kTile256:
+        // (eight waves where both operands' fragments are transposing reads, whose
+        // addresses take sixteen waves' registers: 361 -> 201 us for 2048x8192x8192;
+        // sixteen elsewhere: 203 against 208 and 217 against 220)
+        if constexpr (!PK && !QK)
+          return launch_as<T, PK, QK, 256, 256, 2, 4, 64, 4>(g, stream);
         return launch_as<T, PK, QK, 256, 256, 4, 4, 64, 4>(g, stream);
       default:
         break;
@@ -165,13 +170,6 @@ int run(Product& g, void* workspace, size_t bytes, hipStream_t stream) {
   g.split_chunks = plan.split_chunks;
   char* const space = static_cast<char*>(workspace);
   g.partial = reinterpret_cast<float*>(space + plan.p_bytes + plan.q_bytes);
-  auto fits = [&](const void* p, long stride) {
-    return p == nullptr ||
-           seq::rows_aligned(static_cast<const T*>(p), stride, 16);
-  };
-  g.wide = g.n % 8 == 0 && fits(g.out, g.out_stride) &&
-           fits(g.pre, g.pre_stride) && fits(g.residual, g.residual_stride) &&
-           fits(g.bias, 0);
   if (plan.copy_p || plan.copy_q) {
     Copy copies[2] = {};
     auto copy = [&](const void** at, long* stride, bool k_inner, int rows,

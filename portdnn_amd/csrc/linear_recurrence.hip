@@ -34,9 +34,14 @@ namespace {
 using seq::Pack;
 using seq::pack;
 using seq::sigmoid;
+using seq::sigmoid_alone;
 using seq::unpack;
 
-constexpr int kGroup = 8;  // steps whose loads are in flight together
+// Steps whose loads are in flight together: 8 forward; the gradients, with five
+// operands, keep more waves on a SIMD with 4 (4 x 4096 x 2048 binary16: 176 ->
+// 147 us).
+template <bool BACK>
+constexpr int kSteps = BACK ? 4 : 8;
 
 struct Recurrence {
   int batch, steps, channels;
@@ -63,20 +68,28 @@ __device__ __forceinline__ bool is_reset(float a) {
 
 // What a wave needs of its place: sequence, piece, first channel of the lane.
 struct Place {
-  int b, piece, c, begin, end, length;
+  int b, piece, c, skip, begin, end, length;
   bool on;
 };
 
+// With `turned` the last come first: the walk behind a launch over the same
+// pieces then begins with what that has read last and the caches still hold.
 template <int VEC>
-__device__ __forceinline__ Place place_of(const Recurrence& r) {
+__device__ __forceinline__ Place place_of(const Recurrence& r, bool turned) {
   Place p;
   const int blocks = (r.channels + 64 * VEC - 1) / (64 * VEC);
-  const unsigned at = blockIdx.x * (blockDim.x / 64) + threadIdx.x / 64;
+  const unsigned place = turned ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
+  const unsigned at = place * (blockDim.x / 64) + threadIdx.x / 64;
   const unsigned row = at / blocks;
-  p.c = static_cast<int>(at - row * blocks) * 64 * VEC + (threadIdx.x & 63) * VEC;
+  const int first =
+      static_cast<int>(at - row * blocks) * 64 * VEC + (threadIdx.x & 63) * VEC;
+  // (a row's last channels: see Group; what is before them is not stored)
+  const seq::Group<VEC> group(first, r.channels);
+  p.c = group.c;
+  p.skip = group.skip;
   p.b = static_cast<int>(row / r.pieces);
   p.piece = static_cast<int>(row - static_cast<unsigned>(p.b) * r.pieces);
-  p.on = p.b < r.batch && p.c < r.channels;
+  p.on = p.b < r.batch && first < r.channels;
   if (p.b >= r.batch) p.b = 0;
   p.begin = p.piece * r.piece_steps;
   p.end = min(r.steps, p.begin + r.piece_steps);
@@ -86,13 +99,26 @@ __device__ __forceinline__ Place place_of(const Recurrence& r) {
   return p;
 }
 
+// Stores the lane's own of VEC values.
+template <typename T, int VEC>
+__device__ __forceinline__ void put(T* at, const float (&v)[VEC], int skip) {
+  if (skip == 0) {
+    *reinterpret_cast<typename Pack<T, VEC>::type*>(at) = pack<T, VEC>(v);
+  } else {
+#pragma unroll
+    for (int k = 1; k < VEC; ++k)
+      if (k >= skip) at[k] = static_cast<T>(v[k]);
+  }
+}
+
 // (A, S) of a piece, forward: S behind the piece's steps from a zero state;
 // backward: the gradient in front of it from a zero gradient behind.
 template <typename T, int VEC, bool GATE, bool BACK>
 __global__ void __launch_bounds__(256)
     recurrence_pieces_kernel(Recurrence r) {
   typedef typename Pack<T, VEC>::type V;
-  const Place p = place_of<VEC>(r);
+  constexpr int kGroup = kSteps<BACK>;
+  const Place p = place_of<VEC>(r, false);
   if (!p.on) return;
   const long row = static_cast<long>(p.b) * r.steps;
   const T* const f = static_cast<const T*>(r.f) + row * r.stride + p.c;
@@ -138,15 +164,15 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
       for (int k = 0; k < VEC; ++k) {
         float a, w;
-        sigmoid<T>(fs[k], &a, &w);
+        if (BACK || GATE)
+          a = sigmoid_alone<T>(fs[k]);
+        else
+          sigmoid<T>(fs[k], &a, &w);
         if (BACK) {
           S[k] = fresh[u] ? 0.f : a * (xs[k] + S[k]);
           A[k] = fresh[u] ? -0.f : a * A[k];
         } else {
-          if (GATE) {
-            float rest;
-            sigmoid<T>(is[k], &w, &rest);
-          }
+          if (GATE) w = sigmoid_alone<T>(is[k]);
           S[k] = w * xs[k] + (fresh[u] ? 0.f : a * S[k]);
           A[k] = fresh[u] ? -0.f : a * A[k];
         }
@@ -182,14 +208,28 @@ __global__ void __launch_bounds__(1024)
   auto at = [&](int n) {  // the n-th piece in the walk's order
     return base + static_cast<long>(BACK ? r.pieces - 1 - n : n) * r.channels;
   };
+  // (eight pieces' pairs are under way together)
+  constexpr int kBatch = 8;
+  auto walk = [&](auto step) {
+    for (int n = begin; n < end; n += kBatch) {
+      float a[kBatch], s[kBatch];
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const long where = at(min(n + u, end - 1));
+        a[u] = r.A[where];
+        s[u] = r.S[where];
+      }
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u)
+        if (n + u < end) step(n + u, a[u], s[u]);
+    }
+  };
   float A = 1.f, S = 0.f;
-  if (on) {
-    for (int n = begin; n < end; ++n) {
-      const float a = r.A[at(n)], s = r.S[at(n)];
+  if (on)
+    walk([&](int, float a, float s) {
       S = is_reset(a) ? s : a * S + s;
       A = is_reset(a) ? a : A * a;
-    }
-  }
+    });
   run_a[run][lane] = A;
   run_s[run][lane] = S;
   // (read in front of the barrier: `last` may be the same buffer)
@@ -201,11 +241,10 @@ __global__ void __launch_bounds__(1024)
     const float a = run_a[q][lane];
     state = is_reset(a) ? run_s[q][lane] : a * state + run_s[q][lane];
   }
-  for (int n = begin; n < end; ++n) {
-    const float a = r.A[at(n)], s = r.S[at(n)];
+  walk([&](int n, float a, float s) {
     r.S[at(n)] = state;
     state = is_reset(a) ? s : a * state + s;
-  }
+  });
   if (run == kRuns - 1 && r.last != nullptr) r.last[state_at] = state;
 }
 
@@ -213,7 +252,8 @@ __global__ void __launch_bounds__(1024)
 template <typename T, int VEC, bool GATE>
 __global__ void __launch_bounds__(256) recurrence_walk_kernel(Recurrence r) {
   typedef typename Pack<T, VEC>::type V;
-  const Place p = place_of<VEC>(r);
+  constexpr int kGroup = kSteps<false>;
+  const Place p = place_of<VEC>(r, r.pieces > 1);
   if (!p.on) return;
   const long row = static_cast<long>(p.b) * r.steps;
   const T* const f = static_cast<const T*>(r.f) + row * r.stride + p.c;
@@ -251,25 +291,22 @@ __global__ void __launch_bounds__(256) recurrence_walk_kernel(Recurrence r) {
 #pragma unroll
       for (int k = 0; k < VEC; ++k) {
         float a, w;
-        sigmoid<T>(fs[k], &a, &w);
         if (GATE) {
-          float rest;
-          sigmoid<T>(is[k], &w, &rest);
+          a = sigmoid_alone<T>(fs[k]);
+          w = sigmoid_alone<T>(is[k]);
+        } else {
+          sigmoid<T>(fs[k], &a, &w);
         }
         state[k] = w * xs[k] + (fresh[u] ? 0.f : a * state[k]);
       }
-      *reinterpret_cast<V*>(h + static_cast<long>(first + u) * r.channels) =
-          pack<T, VEC>(state);
+      put<T, VEC>(h + static_cast<long>(first + u) * r.channels, state, p.skip);
     }
   }
   float zero[VEC] = {};
   for (int t = max(p.begin, end); t < p.end; ++t)
-    *reinterpret_cast<V*>(h + static_cast<long>(t) * r.channels) =
-        pack<T, VEC>(zero);
-  if (r.pieces == 1 && r.last != nullptr) {
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) r.last[state_at + k] = state[k];
-  }
+    put<T, VEC>(h + static_cast<long>(t) * r.channels, zero, p.skip);
+  if (r.pieces == 1 && r.last != nullptr)
+    put<float, VEC>(r.last + state_at, state, p.skip);
 }
 
 // The gradients' walk over a piece, from its end, with the gradient that the
@@ -277,7 +314,8 @@ __global__ void __launch_bounds__(256) recurrence_walk_kernel(Recurrence r) {
 template <typename T, int VEC, bool GATE>
 __global__ void __launch_bounds__(256) recurrence_grad_kernel(Recurrence r) {
   typedef typename Pack<T, VEC>::type V;
-  const Place p = place_of<VEC>(r);
+  constexpr int kGroup = kSteps<true>;
+  const Place p = place_of<VEC>(r, r.pieces > 1);
   if (!p.on) return;
   const long row = static_cast<long>(p.b) * r.steps;
   const T* const f = static_cast<const T*>(r.f) + row * r.stride + p.c;
@@ -299,11 +337,11 @@ __global__ void __launch_bounds__(256) recurrence_grad_kernel(Recurrence r) {
 #pragma unroll
   for (int k = 0; k < VEC; ++k) D[k] = from == nullptr ? 0.f : from[k];
   const int end = min(p.end, p.length);
-  const V zero = {};
+  const float zero[VEC] = {};
   for (int t = max(p.begin, end); t < p.end; ++t) {
-    *reinterpret_cast<V*>(dx + t * r.grad_stride) = zero;
-    *reinterpret_cast<V*>(df + t * r.grad_stride) = zero;
-    if (GATE) *reinterpret_cast<V*>(di + t * r.grad_stride) = zero;
+    put<T, VEC>(dx + t * r.grad_stride, zero, p.skip);
+    put<T, VEC>(df + t * r.grad_stride, zero, p.skip);
+    if (GATE) put<T, VEC>(di + t * r.grad_stride, zero, p.skip);
   }
   const int groups = (end - p.begin + kGroup - 1) / kGroup;
   for (int g = groups - 1; g >= 0; --g) {
@@ -354,16 +392,13 @@ __global__ void __launch_bounds__(256) recurrence_grad_kernel(Recurrence r) {
         if (GATE) gi[k] = G * xs[k] * (w * w_rest);
         D[k] = fresh[u] ? 0.f : a * G;
       }
-      *reinterpret_cast<V*>(dx + t * r.grad_stride) = pack<T, VEC>(gx);
-      *reinterpret_cast<V*>(df + t * r.grad_stride) = pack<T, VEC>(gf);
-      if (GATE)
-        *reinterpret_cast<V*>(di + t * r.grad_stride) = pack<T, VEC>(gi);
+      put<T, VEC>(dx + t * r.grad_stride, gx, p.skip);
+      put<T, VEC>(df + t * r.grad_stride, gf, p.skip);
+      if (GATE) put<T, VEC>(di + t * r.grad_stride, gi, p.skip);
     }
   }
-  if (r.pieces == 1 && r.last != nullptr) {
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) r.last[state_at + k] = D[k];
-  }
+  if (r.pieces == 1 && r.last != nullptr)
+    put<float, VEC>(r.last + state_at, D, p.skip);
 }
 
 // How many pieces a sequence is divided into: as many as give the GPU
@@ -380,7 +415,7 @@ void divide_steps(const snn_hip_linear_recurrence_params& p, int* pieces,
   const long want = std::max(1l, kWantedWaves / waves);
   const long most = std::max(1, p.steps / kLeastSteps);
   const int n = static_cast<int>(std::min(want, most));
-  *piece_steps = ceil_div(ceil_div(p.steps, n), kGroup) * kGroup;
+  *piece_steps = ceil_div(ceil_div(p.steps, n), kSteps<false>) * kSteps<false>;
   *pieces = ceil_div(p.steps, *piece_steps);
 }
 
@@ -435,17 +470,7 @@ int launch_recurrence(Recurrence r, const snn_hip_linear_recurrence_params& p,
     r.S = r.A + floats / 2;
   }
   constexpr int VEC = kVec<T>;
-  constexpr unsigned kBytes = VEC * sizeof(T);
-  auto fits = [&](const void* ptr, long stride) {
-    return ptr == nullptr ||
-           seq::rows_aligned(static_cast<const T*>(ptr), stride, kBytes);
-  };
-  const bool wide =
-      p.channels % VEC == 0 && fits(r.x, r.stride) && fits(r.f, r.stride) &&
-      fits(r.i, r.stride) && fits(r.h, p.channels) && fits(r.dh, p.channels) &&
-      fits(r.out_h, p.channels) && fits(r.dx, r.grad_stride) &&
-      fits(r.df, r.grad_stride) && fits(r.di, r.grad_stride);
-  if (wide)
+  if (p.channels >= VEC)
     return r.i != nullptr ? launch_recurrence_as<T, VEC, true, BACK>(r, stream)
                           : launch_recurrence_as<T, VEC, false, BACK>(r, stream);
   return r.i != nullptr ? launch_recurrence_as<T, 1, true, BACK>(r, stream)

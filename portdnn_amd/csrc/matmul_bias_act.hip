@@ -31,23 +31,25 @@ __global__ void __launch_bounds__(256)
   typedef typename Pack<T, VEC>::type V;
   __shared__ float part[8][32 * VEC];
   const int lane = threadIdx.x & 31, line = threadIdx.x >> 5;
-  const int c = (blockIdx.x * 32 + lane) * VEC;
+  const int first = (blockIdx.x * 32 + lane) * VEC;
   const int begin = blockIdx.y * rows, end = min(m, begin + rows);
+  const seq::Group<VEC> at(first, n);
   float sum[VEC] = {};
-  if (c < n) {
+  if (first < n) {
     for (int row = begin + line; row < end; row += 8) {
       float g[VEC];
       seq::unpack<T, VEC>(
-          *reinterpret_cast<const V*>(grad + row * grad_stride + c), g);
+          *reinterpret_cast<const V*>(grad + row * grad_stride + at.c), g);
       if (activation != SNN_HIP_ACTIVATION_NONE) {
-        const long at = static_cast<long>(row) * n + c;
+        const long place = static_cast<long>(row) * n + at.c;
         float v[VEC];
-        seq::unpack<T, VEC>(*reinterpret_cast<const V*>(z + at), v);
+        seq::unpack<T, VEC>(*reinterpret_cast<const V*>(z + place), v);
 #pragma unroll
         for (int i = 0; i < VEC; ++i)
           g[i] *= epi::activation_slope(v[i], activation);
+        // (two lanes write the same values where they overlap)
         if (dz != nullptr)
-          *reinterpret_cast<V*>(dz + at) = seq::pack<T, VEC>(g);
+          *reinterpret_cast<V*>(dz + place) = seq::pack<T, VEC>(g);
       }
 #pragma unroll
       for (int i = 0; i < VEC; ++i) sum[i] += g[i];
@@ -55,7 +57,8 @@ __global__ void __launch_bounds__(256)
   }
   if (sums == nullptr) return;
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) part[line][lane * VEC + i] = sum[i];
+  for (int i = 0; i < VEC; ++i)
+    if (first < n && i >= at.skip) part[line][at.c + i - blockIdx.x * 32 * VEC] = sum[i];
   __syncthreads();
   for (int i = threadIdx.x; i < 32 * VEC; i += 256) {
     const int col = blockIdx.x * 32 * VEC + i;
@@ -261,13 +264,10 @@ int backward(int dtype, const void* grad, const void* lhs, const void* rhs,
   const long grad_stride = or_else(p.output_stride, p.n);
   if (dz != nullptr || sums != nullptr) {
     constexpr int VEC = 16 / sizeof(T);
-    const bool wide =
-        p.n % VEC == 0 &&
-        seq::rows_aligned(static_cast<const T*>(grad), grad_stride, 16) &&
-        (!act || seq::aligned(static_cast<const T*>(z), 16));
     const int s =
-        wide ? launch_activation_grad<T, VEC>(p, grad, z, dz, sums, stream)
-             : launch_activation_grad<T, 1>(p, grad, z, dz, sums, stream);
+        p.n >= VEC
+            ? launch_activation_grad<T, VEC>(p, grad, z, dz, sums, stream)
+            : launch_activation_grad<T, 1>(p, grad, z, dz, sums, stream);
     if (s != SNN_HIP_OK) return s;
   }
   if (sums != nullptr) {

@@ -107,9 +107,10 @@ __device__ __forceinline__ void row_sums(float (&v)[N], float* lds, int* turn) {
   }
 }
 
-// PT values of a row per lane, as PT / VEC accesses: access j of lane l holds
-// the channels (j * lanes + l) * VEC ... + VEC - 1.  Beyond the row's end the
-// values are zero and nothing is stored.
+// PT values of a row per lane, as PT / VEC accesses: access j of lane l is for
+// the channels (j * lanes + l) * VEC ... + VEC - 1 and begins in front of them
+// where the row ends before (see Group).  Values that are another lane's or behind
+// the row's end are zero and are not stored.
 template <typename T, int VEC, int PT, int WAVES>
 struct Slice {
   static constexpr int kLanes = 64 * WAVES;
@@ -119,8 +120,16 @@ struct Slice {
     return WAVES == 1 ? static_cast<int>(threadIdx.x & 63)
                       : static_cast<int>(threadIdx.x);
   }
-  static __device__ __forceinline__ int channel(int j) {
+  static __device__ __forceinline__ int first(int j) {
     return (j * kLanes + lane()) * VEC;
+  }
+  // the channel of value i
+  static __device__ __forceinline__ int channel(int i, int channels) {
+    return min(first(i / VEC), channels - VEC) + i % VEC;
+  }
+  static __device__ __forceinline__ bool inside(int i, int channels) {
+    const int c = first(i / VEC);
+    return c < channels && min(c, channels - VEC) + i % VEC >= c;
   }
   static __device__ __forceinline__ void load(const void* row, int channels,
                                               float (&out)[PT]) {
@@ -128,32 +137,38 @@ struct Slice {
 #pragma unroll
     for (int j = 0; j < PT / VEC; ++j) {
       raw[j] = V{};
-      if (channel(j) < channels)
+      if (first(j) < channels)
         raw[j] = *reinterpret_cast<const V*>(static_cast<const T*>(row) +
-                                             channel(j));
+                                             min(first(j), channels - VEC));
     }
 #pragma unroll
     for (int j = 0; j < PT / VEC; ++j) {
       float part[VEC];
       seq::unpack<T, VEC>(raw[j], part);
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) out[j * VEC + k] = part[k];
+      for (int k = 0; k < VEC; ++k) {
+        const int i = j * VEC + k;
+        out[i] = VEC == 1 || inside(i, channels) ? part[k] : 0.f;
+      }
     }
   }
   static __device__ __forceinline__ void store(void* row, int channels,
                                                const float (&in)[PT]) {
 #pragma unroll
     for (int j = 0; j < PT / VEC; ++j) {
-      float part[VEC];
+      T* const at = static_cast<T*>(row) + first(j);
+      const int skip = first(j) + VEC - channels;  // above zero at the row's end
+      if (skip <= 0) {
+        float part[VEC];
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) part[k] = in[j * VEC + k];
-      if (channel(j) < channels)
-        *reinterpret_cast<V*>(static_cast<T*>(row) + channel(j)) =
-            seq::pack<T, VEC>(part);
+        for (int k = 0; k < VEC; ++k) part[k] = in[j * VEC + k];
+        *reinterpret_cast<V*>(at) = seq::pack<T, VEC>(part);
+      } else {
+#pragma unroll
+        for (int k = 1; k < VEC; ++k)
+          if (k >= skip) at[k - skip] = static_cast<T>(in[j * VEC + k]);
+      }
     }
-  }
-  static __device__ __forceinline__ bool inside(int i, int channels) {
-    return channel(i / VEC) < channels;  // (channels is a multiple of VEC)
   }
 };
 

@@ -132,18 +132,15 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES)
   }
 }
 
-template <typename T, int VEC>
-int launch_residual_norm(const Rows& r, hipStream_t stream) {
-  return norm::by_channels(r.channels, [&](auto waves, auto values) {
-    constexpr int WAVES = decltype(waves)::value, PT = decltype(values)::value;
-    const unsigned groups = static_cast<unsigned>(
-        WAVES == 1 ? (static_cast<long>(r.rows) + 3) / 4 : r.rows);
-    KernelTimer timer(stream);
-    hipLaunchKernelGGL((residual_norm_kernel<T, VEC, PT, WAVES>), dim3(groups),
-                       dim3(WAVES == 1 ? 256 : 64 * WAVES), 0, stream, r);
-    SNN_HIP_CHECK_LAUNCH();
-    return static_cast<int>(SNN_HIP_OK);
-  });
+template <typename T, int VEC, int PT, int WAVES>
+int launch_as(const Rows& r, hipStream_t stream) {
+  const unsigned groups = static_cast<unsigned>(
+      WAVES == 1 ? (static_cast<long>(r.rows) + 3) / 4 : r.rows);
+  KernelTimer timer(stream);
+  hipLaunchKernelGGL((residual_norm_kernel<T, VEC, PT, WAVES>), dim3(groups),
+                     dim3(WAVES == 1 ? 256 : 64 * WAVES), 0, stream, r);
+  SNN_HIP_CHECK_LAUNCH();
+  return SNN_HIP_OK;
 }
 
 template <typename T>
@@ -157,18 +154,12 @@ int residual_norm(const snn_hip_residual_norm_tensors* tensors,
   SNN_REQUIRE(t.normed == nullptr || params->pre_norm != SNN_HIP_NORM_NONE);
   const Rows r = norm::rows_of(t, *params);
   constexpr int VEC = 16 / sizeof(T);
-  auto fits = [&](const void* p, long stride) {
-    return p == nullptr ||
-           seq::rows_aligned(static_cast<const T*>(p), stride, 16);
-  };
-  const bool wide =
-      r.channels % VEC == 0 && fits(t.x, r.x_stride) &&
-      fits(t.gate, r.gate_stride) && fits(t.residual, r.channels) &&
-      fits(t.scale, 0) && fits(t.post_weight, 0) && fits(t.post_bias, 0) &&
-      fits(t.pre_weight, 0) && fits(t.pre_bias, 0) &&
-      fits(t.sum, r.channels) && fits(t.normed, r.channels);
-  return wide ? launch_residual_norm<T, VEC>(r, as_stream(stream))
-              : launch_residual_norm<T, 1>(r, as_stream(stream));
+  if (r.channels < VEC)
+    return launch_as<T, 1, 8, 1>(r, as_stream(stream));
+  return norm::by_channels(r.channels, [&](auto waves, auto values) {
+    return launch_as<T, VEC, decltype(values)::value, decltype(waves)::value>(
+        r, as_stream(stream));
+  });
 }
 
 }  // namespace

@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES)
   auto store_floats = [&](float* to, const float (&v)[PT]) {
 #pragma unroll
     for (int i = 0; i < PT; ++i)
-      if (S::inside(i, channels)) to[S::channel(i / VEC) + i % VEC] = v[i];
+      if (S::inside(i, channels)) to[S::channel(i, channels)] = v[i];
   };
 
   for (int run = blockIdx.x; run < d.runs; run += d.groups) {
@@ -262,38 +262,35 @@ size_t gate_floats(const snn_hip_residual_norm_params& p, const Grad& d) {
              : 0;
 }
 
-template <typename T, int VEC>
-int launch_grad(const Rows& r, const Grad& d, hipStream_t stream) {
-  return norm::by_channels(r.channels, [&](auto waves, auto values) {
-    constexpr int WAVES = decltype(waves)::value, PT = decltype(values)::value;
-    KernelTimer timer(stream);
-    hipLaunchKernelGGL((residual_norm_grad_kernel<T, VEC, PT, WAVES>),
-                       dim3(static_cast<unsigned>(d.groups)),
-                       dim3(WAVES == 1 ? 256 : 64 * WAVES), 0, stream, r, d);
+template <typename T, int VEC, int PT, int WAVES>
+int launch_as(const Rows& r, const Grad& d, hipStream_t stream) {
+  KernelTimer timer(stream);
+  hipLaunchKernelGGL((residual_norm_grad_kernel<T, VEC, PT, WAVES>),
+                     dim3(static_cast<unsigned>(d.groups)),
+                     dim3(WAVES == 1 ? 256 : 64 * WAVES), 0, stream, r, d);
+  SNN_HIP_CHECK_LAUNCH();
+  const unsigned columns = static_cast<unsigned>(ceil_div(r.channels, 64));
+  if (d.sums != nullptr) {
+    const seq::SumOutputs outputs = {{d.g.grad_scale, d.g.grad_post_weight,
+                                 d.g.grad_post_bias, d.g.grad_pre_weight,
+                                 d.g.grad_pre_bias}};
+    hipLaunchKernelGGL(seq::add_rows_kernel<T>, dim3(columns, kSums), dim3(1024),
+                       0, stream, d.sums, outputs, static_cast<T*>(nullptr),
+                       r.channels, d.groups,
+                       static_cast<long>(kSums) * r.channels,
+                       static_cast<long>(r.channels));
     SNN_HIP_CHECK_LAUNCH();
-    const unsigned columns = static_cast<unsigned>(ceil_div(r.channels, 64));
-    if (d.sums != nullptr) {
-      const seq::SumOutputs outputs = {{d.g.grad_scale, d.g.grad_post_weight,
-                                   d.g.grad_post_bias, d.g.grad_pre_weight,
-                                   d.g.grad_pre_bias}};
-      hipLaunchKernelGGL(seq::add_rows_kernel<T>, dim3(columns, kSums), dim3(1024),
-                         0, stream, d.sums, outputs, static_cast<T*>(nullptr),
-                         r.channels, d.groups,
-                         static_cast<long>(kSums) * r.channels,
-                         static_cast<long>(r.channels));
-      SNN_HIP_CHECK_LAUNCH();
-    }
-    if (d.gate_sums != nullptr) {
-      hipLaunchKernelGGL(
-          seq::add_rows_kernel<T>,
-          dim3(columns, static_cast<unsigned>(d.runs / d.per_gate)), dim3(1024),
-          0, stream, d.gate_sums, seq::SumOutputs{}, static_cast<T*>(d.g.grad_gate),
-          r.channels, d.per_gate, static_cast<long>(r.channels),
-          static_cast<long>(d.per_gate) * r.channels);
-      SNN_HIP_CHECK_LAUNCH();
-    }
-    return static_cast<int>(SNN_HIP_OK);
-  });
+  }
+  if (d.gate_sums != nullptr) {
+    hipLaunchKernelGGL(
+        seq::add_rows_kernel<T>,
+        dim3(columns, static_cast<unsigned>(d.runs / d.per_gate)), dim3(1024),
+        0, stream, d.gate_sums, seq::SumOutputs{}, static_cast<T*>(d.g.grad_gate),
+        r.channels, d.per_gate, static_cast<long>(r.channels),
+        static_cast<long>(d.per_gate) * r.channels);
+    SNN_HIP_CHECK_LAUNCH();
+  }
+  return SNN_HIP_OK;
 }
 
 template <typename T>
@@ -341,19 +338,11 @@ int residual_norm_grad(const snn_hip_residual_norm_tensors* tensors,
   if (d.runs / d.per_gate > 65535 && d.gate_sums != nullptr)
     return SNN_HIP_INDEX_EXCEEDED;  // (the grid of the gate's sums)
   constexpr int VEC = 16 / sizeof(T);
-  auto fits = [&](const void* p, long stride) {
-    return p == nullptr ||
-           seq::rows_aligned(static_cast<const T*>(p), stride, 16);
-  };
-  const bool wide =
-      r.channels % VEC == 0 && fits(t.x, r.x_stride) &&
-      fits(t.gate, r.gate_stride) && fits(t.scale, 0) &&
-      fits(t.post_weight, 0) && fits(t.post_bias, 0) && fits(t.pre_weight, 0) &&
-      fits(t.sum, r.channels) && fits(g.grad_sum, r.channels) &&
-      fits(g.grad_normed, r.channels) && fits(g.grad_x, r.channels) &&
-      fits(g.grad_residual, r.channels) && fits(g.grad_gate, r.channels);
-  return wide ? launch_grad<T, VEC>(r, d, as_stream(stream))
-              : launch_grad<T, 1>(r, d, as_stream(stream));
+  if (r.channels < VEC) return launch_as<T, 1, 8, 1>(r, d, as_stream(stream));
+  return norm::by_channels(r.channels, [&](auto waves, auto values) {
+    return launch_as<T, VEC, decltype(values)::value, decltype(waves)::value>(
+        r, d, as_stream(stream));
+  });
 }
 
 }  // namespace

@@ -12,15 +12,26 @@
 namespace snn {
 namespace seq {
 
-// VEC values of T as one access of VEC * sizeof(T) bytes, at an address that
-// is a multiple of that.
+// VEC values of T as one access of VEC * sizeof(T) bytes at any address: the
+// memory takes 16-byte accesses wherever a value may start, so that rows of any
+// length and stride are read and written alike.
 template <typename T, int VEC>
 struct Pack {
-  typedef T type __attribute__((ext_vector_type(VEC)));
+  typedef T type __attribute__((ext_vector_type(VEC), aligned(sizeof(T))));
 };
 template <typename T>
 struct Pack<T, 1> {
   typedef T type;
+};
+
+// Where a lane's VEC neighbouring channels begin: at `c`, or as far in front of
+// it as the row's end asks for; `skip` of them are then the lane's before it and
+// are neither summed nor stored twice.  (Rows of VEC channels at least.)
+template <int VEC>
+struct Group {
+  int c, skip;
+  __device__ __forceinline__ Group(int first, int channels)
+      : c(min(first, channels - VEC)), skip(first - c) {}
 };
 
 template <typename T, int VEC>
@@ -57,6 +68,13 @@ __device__ __forceinline__ void sigmoid(float z, float* s, float* rest) {
   const float small = e * large;
   *s = z >= 0.f ? large : small;
   *rest = z >= 0.f ? small : large;
+}
+
+// sigmoid(z) where the rest is not needed: an exponential that overflows gives
+// the zero that it stands for.
+template <typename T>
+__device__ __forceinline__ float sigmoid_alone(float z) {
+  return __builtin_amdgcn_rcpf(1.f + (sizeof(T) == 2 ? __expf(-z) : expf(-z)));
 }
 
 __device__ __forceinline__ float wave_sum(float v) {
@@ -102,12 +120,6 @@ __global__ void __launch_bounds__(1024)
   out[c] = static_cast<T>(s);
 }
 
-// Do rows of `stride` elements at p start at multiples of `bytes`?
-template <typename T>
-inline bool rows_aligned(const T* p, long stride, unsigned bytes) {
-  return (reinterpret_cast<uintptr_t>(p) % bytes) == 0 &&
-         (static_cast<size_t>(stride) * sizeof(T)) % bytes == 0;
-}
 template <typename T>
 inline bool aligned(const T* p, unsigned bytes) {
   return (reinterpret_cast<uintptr_t>(p) % bytes) == 0;
