@@ -61,26 +61,6 @@ inline int check_operands(const snn_hip_residual_norm_tensors* t,
   return SNN_HIP_OK;
 }
 
-// The gate's factor and its derivative.
-template <typename T>
-__device__ __forceinline__ void gate_of(int kind, float g, float* value,
-                                        float* slope) {
-  if (kind == SNN_HIP_GATE_VALUE) {
-    *value = g;
-    *slope = 1.f;
-    return;
-  }
-  float s, rest;
-  seq::sigmoid<T>(g, &s, &rest);
-  if (kind == SNN_HIP_GATE_SIGMOID) {
-    *value = s;
-    *slope = s * rest;
-  } else {
-    *value = g * s;
-    *slope = s + g * s * rest;
-  }
-}
-
 // Sums over the lanes that share a row: a wave, or all waves of the work-group
 // through LDS.  Two slots in turn, so that one barrier a sum is enough: a wave
 // is past the reads of a slot when it has passed the next sum's barrier.
@@ -110,8 +90,9 @@ __device__ __forceinline__ void row_sums(float (&v)[N], float* lds, int* turn) {
 // PT values of a row per lane, as PT / VEC accesses: access j of lane l is for
 // the channels (j * lanes + l) * VEC ... + VEC - 1 and begins in front of them
 // where the row ends before (see Group).  Values that are another lane's or behind
-// the row's end are zero and are not stored.
-template <typename T, int VEC, int PT, int WAVES>
+// the row's end are zero and are not stored.  WHOLE: rows are a multiple of VEC,
+// so that an access is inside as a whole or not at all.
+template <typename T, int VEC, int PT, int WAVES, bool WHOLE>
 struct Slice {
   static constexpr int kLanes = 64 * WAVES;
   typedef typename seq::Pack<T, VEC>::type V;
@@ -124,33 +105,53 @@ struct Slice {
     return (j * kLanes + lane()) * VEC;
   }
   // the channel of value i
+  static __device__ __forceinline__ int start(int j, int channels) {
+    return WHOLE ? first(j) : min(first(j), channels - VEC);
+  }
   static __device__ __forceinline__ int channel(int i, int channels) {
-    return min(first(i / VEC), channels - VEC) + i % VEC;
+    return start(i / VEC, channels) + i % VEC;
   }
   static __device__ __forceinline__ bool inside(int i, int channels) {
     const int c = first(i / VEC);
-    return c < channels && min(c, channels - VEC) + i % VEC >= c;
+    return c < channels && (WHOLE || start(i / VEC, channels) + i % VEC >= c);
   }
-  static __device__ __forceinline__ void load(const void* row, int channels,
-                                              float (&out)[PT]) {
-    V raw[PT / VEC];
+  static constexpr int kAccesses = PT / VEC;
+  // As they are in memory, which takes fewer registers; `absent` where there is
+  // no row.
+  static __device__ __forceinline__ void fetch(const void* row, int channels,
+                                               V (&raw)[kAccesses],
+                                               float absent = 0.f) {
 #pragma unroll
-    for (int j = 0; j < PT / VEC; ++j) {
-      raw[j] = V{};
-      if (first(j) < channels)
+    for (int j = 0; j < kAccesses; ++j) {
+      float part[VEC];
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) part[k] = absent;
+      raw[j] = seq::pack<T, VEC>(part);
+      if (row != nullptr && first(j) < channels)
         raw[j] = *reinterpret_cast<const V*>(static_cast<const T*>(row) +
-                                             min(first(j), channels - VEC));
+                                             start(j, channels));
     }
+  }
+  static __device__ __forceinline__ void expand(const V (&raw)[kAccesses],
+                                                int channels,
+                                                float (&out)[PT]) {
 #pragma unroll
-    for (int j = 0; j < PT / VEC; ++j) {
+    for (int j = 0; j < kAccesses; ++j) {
       float part[VEC];
       seq::unpack<T, VEC>(raw[j], part);
 #pragma unroll
       for (int k = 0; k < VEC; ++k) {
         const int i = j * VEC + k;
-        out[i] = VEC == 1 || inside(i, channels) ? part[k] : 0.f;
+        // (an access that is outside has not been made)
+        out[i] = WHOLE || inside(i, channels) ? part[k] : 0.f;
       }
     }
+  }
+  static __device__ __forceinline__ void load(const void* row, int channels,
+                                              float (&out)[PT]) {
+    V raw[kAccesses];
+    fetch(row, channels, raw);
+    expand(raw, channels, out);
   }
   static __device__ __forceinline__ void store(void* row, int channels,
                                                const float (&in)[PT]) {
@@ -158,12 +159,12 @@ struct Slice {
     for (int j = 0; j < PT / VEC; ++j) {
       T* const at = static_cast<T*>(row) + first(j);
       const int skip = first(j) + VEC - channels;  // above zero at the row's end
-      if (skip <= 0) {
+      if (WHOLE ? first(j) < channels : skip <= 0) {
         float part[VEC];
 #pragma unroll
         for (int k = 0; k < VEC; ++k) part[k] = in[j * VEC + k];
         *reinterpret_cast<V*>(at) = seq::pack<T, VEC>(part);
-      } else {
+      } else if (!WHOLE) {
 #pragma unroll
         for (int k = 1; k < VEC; ++k)
           if (k >= skip) at[k - skip] = static_cast<T>(in[j * VEC + k]);
@@ -172,10 +173,9 @@ struct Slice {
   }
 };
 
-// Calls `go` with the waves that share a row: at most PT = 8 values per lane up
-// to 8192 channels, 16 beyond.
+// At most PT = 8 values per lane up to 8192 channels, 16 beyond.
 template <typename Go>
-int by_channels(int channels, Go go) {
+int by_length(int channels, Go go) {
   using std::integral_constant;
   if (channels <= 512)
     return go(integral_constant<int, 1>(), integral_constant<int, 8>());
@@ -188,6 +188,19 @@ int by_channels(int channels, Go go) {
   if (channels <= 8192)
     return go(integral_constant<int, 16>(), integral_constant<int, 8>());
   return go(integral_constant<int, 16>(), integral_constant<int, 16>());
+}
+
+// Calls `go` with the waves that share a row, the values per lane, and whether
+// rows are a multiple of VEC.
+template <int VEC, typename Go>
+int by_channels(int channels, Go go) {
+  return channels % VEC == 0
+             ? by_length(channels, [&](auto waves, auto values) {
+                 return go(waves, values, std::true_type());
+               })
+             : by_length(channels, [&](auto waves, auto values) {
+                 return go(waves, values, std::false_type());
+               });
 }
 
 }  // namespace norm

@@ -59,10 +59,10 @@ __device__ __forceinline__ void shifted(float (&v)[PT], const float (&b)[PT]) {
   for (int i = 0; i < PT; ++i) v[i] += b[i];
 }
 
-template <typename T, int VEC, int PT, int WAVES>
+template <typename T, int VEC, int PT, int WAVES, bool WHOLE>
 __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES)
     residual_norm_kernel(Rows r) {
-  typedef norm::Slice<T, VEC, PT, WAVES> S;
+  typedef norm::Slice<T, VEC, PT, WAVES, WHOLE> S;
   __shared__ float lds[WAVES == 1 ? 1 : 4 * WAVES];
   int turn = 0;
   const long row = WAVES == 1
@@ -79,10 +79,11 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES)
   float gate[PT];
   if (r.gate != SNN_HIP_GATE_NONE) {
     S::load(tensor(r.t.gate, row / r.gate_rows * r.gate_stride), channels, gate);
+    if (r.gate != SNN_HIP_GATE_VALUE) {
+      const bool silu = r.gate == SNN_HIP_GATE_SILU;
 #pragma unroll
-    for (int i = 0; i < PT; ++i) {
-      float slope;
-      norm::gate_of<T>(r.gate, gate[i], &gate[i], &slope);
+      for (int i = 0; i < PT; ++i)
+        gate[i] = (silu ? gate[i] : 1.f) * seq::sigmoid_alone<T>(gate[i]);
     }
   }
   float residual[PT];
@@ -132,12 +133,12 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES)
   }
 }
 
-template <typename T, int VEC, int PT, int WAVES>
+template <typename T, int VEC, int PT, int WAVES, bool WHOLE>
 int launch_as(const Rows& r, hipStream_t stream) {
   const unsigned groups = static_cast<unsigned>(
       WAVES == 1 ? (static_cast<long>(r.rows) + 3) / 4 : r.rows);
   KernelTimer timer(stream);
-  hipLaunchKernelGGL((residual_norm_kernel<T, VEC, PT, WAVES>), dim3(groups),
+  hipLaunchKernelGGL((residual_norm_kernel<T, VEC, PT, WAVES, WHOLE>), dim3(groups),
                      dim3(WAVES == 1 ? 256 : 64 * WAVES), 0, stream, r);
   SNN_HIP_CHECK_LAUNCH();
   return SNN_HIP_OK;
@@ -155,11 +156,13 @@ int residual_norm(const snn_hip_residual_norm_tensors* tensors,
   const Rows r = norm::rows_of(t, *params);
   constexpr int VEC = 16 / sizeof(T);
   if (r.channels < VEC)
-    return launch_as<T, 1, 8, 1>(r, as_stream(stream));
-  return norm::by_channels(r.channels, [&](auto waves, auto values) {
-    return launch_as<T, VEC, decltype(values)::value, decltype(waves)::value>(
-        r, as_stream(stream));
-  });
+    return launch_as<T, 1, 8, 1, true>(r, as_stream(stream));
+  return norm::by_channels<VEC>(
+      r.channels, [&](auto waves, auto values, auto whole) {
+        return launch_as<T, VEC, decltype(values)::value,
+                         decltype(waves)::value, decltype(whole)::value>(
+            r, as_stream(stream));
+      });
 }
 
 }  // namespace

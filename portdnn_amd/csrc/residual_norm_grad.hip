@@ -15,7 +15,8 @@
 // Bound by memory: as in the forward kernel rows stay in registers between
 // their row sums, so every operand is read once.  Work-groups walk runs of rows
 // and keep the sums over rows in registers, each lane for its channels; a second
-// launch adds the work-groups' sums in their order.
+// launch adds the work-groups' sums in their order.  A row's two sums are two
+// waits for all its waves, so the next row is on its way meanwhile.
 #include <algorithm>
 
 #include "residual_norm.h"
@@ -25,8 +26,9 @@ namespace snn {
 namespace {
 
 using norm::Rows;
-
-enum { kScale, kPostWeight, kPostBias, kPreWeight, kPreBias, kSums };
+enum { kScale, kPostWeight, kPreWeight, kPostBias, kPreBias, kSums };
+// (... of which there are this many where no bias has a gradient)
+constexpr int kWeightSums = 3;
 static_assert(kSums == seq::kMaxSums, "outputs of a launch");
 
 struct Grad {
@@ -35,31 +37,45 @@ struct Grad {
   // each; without one the rows are one such range.  Work-group w takes the
   // runs w, w + groups, ...
   int gate_span, per_gate, run_rows, runs, groups;
-  float* sums;       // [groups][kSums][channels]
+  float* sums;       // [groups][kSums or kWeightSums][channels]
   float* gate_sums;  // [runs][channels] where per_gate > 1
 };
 
-template <typename T, int VEC, int PT, int WAVES>
+// BIASES: sums for the biases' gradients; SHARED: the gate is shared by rows.
+template <typename T, int VEC, int PT, int WAVES, bool WHOLE, bool BIASES,
+          bool SHARED>
 __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES)
+    __attribute__((amdgpu_waves_per_eu(WAVES == 16 ? 4 : 2)))
     residual_norm_grad_kernel(Rows r, Grad d) {
-  typedef norm::Slice<T, VEC, PT, WAVES> S;
+  typedef norm::Slice<T, VEC, PT, WAVES, WHOLE> S;
+  typedef typename S::V V;
+  constexpr int kOwn = BIASES ? kSums : kWeightSums;
   // (a wave that holds a row alone has its own sums; four of them are added
   // through LDS)
   constexpr int kTeams = WAVES == 1 ? 4 : 1;
+  // (sixteen waves have 128 registers each: none for a row on its way and the
+  // weights)
+  constexpr bool kLean = WAVES == 16;
   __shared__ float lds[WAVES == 1 ? 4 * 64 * PT : 4 * WAVES];
   int turn = 0;
   const int channels = r.channels;
   const float per = 1.f / static_cast<float>(channels);
   const int team = WAVES == 1 ? static_cast<int>(threadIdx.x >> 6) : 0;
-  const bool shared_gate = r.gate != SNN_HIP_GATE_NONE && r.gate_rows > 1;
-  auto tensor = [&](const void* p, long offset) {
-    return static_cast<const void*>(static_cast<const T*>(p) + offset);
-  };
-  float sums[kSums][PT], gate_sum[PT];
+  const bool pre = d.g.grad_normed != nullptr;
+  float sums[kOwn][PT], gate_sum[SHARED ? PT : 1];
 #pragma unroll
-  for (int s = 0; s < kSums; ++s)
+  for (int s = 0; s < kOwn; ++s)
 #pragma unroll
     for (int i = 0; i < PT; ++i) sums[s][i] = 0.f;
+  V pre_weight[S::kAccesses], post_weight[S::kAccesses],
+      post_bias[S::kAccesses], scale[S::kAccesses];
+  auto fetch_weights = [&]() {
+    S::fetch(r.t.pre_weight, channels, pre_weight, 1.f);
+    S::fetch(r.t.post_weight, channels, post_weight, 1.f);
+    S::fetch(r.t.post_bias, channels, post_bias);
+    S::fetch(r.t.scale, channels, scale, 1.f);
+  };
+  if constexpr (!kLean) fetch_weights();
 
   // The teams' sums together, in the first team's registers.
   auto gather = [&](float (&v)[PT]) {
@@ -82,6 +98,32 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES)
       if (S::inside(i, channels)) to[S::channel(i, channels)] = v[i];
   };
 
+  // A row's operands as they come from memory.
+  V next_d[S::kAccesses], next_u[S::kAccesses], next_y[S::kAccesses],
+      next_x[S::kAccesses], next_g[S::kAccesses];
+  float next_stats[4] = {0.f, 0.f, 0.f, 0.f};
+  auto fetch_row = [&](long row) {
+    auto of = [&](const void* p, long stride) {
+      return p == nullptr ? nullptr
+                          : static_cast<const void*>(static_cast<const T*>(p) +
+                                                     row * stride);
+    };
+    S::fetch(of(r.t.x, r.x_stride), channels, next_x);
+    if (pre) {
+      S::fetch(of(d.g.grad_normed, channels), channels, next_u);
+      S::fetch(of(r.t.sum, channels), channels, next_y);
+    }
+    S::fetch(of(d.g.grad_sum, channels), channels, next_d);
+    if (r.gate != SNN_HIP_GATE_NONE)
+      S::fetch(static_cast<const T*>(r.t.gate) +
+                   static_cast<int>(row) / r.gate_rows * r.gate_stride,
+               channels, next_g);
+    if (r.t.stats != nullptr) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) next_stats[i] = r.t.stats[4 * row + i];
+    }
+  };
+
   for (int run = blockIdx.x; run < d.runs; run += d.groups) {
     const int gate_row = run / d.per_gate;
     const long first = static_cast<long>(gate_row) * d.gate_span +
@@ -89,43 +131,39 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES)
     const long last = min(min(first + d.run_rows,
                               (gate_row + 1l) * d.gate_span),
                           static_cast<long>(r.rows));
+    if constexpr (SHARED) {
 #pragma unroll
-    for (int i = 0; i < PT; ++i) gate_sum[i] = 0.f;
+      for (int i = 0; i < PT; ++i) gate_sum[i] = 0.f;
+    }
+    if (!kLean && first + team < last) fetch_row(first + team);
     for (long row = first + team; row < last; row += kTeams) {
       const long at = row * channels;
-      float mean0 = 0.f, rstd0 = 0.f, mean1 = 0.f, rstd1 = 0.f;
-      if (r.t.stats != nullptr) {
-        const float* const s = r.t.stats + 4 * row;
-        mean0 = s[0];
-        rstd0 = s[1];
-        mean1 = s[2];
-        rstd1 = s[3];
+      if constexpr (kLean) {
+        fetch_row(row);
+        fetch_weights();
       }
-      float dy[PT], w[PT];
-#pragma unroll
-      for (int i = 0; i < PT; ++i) dy[i] = 0.f;
-      if (d.g.grad_sum != nullptr)
-        S::load(tensor(d.g.grad_sum, at), channels, dy);
-      float xh[PT];
-      S::load(tensor(r.t.x, row * r.x_stride), channels, xh);
-      if (d.g.grad_normed != nullptr) {
-        float u[PT], yh[PT];
-        S::load(tensor(d.g.grad_normed, at), channels, u);
-        S::load(tensor(r.t.sum, at), channels, yh);
+      float dy[PT], xh[PT], u[PT], yh[PT], gate[PT];
+      S::expand(next_d, channels, dy);
+      S::expand(next_x, channels, xh);
+      if (pre) {
+        S::expand(next_u, channels, u);
+        S::expand(next_y, channels, yh);
+      }
+      if (r.gate != SNN_HIP_GATE_NONE) S::expand(next_g, channels, gate);
+      const float mean0 = next_stats[0], rstd0 = next_stats[1],
+                  mean1 = next_stats[2], rstd1 = next_stats[3];
+      if (!kLean && row + kTeams < last) fetch_row(row + kTeams);
+
+      float w[PT];
+      if (pre) {
+        S::expand(pre_weight, channels, w);
+        float m[2] = {0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < PT; ++i) {
           yh[i] = S::inside(i, channels) ? (yh[i] - mean1) * rstd1 : 0.f;
           sums[kPreWeight][i] += u[i] * yh[i];
-          sums[kPreBias][i] += u[i];
-        }
-        if (r.t.pre_weight != nullptr) {
-          S::load(r.t.pre_weight, channels, w);
-#pragma unroll
-          for (int i = 0; i < PT; ++i) u[i] *= w[i];
-        }
-        float m[2] = {0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < PT; ++i) {
+          if constexpr (BIASES) sums[kPreBias][i] += u[i];
+          u[i] *= w[i];
           m[0] += u[i] * yh[i];
           m[1] += u[i];
         }
@@ -141,61 +179,49 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES)
         S::store(static_cast<T*>(d.g.grad_residual) + at, channels, dy);
 
       // n, of which the gate and the scale have their gradients
-      float n[PT], gate[PT], slope[PT];
+      float n[PT], s[PT];
       if (r.post != SNN_HIP_NORM_NONE) {
 #pragma unroll
         for (int i = 0; i < PT; ++i)
           xh[i] = S::inside(i, channels) ? (xh[i] - mean0) * rstd0 : 0.f;
       }
+      S::expand(post_weight, channels, w);
+      S::expand(post_bias, channels, n);
+      S::expand(scale, channels, s);
 #pragma unroll
-      for (int i = 0; i < PT; ++i) n[i] = xh[i];
-      if (r.t.post_weight != nullptr) {
-        S::load(r.t.post_weight, channels, w);
-#pragma unroll
-        for (int i = 0; i < PT; ++i) n[i] *= w[i];
-      } else {
-#pragma unroll
-        for (int i = 0; i < PT; ++i) w[i] = 1.f;
-      }
-      if (r.t.post_bias != nullptr) {
-        float b[PT];
-        S::load(r.t.post_bias, channels, b);
-#pragma unroll
-        for (int i = 0; i < PT; ++i) n[i] += b[i];
-      }
-      float scale[PT];
-      if (r.t.scale != nullptr) {
-        S::load(r.t.scale, channels, scale);
-      } else {
-#pragma unroll
-        for (int i = 0; i < PT; ++i) scale[i] = 1.f;
-      }
+      for (int i = 0; i < PT; ++i) n[i] += xh[i] * w[i];
       if (r.gate != SNN_HIP_GATE_NONE) {
-        const long gate_at = static_cast<long>(row / r.gate_rows);
-        S::load(tensor(r.t.gate, gate_at * r.gate_stride), channels, gate);
-#pragma unroll
-        for (int i = 0; i < PT; ++i)
-          norm::gate_of<T>(r.gate, gate[i], &gate[i], &slope[i]);
         float dg[PT];
 #pragma unroll
-        for (int i = 0; i < PT; ++i) dg[i] = dy[i] * scale[i] * n[i] * slope[i];
-        if (shared_gate) {
+        for (int i = 0; i < PT; ++i) dg[i] = dy[i] * s[i] * n[i];
+        if (r.gate != SNN_HIP_GATE_VALUE) {
+          const bool silu = r.gate == SNN_HIP_GATE_SILU;
+#pragma unroll
+          for (int i = 0; i < PT; ++i) {
+            float sg, rest;
+            seq::sigmoid<T>(gate[i], &sg, &rest);
+            const float weight = silu ? gate[i] : 1.f;
+            dg[i] *= sg * ((silu ? 1.f : 0.f) + weight * rest);
+            gate[i] = weight * sg;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < PT; ++i) dy[i] *= gate[i];
+        if constexpr (SHARED) {
 #pragma unroll
           for (int i = 0; i < PT; ++i) gate_sum[i] += dg[i];
         } else if (d.g.grad_gate != nullptr) {
           S::store(static_cast<T*>(d.g.grad_gate) + at, channels, dg);
         }
-#pragma unroll
-        for (int i = 0; i < PT; ++i) dy[i] *= gate[i];
       }
       // dy is dy * gate from here on
       float m[2] = {0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < PT; ++i) {
         sums[kScale][i] += dy[i] * n[i];
-        dy[i] *= scale[i];
+        dy[i] *= s[i];
         sums[kPostWeight][i] += dy[i] * xh[i];
-        sums[kPostBias][i] += dy[i];
+        if constexpr (BIASES) sums[kPostBias][i] += dy[i];
         dy[i] *= w[i];
         m[0] += dy[i] * xh[i];
         m[1] += dy[i];
@@ -212,45 +238,54 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES)
         S::store(static_cast<T*>(d.g.grad_x) + at, channels, dy);
       }
     }
-    if (shared_gate && d.g.grad_gate != nullptr) {
-      gather(gate_sum);
-      if (team == 0) {
-        if (d.per_gate > 1)
-          store_floats(d.gate_sums + static_cast<long>(run) * channels,
-                       gate_sum);
-        else
-          S::store(static_cast<T*>(d.g.grad_gate) +
-                       static_cast<long>(gate_row) * channels,
-                   channels, gate_sum);
+    if constexpr (SHARED) {
+      if (d.g.grad_gate != nullptr) {
+        gather(gate_sum);
+        if (team == 0) {
+          if (d.per_gate > 1)
+            store_floats(d.gate_sums + static_cast<long>(run) * channels,
+                         gate_sum);
+          else
+            S::store(static_cast<T*>(d.g.grad_gate) +
+                         static_cast<long>(gate_row) * channels,
+                     channels, gate_sum);
+        }
       }
     }
   }
   if (d.sums == nullptr) return;
   float* const to =
-      d.sums + static_cast<long>(blockIdx.x) * kSums * channels;
+      d.sums + static_cast<long>(blockIdx.x) * kOwn * channels;
 #pragma unroll
-  for (int s = 0; s < kSums; ++s) {
+  for (int s = 0; s < kOwn; ++s) {
     gather(sums[s]);
     if (team == 0) store_floats(to + static_cast<long>(s) * channels, sums[s]);
   }
 }
 
-// Work-groups that walk the rows, and the runs they take.
-constexpr int kMaxGroups = 512;
-constexpr int kLeastRows = 8;  // of a run, so that its sums cost little
+// Work-groups that walk the rows, and the runs they take: eight waves a CU, which
+// leaves each the registers for its sums, the weights and the row on its way
+// (16384 x 2048 bfloat16: 120 us; twelve waves without a row on its way 130,
+// sixteen, whose registers do not fit, 383).
+constexpr int kMostWaves = 8 * 256;
+// Rows of a run at least, so that its sums cost little beside them; fewer where
+// there are few rows, which then wait for one another less (64 x 1024 fp32).
+inline int least_rows(int rows) { return std::min(8, std::max(1, rows / 256)); }
 
 void plan_runs(const snn_hip_residual_norm_params& p, Grad* d) {
   const bool shared = p.gate != SNN_HIP_GATE_NONE && p.gate_rows > 1;
   const int span = shared ? std::min(p.gate_rows, p.rows) : p.rows;
   const int gates = ceil_div(p.rows, span);
+  const int waves = p.channels <= 512 ? 4 : ceil_div(p.channels, 512);
+  const int groups = std::max(256, kMostWaves / waves);
   const int teams = p.channels <= 512 ? 4 : 1;
-  const int target = std::max(
-      kLeastRows * teams, ceil_div(p.rows, kMaxGroups));
+  const int target =
+      std::max(least_rows(p.rows) * teams, ceil_div(p.rows, groups));
   d->gate_span = span;
   d->per_gate = ceil_div(span, target);
   d->run_rows = ceil_div(span, d->per_gate);
   d->runs = gates * d->per_gate;
-  d->groups = std::min(d->runs, kMaxGroups);
+  d->groups = std::min(d->runs, groups);
 }
 
 size_t sum_floats(const snn_hip_residual_norm_params& p, const Grad& d) {
@@ -262,30 +297,44 @@ size_t gate_floats(const snn_hip_residual_norm_params& p, const Grad& d) {
              : 0;
 }
 
-template <typename T, int VEC, int PT, int WAVES>
+template <typename T, int VEC, int PT, int WAVES, bool WHOLE>
 int launch_as(const Rows& r, const Grad& d, hipStream_t stream) {
+  const bool biases =
+      d.g.grad_post_bias != nullptr || d.g.grad_pre_bias != nullptr;
+  const bool shared = r.gate != SNN_HIP_GATE_NONE && r.gate_rows > 1;
+  const auto kernel =
+      biases
+          ? (shared
+                 ? residual_norm_grad_kernel<T, VEC, PT, WAVES, WHOLE, true, true>
+                 : residual_norm_grad_kernel<T, VEC, PT, WAVES, WHOLE, true,
+                                             false>)
+          : (shared
+                 ? residual_norm_grad_kernel<T, VEC, PT, WAVES, WHOLE, false, true>
+                 : residual_norm_grad_kernel<T, VEC, PT, WAVES, WHOLE, false,
+                                             false>);
   KernelTimer timer(stream);
-  hipLaunchKernelGGL((residual_norm_grad_kernel<T, VEC, PT, WAVES>),
-                     dim3(static_cast<unsigned>(d.groups)),
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(d.groups)),
                      dim3(WAVES == 1 ? 256 : 64 * WAVES), 0, stream, r, d);
   SNN_HIP_CHECK_LAUNCH();
   const unsigned columns = static_cast<unsigned>(ceil_div(r.channels, 64));
   if (d.sums != nullptr) {
     const seq::SumOutputs outputs = {{d.g.grad_scale, d.g.grad_post_weight,
-                                 d.g.grad_post_bias, d.g.grad_pre_weight,
-                                 d.g.grad_pre_bias}};
-    hipLaunchKernelGGL(seq::add_rows_kernel<T>, dim3(columns, kSums), dim3(1024),
-                       0, stream, d.sums, outputs, static_cast<T*>(nullptr),
+                                      d.g.grad_pre_weight, d.g.grad_post_bias,
+                                      d.g.grad_pre_bias}};
+    const int own = biases ? static_cast<int>(kSums) : kWeightSums;
+    hipLaunchKernelGGL(seq::add_rows_kernel<T>,
+                       dim3(columns, static_cast<unsigned>(own)), dim3(1024), 0,
+                       stream, d.sums, outputs, static_cast<T*>(nullptr),
                        r.channels, d.groups,
-                       static_cast<long>(kSums) * r.channels,
+                       static_cast<long>(own) * r.channels,
                        static_cast<long>(r.channels));
     SNN_HIP_CHECK_LAUNCH();
   }
   if (d.gate_sums != nullptr) {
     hipLaunchKernelGGL(
         seq::add_rows_kernel<T>,
-        dim3(columns, static_cast<unsigned>(d.runs / d.per_gate)), dim3(1024),
-        0, stream, d.gate_sums, seq::SumOutputs{}, static_cast<T*>(d.g.grad_gate),
+        dim3(columns, static_cast<unsigned>(d.runs / d.per_gate)), dim3(1024), 0,
+        stream, d.gate_sums, seq::SumOutputs{}, static_cast<T*>(d.g.grad_gate),
         r.channels, d.per_gate, static_cast<long>(r.channels),
         static_cast<long>(d.per_gate) * r.channels);
     SNN_HIP_CHECK_LAUNCH();
@@ -338,11 +387,14 @@ int residual_norm_grad(const snn_hip_residual_norm_tensors* tensors,
   if (d.runs / d.per_gate > 65535 && d.gate_sums != nullptr)
     return SNN_HIP_INDEX_EXCEEDED;  // (the grid of the gate's sums)
   constexpr int VEC = 16 / sizeof(T);
-  if (r.channels < VEC) return launch_as<T, 1, 8, 1>(r, d, as_stream(stream));
-  return norm::by_channels(r.channels, [&](auto waves, auto values) {
-    return launch_as<T, VEC, decltype(values)::value, decltype(waves)::value>(
-        r, d, as_stream(stream));
-  });
+  if (r.channels < VEC)
+    return launch_as<T, 1, 8, 1, true>(r, d, as_stream(stream));
+  return norm::by_channels<VEC>(
+      r.channels, [&](auto waves, auto values, auto whole) {
+        return launch_as<T, VEC, decltype(values)::value,
+                         decltype(waves)::value, decltype(whole)::value>(
+            r, d, as_stream(stream));
+      });
 }
 
 }  // namespace
