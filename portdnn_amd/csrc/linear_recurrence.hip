@@ -4,25 +4,35 @@
 //   a_t = sigmoid(f_t),  b_t = w_t x_t,  w_t = sigmoid(i_t) or 1 - a_t
 //   h_t = a_t h_{t-1} + b_t
 //
-// Steps compose: a run of them is h -> A h + S with A = a_t ... a_s, and two
-// runs in turn are (A, S) then (A', S') = (A' A, A' S + S').  A lane owns a few
-// neighbouring channels and walks the steps of a piece of the sequence.  Where
-// the sequences and channels do not fill the GPU, a sequence is divided into
-// pieces: one launch finds every piece's (A, S), a second the state in front
-// of every piece, a third walks the pieces from there.  The gradients run the
-// other way: with D_t = a_t G_t, the gradient that step t hands to step t - 1,
+// and backwards, with D_t = a_t G_t the gradient that step t hands to step t - 1,
 //
 //   G_t = dh_t + D_{t+1}   D_t = a_t dh_t + a_t D_{t+1}
 //   dx_t = G_t w_t   df_t = G_t (h_{t-1} [- x_t]) a_t (1 - a_t)
 //   di_t = G_t x_t w_t (1 - w_t)
 //
-// All of it is bound by memory: a step is about ten operations on the values
-// that it reads and writes once (the inputs of the recurrence itself twice where
-// a sequence is divided).  States and pieces are fp32.
+// Bound by memory: a step is some twenty operations on values that are read and
+// written once.  A lane owns a few neighbouring channels and walks the steps.
+// Where sequences and channels do not fill the GPU with lanes, a sequence is
+// divided: steps compose, a run of them is h -> A h + S, and two runs in turn are
+// (A, S), (A', S') -> (A' A, A' S + S').  A work-group takes a piece of the
+// sequence, every wave a segment of it, which it holds in registers:
+//
+//   1  every wave finds (A, S) of its segment, the work-group's are composed;
+//   2  the piece's (A, S) is published for the pieces behind it;
+//   3  the state in front of the piece is found: the nearest piece before it whose
+//      state behind it is known already, and (A, S) of those between, in turn;
+//   4  the state behind the piece is published, and every wave walks its segment
+//      from the state in front of that.
+//
+// so that every operand is read once all the same.  Pieces are handed out by a
+// counter in their order: a work-group waits only for pieces whose work-groups
+// have begun before it, which therefore end.  The state behind a piece is A s + S
+// of the state in front of it wherever it is computed, so that results do not
+// depend on who waits for whom.  States and pieces are fp32.
 //
 // A reset leaves h_{t-1} out by selection and not by a factor of zero, so that
-// an infinite state does not survive it; steps behind a sequence's length are
-// not read (a = 1, b = 0).
+// an infinite state does not survive it; steps behind a sequence's length do not
+// count (a = 1, b = 0).
 #include <algorithm>
 
 #include "sequence.h"
@@ -37,16 +47,9 @@ using seq::sigmoid;
 using seq::sigmoid_alone;
 using seq::unpack;
 
-// Steps whose loads are in flight together: 8 forward; the gradients, with five
-// operands, keep more waves on a SIMD with 4 (4 x 4096 x 2048 binary16: 176 ->
-// 147 us).
-template <bool BACK>
-constexpr int kSteps = BACK ? 4 : 8;
-
 struct Recurrence {
   int batch, steps, channels;
   long stride, grad_stride;  // of x and the gates, of their gradients
-  int pieces, piece_steps;
   const void *x, *f, *i, *h, *dh;
   const unsigned char* resets;
   const int* lengths;
@@ -54,7 +57,12 @@ struct Recurrence {
   const float* first;    // the state (gradient) that the walk starts from
   float* last;           // ... and ends with
   void *out_h, *dx, *df, *di;
-  float *A, *S;  // [batch][pieces][channels]
+  // The divided walk: pieces, in the walk's order, of `segments` segments.
+  int segments, pieces;
+  unsigned* counter;          // of the pieces handed out
+  unsigned* flags;            // [batch x channel blocks][pieces]: see kNothing
+  unsigned long long* pairs;  // [as flags][64 VEC]: (A, S)
+  unsigned* states;           // [as flags][64 VEC]: behind the piece
 };
 
 template <typename T>
@@ -65,38 +73,8 @@ constexpr int kVec = sizeof(T) == 2 ? 4 : 2;
 __device__ __forceinline__ bool is_reset(float a) {
   return __float_as_uint(a) == 0x80000000u;
 }
-
-// What a wave needs of its place: sequence, piece, first channel of the lane.
-struct Place {
-  int b, piece, c, skip, begin, end, length;
-  bool on;
-};
-
-// With `turned` the last come first: the walk behind a launch over the same
-// pieces then begins with what that has read last and the caches still hold.
-template <int VEC>
-__device__ __forceinline__ Place place_of(const Recurrence& r, bool turned) {
-  Place p;
-  const int blocks = (r.channels + 64 * VEC - 1) / (64 * VEC);
-  const unsigned place = turned ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
-  const unsigned at = place * (blockDim.x / 64) + threadIdx.x / 64;
-  const unsigned row = at / blocks;
-  const int first =
-      static_cast<int>(at - row * blocks) * 64 * VEC + (threadIdx.x & 63) * VEC;
-  // (a row's last channels: see Group; what is before them is not stored)
-  const seq::Group<VEC> group(first, r.channels);
-  p.c = group.c;
-  p.skip = group.skip;
-  p.b = static_cast<int>(row / r.pieces);
-  p.piece = static_cast<int>(row - static_cast<unsigned>(p.b) * r.pieces);
-  p.on = p.b < r.batch && first < r.channels;
-  if (p.b >= r.batch) p.b = 0;
-  p.begin = p.piece * r.piece_steps;
-  p.end = min(r.steps, p.begin + r.piece_steps);
-  p.length = r.lengths == nullptr
-                 ? r.steps
-                 : max(0, min(r.steps, r.lengths[p.b]));
-  return p;
+__device__ __forceinline__ float composed(float a, float s, float state) {
+  return is_reset(a) ? s : a * state + s;
 }
 
 // Stores the lane's own of VEC values.
@@ -111,149 +89,47 @@ __device__ __forceinline__ void put(T* at, const float (&v)[VEC], int skip) {
   }
 }
 
-// (A, S) of a piece, forward: S behind the piece's steps from a zero state;
-// backward: the gradient in front of it from a zero gradient behind.
-template <typename T, int VEC, bool GATE, bool BACK>
-__global__ void __launch_bounds__(256)
-    recurrence_pieces_kernel(Recurrence r) {
-  typedef typename Pack<T, VEC>::type V;
-  constexpr int kGroup = kSteps<BACK>;
-  const Place p = place_of<VEC>(r, false);
-  if (!p.on) return;
-  const long row = static_cast<long>(p.b) * r.steps;
-  const T* const f = static_cast<const T*>(r.f) + row * r.stride + p.c;
-  const T* const x = static_cast<const T*>(r.x) + row * r.stride + p.c;
-  const T* const ig = GATE ? static_cast<const T*>(r.i) + row * r.stride + p.c
-                           : nullptr;
-  const T* const dh =
-      BACK ? static_cast<const T*>(r.dh) + row * r.channels + p.c : nullptr;
-  float A[VEC], S[VEC];
-#pragma unroll
-  for (int k = 0; k < VEC; ++k) {
-    A[k] = 1.f;
-    S[k] = 0.f;
-  }
-  const int end = min(p.end, p.length);
-  const int groups = (end - p.begin + kGroup - 1) / kGroup;
-  for (int g = 0; g < groups; ++g) {
-    V fv[kGroup], xv[kGroup], iv[kGroup];
-    unsigned char fresh[kGroup];
-    const int first = BACK ? p.begin + (groups - 1 - g) * kGroup
-                           : p.begin + g * kGroup;
-#pragma unroll
-    for (int u = 0; u < kGroup; ++u) {
-      const int t = min(first + u, end - 1);
-      fv[u] = *reinterpret_cast<const V*>(f + t * r.stride);
-      if (BACK) {
-        xv[u] = *reinterpret_cast<const V*>(dh + static_cast<long>(t) *
-                                                     r.channels);
-      } else {
-        xv[u] = *reinterpret_cast<const V*>(x + t * r.stride);
-        if (GATE) iv[u] = *reinterpret_cast<const V*>(ig + t * r.stride);
-      }
-      fresh[u] = r.resets == nullptr ? 0 : r.resets[row + t];
-    }
-#pragma unroll
-    for (int n = 0; n < kGroup; ++n) {
-      const int u = BACK ? kGroup - 1 - n : n;
-      if (first + u >= end) continue;
-      float fs[VEC], xs[VEC], is[VEC];
-      unpack<T, VEC>(fv[u], fs);
-      unpack<T, VEC>(xv[u], xs);
-      if (GATE && !BACK) unpack<T, VEC>(iv[u], is);
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) {
-        float a, w;
-        if (BACK || GATE)
-          a = sigmoid_alone<T>(fs[k]);
-        else
-          sigmoid<T>(fs[k], &a, &w);
-        if (BACK) {
-          S[k] = fresh[u] ? 0.f : a * (xs[k] + S[k]);
-          A[k] = fresh[u] ? -0.f : a * A[k];
-        } else {
-          if (GATE) w = sigmoid_alone<T>(is[k]);
-          S[k] = w * xs[k] + (fresh[u] ? 0.f : a * S[k]);
-          A[k] = fresh[u] ? -0.f : a * A[k];
-        }
-      }
-    }
-  }
-  const long at = (static_cast<long>(p.b) * r.pieces + p.piece) * r.channels +
-                  p.c;
-#pragma unroll
-  for (int k = 0; k < VEC; ++k) {
-    r.A[at + k] = A[k];
-    r.S[at + k] = S[k];
-  }
+__device__ __forceinline__ int length_of(const Recurrence& r, int b) {
+  return r.lengths == nullptr ? r.steps
+                              : max(0, min(r.steps, r.lengths[b]));
 }
 
-// The state in front of every piece, over S; `last` behind the last one.  A
-// work-group takes 64 channels of a sequence; each of its 16 waves composes a
-// run of the pieces, the runs' results are composed in turn by every wave up to
-// its own, and the wave walks its run from there.
+// ---- undivided ---------------------------------------------------------------
+
+// Steps whose loads are in flight together: 8 forward; the gradients, with five
+// operands, keep more waves on a SIMD with 4 (4 x 4096 x 2048 binary16: 176 ->
+// 147 us).
 template <bool BACK>
-__global__ void __launch_bounds__(1024)
-    recurrence_join_kernel(Recurrence r) {
-  constexpr int kRuns = 16;
-  __shared__ float run_a[kRuns][64], run_s[kRuns][64];
-  const int lane = threadIdx.x & 63, run = threadIdx.x >> 6;
-  const int blocks = (r.channels + 63) / 64;
-  const int b = blockIdx.x / blocks;
-  const int c = (blockIdx.x - b * blocks) * 64 + lane;
-  const bool on = c < r.channels;
-  const int each = (r.pieces + kRuns - 1) / kRuns;
-  const int begin = min(r.pieces, run * each), end = min(r.pieces, begin + each);
-  const long base = static_cast<long>(b) * r.pieces * r.channels + c;
-  auto at = [&](int n) {  // the n-th piece in the walk's order
-    return base + static_cast<long>(BACK ? r.pieces - 1 - n : n) * r.channels;
-  };
-  // (eight pieces' pairs are under way together)
-  constexpr int kBatch = 8;
-  auto walk = [&](auto step) {
-    for (int n = begin; n < end; n += kBatch) {
-      float a[kBatch], s[kBatch];
-#pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        const long where = at(min(n + u, end - 1));
-        a[u] = r.A[where];
-        s[u] = r.S[where];
-      }
-#pragma unroll
-      for (int u = 0; u < kBatch; ++u)
-        if (n + u < end) step(n + u, a[u], s[u]);
-    }
-  };
-  float A = 1.f, S = 0.f;
-  if (on)
-    walk([&](int, float a, float s) {
-      S = is_reset(a) ? s : a * S + s;
-      A = is_reset(a) ? a : A * a;
-    });
-  run_a[run][lane] = A;
-  run_s[run][lane] = S;
-  // (read in front of the barrier: `last` may be the same buffer)
-  const long state_at = static_cast<long>(b) * r.channels + c;
-  float state = !on || r.first == nullptr ? 0.f : r.first[state_at];
-  __syncthreads();
-  if (!on) return;
-  for (int q = 0; q < run; ++q) {
-    const float a = run_a[q][lane];
-    state = is_reset(a) ? run_s[q][lane] : a * state + run_s[q][lane];
-  }
-  walk([&](int n, float a, float s) {
-    r.S[at(n)] = state;
-    state = is_reset(a) ? s : a * state + s;
-  });
-  if (run == kRuns - 1 && r.last != nullptr) r.last[state_at] = state;
+constexpr int kSteps = BACK ? 4 : 8;
+
+// What a wave needs of its place: sequence and first channel of the lane.
+struct Place {
+  int b, c, skip;
+  bool on;
+};
+template <int VEC>
+__device__ __forceinline__ Place place_of(const Recurrence& r) {
+  Place p;
+  const int blocks = (r.channels + 64 * VEC - 1) / (64 * VEC);
+  const unsigned at = blockIdx.x * (blockDim.x / 64) + threadIdx.x / 64;
+  p.b = static_cast<int>(at / blocks);
+  const int first = static_cast<int>(at - static_cast<unsigned>(p.b) * blocks) *
+                        64 * VEC +
+                    (threadIdx.x & 63) * VEC;
+  // (a row's last channels: see Group; what is before them is not stored)
+  const seq::Group<VEC> group(first, r.channels);
+  p.c = group.c;
+  p.skip = group.skip;
+  p.on = p.b < r.batch && first < r.channels;
+  return p;
 }
 
-// The walk over a piece from the state in front of it.
+// The walk over a sequence.
 template <typename T, int VEC, bool GATE>
 __global__ void __launch_bounds__(256) recurrence_walk_kernel(Recurrence r) {
   typedef typename Pack<T, VEC>::type V;
   constexpr int kGroup = kSteps<false>;
-  const Place p = place_of<VEC>(r, r.pieces > 1);
+  const Place p = place_of<VEC>(r);
   if (!p.on) return;
   const long row = static_cast<long>(p.b) * r.steps;
   const T* const f = static_cast<const T*>(r.f) + row * r.stride + p.c;
@@ -262,15 +138,12 @@ __global__ void __launch_bounds__(256) recurrence_walk_kernel(Recurrence r) {
                            : nullptr;
   T* const h = static_cast<T*>(r.out_h) + row * r.channels + p.c;
   const long state_at = static_cast<long>(p.b) * r.channels + p.c;
-  const float* const from =
-      r.pieces > 1 ? r.S + (static_cast<long>(p.b) * r.pieces + p.piece) *
-                               r.channels + p.c
-                   : r.first == nullptr ? nullptr : r.first + state_at;
+  const float* const from = r.first == nullptr ? nullptr : r.first + state_at;
   float state[VEC];
 #pragma unroll
   for (int k = 0; k < VEC; ++k) state[k] = from == nullptr ? 0.f : from[k];
-  const int end = min(p.end, p.length);
-  for (int first = p.begin; first < end; first += kGroup) {
+  const int end = length_of(r, p.b);
+  for (int first = 0; first < end; first += kGroup) {
     V fv[kGroup], xv[kGroup], iv[kGroup];
     unsigned char fresh[kGroup];
 #pragma unroll
@@ -303,19 +176,18 @@ __global__ void __launch_bounds__(256) recurrence_walk_kernel(Recurrence r) {
     }
   }
   float zero[VEC] = {};
-  for (int t = max(p.begin, end); t < p.end; ++t)
+  for (int t = end; t < r.steps; ++t)
     put<T, VEC>(h + static_cast<long>(t) * r.channels, zero, p.skip);
-  if (r.pieces == 1 && r.last != nullptr)
+  if (r.last != nullptr)
     put<float, VEC>(r.last + state_at, state, p.skip);
 }
 
-// The gradients' walk over a piece, from its end, with the gradient that the
-// step behind it hands over.
+// The gradients' walk over a sequence, from its end.
 template <typename T, int VEC, bool GATE>
 __global__ void __launch_bounds__(256) recurrence_grad_kernel(Recurrence r) {
   typedef typename Pack<T, VEC>::type V;
   constexpr int kGroup = kSteps<true>;
-  const Place p = place_of<VEC>(r, r.pieces > 1);
+  const Place p = place_of<VEC>(r);
   if (!p.on) return;
   const long row = static_cast<long>(p.b) * r.steps;
   const T* const f = static_cast<const T*>(r.f) + row * r.stride + p.c;
@@ -329,25 +201,22 @@ __global__ void __launch_bounds__(256) recurrence_grad_kernel(Recurrence r) {
   T* const di =
       GATE ? static_cast<T*>(r.di) + row * r.grad_stride + p.c : nullptr;
   const long state_at = static_cast<long>(p.b) * r.channels + p.c;
-  const float* const from =
-      r.pieces > 1 ? r.S + (static_cast<long>(p.b) * r.pieces + p.piece) *
-                               r.channels + p.c
-                   : r.first == nullptr ? nullptr : r.first + state_at;
+  const float* const from = r.first == nullptr ? nullptr : r.first + state_at;
   float D[VEC];
 #pragma unroll
   for (int k = 0; k < VEC; ++k) D[k] = from == nullptr ? 0.f : from[k];
-  const int end = min(p.end, p.length);
+  const int end = length_of(r, p.b);
   const float zero[VEC] = {};
-  for (int t = max(p.begin, end); t < p.end; ++t) {
+  for (int t = end; t < r.steps; ++t) {
     put<T, VEC>(dx + t * r.grad_stride, zero, p.skip);
     put<T, VEC>(df + t * r.grad_stride, zero, p.skip);
     if (GATE) put<T, VEC>(di + t * r.grad_stride, zero, p.skip);
   }
-  const int groups = (end - p.begin + kGroup - 1) / kGroup;
+  const int groups = (end + kGroup - 1) / kGroup;
   for (int g = groups - 1; g >= 0; --g) {
     V fv[kGroup], xv[kGroup], iv[kGroup], hv[kGroup], dv[kGroup];
     unsigned char fresh[kGroup];
-    const int first = p.begin + g * kGroup;
+    const int first = g * kGroup;
 #pragma unroll
     for (int u = 0; u < kGroup; ++u) {
       const int t = min(first + u, end - 1);
@@ -397,57 +266,402 @@ __global__ void __launch_bounds__(256) recurrence_grad_kernel(Recurrence r) {
       if (GATE) put<T, VEC>(di + t * r.grad_stride, gi, p.skip);
     }
   }
-  if (r.pieces == 1 && r.last != nullptr)
+  if (r.last != nullptr)
     put<float, VEC>(r.last + state_at, D, p.skip);
 }
 
-// How many pieces a sequence is divided into: as many as give the GPU
-// kWantedWaves waves, of kLeastSteps steps at least so that a piece's fp32
-// pair costs little beside its steps.
-constexpr int kWantedWaves = 4096;
-constexpr int kLeastSteps = 32;
+// ---- divided -----------------------------------------------------------------
 
-template <typename T>
-void divide_steps(const snn_hip_linear_recurrence_params& p, int* pieces,
-                  int* piece_steps) {
-  const long waves =
-      static_cast<long>(p.batch) * ceil_div(p.channels, 64 * kVec<T>);
-  const long want = std::max(1l, kWantedWaves / waves);
-  const long most = std::max(1, p.steps / kLeastSteps);
-  const int n = static_cast<int>(std::min(want, most));
-  *piece_steps = ceil_div(ceil_div(p.steps, n), kSteps<false>) * kSteps<false>;
-  *pieces = ceil_div(p.steps, *piece_steps);
+// What the flag of a piece says: hints for those that wait, which take nothing
+// but words that have arrived.  Not arrived: all bits set, which no value is
+// published as.
+enum : unsigned { kNothing = 0, kPair = 1, kState = 2 };
+constexpr unsigned kNotYet = 0xFFFFFFFFu;
+
+__device__ __forceinline__ unsigned published(float v) {
+  const unsigned bits = __float_as_uint(v);
+  return bits == kNotYet ? 0x7FC00000u : bits;  // (another NaN)
+}
+// Work-groups on other XCDs see these accesses without their L2s in between.
+template <typename W>
+__device__ __forceinline__ void publish(W* at, W v) {
+  __hip_atomic_store(at, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <typename W>
+__device__ __forceinline__ W look(const W* at) {
+  return __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-size_t pair_floats(const snn_hip_linear_recurrence_params& p, int pieces) {
-  return pieces < 2 ? 0
-                    : size_t{2} * static_cast<size_t>(p.batch) * pieces *
-                          p.channels;
+// Sets the counter and the flags to zero, the words to "not arrived".
+__global__ void __launch_bounds__(256)
+    recurrence_clear_kernel(unsigned* zeros, size_t n_zeros,
+                            seq::Pack<unsigned, 4>::type* words,
+                            size_t n_words) {
+  const size_t i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i < n_zeros) zeros[i] = 0u;
+  if (i < n_words)
+    words[i] = seq::Pack<unsigned, 4>::type{kNotYet, kNotYet, kNotYet, kNotYet};
+}
+
+// The state in front of piece `piece` of a row of flags, by the wave that calls.
+template <int VEC>
+__device__ __forceinline__ void state_before(const Recurrence& r, long row,
+                                             int piece, float (&state)[VEC]) {
+  const int lane = threadIdx.x & 63;
+  const long base = row * r.pieces;
+  // The nearest of the 64 pieces before this one with a state, if all between
+  // have pairs: lane l looks at the piece l + 1 before.
+  int back;
+  for (;;) {
+    const int at = piece - 1 - lane;
+    const unsigned flag = at >= 0 ? look(r.flags + base + at) : kNothing;
+    const unsigned long long with_state = __ballot(flag == kState);
+    const unsigned long long with_pair = __ballot(flag != kNothing);
+    back = with_state == 0 ? 64 : __builtin_ctzll(with_state);
+    const unsigned long long between = (1ull << (back & 63)) - 1;
+    if (back < 64 && (with_pair & between) == between) break;
+    __builtin_amdgcn_s_sleep(1);
+  }
+  const long word = static_cast<long>(lane) * VEC;
+  const unsigned* const known =
+      r.states + (base + piece - 1 - back) * (64 * VEC) + word;
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) {
+    unsigned v;
+    while ((v = look(known + k)) == kNotYet) __builtin_amdgcn_s_sleep(1);
+    state[k] = __uint_as_float(v);
+  }
+  // (four pieces' pairs are under way together)
+  constexpr int kBatch = 4;
+  for (int n = back; n > 0; n -= kBatch) {
+    unsigned long long pair[kBatch][VEC];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u)
+#pragma unroll
+      for (int k = 0; k < VEC; ++k)
+        pair[u][k] = look(r.pairs + (base + piece - max(n - u, 1)) * (64 * VEC) +
+                          word + k);
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      if (n - u < 1) break;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        unsigned long long v = pair[u][k];
+        while (v == ~0ull) {
+          __builtin_amdgcn_s_sleep(1);
+          v = look(r.pairs + (base + piece - (n - u)) * (64 * VEC) + word + k);
+        }
+        state[k] = composed(__uint_as_float(static_cast<unsigned>(v)),
+                            __uint_as_float(static_cast<unsigned>(v >> 32)),
+                            state[k]);
+      }
+    }
+  }
+}
+
+// WAVES segments of L steps each are a piece.
+template <typename T, int VEC, bool GATE, bool BACK, int WAVES, int L>
+__global__ void __launch_bounds__(64 * WAVES)
+    recurrence_pass_kernel(Recurrence r) {
+  typedef typename Pack<T, VEC>::type V;
+  __shared__ unsigned handed_out;
+  __shared__ float seg_a[WAVES][VEC][64], seg_s[WAVES][VEC][64];
+  __shared__ float front[VEC][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (threadIdx.x == 0)
+    handed_out = __hip_atomic_fetch_add(r.counter, 1u, __ATOMIC_RELAXED,
+                                        __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  const unsigned tile = __builtin_amdgcn_readfirstlane(handed_out);
+  const int blocks = (r.channels + 64 * VEC - 1) / (64 * VEC);
+  const unsigned rows = static_cast<unsigned>(r.batch) * blocks;
+  const int piece = static_cast<int>(tile / rows);
+  const unsigned row = tile - piece * rows;
+  const int b = static_cast<int>(row / blocks);
+  const int block = static_cast<int>(row - static_cast<unsigned>(b) * blocks);
+  // (a row's last channels: see Group; lanes behind them store nothing)
+  const seq::Group<VEC> group((block * 64 + lane) * VEC, r.channels);
+  const int c = group.c, skip = group.skip;
+  const int length = length_of(r, b);
+  const int segment = piece * WAVES + wave;
+  const int begin =
+      segment >= r.segments
+          ? r.steps
+          : (BACK ? r.segments - 1 - segment : segment) * L;
+  const int stop = min(begin + L, r.steps);  // the segment's end
+  const int end = min(stop, length);         // ... of the steps that count
+
+  const long at0 = static_cast<long>(b) * r.steps;
+  const T* const f = static_cast<const T*>(r.f) + at0 * r.stride + c;
+  const T* const x = static_cast<const T*>(r.x) + at0 * r.stride + c;
+  const T* const ig =
+      GATE ? static_cast<const T*>(r.i) + at0 * r.stride + c : nullptr;
+  auto step_of = [&](int u) { return min(begin + u, max(end, 1) - 1); };
+  V fv[L], xv[L], iv[L], dv[L], hv[L];
+  unsigned char fresh[L];
+#pragma unroll
+  for (int u = 0; u < L; ++u) {
+    const long t = step_of(u);
+    fv[u] = *reinterpret_cast<const V*>(f + t * r.stride);
+    if (BACK) {
+      dv[u] = *reinterpret_cast<const V*>(static_cast<const T*>(r.dh) +
+                                          (at0 + t) * r.channels + c);
+    } else {
+      xv[u] = *reinterpret_cast<const V*>(x + t * r.stride);
+      if (GATE) iv[u] = *reinterpret_cast<const V*>(ig + t * r.stride);
+    }
+    fresh[u] = r.resets == nullptr ? 0 : r.resets[at0 + t];
+  }
+  if (BACK) {  // on their way while the state is found
+#pragma unroll
+    for (int u = 0; u < L; ++u) {
+      const long t = step_of(u);
+      xv[u] = *reinterpret_cast<const V*>(x + t * r.stride);
+      if (GATE) iv[u] = *reinterpret_cast<const V*>(ig + t * r.stride);
+      hv[u] = *reinterpret_cast<const V*>(static_cast<const T*>(r.h) +
+                                          (at0 + max(t - 1, 0l)) * r.channels +
+                                          c);
+    }
+  }
+
+  // (A, S) of the segment; forward a_t and b_t are kept for the walk.
+  float A[VEC], S[VEC];
+  float keep_a[BACK ? 1 : L][VEC], keep_b[BACK ? 1 : L][VEC];
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) {
+    A[k] = 1.f;
+    S[k] = 0.f;
+  }
+#pragma unroll
+  for (int n = 0; n < L; ++n) {
+    const int u = BACK ? L - 1 - n : n;
+    float fs[VEC], xs[VEC], is[VEC];
+    unpack<T, VEC>(fv[u], fs);
+    unpack<T, VEC>(BACK ? dv[u] : xv[u], xs);
+    if (GATE && !BACK) unpack<T, VEC>(iv[u], is);
+    const bool counts = begin + u < end;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      float a, w;
+      if (BACK || GATE)
+        a = sigmoid_alone<T>(fs[k]);
+      else
+        sigmoid<T>(fs[k], &a, &w);
+      if (BACK) {
+        if (counts) {
+          S[k] = fresh[u] ? 0.f : a * (xs[k] + S[k]);
+          A[k] = fresh[u] ? -0.f : a * A[k];
+        }
+      } else {
+        if (GATE) w = sigmoid_alone<T>(is[k]);
+        const float add = w * xs[k];
+        keep_a[u][k] = a;
+        keep_b[u][k] = add;
+        if (counts) {
+          S[k] = add + (fresh[u] ? 0.f : a * S[k]);
+          A[k] = fresh[u] ? -0.f : a * A[k];
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) {
+    seg_a[wave][k][lane] = A[k];
+    seg_s[wave][k][lane] = S[k];
+  }
+  __syncthreads();
+
+  const long state_at = static_cast<long>(b) * r.channels + c;
+  if (wave == 0) {
+    // the piece's pair
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w)
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        const float a = seg_a[w][k][lane];
+        S[k] = composed(a, seg_s[w][k][lane], S[k]);
+        A[k] = is_reset(a) ? a : a * A[k];
+      }
+    const long place = static_cast<long>(row) * r.pieces + piece;
+    const long word = place * (64 * VEC) + static_cast<long>(lane) * VEC;
+    const bool others = piece + 1 < r.pieces;
+    float state[VEC];
+    if (piece == 0) {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k)
+        state[k] = r.first == nullptr ? 0.f : r.first[state_at + k];
+    } else {
+      if (others) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k)
+          publish(r.pairs + word + k,
+                  static_cast<unsigned long long>(published(A[k])) |
+                      static_cast<unsigned long long>(published(S[k])) << 32);
+        if (lane == 0) publish(r.flags + place, static_cast<unsigned>(kPair));
+      }
+      state_before<VEC>(r, row, piece, state);
+    }
+    if (others) {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k)
+        publish(r.states + word + k, published(composed(A[k], S[k], state[k])));
+      if (lane == 0) publish(r.flags + place, static_cast<unsigned>(kState));
+    }
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) front[k][lane] = state[k];
+  }
+  __syncthreads();
+  float state[VEC];
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) state[k] = front[k][lane];
+  for (int w = 0; w < wave; ++w)
+#pragma unroll
+    for (int k = 0; k < VEC; ++k)
+      state[k] = composed(seg_a[w][k][lane], seg_s[w][k][lane], state[k]);
+
+  // the walk over the segment
+  if (!BACK) {
+    T* const h = static_cast<T*>(r.out_h) + at0 * r.channels + c;
+#pragma unroll
+    for (int u = 0; u < L; ++u) {
+      const int t = begin + u;
+      if (t < end) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k)
+          state[k] = keep_b[u][k] + (fresh[u] ? 0.f : keep_a[u][k] * state[k]);
+        put<T, VEC>(h + static_cast<long>(t) * r.channels, state, skip);
+      } else if (t < stop) {
+        const float zero[VEC] = {};
+        put<T, VEC>(h + static_cast<long>(t) * r.channels, zero, skip);
+      }
+    }
+  } else {
+    T* const dx = static_cast<T*>(r.dx) + at0 * r.grad_stride + c;
+    T* const df = static_cast<T*>(r.df) + at0 * r.grad_stride + c;
+    T* const di =
+        GATE ? static_cast<T*>(r.di) + at0 * r.grad_stride + c : nullptr;
+#pragma unroll
+    for (int u = L - 1; u >= 0; --u) {
+      const int t = begin + u;
+      float gx[VEC] = {}, gf[VEC] = {}, gi[VEC] = {};
+      if (t < end) {
+        float fs[VEC], xs[VEC], is[VEC], before[VEC], ds[VEC];
+        unpack<T, VEC>(fv[u], fs);
+        unpack<T, VEC>(xv[u], xs);
+        if (GATE) unpack<T, VEC>(iv[u], is);
+        unpack<T, VEC>(hv[u], before);
+        unpack<T, VEC>(dv[u], ds);
+        if (t == 0) {
+#pragma unroll
+          for (int k = 0; k < VEC; ++k)
+            before[k] = r.initial == nullptr ? 0.f : r.initial[state_at + k];
+        }
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          float a, rest, w, w_rest;
+          sigmoid<T>(fs[k], &a, &rest);
+          if (GATE)
+            sigmoid<T>(is[k], &w, &w_rest);
+          else
+            w = rest;
+          const float G = ds[k] + state[k];
+          const float prior = fresh[u] ? 0.f : before[k];
+          gx[k] = G * w;
+          gf[k] = G * (GATE ? prior : prior - xs[k]) * (a * rest);
+          if (GATE) gi[k] = G * xs[k] * (w * w_rest);
+          state[k] = fresh[u] ? 0.f : a * G;
+        }
+      }
+      if (t < stop) {
+        put<T, VEC>(dx + t * r.grad_stride, gx, skip);
+        put<T, VEC>(df + t * r.grad_stride, gf, skip);
+        if (GATE) put<T, VEC>(di + t * r.grad_stride, gi, skip);
+      }
+    }
+  }
+  // (behind the last segment there are none, or empty ones)
+  if (r.last != nullptr && piece == r.pieces - 1 && wave == WAVES - 1)
+    put<float, VEC>(r.last + state_at, state, skip);
+}
+
+// ---- the choice ----------------------------------------------------------------
+
+#ifndef SNN_REC_FW
+#define SNN_REC_FW 8
+#define SNN_REC_FL 16
+#define SNN_REC_BW 8
+#define SNN_REC_BL 8
+#endif
+template <bool BACK>
+constexpr int kWaves = BACK ? SNN_REC_BW : SNN_REC_FW;
+template <bool BACK>
+constexpr int kSegment = BACK ? SNN_REC_BL : SNN_REC_FL;
+
+// A sequence is divided where its lanes alone are fewer than this many waves, and
+// where it is long enough for the second launch.
+constexpr int kWantedWaves = 4096;
+constexpr int kLeastSteps = 65;
+
+struct Division {
+  int segments, pieces;  // pieces == 0: undivided
+  size_t rows, zeros, words, bytes;
+};
+template <typename T, bool BACK>
+Division divide(const snn_hip_linear_recurrence_params& p) {
+  Division d = {};
+  constexpr int VEC = kVec<T>;
+  d.rows = static_cast<size_t>(p.batch) * ceil_div(p.channels, 64 * VEC);
+  d.segments = ceil_div(p.steps, kSegment<BACK>);
+  if (p.channels < VEC || d.rows >= kWantedWaves || p.steps < kLeastSteps)
+    return d;
+  d.pieces = ceil_div(d.segments, kWaves<BACK>);
+  const size_t places = d.rows * d.pieces;
+  // the counter and the flags, then the states and the pairs
+  d.zeros = (places + 1 + 3) / 4 * 4;
+  d.words = places * (64 * VEC) * 3;
+  d.bytes = (d.zeros + d.words) * sizeof(unsigned);
+  return d;
 }
 
 template <typename T, int VEC, bool GATE, bool BACK>
-int launch_recurrence_as(const Recurrence& r, hipStream_t stream) {
-  const long waves = static_cast<long>(r.batch) * r.pieces *
-                     ceil_div(r.channels, 64 * VEC);
-  if (waves > INT_MAX) return SNN_HIP_INDEX_EXCEEDED;
+int launch_undivided(const Recurrence& r, hipStream_t stream) {
+  const size_t waves =
+      static_cast<size_t>(r.batch) * ceil_div(r.channels, 64 * VEC);
   const dim3 grid(static_cast<unsigned>((waves + 3) / 4)), threads(256);
-  KernelTimer timer(stream);
-  if (r.pieces > 1) {
-    hipLaunchKernelGGL((recurrence_pieces_kernel<T, VEC, GATE, BACK>), grid,
-                       threads, 0, stream, r);
-    SNN_HIP_CHECK_LAUNCH();
-    hipLaunchKernelGGL(
-        (recurrence_join_kernel<BACK>),
-        dim3(static_cast<unsigned>(r.batch * ceil_div(r.channels, 64))),
-        dim3(1024), 0, stream, r);
-    SNN_HIP_CHECK_LAUNCH();
-  }
   if (BACK)
     hipLaunchKernelGGL((recurrence_grad_kernel<T, VEC, GATE>), grid, threads, 0,
                        stream, r);
   else
     hipLaunchKernelGGL((recurrence_walk_kernel<T, VEC, GATE>), grid, threads, 0,
                        stream, r);
+  SNN_HIP_CHECK_LAUNCH();
+  return SNN_HIP_OK;
+}
+
+template <typename T, bool GATE, bool BACK>
+int launch_divided(Recurrence r, const Division& d, void* workspace,
+                   hipStream_t stream) {
+  r.segments = d.segments;
+  r.pieces = d.pieces;
+  unsigned* const at = static_cast<unsigned*>(workspace);
+  r.counter = at;
+  r.flags = at + 1;
+  r.states = at + d.zeros;
+  const size_t slots = d.words / 3;
+  r.pairs = reinterpret_cast<unsigned long long*>(r.states + slots);
+  const size_t most = std::max(d.zeros, d.words / 4);
+  hipLaunchKernelGGL(
+      recurrence_clear_kernel,
+      dim3(static_cast<unsigned>(ceil_div(most, size_t{256}))), dim3(256), 0,
+      stream, at, d.zeros,
+      reinterpret_cast<seq::Pack<unsigned, 4>::type*>(at + d.zeros),
+      d.words / 4);
+  SNN_HIP_CHECK_LAUNCH();
+  hipLaunchKernelGGL(
+      (recurrence_pass_kernel<T, kVec<T>, GATE, BACK, kWaves<BACK>,
+                              kSegment<BACK>>),
+      dim3(static_cast<unsigned>(d.rows * d.pieces)), dim3(64 * kWaves<BACK>), 0,
+      stream, r);
   SNN_HIP_CHECK_LAUNCH();
   return SNN_HIP_OK;
 }
@@ -460,21 +674,25 @@ int launch_recurrence(Recurrence r, const snn_hip_linear_recurrence_params& p,
   r.channels = p.channels;
   r.stride = p.row_stride == 0 ? p.channels : p.row_stride;
   r.grad_stride = p.grad_row_stride == 0 ? p.channels : p.grad_row_stride;
-  divide_steps<T>(p, &r.pieces, &r.piece_steps);
-  const size_t floats = pair_floats(p, r.pieces);
-  if (workspace == nullptr || elems * sizeof(T) < floats * sizeof(float)) {
-    r.pieces = 1;
-    r.piece_steps = p.steps;
-  } else {
-    r.A = static_cast<float*>(workspace);
-    r.S = r.A + floats / 2;
+  KernelTimer timer(stream);
+  const Division d = divide<T, BACK>(p);
+  if (d.pieces > 0 && workspace != nullptr && elems * sizeof(T) >= d.bytes &&
+      d.rows * d.pieces <= INT_MAX) {
+    return r.i != nullptr
+               ? launch_divided<T, true, BACK>(r, d, workspace, stream)
+               : launch_divided<T, false, BACK>(r, d, workspace, stream);
   }
   constexpr int VEC = kVec<T>;
   if (p.channels >= VEC)
-    return r.i != nullptr ? launch_recurrence_as<T, VEC, true, BACK>(r, stream)
-                          : launch_recurrence_as<T, VEC, false, BACK>(r, stream);
-  return r.i != nullptr ? launch_recurrence_as<T, 1, true, BACK>(r, stream)
-                        : launch_recurrence_as<T, 1, false, BACK>(r, stream);
+    return r.i != nullptr ? launch_undivided<T, VEC, true, BACK>(r, stream)
+                          : launch_undivided<T, VEC, false, BACK>(r, stream);
+  return r.i != nullptr ? launch_undivided<T, 1, true, BACK>(r, stream)
+                        : launch_undivided<T, 1, false, BACK>(r, stream);
+}
+
+template <typename T>
+size_t workspace_bytes(const snn_hip_linear_recurrence_params& p) {
+  return std::max(divide<T, false>(p).bytes, divide<T, true>(p).bytes);
 }
 
 int check_recurrence(const snn_hip_linear_recurrence_params* p,
@@ -585,14 +803,10 @@ int snn_hip_linear_recurrence_workspace_size(
   if (required_elems == nullptr || recommended_elems == nullptr ||
       dtype < SNN_HIP_DTYPE_F32 || dtype > SNN_HIP_DTYPE_BF16)
     return SNN_HIP_INVALID_PARAMETER;
-  int pieces, piece_steps;
-  if (dtype == SNN_HIP_DTYPE_F32)
-    snn::divide_steps<float>(*params, &pieces, &piece_steps);
-  else
-    snn::divide_steps<_Float16>(*params, &pieces, &piece_steps);
   *required_elems = 0;
-  *recommended_elems = snn::pair_floats(*params, pieces) *
-                       (dtype == SNN_HIP_DTYPE_F32 ? 1 : 2);
+  *recommended_elems = dtype == SNN_HIP_DTYPE_F32
+                           ? snn::workspace_bytes<float>(*params) / 4
+                           : snn::workspace_bytes<_Float16>(*params) / 2;
   return SNN_HIP_OK;
 }
 
