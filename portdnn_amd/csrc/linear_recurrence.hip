@@ -94,6 +94,18 @@ __device__ __forceinline__ int length_of(const Recurrence& r, int b) {
                               : max(0, min(r.steps, r.lengths[b]));
 }
 
+// Which of the steps `first` ... `first` + n - 1 (n <= 64; as far as they are
+// before `end`) are resets, a bit each: one load for all.
+__device__ __forceinline__ unsigned long long resets_of(const Recurrence& r,
+                                                        long row, int first,
+                                                        int n, int end) {
+  if (r.resets == nullptr) return 0;
+  const int lane = threadIdx.x & 63;
+  const int t = first + lane;
+  const bool on = lane < n && t < end;
+  return __ballot(on && r.resets[row + (on ? t : 0)] != 0);
+}
+
 // ---- undivided ---------------------------------------------------------------
 
 // Steps whose loads are in flight together: 8 forward; the gradients, with five
@@ -102,10 +114,10 @@ __device__ __forceinline__ int length_of(const Recurrence& r, int b) {
 template <bool BACK>
 constexpr int kSteps = BACK ? 4 : 8;
 
-// What a wave needs of its place: sequence and first channel of the lane.
+// What a wave needs of its place: sequence and first channel of the lane.  (Lanes
+// behind a row's channels stay, and store nothing.)
 struct Place {
   int b, c, skip;
-  bool on;
 };
 template <int VEC>
 __device__ __forceinline__ Place place_of(const Recurrence& r) {
@@ -120,7 +132,6 @@ __device__ __forceinline__ Place place_of(const Recurrence& r) {
   const seq::Group<VEC> group(first, r.channels);
   p.c = group.c;
   p.skip = group.skip;
-  p.on = p.b < r.batch && first < r.channels;
   return p;
 }
 
@@ -130,7 +141,7 @@ __global__ void __launch_bounds__(256) recurrence_walk_kernel(Recurrence r) {
   typedef typename Pack<T, VEC>::type V;
   constexpr int kGroup = kSteps<false>;
   const Place p = place_of<VEC>(r);
-  if (!p.on) return;
+  if (p.b >= r.batch) return;
   const long row = static_cast<long>(p.b) * r.steps;
   const T* const f = static_cast<const T*>(r.f) + row * r.stride + p.c;
   const T* const x = static_cast<const T*>(r.x) + row * r.stride + p.c;
@@ -145,14 +156,14 @@ __global__ void __launch_bounds__(256) recurrence_walk_kernel(Recurrence r) {
   const int end = length_of(r, p.b);
   for (int first = 0; first < end; first += kGroup) {
     V fv[kGroup], xv[kGroup], iv[kGroup];
-    unsigned char fresh[kGroup];
+    const unsigned long long resets = resets_of(r, row, first, kGroup, end);
+    auto fresh = [&](int u) { return (resets >> u & 1) != 0; };
 #pragma unroll
     for (int u = 0; u < kGroup; ++u) {
       const int t = min(first + u, end - 1);
       fv[u] = *reinterpret_cast<const V*>(f + t * r.stride);
       xv[u] = *reinterpret_cast<const V*>(x + t * r.stride);
       if (GATE) iv[u] = *reinterpret_cast<const V*>(ig + t * r.stride);
-      fresh[u] = r.resets == nullptr ? 0 : r.resets[row + t];
     }
 #pragma unroll
     for (int u = 0; u < kGroup; ++u) {
@@ -170,7 +181,7 @@ __global__ void __launch_bounds__(256) recurrence_walk_kernel(Recurrence r) {
         } else {
           sigmoid<T>(fs[k], &a, &w);
         }
-        state[k] = w * xs[k] + (fresh[u] ? 0.f : a * state[k]);
+        state[k] = w * xs[k] + (fresh(u) ? 0.f : a * state[k]);
       }
       put<T, VEC>(h + static_cast<long>(first + u) * r.channels, state, p.skip);
     }
@@ -188,7 +199,7 @@ __global__ void __launch_bounds__(256) recurrence_grad_kernel(Recurrence r) {
   typedef typename Pack<T, VEC>::type V;
   constexpr int kGroup = kSteps<true>;
   const Place p = place_of<VEC>(r);
-  if (!p.on) return;
+  if (p.b >= r.batch) return;
   const long row = static_cast<long>(p.b) * r.steps;
   const T* const f = static_cast<const T*>(r.f) + row * r.stride + p.c;
   const T* const x = static_cast<const T*>(r.x) + row * r.stride + p.c;
@@ -215,8 +226,9 @@ __global__ void __launch_bounds__(256) recurrence_grad_kernel(Recurrence r) {
   const int groups = (end + kGroup - 1) / kGroup;
   for (int g = groups - 1; g >= 0; --g) {
     V fv[kGroup], xv[kGroup], iv[kGroup], hv[kGroup], dv[kGroup];
-    unsigned char fresh[kGroup];
     const int first = g * kGroup;
+    const unsigned long long resets = resets_of(r, row, first, kGroup, end);
+    auto fresh = [&](int u) { return (resets >> u & 1) != 0; };
 #pragma unroll
     for (int u = 0; u < kGroup; ++u) {
       const int t = min(first + u, end - 1);
@@ -227,7 +239,6 @@ __global__ void __launch_bounds__(256) recurrence_grad_kernel(Recurrence r) {
           h + static_cast<long>(max(t - 1, 0)) * r.channels);
       dv[u] = *reinterpret_cast<const V*>(dh + static_cast<long>(t) *
                                                    r.channels);
-      fresh[u] = r.resets == nullptr ? 0 : r.resets[row + t];
     }
 #pragma unroll
     for (int u = kGroup - 1; u >= 0; --u) {
@@ -255,11 +266,11 @@ __global__ void __launch_bounds__(256) recurrence_grad_kernel(Recurrence r) {
           w = rest;
         }
         const float G = ds[k] + D[k];
-        const float prior = fresh[u] ? 0.f : before[k];
+        const float prior = fresh(u) ? 0.f : before[k];
         gx[k] = G * w;
         gf[k] = G * (GATE ? prior : prior - xs[k]) * (a * rest);
         if (GATE) gi[k] = G * xs[k] * (w * w_rest);
-        D[k] = fresh[u] ? 0.f : a * G;
+        D[k] = fresh(u) ? 0.f : a * G;
       }
       put<T, VEC>(dx + t * r.grad_stride, gx, p.skip);
       put<T, VEC>(df + t * r.grad_stride, gf, p.skip);
@@ -362,12 +373,14 @@ __device__ __forceinline__ void state_before(const Recurrence& r, long row,
 // WAVES segments of L steps each are a piece.
 template <typename T, int VEC, bool GATE, bool BACK, int WAVES, int L>
 __global__ void __launch_bounds__(64 * WAVES)
+    __attribute__((amdgpu_waves_per_eu(BACK ? 4 : 2)))
     recurrence_pass_kernel(Recurrence r) {
   typedef typename Pack<T, VEC>::type V;
   __shared__ unsigned handed_out;
   __shared__ float seg_a[WAVES][VEC][64], seg_s[WAVES][VEC][64];
   __shared__ float front[VEC][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (threadIdx.x == 0)
     handed_out = __hip_atomic_fetch_add(r.counter, 1u, __ATOMIC_RELAXED,
                                         __HIP_MEMORY_SCOPE_AGENT);
@@ -391,40 +404,47 @@ __global__ void __launch_bounds__(64 * WAVES)
   const int stop = min(begin + L, r.steps);  // the segment's end
   const int end = min(stop, length);         // ... of the steps that count
 
+  // Rows are addressed by the wave (a scalar), channels by the lane's offset.
   const long at0 = static_cast<long>(b) * r.steps;
-  const T* const f = static_cast<const T*>(r.f) + at0 * r.stride + c;
-  const T* const x = static_cast<const T*>(r.x) + at0 * r.stride + c;
-  const T* const ig =
-      GATE ? static_cast<const T*>(r.i) + at0 * r.stride + c : nullptr;
+  const unsigned offset = static_cast<unsigned>(c) * sizeof(T);
+  auto load = [&](const void* p, long stride, long t) {
+    return *reinterpret_cast<const V*>(
+        static_cast<const char*>(p) + (at0 + t) * stride * sizeof(T) + offset);
+  };
+  auto store = [&](void* p, long stride, long t, const float (&v)[VEC]) {
+    put<T, VEC>(reinterpret_cast<T*>(static_cast<char*>(p) +
+                                     (at0 + t) * stride * sizeof(T) + offset),
+                v, skip);
+  };
   auto step_of = [&](int u) { return min(begin + u, max(end, 1) - 1); };
   V fv[L], xv[L], iv[L], dv[L], hv[L];
-  unsigned char fresh[L];
+  const unsigned long long resets = resets_of(r, at0, begin, L, end);
+  auto fresh = [&](int u) { return (resets >> u & 1) != 0; };
 #pragma unroll
   for (int u = 0; u < L; ++u) {
     const long t = step_of(u);
-    fv[u] = *reinterpret_cast<const V*>(f + t * r.stride);
+    fv[u] = load(r.f, r.stride, t);
     if (BACK) {
-      dv[u] = *reinterpret_cast<const V*>(static_cast<const T*>(r.dh) +
-                                          (at0 + t) * r.channels + c);
+      dv[u] = load(r.dh, r.channels, t);
     } else {
-      xv[u] = *reinterpret_cast<const V*>(x + t * r.stride);
-      if (GATE) iv[u] = *reinterpret_cast<const V*>(ig + t * r.stride);
-    }
-    fresh[u] = r.resets == nullptr ? 0 : r.resets[at0 + t];
-  }
-  if (BACK) {  // on their way while the state is found
-#pragma unroll
-    for (int u = 0; u < L; ++u) {
-      const long t = step_of(u);
-      xv[u] = *reinterpret_cast<const V*>(x + t * r.stride);
-      if (GATE) iv[u] = *reinterpret_cast<const V*>(ig + t * r.stride);
-      hv[u] = *reinterpret_cast<const V*>(static_cast<const T*>(r.h) +
-                                          (at0 + max(t - 1, 0l)) * r.channels +
-                                          c);
+      xv[u] = load(r.x, r.stride, t);
+      if (GATE) iv[u] = load(r.i, r.stride, t);
     }
   }
+  // Backwards what only the walk needs is loaded there, kLate steps at a time: held
+  // from the start it takes the registers of a second work-group on the CU
+  // (4 x 4096 x 2048 binary16: 175 -> 129 us).
+  constexpr int kLate = 4;
+  auto load_rest = [&](int u) {
+    const long t = step_of(u);
+    xv[u] = load(r.x, r.stride, t);
+    if (GATE) iv[u] = load(r.i, r.stride, t);
+    hv[u] = load(r.h, r.channels, max(t - 1, 0l));
+  };
 
-  // (A, S) of the segment; forward a_t and b_t are kept for the walk.
+  // (A, S) of the segment.  Forward a_t and b_t are kept for the walk: working them
+  // out again leaves room for more waves and is slower (32768 x 2048 bfloat16: 138
+  // against 121 us).
   float A[VEC], S[VEC];
   float keep_a[BACK ? 1 : L][VEC], keep_b[BACK ? 1 : L][VEC];
 #pragma unroll
@@ -449,8 +469,8 @@ __global__ void __launch_bounds__(64 * WAVES)
         sigmoid<T>(fs[k], &a, &w);
       if (BACK) {
         if (counts) {
-          S[k] = fresh[u] ? 0.f : a * (xs[k] + S[k]);
-          A[k] = fresh[u] ? -0.f : a * A[k];
+          S[k] = fresh(u) ? 0.f : a * (xs[k] + S[k]);
+          A[k] = fresh(u) ? -0.f : a * A[k];
         }
       } else {
         if (GATE) w = sigmoid_alone<T>(is[k]);
@@ -458,8 +478,8 @@ __global__ void __launch_bounds__(64 * WAVES)
         keep_a[u][k] = a;
         keep_b[u][k] = add;
         if (counts) {
-          S[k] = add + (fresh[u] ? 0.f : a * S[k]);
-          A[k] = fresh[u] ? -0.f : a * A[k];
+          S[k] = add + (fresh(u) ? 0.f : a * S[k]);
+          A[k] = fresh(u) ? -0.f : a * A[k];
         }
       }
     }
@@ -519,29 +539,41 @@ __global__ void __launch_bounds__(64 * WAVES)
     for (int k = 0; k < VEC; ++k)
       state[k] = composed(seg_a[w][k][lane], seg_s[w][k][lane], state[k]);
 
+  // (Backwards the gates are worked out again: the barrier keeps the compiler from
+  // holding them, which takes twice the registers of what they come from.)
+  if (BACK) {
+#pragma unroll
+    for (int u = 0; u < L; ++u) {
+      typedef typename Pack<unsigned, sizeof(V) / 4>::type Bits;
+      Bits bits = __builtin_bit_cast(Bits, fv[u]);
+      asm volatile("" : "+v"(bits));
+      fv[u] = __builtin_bit_cast(V, bits);
+    }
+  }
+
   // the walk over the segment
   if (!BACK) {
-    T* const h = static_cast<T*>(r.out_h) + at0 * r.channels + c;
 #pragma unroll
     for (int u = 0; u < L; ++u) {
       const int t = begin + u;
       if (t < end) {
 #pragma unroll
         for (int k = 0; k < VEC; ++k)
-          state[k] = keep_b[u][k] + (fresh[u] ? 0.f : keep_a[u][k] * state[k]);
-        put<T, VEC>(h + static_cast<long>(t) * r.channels, state, skip);
+          state[k] = keep_b[u][k] + (fresh(u) ? 0.f : keep_a[u][k] * state[k]);
+        store(r.out_h, r.channels, t, state);
       } else if (t < stop) {
         const float zero[VEC] = {};
-        put<T, VEC>(h + static_cast<long>(t) * r.channels, zero, skip);
+        store(r.out_h, r.channels, t, zero);
       }
     }
   } else {
-    T* const dx = static_cast<T*>(r.dx) + at0 * r.grad_stride + c;
-    T* const df = static_cast<T*>(r.df) + at0 * r.grad_stride + c;
-    T* const di =
-        GATE ? static_cast<T*>(r.di) + at0 * r.grad_stride + c : nullptr;
 #pragma unroll
     for (int u = L - 1; u >= 0; --u) {
+      if ((L - 1 - u) % kLate == 0) {
+#pragma unroll
+        for (int q = 0; q < kLate; ++q)
+          if (u - q >= 0) load_rest(u - q);
+      }
       const int t = begin + u;
       float gx[VEC] = {}, gf[VEC] = {}, gi[VEC] = {};
       if (t < end) {
@@ -565,17 +597,17 @@ __global__ void __launch_bounds__(64 * WAVES)
           else
             w = rest;
           const float G = ds[k] + state[k];
-          const float prior = fresh[u] ? 0.f : before[k];
+          const float prior = fresh(u) ? 0.f : before[k];
           gx[k] = G * w;
           gf[k] = G * (GATE ? prior : prior - xs[k]) * (a * rest);
           if (GATE) gi[k] = G * xs[k] * (w * w_rest);
-          state[k] = fresh[u] ? 0.f : a * G;
+          state[k] = fresh(u) ? 0.f : a * G;
         }
       }
       if (t < stop) {
-        put<T, VEC>(dx + t * r.grad_stride, gx, skip);
-        put<T, VEC>(df + t * r.grad_stride, gf, skip);
-        if (GATE) put<T, VEC>(di + t * r.grad_stride, gi, skip);
+        store(r.dx, r.grad_stride, t, gx);
+        store(r.df, r.grad_stride, t, gf);
+        if (GATE) store(r.di, r.grad_stride, t, gi);
       }
     }
   }
@@ -586,16 +618,15 @@ __global__ void __launch_bounds__(64 * WAVES)
 
 // ---- the choice ----------------------------------------------------------------
 
-#ifndef SNN_REC_FW
-#define SNN_REC_FW 8
-#define SNN_REC_FL 16
-#define SNN_REC_BW 8
-#define SNN_REC_BL 8
-#endif
+// A piece: waves of a work-group, and the steps of a segment.  Longer pieces make a
+// shorter chain of them, larger segments take registers from the waves of a CU.
+// Forward, 32768 x 2048 bfloat16: 12 x 12 121 us, 16 x 8 and 12 x 8 124, 8 x 16 133,
+// 8 x 12 141, 4 x 16 165.  Gradients, 4 x 4096 x 2048 binary16: 16 x 8 and 8 x 8
+// 129 us, 16 x 4 137, 12 x 8 139, 12 x 12 142.
 template <bool BACK>
-constexpr int kWaves = BACK ? SNN_REC_BW : SNN_REC_FW;
+constexpr int kWaves = BACK ? 16 : 12;
 template <bool BACK>
-constexpr int kSegment = BACK ? SNN_REC_BL : SNN_REC_FL;
+constexpr int kSegment = BACK ? 8 : 12;
 
 // A sequence is divided where its lanes alone are fewer than this many waves, and
 // where it is long enough for the second launch.
