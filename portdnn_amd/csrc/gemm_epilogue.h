@@ -35,6 +35,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "gemm_tile.h"
 #include "sequence.h"
@@ -73,26 +74,45 @@ int run_bf16(Product& g, void* workspace, size_t bytes, hipStream_t stream);
 // orders alone.
 size_t workspace_bytes(const Product& g, int elem_size);
 
-__device__ __forceinline__ float activate(float z, int kind) {
+template <int KIND>
+__device__ __forceinline__ float activate(float z) {
+  if constexpr (KIND == SNN_HIP_ACTIVATION_RELU) {
+    return z < 0.f ? 0.f : z;  // (a NaN stays)
+  } else if constexpr (KIND == SNN_HIP_ACTIVATION_GELU) {
+    return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+  } else {
+    // (1 + tanh(u)) / 2 = sigmoid(2 u)
+    float s, rest;
+    seq::sigmoid<float>(
+        KIND == SNN_HIP_ACTIVATION_SILU
+            ? z
+            : 1.5957691216057308f * (z + 0.044715f * z * z * z),
+        &s, &rest);
+    return z * s;
+  }
+}
+// (the kind is the same for all lanes: one branch for all N)
+template <int N>
+__device__ __forceinline__ void activate(float (&v)[N], int kind) {
+  auto all = [&](auto k) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = activate<decltype(k)::value>(v[i]);
+  };
   switch (kind) {
     case SNN_HIP_ACTIVATION_RELU:
-      return z < 0.f ? 0.f : z;  // (a NaN stays)
+      all(std::integral_constant<int, SNN_HIP_ACTIVATION_RELU>());
+      break;
     case SNN_HIP_ACTIVATION_GELU:
-      return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
-    case SNN_HIP_ACTIVATION_GELU_TANH: {
-      // (1 + tanh(u)) / 2 = sigmoid(2 u)
-      float s, rest;
-      seq::sigmoid<float>(
-          1.5957691216057308f * (z + 0.044715f * z * z * z), &s, &rest);
-      return z * s;
-    }
-    case SNN_HIP_ACTIVATION_SILU: {
-      float s, rest;
-      seq::sigmoid<float>(z, &s, &rest);
-      return z * s;
-    }
+      all(std::integral_constant<int, SNN_HIP_ACTIVATION_GELU>());
+      break;
+    case SNN_HIP_ACTIVATION_GELU_TANH:
+      all(std::integral_constant<int, SNN_HIP_ACTIVATION_GELU_TANH>());
+      break;
+    case SNN_HIP_ACTIVATION_SILU:
+      all(std::integral_constant<int, SNN_HIP_ACTIVATION_SILU>());
+      break;
     default:
-      return z;
+      break;
   }
 }
 
@@ -162,10 +182,7 @@ __device__ __forceinline__ void finish8(const Product& g, int row, int col,
     }
     if (pre != nullptr) store(pre, v);
     if (residual != nullptr) load(residual, add);
-    if (g.activation != SNN_HIP_ACTIVATION_NONE) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = activate(v[i], g.activation);
-    }
+    activate(v, g.activation);
     if (residual != nullptr) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] += add[i];
@@ -173,16 +190,18 @@ __device__ __forceinline__ void finish8(const Product& g, int row, int col,
     store(out, v);
     return;
   }
+  // (a row's last columns, one at a time; the values move up, as an index that is
+  // not known when compiled would put them into LDS)
 #pragma unroll 1
-  for (int i = 0; col + i < g.n; ++i) {
-    float z = v[0];
+  for (; col < g.n; ++col) {
+    float z[1] = {v[0]};
 #pragma unroll
-    for (int k = 1; k < 8; ++k) z = i == k ? v[k] : z;
-    if (bias != nullptr) z += static_cast<float>(bias[col + i]);
-    if (pre != nullptr) pre[col + i] = static_cast<T>(z);
-    z = activate(z, g.activation);
-    if (residual != nullptr) z += static_cast<float>(residual[col + i]);
-    out[col + i] = static_cast<T>(z);
+    for (int i = 0; i < 7; ++i) v[i] = v[i + 1];
+    if (bias != nullptr) z[0] += static_cast<float>(bias[col]);
+    if (pre != nullptr) pre[col] = static_cast<T>(z[0]);
+    activate(z, g.activation);
+    if (residual != nullptr) z[0] += static_cast<float>(residual[col]);
+    out[col] = static_cast<T>(z[0]);
   }
 }
 
