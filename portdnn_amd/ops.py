@@ -807,8 +807,9 @@ def linear_recurrence_grad(grad, x, forget, h, input_gate=None, resets=None,
                            grad_final_state=None, out=None, workspace=None):
     """snn_hip_linear_recurrence_grad: a dict of the gradients of x, forget,
     input_gate (where it is given) and initial_state.  `out` is a [batch, steps,
-    channels * n] tensor that takes those of x, forget and input_gate side by
-    side, the gradient of a projection that they are slices of."""
+    channels * n] tensor, or such a slice of a wider one, that takes those of x,
+    forget and input_gate side by side: the gradient of a projection that they
+    are slices of."""
     batch, steps, channels = shape = x.shape
     dtype = x.dtype
     stride, elems, resets_at, lengths_at = _recurrence_operands(
@@ -818,10 +819,11 @@ def linear_recurrence_grad(grad, x, forget, h, input_gate=None, resets=None,
         got = {name: x.new_empty(shape) for name in names}
         grad_stride = channels
     else:
-        _like(out, (batch, steps, channels * len(names)), dtype)
+        assert out.shape == (batch, steps, channels * len(names)) and \
+            out.dtype == dtype
         got = {name: out[..., i * channels:(i + 1) * channels]
                for i, name in enumerate(names)}
-        grad_stride = channels * len(names)
+        grad_stride = _step_stride(out)
     got["initial_state"] = x.new_empty((batch, channels), dtype=torch.float32)
     if workspace is None:
         if elems:
