@@ -396,8 +396,28 @@ struct Space {
   static constexpr int kStage = kLoads * WAVES * 1024;
 };
 
+// (v >> 8 * bytes), zeros from above.
+__device__ __forceinline__ uint4v shifted_down(uint4v v, int bytes) {
+  typedef unsigned long long Two __attribute__((ext_vector_type(2)));
+  Two w = __builtin_bit_cast(Two, v);
+  if (bytes >= 8) {
+    w = Two{w[1], 0ull};
+    bytes -= 8;
+  }
+  if (bytes >= 8) w = Two{0ull, 0ull};
+  if (bytes > 0 && bytes < 8) {
+    w[0] = w[0] >> (8 * bytes) | w[1] << (64 - 8 * bytes);
+    w[1] >>= 8 * bytes;
+  }
+  return __builtin_bit_cast(uint4v, w);
+}
+
+// The product of a tile by waves that walk the reduction together.  HELD = 0: whole
+// 16-byte pieces at aligned addresses, which go straight to a ring of STAGES chunks
+// in LDS.  Otherwise rows of at least 16 bytes at any address by way of registers,
+// where HELD chunks are under way; LDS holds STAGES = 2.
 template <typename T, bool PK, bool QK, int BM, int BN, int WM, int WN,
-          int CB, int STAGES>
+          int CB, int STAGES, int HELD>
 __device__ __forceinline__ void gemm_body(const Product& g, char* r0, char* r1,
                                           char* r2, char* r3, char* r4) {
   typedef Operand<T, PK, BM, CB> OP;
@@ -460,79 +480,171 @@ __device__ __forceinline__ void gemm_body(const Product& g, char* r0, char* r1,
     }
   };
 
-  // Offsets of the lane's loads within a chunk; the chunk's own place is in
-  // the buffer's base, so that operands may be of any size.
-  unsigned offset[S::kLoads];
-  int order[S::kLoads];  // its reduction index
-#pragma unroll
-  for (int l = 0; l < S::kLoads; ++l) {
-    const int block = wave + l * WAVES;
-    int row, col;
-    bool in;
-    long stride;
-    if (block < OP::kBlocks) {
-      OP::source(block * 1024 + lane * 16, &row, &col);
-      in = PK ? row < rows_left : col < rows_left;
-      stride = g.p_stride;
-      order[l] = PK ? col : row;
-    } else {
-      OQ::source((block - OP::kBlocks) * 1024 + lane * 16, &row, &col);
-      in = block < S::kBlocks && (QK ? row < cols_left : col < cols_left);
-      stride = g.q_stride;
-      order[l] = QK ? col : row;
-    }
-    offset[l] = in ? static_cast<unsigned>((row * stride + col) * sizeof(T))
-                   : kOob;
-  }
-  const char* from_p =
-      reinterpret_cast<const char*>(OP::at(g.p, g.p_stride, row0, k_begin));
-  const char* from_q =
-      reinterpret_cast<const char*>(OQ::at(g.q, g.q_stride, col0, k_begin));
-  const long step_p = PK ? CB : CB * g.p_stride;
-  const long step_q = QK ? CB : CB * g.q_stride;
-  int k_left = k_end - k_begin;
-  auto issue = [&](char* to) {  // the next chunk
-    const __amdgpu_buffer_rsrc_t p = make_rsrc(from_p), q = make_rsrc(from_q);
+  int left = chunks;
+  if constexpr (HELD == 0) {
+    // Offsets of the lane's loads within a chunk; the chunk's own place is in
+    // the buffer's base, so that operands may be of any size.
+    unsigned offset[S::kLoads];
+    int order[S::kLoads];  // its reduction index
 #pragma unroll
     for (int l = 0; l < S::kLoads; ++l) {
       const int block = wave + l * WAVES;
-      const unsigned from = order[l] < k_left ? offset[l] : kOob;
-      if (block < OP::kBlocks)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            p, (lds_ptr)(to + block * 1024), 16, from, 0, 0, 0);
-      else
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            q, (lds_ptr)(to + block * 1024), 16, from, 0, 0, 0);
+      int row, col;
+      bool in;
+      long stride;
+      if (block < OP::kBlocks) {
+        OP::source(block * 1024 + lane * 16, &row, &col);
+        in = PK ? row < rows_left : col < rows_left;
+        stride = g.p_stride;
+        order[l] = PK ? col : row;
+      } else {
+        OQ::source((block - OP::kBlocks) * 1024 + lane * 16, &row, &col);
+        in = block < S::kBlocks && (QK ? row < cols_left : col < cols_left);
+        stride = g.q_stride;
+        order[l] = QK ? col : row;
+      }
+      offset[l] = in ? static_cast<unsigned>((row * stride + col) * sizeof(T))
+                     : kOob;
     }
-    from_p += step_p;
-    from_q += step_q;
-    k_left -= kChunk;
-  };
-  // STAGES - 1 chunks are under way while one is multiplied; behind the last
-  // one the loads are out of range, so that there is always the same number.  A
-  // chunk's place is loaded again behind the barrier that every wave reaches
-  // when it has read it.  (The places are arrays of their own: the compiler
-  // waits for all loads into an array before it reads from it.)
+    const char* from_p =
+        reinterpret_cast<const char*>(OP::at(g.p, g.p_stride, row0, k_begin));
+    const char* from_q =
+        reinterpret_cast<const char*>(OQ::at(g.q, g.q_stride, col0, k_begin));
+    const long step_p = PK ? CB : CB * g.p_stride;
+    const long step_q = QK ? CB : CB * g.q_stride;
+    int k_left = k_end - k_begin;
+    auto issue = [&](char* to) {  // the next chunk
+      const __amdgpu_buffer_rsrc_t p = make_rsrc(from_p), q = make_rsrc(from_q);
 #pragma unroll
-  for (int c = 0; c < STAGES - 1; ++c) issue(ring(c));
-  auto step = [&](int u) {
-    // the chunk is here, and the reads of the one before have returned
-    __builtin_amdgcn_s_waitcnt(kLgkm0 & vmcnt_imm((STAGES - 2) * S::kLoads));
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
-    issue(ring((u + STAGES - 1) % STAGES));
-    compute(ring(u));
-  };
-  int left = chunks;
-  for (; left >= STAGES; left -= STAGES) {
+      for (int l = 0; l < S::kLoads; ++l) {
+        const int block = wave + l * WAVES;
+        const unsigned from = order[l] < k_left ? offset[l] : kOob;
+        if (block < OP::kBlocks)
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(
+              p, (lds_ptr)(to + block * 1024), 16, from, 0, 0, 0);
+        else
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(
+              q, (lds_ptr)(to + block * 1024), 16, from, 0, 0, 0);
+      }
+      from_p += step_p;
+      from_q += step_q;
+      k_left -= kChunk;
+    };
+    // STAGES - 1 chunks are under way while one is multiplied; behind the last
+    // one the loads are out of range, so that there is always the same number.  A
+    // chunk's place is loaded again behind the barrier that every wave reaches
+    // when it has read it.  (The places are arrays of their own: the compiler
+    // waits for all loads into an array before it reads from it.)
 #pragma unroll
-    for (int u = 0; u < STAGES; ++u) step(u);
+    for (int c = 0; c < STAGES - 1; ++c) issue(ring(c));
+    auto step = [&](int u) {
+      // the chunk is here, and the reads of the one before have returned
+      __builtin_amdgcn_s_waitcnt(kLgkm0 & vmcnt_imm((STAGES - 2) * S::kLoads));
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      issue(ring((u + STAGES - 1) % STAGES));
+      compute(ring(u));
+    };
+    for (; left >= STAGES; left -= STAGES) {
+#pragma unroll
+      for (int u = 0; u < STAGES; ++u) step(u);
+    }
+#pragma unroll
+    for (int u = 0; u < STAGES - 1; ++u)
+      if (u < left) step(u);
+  } else {
+    // Where a piece would reach behind its row's end the row's last 16 bytes are
+    // loaded and, on their way into LDS, shifted to where the piece begins: zeros
+    // behind the end of a reduction, anything in columns that are not kept.
+    constexpr int kLoadsP = OP::kBlocks / WAVES;
+    static_assert(OP::kBlocks % WAVES == 0 && OQ::kBlocks % WAVES == 0,
+                  "waves load the same number of blocks of each operand");
+    int offset[S::kLoads], order[S::kLoads], late[S::kLoads];
+#pragma unroll
+    for (int l = 0; l < S::kLoads; ++l) {
+      auto place = [&](auto o, unsigned pos, bool inner, int there, long stride) {
+        typedef decltype(o) O;
+        int row, col;
+        O::source(pos, &row, &col);
+        order[l] = inner ? col : row;
+        const int r = inner ? min(row, there - 1) : row;
+        const int c = inner ? col : min(col, there - O::kPiece);
+        late[l] = (col - c) * static_cast<int>(sizeof(T));
+        offset[l] = static_cast<int>((r * stride + c) * sizeof(T));
+      };
+      const int block = wave + l * WAVES;
+      if (l < kLoadsP)
+        place(OP(), block * 1024 + lane * 16, PK, rows_left, g.p_stride);
+      else
+        place(OQ(), (block - OP::kBlocks) * 1024 + lane * 16, QK, cols_left,
+              g.q_stride);
+    }
+    const char* from_p =
+        reinterpret_cast<const char*>(OP::at(g.p, g.p_stride, row0, k_begin));
+    const char* from_q =
+        reinterpret_cast<const char*>(OQ::at(g.q, g.q_stride, col0, k_begin));
+    const long step_p = PK ? CB : CB * g.p_stride;
+    const long step_q = QK ? CB : CB * g.q_stride;
+    int k_left = k_end - k_begin, k_here = k_left;  // to be loaded, to be stored
+    uint4v held[HELD][S::kLoads];
+    auto load = [&](uint4v (&to)[S::kLoads]) {
+      if (k_left > 0) {
+#pragma unroll
+        for (int l = 0; l < S::kLoads; ++l) {
+          const bool of_p = l < kLoadsP;
+          const bool inner = of_p ? PK : QK;
+          long from = offset[l];
+          if (k_left < kChunk) {
+            const int over =
+                max(0, order[l] - (k_left - (inner ? OP::kPiece : 1)));
+            from -= over * (inner ? 1l : of_p ? g.p_stride : g.q_stride) *
+                    static_cast<long>(sizeof(T));
+          }
+          __builtin_memcpy(&to[l], (of_p ? from_p : from_q) + from, 16);
+        }
+      }
+      from_p += step_p;
+      from_q += step_q;
+      k_left -= kChunk;
+    };
+    auto step = [&](uint4v (&from)[S::kLoads], char* to) {
+#pragma unroll
+      for (int l = 0; l < S::kLoads; ++l) {
+        const bool of_p = l < kLoadsP;
+        uint4v v = from[l];
+        if (of_p ? PK : QK) {
+          if (k_here < kChunk)
+            v = shifted_down(v, max(0, order[l] + OP::kPiece - k_here) *
+                                    static_cast<int>(sizeof(T)));
+        } else {
+          if ((of_p ? rows_left < BM : cols_left < BN))
+            v = shifted_down(v, late[l]);
+          if (order[l] >= k_here) v = uint4v{0u, 0u, 0u, 0u};
+        }
+        *reinterpret_cast<uint4v*>(to + (wave + l * WAVES) * 1024 + lane * 16) = v;
+      }
+      k_here -= kChunk;
+      load(from);
+      // every wave has stored the chunk, and has read the one before
+      __builtin_amdgcn_s_waitcnt(kLgkm0 & vmcnt_imm(63));
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      compute(to);
+    };
+    static_assert(STAGES == 2 && HELD % 2 == 0, "two chunks in LDS");
+#pragma unroll
+    for (int u = 0; u < HELD; ++u) load(held[u]);
+    for (; left >= HELD; left -= HELD) {
+#pragma unroll
+      for (int u = 0; u < HELD; ++u) step(held[u], ring(u % 2));
+    }
+#pragma unroll
+    for (int u = 0; u < HELD - 1; ++u)
+      if (u < left) step(held[u], ring(u % 2));
   }
-#pragma unroll
-  for (int u = 0; u < STAGES - 1; ++u)
-    if (u < left) step(u);
   __builtin_amdgcn_s_waitcnt(kLgkm0 & vmcnt_imm(0));
 
   // The way out.  A wave's part of the tile in passes of kRows rows, a 16-byte
@@ -842,8 +954,8 @@ __global__ void __launch_bounds__(256) gemm_join_kernel(Product g) {
 }
 
 // The kernels of a product: tiles of work-groups that walk the reduction
-// together, tiles whose waves share it (for few rows), and those of the latter
-// that take rows at any address.
+// together, tiles whose waves share it (for few rows), and those that take rows at
+// any address.
 enum Kernel {
   kFew16x16,
   kFew16x32,
@@ -856,6 +968,7 @@ enum Kernel {
   kAny16x16,
   kAny32x32,
   kAny64x32,
+  kAnyTile128,  // rows of 16 bytes at least, tiles within 31 bits
   kKernels
 };
 
@@ -872,14 +985,14 @@ constexpr Shape kShapes16[kKernels] = {
     {64, 128, 1, 256, 4.3f, 0.24f, 0.24f}, {128, 128, 1, 256, 5.2f, 0.42f, 0.42f},
     {128, 128, 1, 512, 5.0f, 0.92f, 0.92f}, {256, 256, 1, 256, 8.0f, 1.5f, 1.5f},
     {16, 16, 4, 768, 3.0f, 0.6f, 1.2f},    {32, 32, 8, 256, 3.0f, 1.8f, 5.5f},
-    {64, 32, 4, 256, 3.0f, 1.55f, 3.6f}};
+    {64, 32, 4, 256, 3.0f, 1.55f, 3.6f},   {128, 128, 1, 256, 5.0f, 0.78f, 0.78f}};
 constexpr Shape kShapes32[kKernels] = {
     {16, 16, 4, 384, 2.3f, 0.33f, 0.5f},   {16, 32, 4, 256, 2.5f, 0.45f, 0.72f},
     {32, 32, 4, 256, 2.5f, 0.6f, 0.8f},    {64, 32, 4, 256, 0.f, 0.f, 0.f},
     {64, 128, 1, 256, 4.3f, 1.0f, 1.0f},   {128, 128, 1, 256, 5.0f, 1.9f, 1.9f},
     {128, 128, 1, 512, 0.f, 0.f, 0.f},     {256, 256, 1, 256, 0.f, 0.f, 0.f},
     {16, 16, 4, 768, 3.0f, 0.9f, 1.2f},    {32, 32, 8, 256, 3.0f, 2.0f, 5.5f},
-    {64, 32, 4, 256, 3.0f, 2.0f, 4.0f}};
+    {64, 32, 4, 256, 3.0f, 2.0f, 4.0f},    {128, 128, 1, 256, 5.0f, 2.15f, 2.15f}};
 
 // How a product is run: the kernel, which operands are copied to rows that start
 // at multiples of 16 bytes, the shares of the reduction.
@@ -900,9 +1013,10 @@ inline long copied_stride(int cols, int elem_size) {
 
 // The kernel and the shares with the least time by the table above; the shares'
 // sums cost a launch and their bytes.  `direct`: whole 16-byte pieces at aligned
-// addresses.  `bytes`: the workspace that is left for the shares.
-inline float choose(const Product& g, int elem_size, bool direct, size_t bytes,
-                    Plan* p) {
+// addresses; `tiled`: what kAnyTile128 takes.  `bytes`: the workspace that is left
+// for the shares.
+inline float choose(const Product& g, int elem_size, bool direct, bool tiled,
+                    size_t bytes, Plan* p) {
   const Shape* const shapes = elem_size == 2 ? kShapes16 : kShapes32;
   const int chunks = ceil_div(g.k, kChunkBytes / elem_size);
   // (operands that an L2 holds)
@@ -912,7 +1026,7 @@ inline float choose(const Product& g, int elem_size, bool direct, size_t bytes,
   for (int kernel = direct ? 0 : kAny16x16;
        kernel < (direct ? kAny16x16 : kKernels); ++kernel) {
     const Shape& s = shapes[kernel];
-    if (s.fixed == 0.f) continue;
+    if (s.fixed == 0.f || (kernel == kAnyTile128 && !tiled)) continue;
 #ifdef SNN_HIP_TUNING
     if (const char* only = std::getenv("SNN_HIP_EPI_KERNEL"))
       if (std::atoi(only) % kAny16x16 != kernel % kAny16x16) continue;
@@ -962,19 +1076,26 @@ inline Plan make_plan(const Product& g, int elem_size, size_t bytes,
   const int m = g.m, n = g.n, k = g.k;
   // Straight to LDS go whole 16-byte pieces, and tiles within 31 bits.
   const int chunk = kChunkBytes / elem_size;
+  auto tile = [&](bool k_inner, int rows, long stride) {
+    return memory_cols(k_inner, rows, k) * static_cast<long>(elem_size) >= 16 &&
+           (k_inner ? 256 : chunk) * stride * elem_size < 0x7FFF0000l;
+  };
   auto direct = [&](bool k_inner, bool aligned, int rows, long stride) {
     return aligned && stride * elem_size % 16 == 0 &&
            memory_cols(k_inner, rows, k) * static_cast<long>(elem_size) % 16 ==
                0 &&
-           (k_inner ? 256 : chunk) * stride * elem_size < 0x7FFF0000l;
+           tile(k_inner, rows, stride);
   };
   const bool p_direct = direct(g.p_k_inner, p_aligned, m, g.p_stride);
   const bool q_direct = direct(g.q_k_inner, q_aligned, n, g.q_stride);
   if (p_direct && q_direct) {
-    choose(g, elem_size, true, bytes, &p);
+    choose(g, elem_size, true, false, bytes, &p);
     return p;
   }
-  const float any = choose(g, elem_size, false, bytes, &p);
+  const float any = choose(g, elem_size, false,
+                           tile(g.p_k_inner, m, g.p_stride) &&
+                               tile(g.q_k_inner, n, g.q_stride),
+                           bytes, &p);
   auto copy_bytes = [&](bool k_inner, int rows) {
     return static_cast<size_t>(memory_rows(k_inner, rows, k)) *
            copied_stride(memory_cols(k_inner, rows, k), elem_size) * elem_size;
@@ -991,7 +1112,8 @@ inline Plan make_plan(const Product& g, int elem_size, size_t bytes,
   copied.q_bytes = q_bytes;
   // (a launch, and the operands read and written)
   const float with_copies =
-      choose(g, elem_size, true, bytes - p_bytes - q_bytes, &copied) + 3.f +
+      choose(g, elem_size, true, false, bytes - p_bytes - q_bytes, &copied) +
+      3.f +
       static_cast<float>(p_bytes + q_bytes) * 0.5e-6f;
 #ifdef SNN_HIP_TUNING
   if (const char* copy = std::getenv("SNN_HIP_EPI_COPY"))

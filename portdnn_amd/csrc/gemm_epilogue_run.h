@@ -10,7 +10,7 @@ namespace snn {
 namespace epi {
 
 template <typename T, bool PK, bool QK, int BM, int BN, int WM, int WN, int CB,
-          int STAGES>
+          int STAGES, int HELD>
 __global__ void __launch_bounds__(64 * WM * WN) gemm_kernel(Product g) {
 #ifdef __HIP_DEVICE_COMPILE__
   constexpr int kStage = Space<BM, BN, WM * WN, CB>::kStage;
@@ -30,14 +30,15 @@ __global__ void __launch_bounds__(64 * WM * WN) gemm_kernel(Product g) {
     __shared__ __align__(1024) char ring4[kStage];
     r4 = ring4;
   }
-  gemm_body<T, PK, QK, BM, BN, WM, WN, CB, STAGES>(g, ring0, ring1, r2, r3, r4);
+  gemm_body<T, PK, QK, BM, BN, WM, WN, CB, STAGES, HELD>(g, ring0, ring1, r2, r3,
+                                                         r4);
 #endif
 }
 
 template <typename T, bool PK, bool QK, int BM, int BN, int WM, int WN, int CB,
-          int STAGES>
+          int STAGES, int HELD = 0>
 int launch_as(const Product& g, hipStream_t stream) {
-  hipLaunchKernelGGL((gemm_kernel<T, PK, QK, BM, BN, WM, WN, CB, STAGES>),
+  hipLaunchKernelGGL((gemm_kernel<T, PK, QK, BM, BN, WM, WN, CB, STAGES, HELD>),
                      dim3(static_cast<unsigned>(g.tiles_m) * g.tiles_n * g.splits),
                      dim3(64 * WM * WN), 0, stream, g);
   SNN_HIP_CHECK_LAUNCH();
@@ -95,6 +96,11 @@ int launch_tile(const Product& g, int kernel, hipStream_t stream) {
       return launch_few<T, PK, QK, 32, 32, 8, 2, false>(g, stream);
     case kAny64x32:
       return launch_few<T, PK, QK, 64, 32, 4, 2, false>(g, stream);
+    case kAnyTile128:
+      // (4095 x 1023 x 1001 binary16: sixteen waves 18.4 us, eight 19.9, four 26; four
+      // chunks under way 21; copies of both operands and their products 25.7.  8191 x
+      // 4095 x 4095: 462 against 266 with copies)
+      return launch_as<T, PK, QK, 128, 128, 4, 4, 128, 2, 2>(g, stream);
     default:
       break;
   }
