@@ -519,6 +519,12 @@ def _step_stride(t):
     return step
 
 
+def _empty_like(t):
+    """A tensor of t's shape whose rows follow one another.  (Taking the layout
+    over is 0.6 us faster than a shape, of small calls of 8.)"""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 def _vector(t, n, dtype):
     """The address of an optional vector of n values."""
     if t is None:
@@ -672,11 +678,11 @@ def residual_norm(x, residual=None, gate=None, scale=None, post=NORM.NONE,
                                              dtype)
     if out is None:
         if keep_sum:
-            out = x.new_empty(shape)
+            out = _empty_like(x)
         sum_at = _at(out)
     else:
         sum_at = _like(out, shape, dtype)
-    normed = x.new_empty(shape) if pre != NORM.NONE else None
+    normed = _empty_like(x) if pre != NORM.NONE else None
     stats = (x.new_empty((rows, 4), dtype=torch.float32) if keep_stats
              else None)
     code = _native.residual_norm(
@@ -703,7 +709,7 @@ def residual_norm_grad(x, sum, stats, grad_sum=None, grad_normed=None,
     that are given."""
     rows, channels = shape = x.shape
     dtype = x.dtype
-    got = {"x": x.new_empty(shape), "residual": x.new_empty(shape)}
+    got = {"x": _empty_like(x), "residual": _empty_like(x)}
     gate_at, gate_stride = None, 0
     if gate is None:
         assert not gate_op, "an operation without a gate"
@@ -781,22 +787,30 @@ def linear_recurrence(x, forget, input_gate=None, resets=None, lengths=None,
     dtype = x.dtype
     stride, elems, resets_at, lengths_at = _recurrence_operands(
         x, forget, input_gate, resets, lengths)
+    state = (batch, channels)
     if out is None:
-        out = x.new_empty(shape)
+        out = _empty_like(x)
+        out_at = out.data_ptr()
+    else:
+        out_at = _like(out, shape, dtype)
+    initial_at = _like(initial_state, state, torch.float32)
     if final_state is None:
-        final_state = x.new_empty((batch, channels), dtype=torch.float32)
+        final_state = x.new_empty(state, dtype=torch.float32)
+        final_at = final_state.data_ptr()
+    elif final_state is initial_state:
+        final_at = initial_at
+    else:
+        final_at = _like(final_state, state, torch.float32)
     if workspace is None:
         if elems:
             workspace = x.new_empty(elems)
     else:
         elems = workspace.numel()
-    state = (batch, channels)
     code = _native.linear_recurrence(
         _address("snn_hip_linear_recurrence" + _TYPES[dtype][0]), x.data_ptr(),
         forget.data_ptr(), _at(input_gate), resets_at, lengths_at,
-        _like(initial_state, state, torch.float32), _like(out, shape, dtype),
-        _like(final_state, state, torch.float32), batch, steps, channels,
-        stride, 0, _at(workspace), elems, _stream())
+        initial_at, out_at, final_at, batch, steps, channels, stride, 0,
+        _at(workspace), elems, _stream())
     if code:
         capi.check(code)
     return out, final_state
@@ -816,7 +830,7 @@ def linear_recurrence_grad(grad, x, forget, h, input_gate=None, resets=None,
         x, forget, input_gate, resets, lengths)
     names = ["x", "forget"] + (["input_gate"] if input_gate is not None else [])
     if out is None:
-        got = {name: x.new_empty(shape) for name in names}
+        got = {name: _empty_like(x) for name in names}
         grad_stride = channels
     else:
         assert out.shape == (batch, steps, channels * len(names)) and \
