@@ -108,11 +108,9 @@ __device__ __forceinline__ unsigned long long resets_of(const Recurrence& r,
 
 // ---- undivided ---------------------------------------------------------------
 
-// Steps whose loads are in flight together: 8 forward; the gradients, with five
-// operands, keep more waves on a SIMD with 4 (4 x 4096 x 2048 binary16: 176 ->
-// 147 us).
-template <bool BACK>
-constexpr int kSteps = BACK ? 4 : 8;
+// Steps whose loads are in flight together.  (64 sequences of 48 x 256 bfloat16
+// forward: 14.8 us, with 8 of them 16.4; 2048 of 64 x 1024: 227 and 222.)
+constexpr int kSteps = 4;
 
 // What a wave needs of its place: sequence and first channel of the lane.  (Lanes
 // behind a row's channels stay, and store nothing.)
@@ -139,7 +137,7 @@ __device__ __forceinline__ Place place_of(const Recurrence& r) {
 template <typename T, int VEC, bool GATE>
 __global__ void __launch_bounds__(256) recurrence_walk_kernel(Recurrence r) {
   typedef typename Pack<T, VEC>::type V;
-  constexpr int kGroup = kSteps<false>;
+  constexpr int kGroup = kSteps;
   const Place p = place_of<VEC>(r);
   if (p.b >= r.batch) return;
   const long row = static_cast<long>(p.b) * r.steps;
@@ -197,7 +195,7 @@ __global__ void __launch_bounds__(256) recurrence_walk_kernel(Recurrence r) {
 template <typename T, int VEC, bool GATE>
 __global__ void __launch_bounds__(256) recurrence_grad_kernel(Recurrence r) {
   typedef typename Pack<T, VEC>::type V;
-  constexpr int kGroup = kSteps<true>;
+  constexpr int kGroup = kSteps;
   const Place p = place_of<VEC>(r);
   if (p.b >= r.batch) return;
   const long row = static_cast<long>(p.b) * r.steps;
@@ -628,10 +626,20 @@ constexpr int kWaves = BACK ? 16 : 12;
 template <bool BACK>
 constexpr int kSegment = BACK ? 8 : 12;
 
-// A sequence is divided where its lanes alone are fewer than this many waves, and
-// where it is long enough for the second launch.
-constexpr int kWantedWaves = 4096;
-constexpr int kLeastSteps = 65;
+// A sequence is divided where there are fewer waves of lanes than this, and where
+// it is long enough for the second launch.  bfloat16 of 1024 channels, us divided
+// and whole, forward | gradients:
+//
+//   4 sequences of 32 steps    13, 11 |  13,  22
+//   4 of 64                    14, 21 |  16,  41
+//   64 of 66                   18, 23 |  22,  48
+//   256 of 128                 71, 60 | 112, 132
+//   512 of 128               131, 109 | 209, 214
+//   1000 of 128              238, 212 | 398, 380
+template <bool BACK>
+constexpr int kWantedWaves = BACK ? 2048 : 512;
+template <bool BACK>
+constexpr int kLeastSteps = BACK ? 24 : 48;
 
 struct Division {
   int segments, pieces;  // pieces == 0: undivided
@@ -643,7 +651,8 @@ Division divide(const snn_hip_linear_recurrence_params& p) {
   constexpr int VEC = kVec<T>;
   d.rows = static_cast<size_t>(p.batch) * ceil_div(p.channels, 64 * VEC);
   d.segments = ceil_div(p.steps, kSegment<BACK>);
-  if (p.channels < VEC || d.rows >= kWantedWaves || p.steps < kLeastSteps)
+  if (p.channels < VEC || d.rows >= kWantedWaves<BACK> ||
+      p.steps < kLeastSteps<BACK>)
     return d;
   d.pieces = ceil_div(d.segments, kWaves<BACK>);
   const size_t places = d.rows * d.pieces;
