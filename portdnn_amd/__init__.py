@@ -1,5 +1,7 @@
 """portdnn_amd: MI355X (gfx950) implementation of portDNN's convolution,
-depthwise-convolution and pooling hot path.
+depthwise-convolution and pooling hot path, and of operators of language
+models over sequences (a matrix product with its epilogue, norms around a
+block, a gated linear recurrence; forward and gradients).
 
 The product is the C-ABI shared library ``libsnn_hip.so`` (declared in
 ``include/snn_hip.h``) and the C++ drop-in headers under ``include/portdnn``.

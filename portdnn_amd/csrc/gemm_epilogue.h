@@ -23,13 +23,25 @@
 // 16-byte pieces are XOR-swizzled so that lanes that read together fall into
 // different banks (swizzle() below).  Where rows start at multiples of 16 bytes
 // the loads go from memory straight to LDS and the swizzle is applied to their
-// source; elsewhere they pass through registers, so that odd sizes cost no copy.
+// source; elsewhere they pass through registers, or the operand is copied first to
+// aligned rows, whichever the estimate finds faster.
 //
 // Q is the instruction's A operand, so a lane ends up with four neighbouring
 // columns of a row.  The tile leaves through LDS, each wave's part in its own
 // place: there a lane picks up eight neighbouring columns, for which the bias, the
 // residual, the activation and the rounding are one piece of code, and stores
 // whole rows.
+//
+// Products of a few rows are bound by the bytes of Q, large ones by the matrix
+// instructions, those between by their first chunks' way from memory and by the
+// way out, which nothing overlaps where the tiles fill the GPU once.  Measured:
+//
+//   1 x 2048 x 8192 bfloat16, silu      9.5 us    34 MB at 3.5 TB/s
+//   24 x 4096 x 4096 binary16           8.9 us    34 MB at 3.8 TB/s
+//   4095 x 1023 x 1001 binary16, gelu  20.9 us    402 TFLOP/s
+//   4096 x 1024 x 1024 fp32            68.7 us    125 TFLOP/s
+//   8192 x 4096 x 8192 bfloat16        411-441 us 1.25-1.34 PFLOP/s; 468 with
+//                                      gelu_tanh and what it is taken of stored
 #ifndef PORTDNN_AMD_CSRC_GEMM_EPILOGUE_H_
 #define PORTDNN_AMD_CSRC_GEMM_EPILOGUE_H_
 
@@ -253,9 +265,10 @@ __device__ __forceinline__ void leave(const Product& g, unsigned split, int row,
   }
   float* const to =
       g.partial + (static_cast<long>(split) * g.m + row) * g.n + col;
-  if (g.n % 8 == 0) {
-    *reinterpret_cast<float4v*>(to) = float4v{v[0], v[1], v[2], v[3]};
-    *reinterpret_cast<float4v*>(to + 4) = float4v{v[4], v[5], v[6], v[7]};
+  if (col + 8 <= g.n) {
+    typedef seq::Pack<float, 4>::type F;  // (rows may start anywhere)
+    *reinterpret_cast<F*>(to) = F{v[0], v[1], v[2], v[3]};
+    *reinterpret_cast<F*>(to + 4) = F{v[4], v[5], v[6], v[7]};
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -922,7 +935,8 @@ __device__ __forceinline__ void gemm_few_body(const Product& g, char* r0,
   }
 }
 
-// Adds the shares of a divided reduction in their order and finishes.
+// Adds the shares of a divided reduction in their order and finishes.  (14 x 3490 x
+// 876 fp32 in eight shares 13.7 us; one share after another 19.1)
 template <typename T>
 __global__ void __launch_bounds__(256) gemm_join_kernel(Product g) {
   const int groups = (g.n + 7) / 8;
@@ -932,24 +946,40 @@ __global__ void __launch_bounds__(256) gemm_join_kernel(Product g) {
   if (row >= g.m) return;
   const long size = static_cast<long>(g.m) * g.n;
   const float* from = g.partial + static_cast<long>(row) * g.n + col;
+  // Four shares at a time, all of whose loads are under way together: behind the
+  // last share that one again, which is not added.
+  constexpr int kBatch = 4;
+  const int last = g.n - 1 - col;
   float v[8] = {};
-  if (g.n % 8 == 0) {
-#pragma unroll 4
-    for (int s = 0; s < g.splits; ++s) {
-      const float4v a = *reinterpret_cast<const float4v*>(from + s * size);
-      const float4v b = *reinterpret_cast<const float4v*>(from + s * size + 4);
+  auto add = [&](auto fetch) {
+    for (int s0 = 0; s0 < g.splits; s0 += kBatch) {
+      float part[kBatch][8];
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u)
+        fetch(from + min(s0 + u, g.splits - 1) * size, part[u]);
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (s0 + u < g.splits) v[i] += part[u][i];
+    }
+  };
+  if (last >= 7)
+    add([](const float* share, float (&to)[8]) {
+      typedef seq::Pack<float, 4>::type F;  // (rows may start anywhere)
+      const F a = *reinterpret_cast<const F*>(share);
+      const F b = *reinterpret_cast<const F*>(share + 4);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        v[i] += a[i];
-        v[4 + i] += b[i];
+        to[i] = a[i];
+        to[4 + i] = b[i];
       }
-    }
-  } else {
-    for (int s = 0; s < g.splits; ++s)
+    });
+  else
+    add([&](const float* share, float (&to)[8]) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (col + i < g.n) v[i] += from[s * size + i];
-  }
+      for (int i = 0; i < 8; ++i) to[i] = share[min(i, last)];
+    });
   finish8<T>(g, row, col, v);
 }
 
@@ -1022,6 +1052,10 @@ inline float choose(const Product& g, int elem_size, bool direct, bool tiled,
   // (operands that an L2 holds)
   const bool cached = (static_cast<double>(g.m) + g.n) * g.k * elem_size < 4e6;
   const float share_mb = static_cast<float>(g.m) * g.n * 4e-6f;
+  // (the operands at 4.2 TB/s, which no division makes faster: 24 x 4096 x 4096
+  // binary16 takes 8.7 us whole, 10.7 in two shares)
+  const float memory =
+      1.f + (static_cast<float>(g.m) + g.n) * g.k * elem_size / 4.2e6f;
   float best = -1.f;
   for (int kernel = direct ? 0 : kAny16x16;
        kernel < (direct ? kAny16x16 : kKernels); ++kernel) {
@@ -1053,9 +1087,10 @@ inline float choose(const Product& g, int elem_size, bool direct, bool tiled,
       float step = g.q_k_inner ? s.step_k : s.step_row;
       if (s.chunks > 1 && cached) step *= 0.6f;
       const float time =
-          static_cast<float>(std::ceil(rounds)) * s.fixed +
-          static_cast<float>(rounds) * steps * step +
-          (splits > 1 ? 2.f + 0.55f * share_mb * splits : 0.f);
+          std::max(static_cast<float>(std::ceil(rounds)) * s.fixed +
+                       static_cast<float>(rounds) * steps * step,
+                   memory) +
+          (splits > 1 ? 2.2f + (0.2f + 0.5f * share_mb) * splits : 0.f);
       if (best < 0.f || time < best) {
         best = time;
         p->kernel = kernel;

@@ -128,7 +128,8 @@ int launch_tile(const Product& g, int kernel, hipStream_t stream) {
   return SNN_HIP_INVALID_ALGORITHM;
 }
 
-// One operand on its way to rows that start at multiples of 16 bytes.
+// One operand on its way to rows that start at multiples of 16 bytes.  (4095 x 1023
+// and 1023 x 1001 binary16: 5.5-10 us, 21 MB read and written.)
 struct Copy {
   const void* in;
   void* out;

