@@ -56,8 +56,11 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES)
   // through LDS)
   constexpr int kTeams = WAVES == 1 ? 4 : 1;
   // (sixteen waves have 128 registers each: none for a row on its way and the
-  // weights)
+  // weights, and LDS holds as many of the sums as fit: 4096 x 8192 fp32 194 us,
+  // with all in registers, of which 65 go to memory, 275)
   constexpr bool kLean = WAVES == 16;
+  constexpr int kInLds = !kLean ? 0 : PT == 8 ? (kOwn < 4 ? kOwn : 4) : 2;
+  __shared__ float own_sums[kLean ? kInLds * PT * 64 * WAVES : 1];
   __shared__ float lds[WAVES == 1 ? 4 * 64 * PT : 4 * WAVES];
   int turn = 0;
   const int channels = r.channels;
@@ -65,19 +68,36 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES)
   const int team = WAVES == 1 ? static_cast<int>(threadIdx.x >> 6) : 0;
   const bool pre = d.g.grad_normed != nullptr;
   float sums[kOwn][PT], gate_sum[SHARED ? PT : 1];
+  auto place = [&](int s, int i) -> float& {
+    return own_sums[(s * PT + i) * (64 * WAVES) + threadIdx.x];
+  };
 #pragma unroll
   for (int s = 0; s < kOwn; ++s)
 #pragma unroll
-    for (int i = 0; i < PT; ++i) sums[s][i] = 0.f;
+    for (int i = 0; i < PT; ++i) {
+      if (s < kInLds)
+        place(s, i) = 0.f;
+      else
+        sums[s][i] = 0.f;
+    }
+  auto add = [&](int s, int i, float v) {
+    if (s < kInLds)
+      place(s, i) += v;
+    else
+      sums[s][i] += v;
+  };
   V pre_weight[S::kAccesses], post_weight[S::kAccesses],
       post_bias[S::kAccesses], scale[S::kAccesses];
-  auto fetch_weights = [&]() {
-    S::fetch(r.t.pre_weight, channels, pre_weight, 1.f);
+  auto fetch_pre = [&]() { S::fetch(r.t.pre_weight, channels, pre_weight, 1.f); };
+  auto fetch_post = [&]() {
     S::fetch(r.t.post_weight, channels, post_weight, 1.f);
     S::fetch(r.t.post_bias, channels, post_bias);
     S::fetch(r.t.scale, channels, scale, 1.f);
   };
-  if constexpr (!kLean) fetch_weights();
+  if constexpr (!kLean) {
+    fetch_pre();
+    fetch_post();
+  }
 
   // The teams' sums together, in the first team's registers.
   auto gather = [&](float (&v)[PT]) {
@@ -142,7 +162,7 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES)
       const long at = row * channels;
       if constexpr (kLean) {
         fetch_row(row);
-        fetch_weights();
+        fetch_pre();
       }
       float dy[PT], xh[PT], u[PT], yh[PT], gate[PT];
       S::expand(next_d, channels, dy);
@@ -163,8 +183,8 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES)
 #pragma unroll
         for (int i = 0; i < PT; ++i) {
           yh[i] = S::inside(i, channels) ? (yh[i] - mean1) * rstd1 : 0.f;
-          sums[kPreWeight][i] += u[i] * yh[i];
-          if constexpr (BIASES) sums[kPreBias][i] += u[i];
+          add(kPreWeight, i, u[i] * yh[i]);
+          if constexpr (BIASES) add(kPreBias, i, u[i]);
           u[i] *= w[i];
           m[0] += u[i] * yh[i];
           m[1] += u[i];
@@ -179,6 +199,7 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES)
       }
       if (d.g.grad_residual != nullptr)
         S::store(static_cast<T*>(d.g.grad_residual) + at, channels, dy);
+      if constexpr (kLean) fetch_post();
 
       // n, of which the gate and the scale have their gradients
       float n[PT], s[PT];
@@ -220,10 +241,10 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES)
       float m[2] = {0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < PT; ++i) {
-        sums[kScale][i] += dy[i] * n[i];
+        add(kScale, i, dy[i] * n[i]);
         dy[i] *= s[i];
-        sums[kPostWeight][i] += dy[i] * xh[i];
-        if constexpr (BIASES) sums[kPostBias][i] += dy[i];
+        add(kPostWeight, i, dy[i] * xh[i]);
+        if constexpr (BIASES) add(kPostBias, i, dy[i]);
         dy[i] *= w[i];
         m[0] += dy[i] * xh[i];
         m[1] += dy[i];
@@ -260,6 +281,10 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES)
       d.sums + static_cast<long>(blockIdx.x) * kOwn * channels;
 #pragma unroll
   for (int s = 0; s < kOwn; ++s) {
+    if (s < kInLds) {
+#pragma unroll
+      for (int i = 0; i < PT; ++i) sums[s][i] = place(s, i);
+    }
     gather(sums[s]);
     if (team == 0) store_floats(to + static_cast<long>(s) * channels, sums[s]);
   }
@@ -393,8 +418,14 @@ int residual_norm_grad(const snn_hip_residual_norm_tensors* tensors,
     return launch_as<T, 1, 8, 1, true>(r, d, as_stream(stream));
   return norm::by_channels<VEC>(
       r.channels, [&](auto waves, auto values, auto whole) {
-        return launch_as<T, VEC, decltype(values)::value,
-                         decltype(waves)::value, decltype(whole)::value>(
+        // (the long rows' kernels have no registers for accesses that begin in
+        // front of what is theirs: 256 x 7195 fp32 75 us, value by value 50, and
+        // 36 since LDS holds sums)
+        constexpr bool kSingly = decltype(waves)::value == 16 &&
+                                 !decltype(whole)::value;
+        return launch_as<T, kSingly ? 1 : VEC, decltype(values)::value,
+                         decltype(waves)::value,
+                         kSingly || decltype(whole)::value>(
             r, d, as_stream(stream));
       });
 }
