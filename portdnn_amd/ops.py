@@ -109,6 +109,16 @@ def _at(t):
     return None if t is None else t.data_ptr()
 
 
+def _room(workspace, t):
+    """The elements of t's type that a caller's workspace, of whatever type, has
+    memory for: what the entry points count a workspace in."""
+    assert workspace.is_contiguous(), "a workspace that is not contiguous"
+    n = workspace.numel()
+    if workspace.dtype is t.dtype:
+        return n
+    return n * workspace.element_size() // t.element_size()
+
+
 def workspace_size(p, direction, algorithm, dtype=None):
     """(required, recommended) elements; with a capi.DTYPE the element type's
     own answer (snn_hip_conv2d_workspace_size_for)."""
@@ -202,9 +212,9 @@ _CONV_FN = {
 def conv2d_raw(inp, fil, out, p, direction, algorithm, workspace=None):
     """Calls the entry point and returns its status code (no exception)."""
     fn = getattr(capi.lib(), _CONV_FN[(direction, inp.dtype)])
-    ws_elems = 0 if workspace is None else workspace.numel()
     return fn(_ptr(inp), _ptr(fil), _ptr(out), ctypes.byref(p), algorithm,
-              _ptr(workspace), ws_elems, _stream())
+              _ptr(workspace),
+              0 if workspace is None else _room(workspace, inp), _stream())
 
 
 def conv2d(inp, fil, p, direction=DIRECTION.FORWARD, algorithm=ALGO.DIRECT,
@@ -223,7 +233,8 @@ def conv2d(inp, fil, p, direction=DIRECTION.FORWARD, algorithm=ALGO.DIRECT,
     code = _native.conv2d(
         _address(_CONV_FN[direction, dtype]), direction, inp.data_ptr(),
         inp.numel(), fil.data_ptr(), fil.numel(), out.data_ptr(), p, algorithm,
-        _at(workspace), 0 if workspace is None else workspace.numel(), _stream())
+        _at(workspace), 0 if workspace is None else _room(workspace, out),
+        _stream())
     if code:
         capi.check(code)
     return out
@@ -249,7 +260,7 @@ def conv2d_bound(inp, fil, out, p, direction, algorithm, workspace=None):
     fn = getattr(capi.lib(), _CONV_FN[(direction, inp.dtype)])
     return _bind(fn, _ptr(inp), _ptr(fil), _ptr(out), ctypes.byref(p),
                  algorithm, _ptr(workspace),
-                 0 if workspace is None else workspace.numel(),
+                 0 if workspace is None else _room(workspace, inp),
                  ctypes.c_void_p(_stream()))
 
 
@@ -258,7 +269,7 @@ def conv2d_prepared_bound(inp, fil, out, p, direction, algorithm, workspace):
     return _bind(capi.lib().snn_hip_conv2d_prepared_f32, direction, _ptr(inp),
                  _ptr(fil), _ptr(out), ctypes.byref(p), algorithm,
                  _ptr(workspace),
-                 0 if workspace is None else workspace.numel(),
+                 0 if workspace is None else _room(workspace, inp),
                  ctypes.c_void_p(_stream()))
 
 
@@ -267,7 +278,7 @@ def conv2d_prepare_filter(fil, p, direction, algorithm, workspace):
     filter alone goes into `workspace`."""
     capi.check(capi.lib().snn_hip_conv2d_prepare_filter_f32(
         direction, _ptr(fil), ctypes.byref(p), algorithm, _ptr(workspace),
-        0 if workspace is None else workspace.numel(), _stream()))
+        0 if workspace is None else _room(workspace, fil), _stream()))
 
 
 def conv2d_prepared(inp, fil, p, direction, algorithm, workspace, out=None):
@@ -278,7 +289,7 @@ def conv2d_prepared(inp, fil, p, direction, algorithm, workspace, out=None):
         out = torch.empty(n_out, dtype=inp.dtype, device=inp.device)
     capi.check(capi.lib().snn_hip_conv2d_prepared_f32(
         direction, _ptr(inp), _ptr(fil), _ptr(out), ctypes.byref(p), algorithm,
-        _ptr(workspace), 0 if workspace is None else workspace.numel(),
+        _ptr(workspace), 0 if workspace is None else _room(workspace, inp),
         _stream()))
     return out
 
@@ -296,7 +307,7 @@ def conv2d_deterministic(inp, fil, p, direction, algorithm, workspace=None,
             workspace = torch.empty(rec, dtype=inp.dtype, device=inp.device)
     capi.check(capi.lib().snn_hip_conv2d_deterministic_f32(
         direction, _ptr(inp), _ptr(fil), _ptr(out), ctypes.byref(p), algorithm,
-        _ptr(workspace), 0 if workspace is None else workspace.numel(),
+        _ptr(workspace), 0 if workspace is None else _room(workspace, inp),
         _stream()))
     return out
 
@@ -313,7 +324,8 @@ def conv2d_bias_act(inp, fil, bias, p, algorithm, relu=True, workspace=None,
     code = _native.conv2d_bias_act(
         _address("snn_hip_conv2d_forward_bias_act_f32"), _at(inp), _at(fil),
         _at(bias), out.data_ptr(), p, algorithm, 1 if relu else 0,
-        _at(workspace), 0 if workspace is None else workspace.numel(), _stream())
+        _at(workspace), 0 if workspace is None else _room(workspace, out),
+        _stream())
     if code:
         capi.check(code)
     return out
@@ -611,7 +623,7 @@ def matmul_bias_act(a, b, bias=None, residual=None,
         if elems:
             workspace = a.new_empty(elems)
     else:
-        elems = workspace.numel()
+        elems = _room(workspace, a)
     code = _native.matmul_bias_act(
         fn, a.data_ptr(), b.data_ptr(), _vector(bias, n, dtype), add,
         out.data_ptr(), _at(z), m, k, n, trans_a, trans_b, activation, a_stride,
@@ -641,7 +653,7 @@ def matmul_bias_act_grad(grad, a, b, pre_activation=None,
         if elems:
             workspace = a.new_empty(elems)
     else:
-        elems = workspace.numel()
+        elems = _room(workspace, a)
     code = _native.matmul_bias_act_grad(
         fn, grad.data_ptr(), a.data_ptr(), b.data_ptr(),
         _like(pre_activation, (m, n), dtype), _at(grad_a), _at(grad_b),
@@ -737,6 +749,8 @@ def residual_norm_grad(x, sum, stats, grad_sum=None, grad_normed=None,
                 ResidualNormParams(rows=rows, channels=channels, gate=gate_op,
                                    gate_rows=gate_rows), _TYPES[dtype][1]))
         workspace = x.new_empty(elems)
+    else:
+        elems = _room(workspace, x)
     code = _native.residual_norm_grad(
         _address("snn_hip_residual_norm_grad" + _TYPES[dtype][0]),
         x.data_ptr(), None, gate_at, addresses["scale"],
@@ -750,7 +764,7 @@ def residual_norm_grad(x, sum, stats, grad_sum=None, grad_normed=None,
         _at(got.get("post_bias")), _at(got.get("pre_weight")),
         _at(got.get("pre_bias")), rows, channels, post, pre, gate_op, gate_rows,
         _row_stride(x), gate_stride, eps, workspace.data_ptr(),
-        workspace.numel(), _stream())
+        elems, _stream())
     if code:
         capi.check(code)
     return got
@@ -805,7 +819,7 @@ def linear_recurrence(x, forget, input_gate=None, resets=None, lengths=None,
         if elems:
             workspace = x.new_empty(elems)
     else:
-        elems = workspace.numel()
+        elems = _room(workspace, x)
     code = _native.linear_recurrence(
         _address("snn_hip_linear_recurrence" + _TYPES[dtype][0]), x.data_ptr(),
         forget.data_ptr(), _at(input_gate), resets_at, lengths_at,
@@ -843,7 +857,7 @@ def linear_recurrence_grad(grad, x, forget, h, input_gate=None, resets=None,
         if elems:
             workspace = x.new_empty(elems)
     else:
-        elems = workspace.numel()
+        elems = _room(workspace, x)
     state = (batch, channels)
     code = _native.linear_recurrence_grad(
         _address("snn_hip_linear_recurrence_grad" + _TYPES[dtype][0]),
