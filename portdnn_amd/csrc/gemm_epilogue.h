@@ -165,8 +165,11 @@ __device__ __forceinline__ float activation_slope(float z, int kind) {
       float s, rest;
       seq::sigmoid<float>(
           1.5957691216057308f * (z + 0.044715f * z * z * z), &s, &rest);
-      return s + z * s * rest * 1.5957691216057308f *
-                     (1.f + 0.134145f * z * z);
+      // (s * rest is exactly zero long before |z| = 64, and would be multiplied by an
+      // infinite z^2 from 1.8e19 on)
+      const float near = fminf(fmaxf(z, -64.f), 64.f);
+      return s + near * s * rest * 1.5957691216057308f *
+                     (1.f + 0.134145f * near * near);
     }
     case SNN_HIP_ACTIVATION_SILU: {
       float s, rest;
