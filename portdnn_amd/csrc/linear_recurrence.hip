@@ -74,10 +74,26 @@ struct Recurrence {
 template <typename T>
 constexpr int kVec = sizeof(T) == 2 ? 4 : 2;
 
-// A piece with a reset has A = -0, which the factors behind it leave as it is; a
-// product that has only become too small is +0.
+// The gate a of a logit, with 1 - a where it is asked for.  Above zero, as sigmoid
+// is: an infinite state stays infinite behind a gate that fp32 has no value for.
+template <typename T>
+__device__ __forceinline__ float gate_of(float z) {
+  return sigmoid_alone<T>(z) + 0x1p-126f;
+}
+template <typename T>
+__device__ __forceinline__ void gate_of(float z, float* a, float* rest) {
+  sigmoid<T>(z, a, rest);
+  *a += 0x1p-126f;
+}
+
+// A run of steps with a reset has A = -0, which the factors behind it leave as it
+// is; products that become too small are the smallest value above zero, for the same
+// reason (as bits: zero has none set).
 __device__ __forceinline__ bool is_reset(float a) {
   return __float_as_uint(a) == 0x80000000u;
+}
+__device__ __forceinline__ float above_zero(float a) {
+  return __uint_as_float(max(__float_as_uint(a), 1u));
 }
 __device__ __forceinline__ float composed(float a, float s, float state) {
   return is_reset(a) ? s : a * state + s;
@@ -180,10 +196,10 @@ __global__ void __launch_bounds__(256) recurrence_walk_kernel(Recurrence r) {
       for (int k = 0; k < VEC; ++k) {
         float a, w;
         if (GATE) {
-          a = sigmoid_alone<T>(fs[k]);
+          a = gate_of<T>(fs[k]);
           w = sigmoid_alone<T>(is[k]);
         } else {
-          sigmoid<T>(fs[k], &a, &w);
+          gate_of<T>(fs[k], &a, &w);
         }
         state[k] = w * xs[k] + (fresh(u) ? 0.f : a * state[k]);
       }
@@ -263,7 +279,7 @@ __global__ void __launch_bounds__(256) recurrence_grad_kernel(Recurrence r) {
 #pragma unroll
       for (int k = 0; k < VEC; ++k) {
         float a, rest, w, w_rest;
-        sigmoid<T>(fs[k], &a, &rest);
+        gate_of<T>(fs[k], &a, &rest);
         if (GATE) {
           sigmoid<T>(is[k], &w, &w_rest);
         } else {
@@ -468,9 +484,9 @@ __global__ void __launch_bounds__(64 * WAVES)
     for (int k = 0; k < VEC; ++k) {
       float a, w;
       if (BACK || GATE)
-        a = sigmoid_alone<T>(fs[k]);
+        a = gate_of<T>(fs[k]);
       else
-        sigmoid<T>(fs[k], &a, &w);
+        gate_of<T>(fs[k], &a, &w);
       if (BACK) {
         if (counts) {
           S[k] = fresh(u) ? 0.f : a * (xs[k] + S[k]);
@@ -490,6 +506,7 @@ __global__ void __launch_bounds__(64 * WAVES)
   }
 #pragma unroll
   for (int k = 0; k < VEC; ++k) {
+    A[k] = above_zero(A[k]);
     seg_a[wave][k][lane] = A[k];
     seg_s[wave][k][lane] = S[k];
   }
@@ -504,7 +521,7 @@ __global__ void __launch_bounds__(64 * WAVES)
       for (int k = 0; k < VEC; ++k) {
         const float a = seg_a[w][k][lane];
         S[k] = composed(a, seg_s[w][k][lane], S[k]);
-        A[k] = is_reset(a) ? a : a * A[k];
+        A[k] = is_reset(a) ? a : above_zero(a * A[k]);
       }
     const long place = static_cast<long>(row) * r.pieces + piece;
     const long word = place * (64 * VEC) + static_cast<long>(lane) * VEC;
@@ -595,7 +612,7 @@ __global__ void __launch_bounds__(64 * WAVES)
 #pragma unroll
         for (int k = 0; k < VEC; ++k) {
           float a, rest, w, w_rest;
-          sigmoid<T>(fs[k], &a, &rest);
+          gate_of<T>(fs[k], &a, &rest);
           if (GATE)
             sigmoid<T>(is[k], &w, &w_rest);
           else
