@@ -96,7 +96,11 @@ def _struct(name, fields, defaults, types={}):
         def __init__(self, **kw):
             super().__init__()
             for f in fields:
-                setattr(self, f, kw.pop(f, defaults.get(f, 0)))
+                v = kw.pop(f, defaults.get(f, 0))
+                # (ctypes cuts numbers off that a field does not hold)
+                if f not in types and not -1 << 31 <= v < 1 << 31:
+                    raise OverflowError("%s: %d is beyond 31 bits" % (f, v))
+                setattr(self, f, v)
             if kw:
                 raise TypeError("unknown fields: %s" % sorted(kw))
 

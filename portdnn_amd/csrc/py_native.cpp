@@ -13,6 +13,7 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <climits>
 #include <cstddef>
 #include <cstdint>
 
@@ -50,6 +51,10 @@ class Args {
     if (!ok) return 0;
     const long v = PyLong_AsLong(o);
     if (v == -1 && PyErr_Occurred()) ok = false;
+    if (ok && (v < INT_MIN || v > INT_MAX)) {
+      PyErr_Format(PyExc_OverflowError, "%ld is beyond 31 bits", v);
+      ok = false;
+    }
     return static_cast<int>(v);
   }
   double real() {
