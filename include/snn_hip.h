@@ -555,7 +555,8 @@ SNN_HIP_API int snn_hip_binaryop_f16(const void* lhs, const void* rhs,
  * in place); no other operand may overlap an output.
  *
  * Every dimension is positive and every row shorter than 2^30 bytes; tensors
- * may be of any size beyond that.  A workspace of the recommended size lets
+ * may be of any size beyond that, as far as a grid holds the output's tiles
+ * (SNN_HIP_INDEX_EXCEEDED; from 2^35 values on).  A workspace of the recommended size lets
  * products with few output tiles share their reduction between work-groups (the
  * parts are added in a fixed order: two calls with the same arguments, workspace
  * included, return the same bits) and holds copies of operands whose rows do not

@@ -1008,24 +1008,25 @@ enum Kernel {
 // What the choice goes by, measured: microseconds of a round of `slots`
 // work-groups that does not go into its steps, and of a step (`chunks` 128-byte
 // chunks of the reduction) with Q K inner and row inner; 0: not for this type.
+// `waves` of a work-group, at most.
 struct Shape {
-  int bm, bn, chunks, slots;
+  int bm, bn, chunks, slots, waves;
   float fixed, step_k, step_row;
 };
 constexpr Shape kShapes16[kKernels] = {
-    {16, 16, 4, 384, 2.3f, 0.43f, 0.6f},   {16, 32, 4, 256, 2.5f, 0.49f, 0.62f},
-    {32, 32, 4, 256, 2.5f, 0.42f, 0.7f},   {64, 32, 4, 256, 2.8f, 0.55f, 0.88f},
-    {64, 128, 1, 256, 4.3f, 0.24f, 0.24f}, {128, 128, 1, 256, 5.2f, 0.42f, 0.42f},
-    {128, 128, 1, 512, 5.0f, 0.92f, 0.92f}, {256, 256, 1, 256, 8.0f, 1.5f, 1.5f},
-    {16, 16, 4, 768, 3.0f, 0.6f, 1.2f},    {32, 32, 8, 256, 3.0f, 1.8f, 5.5f},
-    {64, 32, 4, 256, 3.0f, 1.55f, 3.6f},   {128, 128, 1, 256, 5.0f, 0.78f, 0.78f}};
+    {16, 16, 4, 384, 4, 2.3f, 0.43f, 0.6f}, {16, 32, 4, 256, 4, 2.5f, 0.49f, 0.62f},
+    {32, 32, 4, 256, 4, 2.5f, 0.42f, 0.7f}, {64, 32, 4, 256, 4, 2.8f, 0.55f, 0.88f},
+    {64, 128, 1, 256, 8, 4.3f, 0.24f, 0.24f}, {128, 128, 1, 256, 8, 5.2f, 0.42f, 0.42f},
+    {128, 128, 1, 512, 8, 5.0f, 0.92f, 0.92f}, {256, 256, 1, 256, 16, 8.0f, 1.5f, 1.5f},
+    {16, 16, 4, 768, 4, 3.0f, 0.6f, 1.2f}, {32, 32, 8, 256, 8, 3.0f, 1.8f, 5.5f},
+    {64, 32, 4, 256, 4, 3.0f, 1.55f, 3.6f}, {128, 128, 1, 256, 16, 5.0f, 0.78f, 0.78f}};
 constexpr Shape kShapes32[kKernels] = {
-    {16, 16, 4, 384, 2.3f, 0.33f, 0.5f},   {16, 32, 4, 256, 2.5f, 0.45f, 0.72f},
-    {32, 32, 4, 256, 2.5f, 0.6f, 0.8f},    {64, 32, 4, 256, 0.f, 0.f, 0.f},
-    {64, 128, 1, 256, 4.3f, 1.0f, 1.0f},   {128, 128, 1, 256, 5.0f, 1.9f, 1.9f},
-    {128, 128, 1, 512, 0.f, 0.f, 0.f},     {256, 256, 1, 256, 0.f, 0.f, 0.f},
-    {16, 16, 4, 768, 3.0f, 0.9f, 1.2f},    {32, 32, 8, 256, 3.0f, 2.0f, 5.5f},
-    {64, 32, 4, 256, 3.0f, 2.0f, 4.0f},    {128, 128, 1, 256, 5.0f, 2.15f, 2.15f}};
+    {16, 16, 4, 384, 4, 2.3f, 0.33f, 0.5f}, {16, 32, 4, 256, 4, 2.5f, 0.45f, 0.72f},
+    {32, 32, 4, 256, 4, 2.5f, 0.6f, 0.8f}, {64, 32, 4, 256, 4, 0.f, 0.f, 0.f},
+    {64, 128, 1, 256, 8, 4.3f, 1.0f, 1.0f}, {128, 128, 1, 256, 8, 5.0f, 1.9f, 1.9f},
+    {128, 128, 1, 512, 8, 0.f, 0.f, 0.f}, {256, 256, 1, 256, 8, 0.f, 0.f, 0.f},
+    {16, 16, 4, 768, 4, 3.0f, 0.9f, 1.2f}, {32, 32, 8, 256, 8, 3.0f, 2.0f, 5.5f},
+    {64, 32, 4, 256, 4, 3.0f, 2.0f, 4.0f}, {128, 128, 1, 256, 16, 5.0f, 2.15f, 2.15f}};
 
 // How a product is run: the kernel, which operands are copied to rows that start
 // at multiples of 16 bytes, the shares of the reduction.
@@ -1045,7 +1046,7 @@ inline long copied_stride(int cols, int elem_size) {
 }
 
 // The kernel and the shares with the least time by the table above; the shares'
-// sums cost a launch and their bytes.  `direct`: whole 16-byte pieces at aligned
+// sums cost a launch and their bytes; below zero: no grid holds the tiles.  `direct`: whole 16-byte pieces at aligned
 // addresses; `tiled`: what kAnyTile128 takes.  `bytes`: the workspace that is left
 // for the shares.
 inline float choose(const Product& g, int elem_size, bool direct, bool tiled,
@@ -1080,6 +1081,7 @@ inline float choose(const Product& g, int elem_size, bool direct, bool tiled,
         break;
       const int split_chunks = ceil_div(chunks, want);
       const int splits = ceil_div(chunks, split_chunks);
+      if (tiles * splits > UINT_MAX / (64u * s.waves)) break;
       double rounds = std::ceil(tiles * splits / s.slots);
       if (s.slots == 512)  // work-groups that are alone on their CU are faster
         rounds += std::max(0.55, std::min(1.0, tiles * splits / 512 -
@@ -1107,7 +1109,8 @@ inline float choose(const Product& g, int elem_size, bool direct, bool tiled,
   return best;
 }
 
-// `bytes`: the workspace.  `p_aligned`, `q_aligned`: of the pointers.
+// `bytes`: the workspace.  `p_aligned`, `q_aligned`: of the pointers.  No shares
+// (splits == 0): no grid holds the tiles.
 inline Plan make_plan(const Product& g, int elem_size, size_t bytes,
                       bool p_aligned, bool q_aligned) {
   Plan p = {};
@@ -1141,7 +1144,8 @@ inline Plan make_plan(const Product& g, int elem_size, size_t bytes,
   const size_t p_bytes = p_direct ? 0 : copy_bytes(g.p_k_inner, m);
   const size_t q_bytes = q_direct ? 0 : copy_bytes(g.q_k_inner, n);
   const int reach = 0x7FFF0000 / 256 / elem_size;
-  if (p_bytes + q_bytes > bytes || m >= reach || n >= reach || k >= reach)
+  if (p_bytes + q_bytes > bytes || m >= reach || n >= reach || k >= reach ||
+      !seq::grid_fits((p_bytes + q_bytes) / 4096 + 2, 256))
     return p;
   Plan copied = {};
   copied.copy_p = !p_direct;
@@ -1149,15 +1153,16 @@ inline Plan make_plan(const Product& g, int elem_size, size_t bytes,
   copied.p_bytes = p_bytes;
   copied.q_bytes = q_bytes;
   // (a launch, and the operands read and written)
+  const float product =
+      choose(g, elem_size, true, false, bytes - p_bytes - q_bytes, &copied);
   const float with_copies =
-      choose(g, elem_size, true, false, bytes - p_bytes - q_bytes, &copied) +
-      3.f +
-      static_cast<float>(p_bytes + q_bytes) * 0.5e-6f;
+      product + 3.f + static_cast<float>(p_bytes + q_bytes) * 0.5e-6f;
+  if (product < 0.f) return p;
 #ifdef SNN_HIP_TUNING
   if (const char* copy = std::getenv("SNN_HIP_EPI_COPY"))
     return std::atoi(copy) != 0 ? copied : p;
 #endif
-  return with_copies < any ? copied : p;
+  return any < 0.f || with_copies < any ? copied : p;
 }
 
 }  // namespace epi

@@ -169,8 +169,7 @@ int run(Product& g, void* workspace, size_t bytes, hipStream_t stream) {
   const Plan plan = make_plan(g, sizeof(T), bytes,
                               seq::aligned(static_cast<const T*>(g.p), 16),
                               seq::aligned(static_cast<const T*>(g.q), 16));
-  if (static_cast<size_t>(plan.tiles_m) * plan.tiles_n * plan.splits > INT_MAX)
-    return SNN_HIP_INDEX_EXCEEDED;
+  if (plan.splits == 0) return SNN_HIP_INDEX_EXCEEDED;
   g.tiles_m = plan.tiles_m;
   g.tiles_n = plan.tiles_n;
   g.splits = plan.splits;

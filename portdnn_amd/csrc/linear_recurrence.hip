@@ -143,9 +143,10 @@ template <int VEC>
 __device__ __forceinline__ Place place_of(const Recurrence& r) {
   Place p;
   const int blocks = (r.channels + 64 * VEC - 1) / (64 * VEC);
-  const unsigned at = blockIdx.x * (blockDim.x / 64) + threadIdx.x / 64;
-  p.b = static_cast<int>(at / blocks);
-  const int first = static_cast<int>(at - static_cast<unsigned>(p.b) * blocks) *
+  const unsigned at = seq::group_of_grid() * (blockDim.x / 64) + threadIdx.x / 64;
+  const unsigned b = at / blocks;
+  p.b = static_cast<int>(min(b, static_cast<unsigned>(r.batch)));
+  const int first = static_cast<int>(at - b * blocks) *
                         64 * VEC +
                     (threadIdx.x & 63) * VEC;
   // (a row's last channels: see Group; what is before them is not stored)
@@ -677,8 +678,10 @@ Division divide(const snn_hip_linear_recurrence_params& p) {
   if (p.channels < VEC || d.rows >= kWantedWaves<BACK> ||
       p.steps < kLeastSteps<BACK>)
     return d;
-  d.pieces = ceil_div(d.segments, kWaves<BACK>);
-  const size_t places = d.rows * d.pieces;
+  const int pieces = ceil_div(d.segments, kWaves<BACK>);
+  const size_t places = d.rows * pieces;
+  if (!seq::grid_fits(places, 64 * kWaves<BACK>)) return d;
+  d.pieces = pieces;
   // the counter and the flags, then the states and the pairs
   d.zeros = (places + 1 + 3) / 4 * 4;
   d.words = places * (64 * VEC) * 3;
@@ -690,7 +693,7 @@ template <typename T, int VEC, bool GATE, bool BACK>
 int launch_undivided(const Recurrence& r, hipStream_t stream) {
   const size_t waves =
       static_cast<size_t>(r.batch) * ceil_div(r.channels, 64 * VEC);
-  const dim3 grid(static_cast<unsigned>((waves + 3) / 4)), threads(256);
+  const dim3 grid = seq::grid_of(ceil_div(waves, size_t{4})), threads(256);
   if (BACK)
     hipLaunchKernelGGL((recurrence_grad_kernel<T, VEC, GATE>), grid, threads, 0,
                        stream, r);
@@ -739,8 +742,7 @@ int launch_recurrence(Recurrence r, const snn_hip_linear_recurrence_params& p,
   r.grad_stride = p.grad_row_stride == 0 ? p.channels : p.grad_row_stride;
   KernelTimer timer(stream);
   const Division d = divide<T, BACK>(p);
-  if (d.pieces > 0 && workspace != nullptr && elems * sizeof(T) >= d.bytes &&
-      d.rows * d.pieces <= INT_MAX) {
+  if (d.pieces > 0 && workspace != nullptr && elems * sizeof(T) >= d.bytes) {
     return r.i != nullptr
                ? launch_divided<T, true, BACK>(r, d, workspace, stream)
                : launch_divided<T, false, BACK>(r, d, workspace, stream);
@@ -765,7 +767,7 @@ int check_recurrence(const snn_hip_linear_recurrence_params* p,
   SNN_REQUIRE(p->row_stride == 0 || p->row_stride >= p->channels);
   SNN_REQUIRE(p->grad_row_stride == 0 || p->grad_row_stride >= p->channels);
   SNN_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15u) == 0);
-  // (the grids count waves and 64-channel blocks in 31 bits)
+  // (waves are counted in 31 bits)
   if (static_cast<size_t>(p->batch) * ceil_div(p->channels, 64) > INT_MAX)
     return SNN_HIP_INDEX_EXCEEDED;
   return SNN_HIP_OK;

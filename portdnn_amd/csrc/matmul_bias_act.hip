@@ -274,8 +274,7 @@ int backward(int dtype, const void* grad, const void* lhs, const void* rhs,
   if (sums != nullptr) {
     hipLaunchKernelGGL(
         seq::add_rows_kernel<T>,
-        dim3(static_cast<unsigned>(ceil_div(p.n, 64)), 1), dim3(1024), 0,
-        stream, sums, seq::SumOutputs{}, static_cast<T*>(grad_bias), p.n,
+        seq::columns_grid(p.n, 1), dim3(1024), 0, stream, sums, seq::SumOutputs{}, static_cast<T*>(grad_bias), p.n,
         ceil_div(p.m, rows_per_group(p.m, p.n)), static_cast<long>(p.n), 0l);
     SNN_HIP_CHECK_LAUNCH();
   }

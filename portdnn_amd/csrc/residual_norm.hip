@@ -68,8 +68,8 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES)
   __shared__ float lds[WAVES == 1 ? 1 : 4 * WAVES];
   int turn = 0;
   const long row = WAVES == 1
-                       ? static_cast<long>(blockIdx.x) * 4 + (threadIdx.x >> 6)
-                       : static_cast<long>(blockIdx.x);
+                       ? seq::group_of_grid() * 4l + (threadIdx.x >> 6)
+                       : static_cast<long>(seq::group_of_grid());
   if (row >= r.rows) return;
   const int channels = r.channels;
   const long at = row * channels;
@@ -137,11 +137,10 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES)
 
 template <typename T, int VEC, int PT, int WAVES, bool WHOLE>
 int launch_as(const Rows& r, hipStream_t stream) {
-  const unsigned groups = static_cast<unsigned>(
-      WAVES == 1 ? (static_cast<long>(r.rows) + 3) / 4 : r.rows);
+  const size_t rows = r.rows, groups = WAVES == 1 ? ceil_div(rows, size_t{4}) : rows;
   KernelTimer timer(stream);
-  hipLaunchKernelGGL((residual_norm_kernel<T, VEC, PT, WAVES, WHOLE>), dim3(groups),
-                     dim3(WAVES == 1 ? 256 : 64 * WAVES), 0, stream, r);
+  hipLaunchKernelGGL((residual_norm_kernel<T, VEC, PT, WAVES, WHOLE>),
+                     seq::grid_of(groups), dim3(WAVES == 1 ? 256 : 64 * WAVES), 0, stream, r);
   SNN_HIP_CHECK_LAUNCH();
   return SNN_HIP_OK;
 }

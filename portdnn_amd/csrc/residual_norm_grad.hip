@@ -343,14 +343,13 @@ int launch_as(const Rows& r, const Grad& d, hipStream_t stream) {
   hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(d.groups)),
                      dim3(WAVES == 1 ? 256 : 64 * WAVES), 0, stream, r, d);
   SNN_HIP_CHECK_LAUNCH();
-  const unsigned columns = static_cast<unsigned>(ceil_div(r.channels, 64));
   if (d.sums != nullptr) {
     const seq::SumOutputs outputs = {{d.g.grad_scale, d.g.grad_post_weight,
                                       d.g.grad_pre_weight, d.g.grad_post_bias,
                                       d.g.grad_pre_bias}};
     const int own = biases ? static_cast<int>(kSums) : kWeightSums;
     hipLaunchKernelGGL(seq::add_rows_kernel<T>,
-                       dim3(columns, static_cast<unsigned>(own)), dim3(1024), 0,
+                       seq::columns_grid(r.channels, own), dim3(1024), 0,
                        stream, d.sums, outputs, static_cast<T*>(nullptr),
                        r.channels, d.groups,
                        static_cast<long>(own) * r.channels,
@@ -360,7 +359,7 @@ int launch_as(const Rows& r, const Grad& d, hipStream_t stream) {
   if (d.gate_sums != nullptr) {
     hipLaunchKernelGGL(
         seq::add_rows_kernel<T>,
-        dim3(columns, static_cast<unsigned>(d.runs / d.per_gate)), dim3(1024), 0,
+        seq::columns_grid(r.channels, d.runs / d.per_gate), dim3(1024), 0,
         stream, d.gate_sums, seq::SumOutputs{}, static_cast<T*>(d.g.grad_gate),
         r.channels, d.per_gate, static_cast<long>(r.channels),
         static_cast<long>(d.per_gate) * r.channels);

@@ -5,6 +5,7 @@
 #ifndef PORTDNN_AMD_CSRC_SEQUENCE_H_
 #define PORTDNN_AMD_CSRC_SEQUENCE_H_
 
+#include <algorithm>
 #include <type_traits>
 
 #include "snn_common.h"
@@ -83,10 +84,26 @@ __device__ __forceinline__ float wave_sum(float v) {
   return v;
 }
 
+// A dimension of a grid holds at most 2^32 - 1 work-items.
+inline bool grid_fits(size_t groups, unsigned threads) {
+  return groups <= UINT_MAX / threads;
+}
+// Where there may be more work-groups than that, they continue along y, 2^20 at a
+// time; the last of these may not exist.
+constexpr unsigned kGroupsOfX = 1u << 20;
+inline dim3 grid_of(size_t groups) {
+  return dim3(static_cast<unsigned>(std::min(groups, size_t{kGroupsOfX})),
+              static_cast<unsigned>(ceil_div(groups, size_t{kGroupsOfX})));
+}
+__device__ __forceinline__ unsigned group_of_grid() {
+  return blockIdx.x + blockIdx.y * kGroupsOfX;
+}
+
 // Adds up partial sums: out[c] = sum over `count` rows of `in`, `stride` floats
 // apart.  blockIdx.y is the output, `step` floats behind the one before: row
 // blockIdx.y of `rows_out`, or one of `outputs` (null: not wanted).  16 waves
-// share a column's rows, and their sums are added in order.
+// share a column's rows, and their sums are added in order.  Columns continue along
+// z (columns_grid).
 constexpr int kMaxSums = 5;
 struct SumOutputs {
   void* out[kMaxSums];
@@ -102,7 +119,7 @@ __global__ void __launch_bounds__(1024)
                      : static_cast<T*>(outputs.out[blockIdx.y]);
   if (out == nullptr) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int c = blockIdx.x * 64 + lane;
+  const int c = (blockIdx.x + blockIdx.z * kGroupsOfX) * 64 + lane;
   in += blockIdx.y * step + c;
   const int each = (count + 15) / 16;
   const int begin = min(count, wave * each), end = min(count, begin + each);
@@ -118,6 +135,11 @@ __global__ void __launch_bounds__(1024)
 #pragma unroll
   for (int w = 0; w < 16; ++w) s += part[w][lane];
   out[c] = static_cast<T>(s);
+}
+
+inline dim3 columns_grid(int channels, int outputs) {
+  const dim3 columns = grid_of(ceil_div(channels, 64));
+  return dim3(columns.x, static_cast<unsigned>(outputs), columns.y);
 }
 
 template <typename T>

@@ -1,0 +1,40 @@
+"""Work-groups that no grid holds: decided on the host.  Nothing is launched."""
+import ctypes
+
+import pytest
+
+from portdnn_amd import capi
+from portdnn_amd.capi import DTYPE, STATUS, LinearRecurrenceParams, MatmulBiasActParams
+
+FAKE = 0x1000  # never dereferenced
+TYPES = ["f32", "f16", "bf16"]
+
+
+@pytest.mark.parametrize("suffix", TYPES)
+def test_products_of_more_tiles_than_a_grid_holds(suffix):
+    p = MatmulBiasActParams(m=1 << 21, k=64, n=1 << 20)
+    fn = getattr(capi.lib(), "snn_hip_matmul_bias_act_" + suffix)
+    for n in (1 << 20, (1 << 20) + 1):
+        p.n = n
+        assert fn(FAKE, FAKE, None, None, FAKE, None, ctypes.byref(p), None, 0,
+                  None) == STATUS.INDEX_EXCEEDED
+
+
+@pytest.mark.parametrize("suffix", TYPES)
+def test_sequences_are_divided_as_far_as_a_grid_holds_the_pieces(suffix):
+    """128 steps to a piece of 1024 lanes, 144 to one of 768."""
+    query = capi.lib().snn_hip_linear_recurrence_workspace_size
+    required, recommended = ctypes.c_size_t(), ctypes.c_size_t()
+
+    def elems(steps, batch=1):
+        p = LinearRecurrenceParams(batch=batch, steps=steps, channels=8)
+        assert query(ctypes.byref(p), getattr(DTYPE, suffix.upper()),
+                     ctypes.byref(required), ctypes.byref(recommended)) == 0
+        return recommended.value
+
+    limit = (1 << 32) - 1
+    assert elems(limit // 1024 * 128) > 0
+    assert elems(limit // 768 * 144) > 0
+    assert elems(limit // 768 * 144 + 1) == 0
+    assert elems(limit // 768 // 100 * 144, batch=100) > 0
+    assert elems(limit // 768 // 100 * 144 + 144, batch=100) == 0
