@@ -73,7 +73,10 @@ class KernelTimer {
 
 constexpr int kWave = 64;
 
-inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
+// (without a sum that 31 bits do not hold)
+inline int ceil_div(int a, int b) {
+  return a > 0 ? (a - 1) / b + 1 : (a + b - 1) / b;
+}
 inline unsigned ceil_div(unsigned a, unsigned b) { return (a + b - 1) / b; }
 inline size_t ceil_div(size_t a, size_t b) { return (a + b - 1) / b; }
 

@@ -107,3 +107,23 @@ def test_sums_of_many_columns():
         v = part.double()
         ref.check(bias[p], (v.sum(0), v.abs().sum(0)), 64)
     assert _only_there(bias, places)
+
+
+def test_sums_over_many_rows():
+    """More rows than 2^30, of one channel: x + scale y and its gradients."""
+    rows = (1 << 30) + 75
+    places = _places(rows, 1 << 29)
+    x, xs = _filled((rows, 1), places, 8)
+    dy, ds = _filled((rows, 1), places, 9)
+    scale = torch.tensor([0.75], dtype=F16, device="cuda")
+    y, _, _ = ops.residual_norm(x, residual=x, scale=scale)
+    got = ops.residual_norm_grad(x, y, None, grad_sum=dy, scale=scale)
+    for p, part, d in zip(places, xs, ds):
+        v, w = part.double(), d.double()
+        ref.check(y[p], (1.75 * v, 1.75 * v.abs()), 8)
+        ref.check(got["x"][p], (0.75 * w, 0.75 * w.abs()), 8)
+        assert torch.equal(got["residual"][p].cpu(), d)
+    assert _only_there(y, places) and _only_there(got["x"], places)
+    each = torch.cat([v.double() * w.double() for v, w in zip(xs, ds)])
+    # (120 terms that are not zero, added along 2^18 rows a wave and joined)
+    ref.check(got["scale"], (each.sum(0), each.abs().sum(0)), 256)

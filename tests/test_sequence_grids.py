@@ -4,7 +4,8 @@ import ctypes
 import pytest
 
 from portdnn_amd import capi
-from portdnn_amd.capi import DTYPE, STATUS, LinearRecurrenceParams, MatmulBiasActParams
+from portdnn_amd.capi import (DTYPE, GATE, STATUS, LinearRecurrenceParams,
+                              MatmulBiasActParams, ResidualNormParams)
 
 FAKE = 0x1000  # never dereferenced
 TYPES = ["f32", "f16", "bf16"]
@@ -38,3 +39,20 @@ def test_sequences_are_divided_as_far_as_a_grid_holds_the_pieces(suffix):
     assert elems(limit // 768 * 144 + 1) == 0
     assert elems(limit // 768 // 100 * 144, batch=100) > 0
     assert elems(limit // 768 // 100 * 144 + 144, batch=100) == 0
+
+
+@pytest.mark.parametrize("suffix", TYPES)
+@pytest.mark.parametrize("gate_rows", [0, 2, 3, 1 << 20, (1 << 31) - 1])
+def test_sums_over_as_many_rows_as_there_may_be(suffix, gate_rows):
+    """Of at most 2048 work-groups, and as many of a shared gate's rows, per channel."""
+    query = capi.lib().snn_hip_residual_norm_grad_workspace_size
+    required, recommended = ctypes.c_size_t(), ctypes.c_size_t()
+    for rows in ((1 << 30) + 1, (1 << 31) - 1):
+        p = ResidualNormParams(
+            rows=rows, channels=2, gate=GATE.VALUE if gate_rows else GATE.NONE,
+            gate_rows=max(1, gate_rows))
+        assert query(ctypes.byref(p), getattr(DTYPE, suffix.upper()),
+                     ctypes.byref(required), ctypes.byref(recommended)) == 0
+        size = 4 if suffix == "f32" else 2
+        # (five sums, and runs of a gate's rows: no more than two for each group)
+        assert 0 < required.value * size <= (5 + 2) * 2048 * 2 * 4
