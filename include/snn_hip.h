@@ -796,7 +796,10 @@ SNN_HIP_API int snn_hip_linear_recurrence_grad_bf16(
     void* grad_x, void* grad_forget, void* grad_input_gate,
     float* grad_initial_state, const snn_hip_linear_recurrence_params* params,
     void* workspace, size_t workspace_elems, void* stream);
-/* Workspace of either call, in elements of `dtype`; none is required. */
+/* Workspace of either call, in elements of `dtype`; none is required.  Sequences
+ * of more than 2^31 - 65 steps or 2^31 - 1025 channels, and more than 2^31 - 1
+ * sequences times blocks of 64 channels, are SNN_HIP_INDEX_EXCEEDED here and in
+ * the calls. */
 SNN_HIP_API int snn_hip_linear_recurrence_workspace_size(
     const snn_hip_linear_recurrence_params* params, int dtype,
     size_t* required_elems, size_t* recommended_elems);

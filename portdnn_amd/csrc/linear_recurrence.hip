@@ -767,8 +767,10 @@ int check_recurrence(const snn_hip_linear_recurrence_params* p,
   SNN_REQUIRE(p->row_stride == 0 || p->row_stride >= p->channels);
   SNN_REQUIRE(p->grad_row_stride == 0 || p->grad_row_stride >= p->channels);
   SNN_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15u) == 0);
-  // (waves are counted in 31 bits)
-  if (static_cast<size_t>(p->batch) * ceil_div(p->channels, 64) > INT_MAX)
+  // (waves, and steps and channels of a group behind the last one, are counted in 31
+  // bits)
+  if (static_cast<size_t>(p->batch) * ceil_div(p->channels, 64) > INT_MAX ||
+      p->steps > INT_MAX - 64 || p->channels > INT_MAX - 1024)
     return SNN_HIP_INDEX_EXCEEDED;
   return SNN_HIP_OK;
 }

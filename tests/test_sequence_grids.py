@@ -56,3 +56,28 @@ def test_sums_over_as_many_rows_as_there_may_be(suffix, gate_rows):
         size = 4 if suffix == "f32" else 2
         # (five sums, and runs of a gate's rows: no more than two for each group)
         assert 0 < required.value * size <= (5 + 2) * 2048 * 2 * 4
+
+
+@pytest.mark.parametrize("suffix", TYPES)
+def test_steps_and_channels_that_cannot_be_counted_on(suffix):
+    """A walk counts some steps, and a work-group some channels, beyond the last."""
+    query = capi.lib().snn_hip_linear_recurrence_workspace_size
+    n = ctypes.c_size_t()
+    most = (1 << 31) - 1
+    for steps, channels, want in ((most - 64, 1, STATUS.OK),
+                                  (most - 63, 1, STATUS.INDEX_EXCEEDED),
+                                  (most, 1, STATUS.INDEX_EXCEEDED),
+                                  (1, most - 1024, STATUS.OK),
+                                  (1, most - 1023, STATUS.INDEX_EXCEEDED),
+                                  (1, most, STATUS.INDEX_EXCEEDED)):
+        p = LinearRecurrenceParams(batch=1, steps=steps, channels=channels)
+        assert query(ctypes.byref(p), getattr(DTYPE, suffix.upper()),
+                     ctypes.byref(n), ctypes.byref(n)) == want
+        if want != STATUS.OK:
+            name = "snn_hip_linear_recurrence"
+            assert getattr(capi.lib(), "%s_%s" % (name, suffix))(
+                FAKE, FAKE, None, None, None, None, FAKE, None, ctypes.byref(p),
+                None, 0, None) == want
+            assert getattr(capi.lib(), "%s_grad_%s" % (name, suffix))(
+                FAKE, None, FAKE, FAKE, None, None, None, None, FAKE, FAKE,
+                FAKE, None, None, ctypes.byref(p), None, 0, None) == want
