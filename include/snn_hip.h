@@ -619,6 +619,25 @@ SNN_HIP_API int snn_hip_matmul_bias_act_grad_bf16(
 SNN_HIP_API int snn_hip_matmul_bias_act_workspace_size(
     const snn_hip_matmul_bias_act_params* params, int grad, int dtype,
     size_t* required_elems, size_t* recommended_elems);
+/* Diagnostics for tests of the kernels: what a product runs on, given a workspace
+ * of `workspace_elems`, and operands that start at multiples of 16 bytes or do not.
+ * `product` is 0 for the forward call, 1 and 2 for grad_lhs and grad_rhs of a call
+ * for all three gradients.  The result's rows are the first operand's. */
+typedef struct snn_hip_matmul_bias_act_plan {
+  int tile_rows;
+  int tile_cols;
+  int shared;       /* 1: a tile's reduction is shared by the work-group's waves */
+  int any_address;  /* 1: operands by way of registers, 0: straight to LDS */
+  int pair;         /* 1: two work-groups to a CU */
+  int first_inner;  /* 1: the reduction is contiguous in the first operand */
+  int second_inner; /* ... and in the second */
+  int first_copied; /* 1: copied to aligned rows first */
+  int second_copied;
+  int shares;       /* of the reduction, each by a work-group of its own */
+} snn_hip_matmul_bias_act_plan;
+SNN_HIP_API int snn_hip_matmul_bias_act_planned(
+    const snn_hip_matmul_bias_act_params* params, int product, int dtype,
+    int aligned, size_t workspace_elems, snn_hip_matmul_bias_act_plan* plan);
 
 /* The norms before and after a block, with its gate and residual scale, in
  * one pass over the rows:

@@ -136,6 +136,11 @@ MatmulBiasActParams = _struct(
     ["m", "k", "n", "transpose_lhs", "transpose_rhs", "activation",
      "lhs_stride", "rhs_stride", "residual_stride", "output_stride"], {})
 
+MATMUL_PLAN = ["tile_rows", "tile_cols", "shared", "any_address", "pair",
+               "first_inner", "second_inner", "first_copied", "second_copied",
+               "shares"]
+MatmulBiasActPlan = _struct("MatmulBiasActPlan", MATMUL_PLAN, {})
+
 ResidualNormParams = _struct(
     "ResidualNormParams",
     ["rows", "channels", "post_norm", "pre_norm", "gate", "gate_rows",
@@ -229,6 +234,7 @@ SIGNATURES = {
                              ctypes.POINTER(_I), _I, _I, _P],
     "snn_hip_matmul_bias_act_workspace_size": [
         _P, _I, _I, ctypes.POINTER(_SZ), ctypes.POINTER(_SZ)],
+    "snn_hip_matmul_bias_act_planned": [_P, _I, _I, _I, _SZ, _P],
     "snn_hip_residual_norm_grad_workspace_size": [
         _P, _I, ctypes.POINTER(_SZ), ctypes.POINTER(_SZ)],
     "snn_hip_linear_recurrence_workspace_size": [

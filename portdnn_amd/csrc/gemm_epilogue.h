@@ -1028,6 +1028,10 @@ constexpr Shape kShapes32[kKernels] = {
     {16, 16, 4, 768, 4, 3.0f, 0.9f, 1.2f}, {32, 32, 8, 256, 8, 3.0f, 2.0f, 5.5f},
     {64, 32, 4, 256, 4, 3.0f, 2.0f, 4.0f}, {128, 128, 1, 256, 16, 5.0f, 2.15f, 2.15f}};
 
+inline const Shape& shape_of(int elem_size, int kernel) {
+  return (elem_size == 2 ? kShapes16 : kShapes32)[kernel];
+}
+
 // How a product is run: the kernel, which operands are copied to rows that start
 // at multiples of 16 bytes, the shares of the reduction.
 struct Plan {
@@ -1051,7 +1055,6 @@ inline long copied_stride(int cols, int elem_size) {
 // for the shares.
 inline float choose(const Product& g, int elem_size, bool direct, bool tiled,
                     size_t bytes, Plan* p) {
-  const Shape* const shapes = elem_size == 2 ? kShapes16 : kShapes32;
   const int chunks = ceil_div(g.k, kChunkBytes / elem_size);
   // (operands that an L2 holds)
   const bool cached = (static_cast<double>(g.m) + g.n) * g.k * elem_size < 4e6;
@@ -1063,7 +1066,7 @@ inline float choose(const Product& g, int elem_size, bool direct, bool tiled,
   float best = -1.f;
   for (int kernel = direct ? 0 : kAny16x16;
        kernel < (direct ? kAny16x16 : kKernels); ++kernel) {
-    const Shape& s = shapes[kernel];
+    const Shape& s = shape_of(elem_size, kernel);
     if (s.fixed == 0.f || (kernel == kAnyTile128 && !tiled)) continue;
 #ifdef SNN_HIP_TUNING
     if (const char* only = std::getenv("SNN_HIP_EPI_KERNEL"))

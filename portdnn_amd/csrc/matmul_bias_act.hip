@@ -364,4 +364,48 @@ int snn_hip_matmul_bias_act_workspace_size(
   return SNN_HIP_OK;
 }
 
+int snn_hip_matmul_bias_act_planned(
+    const snn_hip_matmul_bias_act_params* params, int product, int dtype,
+    int aligned, size_t workspace_elems, snn_hip_matmul_bias_act_plan* plan) {
+  if (dtype < SNN_HIP_DTYPE_F32 || dtype > SNN_HIP_DTYPE_BF16 || product < 0 ||
+      product > 2 || plan == nullptr)
+    return SNN_HIP_INVALID_PARAMETER;
+  const int size = snn::elem_size(dtype);
+  const int v = snn::check(params, size, nullptr);
+  if (v != SNN_HIP_OK) return v;
+  const bool at16 = aligned != 0;
+  size_t bytes = workspace_elems * size;
+  snn::epi::Product g;
+  bool p_at16 = at16, q_at16 = at16;
+  if (product == 0) {
+    g = snn::forward_product(*params);
+  } else {
+    const snn::GradSpace s = snn::grad_space(*params, size);
+    if (bytes < s.dz + s.sums) return SNN_HIP_INSUFFICIENT_WORKSPACE;
+    bytes -= s.dz + s.sums;
+    const long stride =
+        s.dz > 0 ? params->n : snn::or_else(params->output_stride, params->n);
+    g = product == 1 ? snn::lhs_product(*params, nullptr, stride, nullptr)
+                     : snn::rhs_product(*params, nullptr, stride, nullptr);
+    // (the gradient in front of the activation is in the workspace)
+    const bool first = product == 1 ? params->transpose_lhs == 0
+                                    : params->transpose_rhs != 0;
+    if (s.dz > 0) (first ? p_at16 : q_at16) = true;
+  }
+  const snn::epi::Plan p = snn::epi::make_plan(g, size, bytes, p_at16, q_at16);
+  if (p.splits == 0) return SNN_HIP_INDEX_EXCEEDED;
+  const snn::epi::Shape& shape = snn::epi::shape_of(size, p.kernel);
+  *plan = {shape.bm,
+           shape.bn,
+           shape.chunks > 1,
+           p.kernel >= snn::epi::kAny16x16,
+           p.kernel == snn::epi::kTile128Pair,
+           g.p_k_inner,
+           g.q_k_inner,
+           p.copy_p,
+           p.copy_q,
+           p.splits};
+  return SNN_HIP_OK;
+}
+
 }  // extern "C"

@@ -595,6 +595,25 @@ def _matmul_plan(key, a, b, grad, activation, trans_a, trans_b):
                        p.rhs_stride, out_stride, elems))
 
 
+def matmul_plan(m, k, n, dtype, product=0, activation=ACTIVATION.NONE,
+                trans_a=False, trans_b=False, aligned=True, workspace_elems=None,
+                **strides):
+    """What a product runs on (snn_hip_matmul_bias_act_planned), a dict by the names
+    of capi.MATMUL_PLAN; by default with the recommended workspace."""
+    p = MatmulBiasActParams(m=m, k=k, n=n, transpose_lhs=int(trans_a),
+                            transpose_rhs=int(trans_b), activation=activation,
+                            **strides)
+    code = _TYPES[dtype][1]
+    if workspace_elems is None:
+        workspace_elems = _workspace("snn_hip_matmul_bias_act_workspace_size", p,
+                                     int(product > 0), code)
+    plan = capi.MatmulBiasActPlan()
+    capi.check(capi.lib().snn_hip_matmul_bias_act_planned(
+        ctypes.byref(p), product, code, int(aligned), workspace_elems,
+        ctypes.byref(plan)))
+    return {name: getattr(plan, name) for name in capi.MATMUL_PLAN}
+
+
 def matmul_bias_act(a, b, bias=None, residual=None,
                     activation=ACTIVATION.NONE, trans_a=False, trans_b=False,
                     keep_pre_activation=False, out=None, workspace=None):
@@ -883,7 +902,7 @@ __all__ = [
     "default_algorithm",
     "depthwise_conv2d", "depthwise_params", "depthwise_sizes",
     "linear_recurrence", "linear_recurrence_grad", "matmul", "matmul_bias_act",
-    "matmul_bias_act_grad",
+    "matmul_bias_act_grad", "matmul_plan",
     "pointwise_forward", "pointwise_grad", "pool_params", "pooling_avg_grad",
     "pooling_forward", "pooling_max_grad", "residual_norm",
     "residual_norm_grad", "workspace_size",
