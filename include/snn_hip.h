@@ -596,8 +596,9 @@ SNN_HIP_API int snn_hip_matmul_bias_act_bf16(
  * values.  Any of the three may be NULL and is then not computed; lhs is needed
  * for grad_rhs and rhs for grad_lhs only.  grad_bias and, where there is an
  * activation, the products (which need the gradient with respect to
- * pre_activation, rounded to the data type) take workspace:
- * SNN_HIP_INSUFFICIENT_WORKSPACE without the required size. */
+ * pre_activation, rounded to the data type: in binary16 it is infinite beyond
+ * 65504) take workspace: SNN_HIP_INSUFFICIENT_WORKSPACE without the required
+ * size. */
 SNN_HIP_API int snn_hip_matmul_bias_act_grad_f32(
     const void* grad_output, const void* lhs, const void* rhs,
     const void* pre_activation, void* grad_lhs, void* grad_rhs,

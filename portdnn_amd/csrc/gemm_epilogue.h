@@ -37,8 +37,8 @@
 // way out, which nothing overlaps where the tiles fill the GPU once.  Measured:
 //
 //   1 x 2048 x 8192 bfloat16, silu      9.5 us    34 MB at 3.5 TB/s
-//   24 x 4096 x 4096 binary16           8.9 us    34 MB at 3.8 TB/s
-//   4095 x 1023 x 1001 binary16, gelu  20.9 us    402 TFLOP/s
+//   24 x 4096 x 4096 binary16           8.8 us    34 MB at 3.9 TB/s
+//   4095 x 1023 x 1001 binary16, gelu  21.2 us    396 TFLOP/s
 //   4096 x 1024 x 1024 fp32            68.7 us    125 TFLOP/s
 //   8192 x 4096 x 8192 bfloat16        411-441 us 1.25-1.34 PFLOP/s; 468 with
 //                                      gelu_tanh and what it is taken of stored

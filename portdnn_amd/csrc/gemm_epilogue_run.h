@@ -97,9 +97,9 @@ int launch_tile(const Product& g, int kernel, hipStream_t stream) {
     case kAny64x32:
       return launch_few<T, PK, QK, 64, 32, 4, 2, false>(g, stream);
     case kAnyTile128:
-      // (4095 x 1023 x 1001 binary16: sixteen waves 18.4 us, eight 19.9, four 26; four
-      // chunks under way 21; copies of both operands and their products 25.7.  8191 x
-      // 4095 x 4095: 462 against 266 with copies)
+      // (4095 x 1023 x 1001 binary16, the product alone: sixteen waves 18.4 us, eight
+      // 19.9, four 26; four chunks under way 21; copies of both operands and their
+      // products 25.7.  8191 x 4095 x 4095: 462 against 266 with copies)
       return launch_as<T, PK, QK, 128, 128, 4, 4, 128, 2, 2>(g, stream);
     default:
       break;

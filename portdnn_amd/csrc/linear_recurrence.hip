@@ -30,11 +30,11 @@
 // of the state in front of it wherever it is computed, so that results do not
 // depend on who waits for whom.  States and pieces are fp32.
 //
-// One sequence of 32768 x 2048 bfloat16: 120 us, 403 MB at 3.4 TB/s (with two passes
-// over the operands 151); a gradient of 4 x 4096 x 2048 binary16 with both gates 128
-// us, 537 MB at 4.2 TB/s.  What is left is the wait of a CU's few waves for the
-// states, as their segments fill the registers.  A token of 64 x 4096 fp32: 4.4 us, a
-// launch's latency.
+// One sequence of 32768 x 2048 bfloat16: 121.5 us, 403 MB at 3.3 TB/s (with two passes
+// over the operands 151); a gradient of 4 x 4096 x 2048 binary16 with both gates 131
+// us, 537 MB at 4.1 TB/s.  What is left is the wait of a CU's few waves for the
+// states, as their segments fill the registers.  A token of 64 x 4096 fp32: 3.8-4.6 us,
+// a launch's latency.
 //
 // A reset leaves h_{t-1} out by selection and not by a factor of zero, so that
 // an infinite state does not survive it; steps behind a sequence's length do not
@@ -131,7 +131,7 @@ __device__ __forceinline__ unsigned long long resets_of(const Recurrence& r,
 // ---- undivided ---------------------------------------------------------------
 
 // Steps whose loads are in flight together.  (64 sequences of 48 x 256 bfloat16
-// forward: 14.8 us, with 8 of them 16.4; 2048 of 64 x 1024: 227 and 222.)
+// forward, whole: 15 us, with 8 of them 16.4.)
 constexpr int kSteps = 4;
 
 // What a wave needs of its place: sequence and first channel of the lane.  (Lanes
@@ -651,15 +651,20 @@ template <bool BACK>
 constexpr int kSegment = BACK ? 8 : 12;
 
 // A sequence is divided where there are fewer waves of lanes than this, and where
-// it is long enough for the second launch.  bfloat16 of 1024 channels, us divided
-// and whole, forward | gradients:
+// it is long enough for the second launch.  bfloat16 of 1024 channels, four waves a
+// sequence, us divided and whole, forward | gradients; in brackets with an input gate:
 //
-//   4 sequences of 32 steps    13, 11 |  13,  22
-//   4 of 64                    14, 21 |  16,  41
-//   64 of 66                   18, 23 |  22,  48
-//   256 of 128                 71, 60 | 112, 132
-//   512 of 128               131, 109 | 209, 214
-//   1000 of 128              238, 212 | 398, 380
+//   4 sequences of 32 steps    12, 10 |  12,  18
+//   4 of 64                    13, 19 |  14,  32
+//   64 of 66                   17, 26 |  20,  39
+//   128 of 128                 33, 49 |  54,  93   (39,  67 |  62, 116)
+//   128 of 512               119, 272 | 206, 357
+//   256 of 128                 61, 78 | 102, 104   (73,  80 | 121, 135)
+//   512 of 128               111, 101 | 187, 176  (133, 115 | 227, 231)
+//   1000 of 128              205, 161 | 352, 318  (248, 214 | 433, 432)
+//
+// (by which the forward walk would be divided up to 1024 waves: its threshold is from
+// kernels before these)
 template <bool BACK>
 constexpr int kWantedWaves = BACK ? 2048 : 512;
 template <bool BACK>

@@ -17,7 +17,7 @@
 // and keep the sums over rows in registers, each lane for its channels; a second
 // launch adds the work-groups' sums in their order.  A row's two sums are two
 // waits for all its waves, so the next row is on its way meanwhile.  16384 x 2048
-// bfloat16 with both norms, a gate and its weights' sums: 112-116 us, 537 MB at
+// bfloat16 with both norms, a gate and its weights' sums: 111-117 us, 537 MB at
 // 4.6-4.8 TB/s, and 5 for the second launch.
 #include <algorithm>
 
