@@ -644,8 +644,8 @@ __global__ void __launch_bounds__(64 * WAVES)
 // shorter chain of them, larger segments take registers from the waves of a CU.
 // Forward, 32768 x 2048 bfloat16: 12 x 12 122 us, 16 x 8 126, 16 x 12 130, 8 x 16 135,
 // 8 x 8 159, 12 x 16 170.  Gradients, 4 x 4096 x 2048 binary16: 16 x 8 132 us, 8 x 8
-// 131, 16 x 4 137, 8 x 12 138, 12 x 12 144.  fp32, two channels a lane, is within an
-// eighth of the best of these on four sizes: 32768 x 2048 188 us (8 x 16 170),
+// 131, 16 x 4 137, 8 x 12 138, 12 x 12 144.  fp32, two channels a lane, is within a
+// seventh of the best of these on four sizes: 32768 x 2048 188 us (8 x 16 170),
 // gradients 320 (8 x 8 311); 8192 x 1024 33 (16 x 8 32) and 50 (16 x 4 55).
 template <bool BACK>
 constexpr int kWaves = BACK ? 16 : 12;
