@@ -824,6 +824,252 @@ SNN_HIP_API int snn_hip_linear_recurrence_workspace_size(
     const snn_hip_linear_recurrence_params* params, int dtype,
     size_t* required_elems, size_t* recommended_elems);
 
+/* ---- a linear-attention block ------------------------------------------------
+ * What a block of linear attention takes beside the operators above: a product
+ * gated by another, positions by rotation, and the attention itself, a
+ * recurrence whose state is a matrix for each head.  Types, strides, rounding
+ * and workspaces as above. */
+
+/* output = act(lhs op(gate_weight) + gate_bias) * (lhs op(up_weight) + up_bias):
+ * the first half of a gated feed-forward part, both products in one pass over
+ * lhs.  (Its second half is a matrix product with a residual.)
+ *
+ * lhs is m x k; both weights are stored k x n, or n x k when transpose_rhs, with
+ * one stride, so that they may be the two halves of one matrix.  The biases hold
+ * n values; either may be NULL.  gate and up, m x n without a stride, both NULL or
+ * both there, receive the two factors' values in front of the activation, which
+ * the gradients take.  No operand may overlap an output.  Sizes, workspace and
+ * order of sums as in snn_hip_matmul_bias_act. */
+typedef struct snn_hip_gated_matmul_params {
+  int m;
+  int k;
+  int n;
+  int transpose_rhs;
+  int activation; /* a snn_hip_activation */
+  int lhs_stride;
+  int rhs_stride;    /* of both weights */
+  int output_stride; /* of output and grad_output */
+} snn_hip_gated_matmul_params;
+SNN_HIP_API int snn_hip_gated_matmul_f32(
+    const void* lhs, const void* gate_weight, const void* up_weight,
+    const void* gate_bias, const void* up_bias, void* output, void* gate,
+    void* up, const snn_hip_gated_matmul_params* params, void* workspace,
+    size_t workspace_elems, void* stream);
+SNN_HIP_API int snn_hip_gated_matmul_f16(
+    const void* lhs, const void* gate_weight, const void* up_weight,
+    const void* gate_bias, const void* up_bias, void* output, void* gate,
+    void* up, const snn_hip_gated_matmul_params* params, void* workspace,
+    size_t workspace_elems, void* stream);
+SNN_HIP_API int snn_hip_gated_matmul_bf16(
+    const void* lhs, const void* gate_weight, const void* up_weight,
+    const void* gate_bias, const void* up_bias, void* output, void* gate,
+    void* up, const snn_hip_gated_matmul_params* params, void* workspace,
+    size_t workspace_elems, void* stream);
+/* The gradients; gate and up are what the forward call wrote.  grad_lhs and the
+ * weights' gradients are stored as those are, without a stride; each of the five
+ * may be NULL and is then not computed.  lhs is needed for the weights' gradients
+ * and both weights for grad_lhs only.  The gradients of the two factors, rounded to
+ * the data type, and the biases' sums take workspace:
+ * SNN_HIP_INSUFFICIENT_WORKSPACE without the required size. */
+SNN_HIP_API int snn_hip_gated_matmul_grad_f32(
+    const void* grad_output, const void* lhs, const void* gate_weight,
+    const void* up_weight, const void* gate, const void* up, void* grad_lhs,
+    void* grad_gate_weight, void* grad_up_weight, void* grad_gate_bias,
+    void* grad_up_bias, const snn_hip_gated_matmul_params* params,
+    void* workspace, size_t workspace_elems, void* stream);
+SNN_HIP_API int snn_hip_gated_matmul_grad_f16(
+    const void* grad_output, const void* lhs, const void* gate_weight,
+    const void* up_weight, const void* gate, const void* up, void* grad_lhs,
+    void* grad_gate_weight, void* grad_up_weight, void* grad_gate_bias,
+    void* grad_up_bias, const snn_hip_gated_matmul_params* params,
+    void* workspace, size_t workspace_elems, void* stream);
+SNN_HIP_API int snn_hip_gated_matmul_grad_bf16(
+    const void* grad_output, const void* lhs, const void* gate_weight,
+    const void* up_weight, const void* gate, const void* up, void* grad_lhs,
+    void* grad_gate_weight, void* grad_up_weight, void* grad_gate_bias,
+    void* grad_up_bias, const snn_hip_gated_matmul_params* params,
+    void* workspace, size_t workspace_elems, void* stream);
+/* Workspace of the forward call (grad == 0) or of the gradients, in elements of
+ * `dtype`. */
+SNN_HIP_API int snn_hip_gated_matmul_workspace_size(
+    const snn_hip_gated_matmul_params* params, int grad, int dtype,
+    size_t* required_elems, size_t* recommended_elems);
+
+/* Positions by rotation.  Of each head's `channels` the first `turned` form pairs
+ * (a, b), channel i with i + turned / 2 (HALVES) or 2 i with 2 i + 1 (PAIRS), and
+ * pair i of a token at position p becomes
+ *
+ *   magnitude (a cos w - b sin w),  magnitude (a sin w + b cos w)
+ *
+ * with w = 2 pi p frequencies[i], or -w where `inverse` is set: the gradient of
+ * the forward call is the inverse call on the output's gradient.  The other
+ * channels are copied as they are.  Angles are reduced in 64 bits, so that far
+ * positions lose nothing.
+ *
+ * input is [batch][steps][heads][channels] with row_stride elements from step to
+ * step (steps * row_stride from sequence to sequence), output the same with
+ * output_row_stride, so that both may be slices of a projection's rows; output may
+ * be input with the same stride (in place), otherwise they may not overlap.
+ * `positions` is NULL where params->positions is NONE (a token's position is its
+ * step), [batch] ints for FIRST (the position of step 0, the others follow) or
+ * [batch][steps] for EACH.  2^32 or more lanes, tokens times groups of 16 bytes of a
+ * head, are SNN_HIP_INDEX_EXCEEDED. */
+typedef enum snn_hip_rotary_layout {
+  SNN_HIP_ROTARY_HALVES = 0,
+  SNN_HIP_ROTARY_PAIRS = 1
+} snn_hip_rotary_layout;
+typedef enum snn_hip_rotary_positions {
+  SNN_HIP_ROTARY_POSITIONS_NONE = 0,
+  SNN_HIP_ROTARY_POSITIONS_FIRST = 1,
+  SNN_HIP_ROTARY_POSITIONS_EACH = 2
+} snn_hip_rotary_positions;
+typedef struct snn_hip_rotary_params {
+  int batch;
+  int steps;
+  int heads;
+  int channels; /* of a head */
+  int turned;   /* even, 2 ... channels */
+  int layout;   /* a snn_hip_rotary_layout */
+  int positions; /* a snn_hip_rotary_positions */
+  int inverse;
+  int row_stride;
+  int output_row_stride;
+  float magnitude;
+} snn_hip_rotary_params;
+SNN_HIP_API int snn_hip_rotary_f32(const void* input, const double* frequencies,
+                                   const int* positions, void* output,
+                                   const snn_hip_rotary_params* params,
+                                   void* stream);
+SNN_HIP_API int snn_hip_rotary_f16(const void* input, const double* frequencies,
+                                   const int* positions, void* output,
+                                   const snn_hip_rotary_params* params,
+                                   void* stream);
+SNN_HIP_API int snn_hip_rotary_bf16(const void* input,
+                                    const double* frequencies,
+                                    const int* positions, void* output,
+                                    const snn_hip_rotary_params* params,
+                                    void* stream);
+/* The frequencies of turned / 2 pairs, in turns from one position to the next:
+ * base^(-2 i / turned) / (2 pi), written to `frequencies` in host memory, which the
+ * calls above take from device memory.  For contexts `factor` times the `context`
+ * tokens that a model has been trained on:
+ *
+ *   POSITIONS  every frequency divided by factor;
+ *   BASE       the base times factor^(turned / (turned - 2)): the first pair stays,
+ *              the last is divided by factor;
+ *   BANDS      pairs of at least `high` turns within the context stay, those of
+ *              at most `low` are divided by factor, between them the two are
+ *              mixed in proportion to the turns.
+ *
+ * `context`, `low` and `high` are read for BANDS only. */
+typedef enum snn_hip_rotary_scaling {
+  SNN_HIP_ROTARY_SCALING_NONE = 0,
+  SNN_HIP_ROTARY_SCALING_POSITIONS = 1,
+  SNN_HIP_ROTARY_SCALING_BASE = 2,
+  SNN_HIP_ROTARY_SCALING_BANDS = 3
+} snn_hip_rotary_scaling;
+SNN_HIP_API int snn_hip_rotary_frequencies(int turned, double base, int scaling,
+                                           double factor, double context,
+                                           double low, double high,
+                                           double* frequencies);
+
+/* Linear attention with a decay for each head: a state of keys x values floats
+ * for each head of each sequence,
+ *
+ *   S_t = a S_{t-1} + k_t^T v_t        a = exp(decay[head])
+ *   o_t = scale q_t S_t
+ *
+ * q and k are [batch][steps][key_heads][keys], v and output
+ * [batch][steps][heads][values]; heads is a multiple of key_heads, and head h reads
+ * the queries and keys of head h / (heads / key_heads).  q, k and v have row
+ * strides of their own, elements from step to step (steps times that from sequence
+ * to sequence), so that they may be slices of one projection's rows; output has
+ * none.  decay holds `heads` floats, logarithms: 0 for a state that keeps
+ * everything; values above 0 are taken as 0, values below -10000 as -10000.  Decays
+ * are constants of the model and have no gradient here.
+ *
+ * initial_state and final_state are [batch][heads][keys][values] floats (NULL: zero,
+ * not wanted) and may be one buffer: a single token is a call with one step that
+ * updates the state in place.  resets ([batch][steps] bytes, NULL: none): where it
+ * is not zero a S_{t-1} is left out, whatever it is.  lengths ([batch] ints, NULL:
+ * all steps; clamped to 0 ... steps): steps from there on are not read, their
+ * outputs are zero, and final_state is the state behind the last step that counts
+ * (the initial state for a length of zero).  Outputs of a step depend on no later
+ * step and on no step in front of a reset, whatever values those hold.
+ *
+ * A few steps are taken one after the other, more in blocks: of each block of steps
+ * the products q_t k_s, weighted by their decays, and the states come from the
+ * matrix instructions.  These take scale q_t k_s rounded to the data type (in
+ * binary16: infinite beyond 65504), the states and the weighted values as two
+ * values of the data type each; sums and states are fp32.  Long sequences are
+ * divided into pieces that run beside one another, given a workspace of the
+ * recommended size.  The order of operations is fixed by the sizes and the
+ * workspace.  At most 256 channels of a key or a value. */
+typedef struct snn_hip_linear_attention_params {
+  int batch;
+  int steps;
+  int heads;     /* of values, states, decays and outputs */
+  int key_heads; /* of queries and keys */
+  int keys;      /* channels of a query or key */
+  int values;    /* channels of a value */
+  int q_stride;
+  int k_stride;
+  int v_stride;
+  int grad_q_stride;
+  int grad_k_stride;
+  int grad_v_stride;
+  float scale;
+} snn_hip_linear_attention_params;
+SNN_HIP_API int snn_hip_linear_attention_f32(
+    const void* q, const void* k, const void* v, const float* decay,
+    const unsigned char* resets, const int* lengths, const float* initial_state,
+    void* output, float* final_state,
+    const snn_hip_linear_attention_params* params, void* workspace,
+    size_t workspace_elems, void* stream);
+SNN_HIP_API int snn_hip_linear_attention_f16(
+    const void* q, const void* k, const void* v, const float* decay,
+    const unsigned char* resets, const int* lengths, const float* initial_state,
+    void* output, float* final_state,
+    const snn_hip_linear_attention_params* params, void* workspace,
+    size_t workspace_elems, void* stream);
+SNN_HIP_API int snn_hip_linear_attention_bf16(
+    const void* q, const void* k, const void* v, const float* decay,
+    const unsigned char* resets, const int* lengths, const float* initial_state,
+    void* output, float* final_state,
+    const snn_hip_linear_attention_params* params, void* workspace,
+    size_t workspace_elems, void* stream);
+/* The gradients.  grad_final_state may be NULL.  grad_q, grad_k and grad_v have
+ * strides of their own and are zero from a sequence's length on; each of the four
+ * outputs may be NULL and is then not computed.  No output may overlap an input.
+ * Where key_heads is not heads, the sums over the heads that share a query or key
+ * take workspace: SNN_HIP_INSUFFICIENT_WORKSPACE without the required size. */
+SNN_HIP_API int snn_hip_linear_attention_grad_f32(
+    const void* grad_output, const float* grad_final_state, const void* q,
+    const void* k, const void* v, const float* decay,
+    const unsigned char* resets, const int* lengths, const float* initial_state,
+    void* grad_q, void* grad_k, void* grad_v, float* grad_initial_state,
+    const snn_hip_linear_attention_params* params, void* workspace,
+    size_t workspace_elems, void* stream);
+SNN_HIP_API int snn_hip_linear_attention_grad_f16(
+    const void* grad_output, const float* grad_final_state, const void* q,
+    const void* k, const void* v, const float* decay,
+    const unsigned char* resets, const int* lengths, const float* initial_state,
+    void* grad_q, void* grad_k, void* grad_v, float* grad_initial_state,
+    const snn_hip_linear_attention_params* params, void* workspace,
+    size_t workspace_elems, void* stream);
+SNN_HIP_API int snn_hip_linear_attention_grad_bf16(
+    const void* grad_output, const float* grad_final_state, const void* q,
+    const void* k, const void* v, const float* decay,
+    const unsigned char* resets, const int* lengths, const float* initial_state,
+    void* grad_q, void* grad_k, void* grad_v, float* grad_initial_state,
+    const snn_hip_linear_attention_params* params, void* workspace,
+    size_t workspace_elems, void* stream);
+/* Workspace of the forward call (grad == 0) or of the gradients, in elements of
+ * `dtype`; the forward call requires none. */
+SNN_HIP_API int snn_hip_linear_attention_workspace_size(
+    const snn_hip_linear_attention_params* params, int grad, int dtype,
+    size_t* required_elems, size_t* recommended_elems);
+
 #ifdef __cplusplus
 }
 #endif

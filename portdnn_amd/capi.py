@@ -67,6 +67,24 @@ class GATE:
     SILU = 3
 
 
+class ROTARY:
+    HALVES = 0
+    PAIRS = 1
+
+
+class ROTARY_POSITIONS:
+    NONE = 0
+    FIRST = 1
+    EACH = 2
+
+
+class ROTARY_SCALING:
+    NONE = 0
+    POSITIONS = 1
+    BASE = 2
+    BANDS = 3
+
+
 class POOL_OP:
     MAX = 0
     MAX_WITH_NAN = 1
@@ -165,6 +183,24 @@ LinearRecurrenceParams = _struct(
     "LinearRecurrenceParams",
     ["batch", "steps", "channels", "row_stride", "grad_row_stride"], {})
 
+GatedMatmulParams = _struct(
+    "GatedMatmulParams",
+    ["m", "k", "n", "transpose_rhs", "activation", "lhs_stride", "rhs_stride",
+     "output_stride"], {})
+
+RotaryParams = _struct(
+    "RotaryParams",
+    ["batch", "steps", "heads", "channels", "turned", "layout", "positions",
+     "inverse", "row_stride", "output_row_stride", "magnitude"],
+    {"magnitude": 1.0}, {"magnitude": ctypes.c_float})
+
+LinearAttentionParams = _struct(
+    "LinearAttentionParams",
+    ["batch", "steps", "heads", "key_heads", "keys", "values", "q_stride",
+     "k_stride", "v_stride", "grad_q_stride", "grad_k_stride",
+     "grad_v_stride", "scale"],
+    {"scale": 1.0}, {"scale": ctypes.c_float})
+
 _P = ctypes.c_void_p
 _SZ = ctypes.c_size_t
 _I = ctypes.c_int
@@ -239,6 +275,12 @@ SIGNATURES = {
         _P, _I, ctypes.POINTER(_SZ), ctypes.POINTER(_SZ)],
     "snn_hip_linear_recurrence_workspace_size": [
         _P, _I, ctypes.POINTER(_SZ), ctypes.POINTER(_SZ)],
+    "snn_hip_gated_matmul_workspace_size": [
+        _P, _I, _I, ctypes.POINTER(_SZ), ctypes.POINTER(_SZ)],
+    "snn_hip_rotary_frequencies": [
+        _I, ctypes.c_double, _I] + [ctypes.c_double] * 4 + [_P],
+    "snn_hip_linear_attention_workspace_size": [
+        _P, _I, _I, ctypes.POINTER(_SZ), ctypes.POINTER(_SZ)],
 }
 for _type in ("f32", "f16", "bf16"):
     SIGNATURES["snn_hip_matmul_bias_act_" + _type] = [_P] * 8 + [_SZ, _P]
@@ -247,6 +289,12 @@ for _type in ("f32", "f16", "bf16"):
     SIGNATURES["snn_hip_residual_norm_grad_" + _type] = [_P] * 4 + [_SZ, _P]
     SIGNATURES["snn_hip_linear_recurrence_" + _type] = [_P] * 10 + [_SZ, _P]
     SIGNATURES["snn_hip_linear_recurrence_grad_" + _type] = (
+        [_P] * 15 + [_SZ, _P])
+    SIGNATURES["snn_hip_gated_matmul_" + _type] = [_P] * 10 + [_SZ, _P]
+    SIGNATURES["snn_hip_gated_matmul_grad_" + _type] = [_P] * 13 + [_SZ, _P]
+    SIGNATURES["snn_hip_rotary_" + _type] = [_P] * 6
+    SIGNATURES["snn_hip_linear_attention_" + _type] = [_P] * 11 + [_SZ, _P]
+    SIGNATURES["snn_hip_linear_attention_grad_" + _type] = (
         [_P] * 15 + [_SZ, _P])
 
 _lib = None

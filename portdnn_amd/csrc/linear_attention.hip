@@ -1,0 +1,684 @@
+// The entry points of linear attention (the walks over blocks of steps:
+// linear_attention.h), the walk over a few steps and the sums along pieces.
+#include <algorithm>
+#include <cmath>
+
+#include "linear_attention.h"
+
+namespace snn {
+namespace {
+
+using att::Problem;
+using att::Walk;
+using seq::Pack;
+
+// ---- a few steps ---------------------------------------------------------------
+
+constexpr int kFewSteps = 16;
+
+struct Few {
+  const void *q, *k, *v;
+  void* out;
+  long q_row, k_row, v_row;
+  int batch, heads, share, steps, keys, values, slices;
+  const float* decay;
+  const unsigned char* resets;
+  const int* lengths;
+  const float* initial;
+  float* final;
+  float scale;
+};
+
+// One step after the other, all in fp32: a work-group owns 64 values of a head's
+// state, a lane four neighbouring values of every sixteenth key.  Bound by the state,
+// which is read and written once.
+template <typename T, int R>
+__global__ void __launch_bounds__(256) few_steps_kernel(Few p) {
+  __shared__ float q_of[kFewSteps][16 * R], k_of[kFewSteps][16 * R];
+  __shared__ float sums[kFewSteps][4][64];
+  typedef Pack<float, 4>::type F;
+  const unsigned at = seq::group_of_grid();
+  const unsigned bh = at / p.slices, slice = at - bh * p.slices;
+  const unsigned b = bh / p.heads, h = bh - b * p.heads;
+  if (b >= static_cast<unsigned>(p.batch)) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int first_key = tid / 16;
+  const int col = slice * 64 + tid % 16 * 4;
+  const int cols = max(0, min(4, p.values - col));
+  const long row = static_cast<long>(b) * p.steps;
+  const long state_at =
+      static_cast<long>(bh) * p.keys * p.values + min(col, p.values - 1);
+  const int length = p.lengths == nullptr
+                         ? p.steps
+                         : max(0, min(p.steps, p.lengths[b]));
+
+  float state[R][4];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int key = first_key + 16 * i;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) state[i][c] = 0.f;
+    if (p.initial != nullptr && key < p.keys) {
+      const float* const from =
+          p.initial + state_at + static_cast<long>(key) * p.values;
+      if (cols == 4) {
+        const F f = *reinterpret_cast<const F*>(from);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) state[i][c] = f[c];
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (c < cols) state[i][c] = from[c];
+      }
+    }
+  }
+  const T* const q = static_cast<const T*>(p.q) + row * p.q_row +
+                     static_cast<long>(h / p.share) * p.keys;
+  const T* const k = static_cast<const T*>(p.k) + row * p.k_row +
+                     static_cast<long>(h / p.share) * p.keys;
+  const T* const v = static_cast<const T*>(p.v) + row * p.v_row +
+                     static_cast<long>(h) * p.values + col;
+  for (int e = tid; e < length * 16 * R; e += 256) {
+    const int t = e / (16 * R), key = e % (16 * R);
+    const bool in = key < p.keys;
+    q_of[t][key] = in ? static_cast<float>(q[t * p.q_row + key]) : 0.f;
+    k_of[t][key] = in ? static_cast<float>(k[t * p.k_row + key]) : 0.f;
+  }
+  const float a = expf(att::log_decay(p.decay, h));
+  __syncthreads();
+  for (int t = 0; t < length; ++t) {
+    float x[4] = {};
+    const T* const from = v + t * p.v_row;
+    if (cols == 4) {
+      seq::unpack<T, 4>(
+          *reinterpret_cast<const typename Pack<T, 4>::type*>(from), x);
+    } else {
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (c < cols) x[c] = static_cast<float>(from[c]);
+    }
+    const bool fresh = p.resets != nullptr && p.resets[row + t] != 0;
+    float sum[4] = {};
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const float key = k_of[t][first_key + 16 * i];
+      const float query = q_of[t][first_key + 16 * i];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        state[i][c] = key * x[c] + (fresh ? 0.f : a * state[i][c]);
+        // (keys that do not exist hold zeros)
+        sum[c] += query * state[i][c];
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      sum[c] += __shfl_xor(sum[c], 16);
+      sum[c] += __shfl_xor(sum[c], 32);
+      if (lane < 16) sums[t][wave][lane * 4 + c] = sum[c];
+    }
+  }
+  __syncthreads();
+  T* const out = static_cast<T*>(p.out) +
+                 (row * p.heads + h) * static_cast<long>(p.values) + slice * 64;
+  for (int e = tid; e < p.steps * 64; e += 256) {
+    const int t = e / 64, c = e % 64;
+    if (static_cast<int>(slice * 64) + c >= p.values) continue;
+    float s = 0.f;
+    if (t < length) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) s += sums[t][u][c];
+    }
+    out[t * static_cast<long>(p.heads) * p.values + c] =
+        static_cast<T>(s * p.scale);
+  }
+  if (p.final == nullptr) return;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int key = first_key + 16 * i;
+    if (key >= p.keys) continue;
+    float* const to = p.final + state_at + static_cast<long>(key) * p.values;
+    if (cols == 4) {
+      *reinterpret_cast<F*>(to) =
+          F{state[i][0], state[i][1], state[i][2], state[i][3]};
+    } else {
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (c < cols) to[c] = state[i][c];
+    }
+  }
+}
+
+template <typename T>
+int run_few(const Few& f, hipStream_t stream) {
+  const dim3 grid = seq::grid_of(static_cast<size_t>(f.batch) * f.heads *
+                                 f.slices);
+  if (f.keys <= 64)
+    hipLaunchKernelGGL((few_steps_kernel<T, 4>), grid, dim3(256), 0, stream, f);
+  else if (f.keys <= 128)
+    hipLaunchKernelGGL((few_steps_kernel<T, 8>), grid, dim3(256), 0, stream, f);
+  else
+    hipLaunchKernelGGL((few_steps_kernel<T, 16>), grid, dim3(256), 0, stream, f);
+  SNN_HIP_CHECK_LAUNCH();
+  return SNN_HIP_OK;
+}
+
+// ---- along the pieces ------------------------------------------------------------
+
+// The pieces' own states become the states in front of them, in the walk's order.
+struct Chain {
+  float* states;
+  const int* carries;
+  const float* initial;
+};
+struct Chains {
+  Chain chain[2];
+  int heads, pieces, piece_steps, steps;
+  long size;  // of a state
+  const float* decay;
+  const int* lengths;
+};
+__global__ void __launch_bounds__(256) chain_kernel(Chains p) {
+  const Chain& c = p.chain[blockIdx.z];
+  const int bh = blockIdx.y;
+  const long at = static_cast<long>(blockIdx.x) * 256 + threadIdx.x;
+  if (at >= p.size) return;
+  const int b = bh / p.heads, h = bh - b * p.heads;
+  const int length = p.lengths == nullptr
+                         ? p.steps
+                         : max(0, min(p.steps, p.lengths[b]));
+  const float log_a = att::log_decay(p.decay, h);
+  const float whole = expf(p.piece_steps * log_a);
+  float state = c.initial == nullptr ? 0.f : c.initial[bh * p.size + at];
+  float* to = c.states + static_cast<long>(bh) * p.pieces * p.size + at;
+  const int* const carries = c.carries + static_cast<long>(bh) * p.pieces;
+  for (int i = 0; i < p.pieces; ++i, to += p.size) {
+    // (the last piece has left no state of its own, and those behind it none at all)
+    const bool on = static_cast<long>(i + 1) * p.piece_steps < length;
+    const float own = on ? *to : 0.f;
+    *to = state;
+    if (!on) break;
+    state = (carries[i] != 0 ? whole * state : 0.f) + own;
+  }
+}
+
+// ---- gradients of shared heads ---------------------------------------------------
+
+// out[row][g][c] = sum over the group's heads of in[row][g * share + i][c].
+template <typename T>
+__global__ void __launch_bounds__(256)
+    share_kernel(const float* __restrict__ in, T* __restrict__ out, size_t rows,
+                 long out_row, int groups, int share, int keys) {
+  const size_t size = static_cast<size_t>(groups) * keys;
+  for (size_t at = (blockIdx.x + static_cast<size_t>(blockIdx.y) *
+                                     seq::kGroupsOfX) * 256 + threadIdx.x;
+       at < rows * size;
+       at += static_cast<size_t>(gridDim.x) * gridDim.y * 256) {
+    const size_t row = at / size, rest = at - row * size;
+    const size_t g = rest / keys, c = rest - g * keys;
+    const float* const from = in + ((row * groups + g) * share) * keys + c;
+    float s = 0.f;
+    for (int i = 0; i < share; ++i) s += from[static_cast<long>(i) * keys];
+    out[row * out_row + rest] = static_cast<T>(s);
+  }
+}
+
+// ---- entry points ------------------------------------------------------------------
+
+int check(const snn_hip_linear_attention_params* p, const void* workspace) {
+  if (p == nullptr) return SNN_HIP_INVALID_PARAMETER;
+  SNN_REQUIRE(p->batch > 0 && p->steps > 0 && p->heads > 0 &&
+              p->key_heads > 0 && p->keys > 0 && p->values > 0);
+  SNN_REQUIRE(p->heads % p->key_heads == 0);
+  SNN_REQUIRE(p->keys <= 256 && p->values <= 256);
+  SNN_REQUIRE(std::isfinite(p->scale));
+  const long of_keys = static_cast<long>(p->key_heads) * p->keys;
+  const long of_values = static_cast<long>(p->heads) * p->values;
+  auto stride_ok = [](int stride, long row) {
+    return stride == 0 || stride >= row;
+  };
+  SNN_REQUIRE(stride_ok(p->q_stride, of_keys) && stride_ok(p->k_stride, of_keys) &&
+              stride_ok(p->v_stride, of_values));
+  SNN_REQUIRE(stride_ok(p->grad_q_stride, of_keys) &&
+              stride_ok(p->grad_k_stride, of_keys) &&
+              stride_ok(p->grad_v_stride, of_values));
+  SNN_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15u) == 0);
+  // (steps and places of pieces are counted in 31 bits, heads in a grid's y)
+  const size_t heads = static_cast<size_t>(p->batch) * p->heads;
+  if (p->steps > (1 << 30) || heads > (1u << 20)) return SNN_HIP_INDEX_EXCEEDED;
+  return SNN_HIP_OK;
+}
+
+long or_else(int stride, long row) { return stride == 0 ? row : stride; }
+size_t round16(size_t bytes) { return (bytes + 15) / 16 * 16; }
+int class_of(int keys) { return keys <= 64 ? 64 : keys <= 128 ? 128 : 256; }
+
+// Waves of a work-group, and the work-groups that share the values.
+int waves_of(int values) { return values > 64 ? 8 : 4; }
+int slices_of(int values) { return ceil_div(values, 16 * waves_of(values)); }
+
+// How a sequence is divided: enough work-groups for the GPU, pieces that are long
+// beside their states.
+struct Division {
+  int pieces, piece_steps;
+};
+Division divide(const snn_hip_linear_attention_params& p, int units, int block,
+                size_t bytes, int states) {
+  const int blocks = ceil_div(p.steps, block);
+  const size_t groups = static_cast<size_t>(p.batch) * p.heads * units;
+  int pieces = static_cast<int>(
+      std::min<size_t>(512 / std::min<size_t>(groups, 512), blocks / 4));
+#ifdef SNN_HIP_TUNING
+  if (const char* want = std::getenv("SNN_HIP_ATT_PIECES"))
+    pieces = std::min(std::atoi(want), blocks);
+#endif
+  pieces = std::max(pieces, 1);
+  const int each = ceil_div(blocks, pieces);
+  pieces = ceil_div(blocks, each);
+  const size_t heads = static_cast<size_t>(p.batch) * p.heads * pieces;
+  const size_t need =
+      states * (round16(heads * p.keys * p.values * sizeof(float)) +
+                round16(heads * sizeof(int)));
+  if (pieces == 1 || need > bytes) return {1, blocks * block};
+  return {pieces, each * block};
+}
+size_t division_bytes(const snn_hip_linear_attention_params& p,
+                      const Division& d, int states) {
+  if (d.pieces == 1) return 0;
+  const size_t heads = static_cast<size_t>(p.batch) * p.heads * d.pieces;
+  return states * (round16(heads * p.keys * p.values * sizeof(float)) +
+                   round16(heads * sizeof(int)));
+}
+
+int forward_units(const snn_hip_linear_attention_params& p) {
+  return slices_of(p.values);
+}
+int grad_units(const snn_hip_linear_attention_params& p) {
+  return 2 * slices_of(p.keys) + slices_of(p.values);
+}
+int block_of(int elem_size) { return elem_size == 2 ? 64 : 32; }
+
+// fp32 gradients of q and k by heads, where heads share them.
+size_t shared_bytes(const snn_hip_linear_attention_params& p) {
+  return p.heads == p.key_heads
+             ? 0
+             : round16(static_cast<size_t>(p.batch) * p.steps * p.heads *
+                       p.keys * sizeof(float));
+}
+
+template <typename T>
+int run_class(const Problem& p, int keys_class, int waves, bool outputs,
+              hipStream_t stream) {
+  const size_t groups =
+      static_cast<size_t>(p.units) * p.batch * p.heads * p.pieces;
+  if (!seq::grid_fits(groups, 64 * waves)) return SNN_HIP_INDEX_EXCEEDED;
+  if (std::is_same<T, float>::value)
+    return att::run_walks_f32(p, keys_class, waves, outputs, stream);
+  if (std::is_same<T, _Float16>::value)
+    return att::run_walks_f16(p, keys_class, waves, outputs, stream);
+  return att::run_walks_bf16(p, keys_class, waves, outputs, stream);
+}
+
+Problem problem_of(const snn_hip_linear_attention_params& p, const Division& d,
+                   const float* decay, const unsigned char* resets,
+                   const int* lengths) {
+  Problem g = {};
+  g.batch = p.batch;
+  g.heads = p.heads;
+  g.steps = p.steps;
+  g.pieces = d.pieces;
+  g.piece_steps = d.piece_steps;
+  g.decay = decay;
+  g.resets = resets;
+  g.lengths = lengths;
+  return g;
+}
+void add(Problem* g, const Walk& w) {
+  g->walk[g->walks] = w;
+  g->walk[g->walks].slices = slices_of(w.values);
+  g->units += g->walk[g->walks].slices;
+  ++g->walks;
+}
+// Walks of one class of keys and one width of slices go together.
+template <typename T>
+int run_all(const Problem& base, const Walk* walks, int n, bool outputs,
+            hipStream_t stream) {
+  bool done[att::kMostWalks] = {};
+  for (int i = 0; i < n; ++i) {
+    if (done[i]) continue;
+    const int keys = class_of(walks[i].keys);
+    const int waves = waves_of(walks[i].values);
+    Problem g = base;
+    for (int j = i; j < n; ++j) {
+      if (done[j] || class_of(walks[j].keys) != keys ||
+          waves_of(walks[j].values) != waves)
+        continue;
+      add(&g, walks[j]);
+      done[j] = true;
+    }
+    const int s = run_class<T>(g, keys, waves, outputs, stream);
+    if (s != SNN_HIP_OK) return s;
+  }
+  return SNN_HIP_OK;
+}
+// The states in front of the pieces of one or two walks.
+template <typename T>
+int run_pieces(const snn_hip_linear_attention_params& p, const Problem& base,
+               const Walk* walks, int n, hipStream_t stream) {
+  const int s = run_all<T>(base, walks, n, false, stream);
+  if (s != SNN_HIP_OK) return s;
+  Chains c = {};
+  for (int i = 0; i < n; ++i)
+    c.chain[i] = {walks[i].states, walks[i].carries, walks[i].initial};
+  c.heads = p.heads;
+  c.pieces = base.pieces;
+  c.piece_steps = base.piece_steps;
+  c.steps = p.steps;
+  c.size = static_cast<long>(p.keys) * p.values;
+  c.decay = base.decay;
+  c.lengths = base.lengths;
+  hipLaunchKernelGGL(
+      chain_kernel,
+      dim3(static_cast<unsigned>(ceil_div(static_cast<size_t>(c.size), size_t{256})),
+           static_cast<unsigned>(p.batch) * p.heads, static_cast<unsigned>(n)),
+      dim3(256), 0, stream, c);
+  SNN_HIP_CHECK_LAUNCH();
+  return SNN_HIP_OK;
+}
+// Places of a walk's states and carries.
+char* place_states(const snn_hip_linear_attention_params& p, int pieces,
+                   char* at, Walk* w) {
+  const size_t heads = static_cast<size_t>(p.batch) * p.heads * pieces;
+  w->states = reinterpret_cast<float*>(at);
+  at += round16(heads * p.keys * p.values * sizeof(float));
+  w->carries = reinterpret_cast<int*>(at);
+  return at + round16(heads * sizeof(int));
+}
+
+template <typename T>
+int forward(const void* q, const void* k, const void* v, const float* decay,
+            const unsigned char* resets, const int* lengths,
+            const float* initial, void* output, float* final,
+            const snn_hip_linear_attention_params* params, void* workspace,
+            size_t elems, void* stream_arg) {
+  const int valid = check(params, workspace);
+  if (valid != SNN_HIP_OK) return valid;
+  const snn_hip_linear_attention_params& p = *params;
+  SNN_REQUIRE(q != nullptr && k != nullptr && v != nullptr && decay != nullptr &&
+              output != nullptr);
+  const hipStream_t stream = as_stream(stream_arg);
+  const long of_keys = static_cast<long>(p.key_heads) * p.keys;
+  const long of_values = static_cast<long>(p.heads) * p.values;
+  KernelTimer timer(stream);
+  if (p.steps <= kFewSteps) {
+    Few f = {};
+    f.q = q;
+    f.k = k;
+    f.v = v;
+    f.out = output;
+    f.q_row = or_else(p.q_stride, of_keys);
+    f.k_row = or_else(p.k_stride, of_keys);
+    f.v_row = or_else(p.v_stride, of_values);
+    f.batch = p.batch;
+    f.heads = p.heads;
+    f.share = p.heads / p.key_heads;
+    f.steps = p.steps;
+    f.keys = p.keys;
+    f.values = p.values;
+    f.slices = ceil_div(p.values, 64);
+    f.decay = decay;
+    f.resets = resets;
+    f.lengths = lengths;
+    f.initial = initial;
+    f.final = final;
+    f.scale = p.scale;
+    return run_few<T>(f, stream);
+  }
+  Walk w = {};
+  w.q = q;
+  w.k = k;
+  w.v = v;
+  w.out = output;
+  w.q_row = or_else(p.q_stride, of_keys);
+  w.k_row = or_else(p.k_stride, of_keys);
+  w.v_row = or_else(p.v_stride, of_values);
+  w.out_row = of_values;
+  w.q_share = w.k_share = p.heads / p.key_heads;
+  w.v_share = 1;
+  w.keys = p.keys;
+  w.values = p.values;
+  w.initial = initial;
+  w.final = final;
+  w.weight = p.scale;
+  w.reach_weight = p.scale;
+  w.state_weight = 1.f;
+  const Division d =
+      divide(p, forward_units(p), block_of(sizeof(T)),
+             workspace == nullptr ? 0 : elems * sizeof(T), 1);
+  const Problem base = problem_of(p, d, decay, resets, lengths);
+  if (d.pieces > 1) {
+    place_states(p, d.pieces, static_cast<char*>(workspace), &w);
+    const int s = run_pieces<T>(p, base, &w, 1, stream);
+    if (s != SNN_HIP_OK) return s;
+  }
+  return run_all<T>(base, &w, 1, true, stream);
+}
+
+template <typename T>
+int share_sum(const snn_hip_linear_attention_params& p, const float* in,
+              void* out, int stride, hipStream_t stream) {
+  const long width = static_cast<long>(p.key_heads) * p.keys;
+  const size_t rows = static_cast<size_t>(p.batch) * p.steps;
+  const size_t groups = std::min<size_t>(
+      ceil_div(rows * static_cast<size_t>(width), size_t{256}), 1u << 20);
+  hipLaunchKernelGGL(share_kernel<T>, seq::grid_of(groups), dim3(256), 0, stream,
+                     in, static_cast<T*>(out), rows, or_else(stride, width),
+                     p.key_heads, p.heads / p.key_heads, p.keys);
+  SNN_HIP_CHECK_LAUNCH();
+  return SNN_HIP_OK;
+}
+
+template <typename T>
+int backward(const void* grad, const float* grad_final, const void* q,
+             const void* k, const void* v, const float* decay,
+             const unsigned char* resets, const int* lengths,
+             const float* initial, void* grad_q, void* grad_k, void* grad_v,
+             float* grad_initial, const snn_hip_linear_attention_params* params,
+             void* workspace, size_t elems, void* stream_arg) {
+  const int valid = check(params, workspace);
+  if (valid != SNN_HIP_OK) return valid;
+  const snn_hip_linear_attention_params& p = *params;
+  SNN_REQUIRE(grad != nullptr && q != nullptr && k != nullptr && v != nullptr &&
+              decay != nullptr);
+  SNN_REQUIRE(grad_q != nullptr || grad_k != nullptr || grad_v != nullptr ||
+              grad_initial != nullptr);
+  const hipStream_t stream = as_stream(stream_arg);
+  const long of_keys = static_cast<long>(p.key_heads) * p.keys;
+  const long of_values = static_cast<long>(p.heads) * p.values;
+  const int share = p.heads / p.key_heads;
+  const size_t each = shared_bytes(p);
+  const size_t shared = each * ((grad_q != nullptr) + (grad_k != nullptr));
+  const size_t bytes = workspace == nullptr ? 0 : elems * sizeof(T);
+  if (bytes < shared) return SNN_HIP_INSUFFICIENT_WORKSPACE;
+  char* at = static_cast<char*>(workspace);
+  float *q_sums = nullptr, *k_sums = nullptr;
+  if (each > 0 && grad_q != nullptr) {
+    q_sums = reinterpret_cast<float*>(at);
+    at += each;
+  }
+  if (each > 0 && grad_k != nullptr) {
+    k_sums = reinterpret_cast<float*>(at);
+    at += each;
+  }
+  const long q_row = or_else(p.q_stride, of_keys);
+  const long k_row = or_else(p.k_stride, of_keys);
+  const long v_row = or_else(p.v_stride, of_values);
+
+  Walk of_q = {}, of_k = {}, of_v = {}, front = {};
+  of_q.q = grad;
+  of_q.q_row = of_values;
+  of_q.q_share = 1;
+  of_q.k = v;
+  of_q.k_row = v_row;
+  of_q.k_share = 1;
+  of_q.v = k;
+  of_q.v_row = k_row;
+  of_q.v_share = share;
+  of_q.keys = p.values;
+  of_q.values = p.keys;
+  of_q.initial = initial;
+  of_q.transposed = 1;
+  of_q.weight = of_q.reach_weight = p.scale;
+  of_q.state_weight = 1.f;
+
+  of_k.q = v;
+  of_k.q_row = v_row;
+  of_k.q_share = 1;
+  of_k.k = grad;
+  of_k.k_row = of_values;
+  of_k.k_share = 1;
+  of_k.v = q;
+  of_k.v_row = q_row;
+  of_k.v_share = share;
+  of_k.keys = p.values;
+  of_k.values = p.keys;
+  of_k.initial = grad_final;
+  of_k.transposed = 1;
+  of_k.from_end = 1;
+  of_k.weight = of_k.state_weight = p.scale;
+  of_k.reach_weight = 1.f;
+
+  of_v.q = k;
+  of_v.q_row = k_row;
+  of_v.q_share = share;
+  of_v.k = q;
+  of_v.k_row = q_row;
+  of_v.k_share = share;
+  of_v.v = grad;
+  of_v.v_row = of_values;
+  of_v.v_share = 1;
+  of_v.out = grad_v;
+  of_v.out_row = or_else(p.grad_v_stride, of_values);
+  of_v.keys = p.keys;
+  of_v.values = p.values;
+  of_v.initial = grad_final;
+  of_v.final = grad_initial;
+  of_v.from_end = 1;
+  of_v.weight = of_v.state_weight = p.scale;
+  of_v.reach_weight = 1.f;
+
+  auto output = [&](Walk* w, void* out, int stride, float* sums) {
+    w->out = sums != nullptr ? sums : out;
+    w->out_float = sums != nullptr;
+    w->out_row = sums != nullptr ? static_cast<long>(p.heads) * p.keys
+                                 : or_else(stride, of_keys);
+  };
+  output(&of_q, grad_q, p.grad_q_stride, q_sums);
+  output(&of_k, grad_k, p.grad_k_stride, k_sums);
+
+  KernelTimer timer(stream);
+  const Division d =
+      divide(p, grad_units(p), block_of(sizeof(T)), bytes - shared, 2);
+  const Problem base = problem_of(p, d, decay, resets, lengths);
+  if (d.pieces > 1) {
+    // the states from the front, as the forward pass has them, and from the end
+    front = {};
+    front.k = k;
+    front.k_row = k_row;
+    front.k_share = share;
+    front.v = v;
+    front.v_row = v_row;
+    front.v_share = 1;
+    front.q_share = 1;
+    front.keys = p.keys;
+    front.values = p.values;
+    front.initial = initial;
+    front.state_weight = 1.f;
+    at = place_states(p, d.pieces, at, &front);
+    place_states(p, d.pieces, at, &of_v);
+    of_q.states = front.states;
+    of_k.states = of_v.states;
+    Walk both[2];
+    int n = 0;
+    if (grad_q != nullptr) both[n++] = front;
+    if (grad_k != nullptr || grad_v != nullptr || grad_initial != nullptr)
+      both[n++] = of_v;
+    const int s = run_pieces<T>(p, base, both, n, stream);
+    if (s != SNN_HIP_OK) return s;
+  }
+  Walk walks[att::kMostWalks];
+  int n = 0;
+  if (grad_q != nullptr) walks[n++] = of_q;
+  if (grad_k != nullptr) walks[n++] = of_k;
+  if (grad_v != nullptr || grad_initial != nullptr) walks[n++] = of_v;
+  int s = run_all<T>(base, walks, n, true, stream);
+  if (s == SNN_HIP_OK && q_sums != nullptr)
+    s = share_sum<T>(p, q_sums, grad_q, p.grad_q_stride, stream);
+  if (s == SNN_HIP_OK && k_sums != nullptr)
+    s = share_sum<T>(p, k_sums, grad_k, p.grad_k_stride, stream);
+  return s;
+}
+
+}  // namespace
+}  // namespace snn
+
+#define SNN_LINEAR_ATTENTION(suffix, T)                                        \
+  int snn_hip_linear_attention_##suffix(                                       \
+      const void* q, const void* k, const void* v, const float* decay,         \
+      const unsigned char* resets, const int* lengths,                         \
+      const float* initial_state, void* output, float* final_state,            \
+      const snn_hip_linear_attention_params* params, void* workspace,          \
+      size_t workspace_elems, void* stream) {                                  \
+    return snn::forward<T>(q, k, v, decay, resets, lengths, initial_state,     \
+                           output, final_state, params, workspace,             \
+                           workspace_elems, stream);                           \
+  }                                                                            \
+  int snn_hip_linear_attention_grad_##suffix(                                  \
+      const void* grad_output, const float* grad_final_state, const void* q,   \
+      const void* k, const void* v, const float* decay,                        \
+      const unsigned char* resets, const int* lengths,                         \
+      const float* initial_state, void* grad_q, void* grad_k, void* grad_v,    \
+      float* grad_initial_state,                                               \
+      const snn_hip_linear_attention_params* params, void* workspace,          \
+      size_t workspace_elems, void* stream) {                                  \
+    return snn::backward<T>(grad_output, grad_final_state, q, k, v, decay,     \
+                            resets, lengths, initial_state, grad_q, grad_k,    \
+                            grad_v, grad_initial_state, params, workspace,     \
+                            workspace_elems, stream);                          \
+  }
+
+extern "C" {
+
+SNN_LINEAR_ATTENTION(f32, float)
+SNN_LINEAR_ATTENTION(f16, _Float16)
+SNN_LINEAR_ATTENTION(bf16, __bf16)
+
+int snn_hip_linear_attention_workspace_size(
+    const snn_hip_linear_attention_params* params, int grad, int dtype,
+    size_t* required_elems, size_t* recommended_elems) {
+  if (dtype < SNN_HIP_DTYPE_F32 || dtype > SNN_HIP_DTYPE_BF16 ||
+      required_elems == nullptr || recommended_elems == nullptr)
+    return SNN_HIP_INVALID_PARAMETER;
+  const int valid = snn::check(params, nullptr);
+  if (valid != SNN_HIP_OK) return valid;
+  const size_t size = dtype == SNN_HIP_DTYPE_F32 ? 4 : 2;
+  const int block = snn::block_of(static_cast<int>(size));
+  if (grad != 0) {
+    const size_t shared = 2 * snn::shared_bytes(*params);
+    const snn::Division d = snn::divide(*params, snn::grad_units(*params), block,
+                                        ~size_t{0}, 2);
+    *required_elems = shared / size;
+    *recommended_elems =
+        (shared + snn::division_bytes(*params, d, 2)) / size;
+  } else {
+    *required_elems = 0;
+    *recommended_elems = 0;
+    if (params->steps > snn::kFewSteps) {
+      const snn::Division d = snn::divide(
+          *params, snn::forward_units(*params), block, ~size_t{0}, 1);
+      *recommended_elems = snn::division_bytes(*params, d, 1) / size;
+    }
+  }
+  return SNN_HIP_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,13 @@
+// The kernels of linear_attention.h for binary16.
+#include "linear_attention.h"
+
+namespace snn {
+namespace att {
+
+int run_walks_f16(const Problem& p, int keys_class, int waves, bool outputs,
+                 hipStream_t stream) {
+  return run_walks<_Float16>(p, keys_class, waves, outputs, stream);
+}
+
+}  // namespace att
+}  // namespace snn

@@ -509,6 +509,161 @@ PyObject* linear_recurrence_grad(PyObject*, PyObject* const* args,
   });
 }
 
+void read_params(Args& a, snn_hip_gated_matmul_params* p) {
+  p->m = a.integer();
+  p->k = a.integer();
+  p->n = a.integer();
+  p->transpose_rhs = a.integer();
+  p->activation = a.integer();
+  p->lhs_stride = a.integer();
+  p->rhs_stride = a.integer();
+  p->output_stride = a.integer();
+}
+
+// (fn, lhs, gate_weight, up_weight, gate_bias, up_bias, output, gate, up,
+//  <8 numbers>, workspace, elements, stream)
+PyObject* gated_matmul(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 20);
+  if (!a.ok) return nullptr;
+  using Fn = int (*)(const void*, const void*, const void*, const void*,
+                     const void*, void*, void*, void*,
+                     const snn_hip_gated_matmul_params*, void*, size_t, void*);
+  const Fn fn = reinterpret_cast<Fn>(a.pointer());
+  void* t[8];
+  for (void*& p : t) p = a.pointer();
+  snn_hip_gated_matmul_params params;
+  read_params(a, &params);
+  void* const workspace = a.pointer();
+  const size_t elems = a.size();
+  void* const stream = a.pointer();
+  return launch(a, [&] {
+    return fn(t[0], t[1], t[2], t[3], t[4], t[5], t[6], t[7], &params, workspace,
+              elems, stream);
+  });
+}
+
+// (fn, grad_output, lhs, gate_weight, up_weight, gate, up, grad_lhs,
+//  grad_gate_weight, grad_up_weight, grad_gate_bias, grad_up_bias, <8 numbers>,
+//  workspace, elements, stream)
+PyObject* gated_matmul_grad(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 23);
+  if (!a.ok) return nullptr;
+  using Fn = int (*)(const void*, const void*, const void*, const void*,
+                     const void*, const void*, void*, void*, void*, void*, void*,
+                     const snn_hip_gated_matmul_params*, void*, size_t, void*);
+  const Fn fn = reinterpret_cast<Fn>(a.pointer());
+  void* t[11];
+  for (void*& p : t) p = a.pointer();
+  snn_hip_gated_matmul_params params;
+  read_params(a, &params);
+  void* const workspace = a.pointer();
+  const size_t elems = a.size();
+  void* const stream = a.pointer();
+  return launch(a, [&] {
+    return fn(t[0], t[1], t[2], t[3], t[4], t[5], t[6], t[7], t[8], t[9], t[10],
+              &params, workspace, elems, stream);
+  });
+}
+
+// (fn, input, frequencies, positions, output, <10 numbers>, magnitude, stream)
+PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 17);
+  if (!a.ok) return nullptr;
+  using Fn = int (*)(const void*, const double*, const int*, void*,
+                     const snn_hip_rotary_params*, void*);
+  const Fn fn = reinterpret_cast<Fn>(a.pointer());
+  const void* const input = a.pointer();
+  const double* const frequencies = static_cast<const double*>(a.pointer());
+  const int* const positions = static_cast<const int*>(a.pointer());
+  void* const output = a.pointer();
+  snn_hip_rotary_params p;
+  p.batch = a.integer();
+  p.steps = a.integer();
+  p.heads = a.integer();
+  p.channels = a.integer();
+  p.turned = a.integer();
+  p.layout = a.integer();
+  p.positions = a.integer();
+  p.inverse = a.integer();
+  p.row_stride = a.integer();
+  p.output_row_stride = a.integer();
+  p.magnitude = static_cast<float>(a.real());
+  void* const stream = a.pointer();
+  return launch(a, [&] {
+    return fn(input, frequencies, positions, output, &p, stream);
+  });
+}
+
+void read_params(Args& a, snn_hip_linear_attention_params* p) {
+  p->batch = a.integer();
+  p->steps = a.integer();
+  p->heads = a.integer();
+  p->key_heads = a.integer();
+  p->keys = a.integer();
+  p->values = a.integer();
+  p->q_stride = a.integer();
+  p->k_stride = a.integer();
+  p->v_stride = a.integer();
+  p->grad_q_stride = a.integer();
+  p->grad_k_stride = a.integer();
+  p->grad_v_stride = a.integer();
+  p->scale = static_cast<float>(a.real());
+}
+
+// (fn, q, k, v, decay, resets, lengths, initial_state, output, final_state,
+//  <12 numbers>, scale, workspace, elements, stream)
+PyObject* linear_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 26);
+  if (!a.ok) return nullptr;
+  using Fn = int (*)(const void*, const void*, const void*, const float*,
+                     const unsigned char*, const int*, const float*, void*,
+                     float*, const snn_hip_linear_attention_params*, void*,
+                     size_t, void*);
+  const Fn fn = reinterpret_cast<Fn>(a.pointer());
+  void* t[9];
+  for (void*& p : t) p = a.pointer();
+  snn_hip_linear_attention_params params;
+  read_params(a, &params);
+  void* const workspace = a.pointer();
+  const size_t elems = a.size();
+  void* const stream = a.pointer();
+  return launch(a, [&] {
+    return fn(t[0], t[1], t[2], static_cast<const float*>(t[3]),
+              static_cast<const unsigned char*>(t[4]),
+              static_cast<const int*>(t[5]), static_cast<const float*>(t[6]),
+              t[7], static_cast<float*>(t[8]), &params, workspace, elems, stream);
+  });
+}
+
+// (fn, grad_output, grad_final_state, q, k, v, decay, resets, lengths,
+//  initial_state, grad_q, grad_k, grad_v, grad_initial_state, <12 numbers>, scale,
+//  workspace, elements, stream)
+PyObject* linear_attention_grad(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 30);
+  if (!a.ok) return nullptr;
+  using Fn = int (*)(const void*, const float*, const void*, const void*,
+                     const void*, const float*, const unsigned char*, const int*,
+                     const float*, void*, void*, void*, float*,
+                     const snn_hip_linear_attention_params*, void*, size_t,
+                     void*);
+  const Fn fn = reinterpret_cast<Fn>(a.pointer());
+  void* t[13];
+  for (void*& p : t) p = a.pointer();
+  snn_hip_linear_attention_params params;
+  read_params(a, &params);
+  void* const workspace = a.pointer();
+  const size_t elems = a.size();
+  void* const stream = a.pointer();
+  return launch(a, [&] {
+    return fn(t[0], static_cast<const float*>(t[1]), t[2], t[3], t[4],
+              static_cast<const float*>(t[5]),
+              static_cast<const unsigned char*>(t[6]),
+              static_cast<const int*>(t[7]), static_cast<const float*>(t[8]),
+              t[9], t[10], t[11], static_cast<float*>(t[12]), &params, workspace,
+              elems, stream);
+  });
+}
+
 #define SNN_PY_METHOD(name)                                              \
   {                                                                      \
     #name,                                                               \
@@ -529,6 +684,11 @@ PyMethodDef methods[] = {SNN_PY_METHOD(conv2d),
                          SNN_PY_METHOD(residual_norm_grad),
                          SNN_PY_METHOD(linear_recurrence),
                          SNN_PY_METHOD(linear_recurrence_grad),
+                         SNN_PY_METHOD(gated_matmul),
+                         SNN_PY_METHOD(gated_matmul_grad),
+                         SNN_PY_METHOD(rotary),
+                         SNN_PY_METHOD(linear_attention),
+                         SNN_PY_METHOD(linear_attention_grad),
                          {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods,

@@ -9,7 +9,8 @@ import torch
 
 from . import _native, capi
 from .capi import ACTIVATION, ALGO, BINARY_OP, DIRECTION, DTYPE, GATE, NORM, \
-    POINTWISE_OP, POOL_OP, STATUS, ConvParams, DepthwiseParams, \
+    POINTWISE_OP, POOL_OP, ROTARY, ROTARY_POSITIONS, ROTARY_SCALING, STATUS, \
+    ConvParams, DepthwiseParams, GatedMatmulParams, LinearAttentionParams, \
     LinearRecurrenceParams, MatmulBiasActParams, PoolParams, ResidualNormParams
 
 
@@ -892,20 +893,295 @@ def linear_recurrence_grad(grad, x, forget, h, input_gate=None, resets=None,
     return got
 
 
+# ---- a linear-attention block ------------------------------------------------
+# Heads are a dimension of their own: [batch, steps, heads, channels] tensors whose
+# heads follow one another, and whose rows of heads may be slices of wider ones.
+
+
+def _gated_plan(key, a, w_gate, w_up, grad, activation, trans_b):
+    dtype = a.dtype
+    m, k = a.shape
+    n = w_gate.shape[0] if trans_b else w_gate.shape[1]
+    stride = _row_stride(w_gate)
+    assert (w_gate.shape[1] if trans_b else w_gate.shape[0]) == k
+    assert w_up.shape == w_gate.shape and _row_stride(w_up) == stride
+    assert w_gate.dtype == dtype and w_up.dtype == dtype
+    suffix, code = _TYPES[dtype]
+    out_stride = 0
+    if grad is not None:
+        assert grad.shape == (m, n) and grad.dtype == dtype
+        out_stride = _row_stride(grad)
+    p = GatedMatmulParams(
+        m=m, k=k, n=n, transpose_rhs=int(trans_b), activation=activation,
+        lhs_stride=_row_stride(a), rhs_stride=stride, output_stride=out_stride)
+    elems = _workspace("snn_hip_gated_matmul_workspace_size", p,
+                       int(grad is not None), code)
+    name = "snn_hip_gated_matmul" + ("_grad" if grad is not None else "")
+    return _keep(key, (_address(name + suffix), m, k, n, p.lhs_stride, stride,
+                       out_stride, elems))
+
+
+def gated_matmul(a, w_gate, w_up, bias_gate=None, bias_up=None,
+                 activation=ACTIVATION.SILU, trans_b=False,
+                 keep_pre_activation=False, out=None, workspace=None):
+    """snn_hip_gated_matmul: act(a w_gate + bias_gate) * (a w_up + bias_up).  With
+    keep_pre_activation returns (output, gate, up), of which the gradients take
+    the second and third: the two factors in front of the activation."""
+    dtype = a.dtype
+    key = ("gated", a.shape, a.stride(), w_gate.shape, w_gate.stride(),
+           w_up.shape, w_up.stride(), dtype, w_gate.dtype, w_up.dtype,
+           activation, trans_b)
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _gated_plan(key, a, w_gate, w_up, None, activation, trans_b)
+    fn, m, k, n, a_stride, b_stride, _, elems = plan
+    if out is None:
+        out = a.new_empty((m, n))
+        out_stride = n
+    else:
+        assert out.shape == (m, n) and out.dtype == dtype
+        out_stride = _row_stride(out)
+    gate = up = None
+    if keep_pre_activation:
+        gate, up = a.new_empty((m, n)), a.new_empty((m, n))
+    if workspace is None:
+        if elems:
+            workspace = a.new_empty(elems)
+    else:
+        elems = _room(workspace, a)
+    code = _native.gated_matmul(
+        fn, a.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(),
+        _vector(bias_gate, n, dtype), _vector(bias_up, n, dtype),
+        out.data_ptr(), _at(gate), _at(up), m, k, n, trans_b, activation,
+        a_stride, b_stride, out_stride, _at(workspace), elems, _stream())
+    if code:
+        capi.check(code)
+    return (out, gate, up) if keep_pre_activation else out
+
+
+def gated_matmul_grad(grad, a, w_gate, w_up, gate, up,
+                      activation=ACTIVATION.SILU, trans_b=False, bias=True,
+                      need_a=True, need_b=True, workspace=None):
+    """snn_hip_gated_matmul_grad: the gradients of a, w_gate, w_up, bias_gate and
+    bias_up, None for those that are not wanted."""
+    dtype = a.dtype
+    key = ("gated", a.shape, a.stride(), w_gate.shape, w_gate.stride(),
+           w_up.shape, w_up.stride(), grad.shape, grad.stride(), dtype,
+           w_gate.dtype, w_up.dtype, grad.dtype, activation, trans_b)
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _gated_plan(key, a, w_gate, w_up, grad, activation, trans_b)
+    fn, m, k, n, a_stride, b_stride, grad_stride, elems = plan
+    grad_a = a.new_empty(a.shape) if need_a else None
+    grad_gate = a.new_empty(w_gate.shape) if need_b else None
+    grad_up = a.new_empty(w_gate.shape) if need_b else None
+    bias_gate = a.new_empty(n) if bias else None
+    bias_up = a.new_empty(n) if bias else None
+    if workspace is None:
+        if elems:
+            workspace = a.new_empty(elems)
+    else:
+        elems = _room(workspace, a)
+    code = _native.gated_matmul_grad(
+        fn, grad.data_ptr(), a.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(),
+        _like(gate, (m, n), dtype), _like(up, (m, n), dtype), _at(grad_a),
+        _at(grad_gate), _at(grad_up), _at(bias_gate), _at(bias_up), m, k, n,
+        trans_b, activation, a_stride, b_stride, grad_stride, _at(workspace),
+        elems, _stream())
+    if code:
+        capi.check(code)
+    return grad_a, grad_gate, grad_up, bias_gate, bias_up
+
+
+def _head_stride(t):
+    """Elements from step to step of a [batch, steps, heads, channels] tensor."""
+    batch, steps, heads, channels = t.shape
+    outer, step, head, unit = t.stride()
+    width = heads * channels
+    assert unit == 1 or channels == 1, "channels are not contiguous"
+    assert head == channels or heads == 1, "heads do not follow one another"
+    if steps == 1:
+        step = outer if batch > 1 else width
+    else:
+        assert batch == 1 or outer == steps * step, \
+            "sequences do not follow one another"
+    assert step >= width
+    return step
+
+
+def rotary_frequencies(turned, base=10000.0, scaling=ROTARY_SCALING.NONE,
+                       factor=1.0, context=0.0, low=1.0, high=32.0,
+                       device="cuda"):
+    """snn_hip_rotary_frequencies: the float64 table that `rotary` takes, turns
+    from one position to the next of turned / 2 pairs, on `device`."""
+    table = torch.empty(max(turned, 0) // 2, dtype=torch.float64)
+    capi.check(capi.lib().snn_hip_rotary_frequencies(
+        turned, base, scaling, factor, context, low, high, table.data_ptr()))
+    return table.to(device)
+
+
+def rotary(x, frequencies, positions=None, layout=ROTARY.HALVES, magnitude=1.0,
+           inverse=False, out=None):
+    """snn_hip_rotary over a [batch, steps, heads, channels] tensor, of whose
+    channels the first 2 * len(frequencies) are turned.  positions: None (a token's
+    step), an int32 [batch] tensor (of step 0) or [batch, steps] one.  `out` may be
+    x.  The gradient is the call with `inverse` on the output's gradient."""
+    batch, steps, heads, channels = shape = x.shape
+    dtype = x.dtype
+    assert frequencies.dtype is torch.float64 and frequencies.dim() == 1 and \
+        frequencies.is_contiguous()
+    kind = ROTARY_POSITIONS.NONE
+    if positions is not None:
+        kind = ROTARY_POSITIONS.FIRST
+        if positions.dim() != 1:
+            kind = ROTARY_POSITIONS.EACH
+        assert positions.dtype is torch.int32 and positions.is_contiguous() and \
+            positions.shape == shape[:positions.dim()]
+    stride = _head_stride(x)
+    if out is None:
+        out = x.new_empty(shape)
+        out_stride = heads * channels
+    elif out is x:
+        out_stride = stride
+    else:
+        assert out.shape == shape and out.dtype == dtype
+        out_stride = _head_stride(out)
+    code = _native.rotary(
+        _address("snn_hip_rotary" + _TYPES[dtype][0]), x.data_ptr(),
+        frequencies.data_ptr(), _at(positions), out.data_ptr(), batch, steps,
+        heads, channels, 2 * frequencies.shape[0], layout, kind, inverse, stride,
+        out_stride, magnitude, _stream())
+    if code:
+        capi.check(code)
+    return out
+
+
+def _attention_operands(q, k, v, decay, resets, lengths, grad):
+    """Sizes, strides, the workspace's elements and the small operands'
+    addresses."""
+    key = ("attention", q.shape, q.stride(), k.shape, k.stride(), v.shape,
+           v.stride(), q.dtype, k.dtype, v.dtype, grad)
+    plan = _plans.get(key)
+    if plan is None:
+        batch, steps, key_heads, keys = q.shape
+        heads, values = v.shape[2:]
+        assert k.shape == q.shape and v.shape[:2] == q.shape[:2]
+        assert k.dtype == q.dtype and v.dtype == q.dtype
+        strides = _head_stride(q), _head_stride(k), _head_stride(v)
+        params = LinearAttentionParams(
+            batch=batch, steps=steps, heads=heads, key_heads=key_heads,
+            keys=keys, values=values)
+        plan = _keep(key, (
+            (batch, steps, heads, key_heads, keys, values) + strides,
+            _workspace("snn_hip_linear_attention_workspace_size", params,
+                       int(grad), _TYPES[q.dtype][1])))
+    sizes, elems = plan
+    return sizes, elems, _vector(decay, sizes[2], torch.float32), \
+        _like(resets, sizes[:2], torch.uint8), \
+        _vector(lengths, sizes[0], torch.int32)
+
+
+def linear_attention(q, k, v, decay, resets=None, lengths=None,
+                     initial_state=None, scale=1.0, out=None, final_state=None,
+                     workspace=None):
+    """snn_hip_linear_attention: q and k are [batch, steps, key_heads, keys], v is
+    [batch, steps, heads, values]; decay holds the logarithms of the heads' decays
+    (fp32), resets is a uint8 [batch, steps] tensor, lengths an int32 [batch] one,
+    states are fp32 [batch, heads, keys, values].  Returns (output, final state);
+    final_state may be initial_state, which is then updated in place."""
+    sizes, elems, decay_at, resets_at, lengths_at = _attention_operands(
+        q, k, v, decay, resets, lengths, False)
+    batch, steps, heads, _, keys, values = sizes[:6]
+    dtype = q.dtype
+    if out is None:
+        out = v.new_empty(v.shape)
+        out_at = out.data_ptr()
+    else:
+        out_at = _like(out, v.shape, dtype)
+    state = (batch, heads, keys, values)
+    initial_at = _like(initial_state, state, torch.float32)
+    if final_state is None:
+        final_state = q.new_empty(state, dtype=torch.float32)
+        final_at = final_state.data_ptr()
+    elif final_state is initial_state:
+        final_at = initial_at
+    else:
+        final_at = _like(final_state, state, torch.float32)
+    if workspace is None:
+        if elems:
+            workspace = q.new_empty(elems)
+    else:
+        elems = _room(workspace, q)
+    code = _native.linear_attention(
+        _address("snn_hip_linear_attention" + _TYPES[dtype][0]), q.data_ptr(),
+        k.data_ptr(), v.data_ptr(), decay_at, resets_at, lengths_at, initial_at,
+        out_at, final_at, *sizes, 0, 0, 0, scale, _at(workspace), elems,
+        _stream())
+    if code:
+        capi.check(code)
+    return out, final_state
+
+
+def linear_attention_grad(grad, q, k, v, decay, resets=None, lengths=None,
+                          initial_state=None, grad_final_state=None, scale=1.0,
+                          out=None, workspace=None):
+    """snn_hip_linear_attention_grad: a dict of the gradients of q, k, v and
+    initial_state.  `out` is a [batch, steps, 2 * key_heads * keys + heads * values]
+    tensor, or such a slice of a wider one, that takes those of q, k and v side by
+    side: the gradient of a projection that they are slices of."""
+    sizes, elems, decay_at, resets_at, lengths_at = _attention_operands(
+        q, k, v, decay, resets, lengths, True)
+    batch, steps, heads, key_heads, keys, values = sizes[:6]
+    dtype = q.dtype
+    if out is None:
+        got = {"q": q.new_empty(q.shape), "k": k.new_empty(k.shape),
+               "v": v.new_empty(v.shape)}
+        strides = 0, 0, 0
+    else:
+        n, m = key_heads * keys, heads * values
+        assert out.shape == (batch, steps, 2 * n + m) and out.dtype == dtype
+        got = {"q": out[..., :n].unflatten(2, (key_heads, keys)),
+               "k": out[..., n:2 * n].unflatten(2, (key_heads, keys)),
+               "v": out[..., 2 * n:].unflatten(2, (heads, values))}
+        strides = (_step_stride(out),) * 3
+    state = (batch, heads, keys, values)
+    got["initial_state"] = q.new_empty(state, dtype=torch.float32)
+    if workspace is None:
+        if elems:
+            workspace = q.new_empty(elems)
+    else:
+        elems = _room(workspace, q)
+    code = _native.linear_attention_grad(
+        _address("snn_hip_linear_attention_grad" + _TYPES[dtype][0]),
+        _like(grad, v.shape, dtype),
+        _like(grad_final_state, state, torch.float32), q.data_ptr(),
+        k.data_ptr(), v.data_ptr(), decay_at, resets_at, lengths_at,
+        _like(initial_state, state, torch.float32), got["q"].data_ptr(),
+        got["k"].data_ptr(), got["v"].data_ptr(),
+        got["initial_state"].data_ptr(), *sizes, *strides, scale,
+        _at(workspace), elems, _stream())
+    if code:
+        capi.check(code)
+    return got
+
+
 __all__ = [
     "ACTIVATION", "ALGO", "BINARY_OP", "DIRECTION", "GATE", "NORM",
-    "POINTWISE_OP", "POOL_OP", "STATUS",
+    "POINTWISE_OP", "POOL_OP", "ROTARY", "ROTARY_POSITIONS", "ROTARY_SCALING",
+    "STATUS",
     "ConvParams", "DepthwiseParams", "PoolParams", "add_padding_to",
     "binaryop", "binaryop_raw", "calculate_padding", "conv2d",
     "conv2d_bias_act", "conv2d_prepare_filter", "conv2d_prepared",
     "conv2d_raw", "conv_flops", "conv_params", "conv_sizes",
     "default_algorithm",
     "depthwise_conv2d", "depthwise_params", "depthwise_sizes",
+    "gated_matmul", "gated_matmul_grad", "linear_attention",
+    "linear_attention_grad",
     "linear_recurrence", "linear_recurrence_grad", "matmul", "matmul_bias_act",
     "matmul_bias_act_grad", "matmul_plan",
     "pointwise_forward", "pointwise_grad", "pool_params", "pooling_avg_grad",
     "pooling_forward", "pooling_max_grad", "residual_norm",
-    "residual_norm_grad", "workspace_size",
+    "residual_norm_grad", "rotary", "rotary_frequencies", "workspace_size",
 ]
 
 
