@@ -49,6 +49,7 @@ namespace snn {
 namespace att {
 
 using epi::float4v;
+using epi::lds_ptr;
 using epi::lds_short4_ptr;
 using epi::short4v;
 using epi::uint4v;
@@ -260,28 +261,39 @@ __device__ __forceinline__ Part part_of(const Problem& p) {
   return r;
 }
 
-// D: the keys, rounded up; WAVES: of a work-group, with 16 values each.
-template <typename T, int D, int WAVES, bool OUTPUT>
-__global__ void __launch_bounds__(64 * WAVES, 2)
-    walk_kernel(Problem p) {
-#ifdef __HIP_DEVICE_COMPILE__
+// D: the keys, rounded up; WAVES: of a work-group, with 16 values each.  DIRECT: rows of
+// whole 16-byte pieces at aligned addresses, which go straight to LDS, STAGES blocks
+// in a ring; otherwise they pass through registers, where one block is under way.
+//
+// LDS holds three blocks of 128 keys, q and 128 values, or two work-groups of a CU
+// with two blocks each.
+template <int D, bool OUTPUT>
+constexpr int kStages = OUTPUT && D == 128 ? 3 : 2;
+template <int D, int WAVES, bool OUTPUT>
+constexpr int kWavesOfSimd = D == 256                ? 1
+                             : OUTPUT && D == 128 ? WAVES / 4
+                                                    : WAVES / 2;
+
+template <typename T, int D, int WAVES, bool OUTPUT, bool DIRECT>
+__device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* ring1,
+                                          char* ring2, char* p_tile, float* power,
+                                          int* all_resets_to) {
   constexpr int E = sizeof(T), C = kBlock<T>, BV = 16 * WAVES;
   constexpr int kThreads = 64 * WAVES;
-  constexpr int KB = 64 / E;      // reductions of a fragment
+  constexpr int KB = 64 / E;       // reductions of a fragment
   constexpr int HALVES = KB / 16;  // state tiles of a block of KB keys
   constexpr int BLOCKS = D / KB, TT = C / 16, SB = C / KB;
   constexpr int PT = (TT * TT + WAVES - 1) / WAVES;  // tiles of q k of a wave
+  constexpr int kPer = 16 / E;
+  constexpr int STAGES = DIRECT ? kStages<D, OUTPUT> : 1;
   typedef Tile<T, D> Keys;
   typedef Tile<T, BV> Values;
   typedef Tile<T, C> Weights;
   constexpr int kLoadsK = C * Keys::kPieces / kThreads;
   constexpr int kLoadsV = C * Values::kPieces / kThreads;
-  __shared__ __align__(1024) char q_tile[OUTPUT ? C * Keys::kPitch : 16];
-  __shared__ __align__(1024) char k_tile[C * Keys::kPitch];
-  __shared__ __align__(1024) char v_tile[C * Values::kPitch];
-  __shared__ __align__(1024) char p_tile[OUTPUT ? C * Weights::kPitch : 16];
-  __shared__ float power[C + 1];
-  __shared__ int resets_to[C];  // in front of a row that count against it
+  // a block in LDS: k, v, q
+  constexpr int kVAt = C * Keys::kPitch, kQAt = kVAt + C * Values::kPitch;
+  auto ring = [&](int u) { return u == 0 ? ring0 : u == 1 ? ring1 : ring2; };
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -297,8 +309,13 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
   const float log_a = log_decay(p.decay, part.h);
   if (tid <= C) power[tid] = tid == 0 ? 1.f : expf(tid * log_a);
   __syncthreads();
+  // The weights of v in the state behind the block, for a whole one and behind that for
+  // the one at hand.
+  float* const into = power + C + 4;
+  if (tid < C) into[tid] = w.state_weight * power[C - (from_end ? 0 : 1) - tid];
+  __syncthreads();
 
-  const int col0 = part.slice * BV + wave * 16;  // of the wave's values
+  const int value0 = part.slice * BV, col0 = value0 + wave * 16;
   const long row_base = static_cast<long>(part.b) * p.steps;
   const T* const q = OUTPUT ? static_cast<const T*>(w.q) +
                                   row_base * w.q_row +
@@ -307,14 +324,21 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
   const T* const k = static_cast<const T*>(w.k) + row_base * w.k_row +
                      static_cast<long>(part.h / w.k_share) * w.keys;
   const T* const v = static_cast<const T*>(w.v) + row_base * w.v_row +
-                     static_cast<long>(part.h / w.v_share) * w.values;
-  // the step of a place in the walk's order
+                     static_cast<long>(part.h / w.v_share) * w.values + value0;
+  // The step of a place in the walk's order; a block's lowest step (which may be in
+  // front of the sequence, where the block's rows do not exist) and a row's distance
+  // from it.
   auto step_of = [&](int place) {
     return from_end ? length - 1 - place : place;
   };
+  auto lowest = [&](int place) {
+    return from_end ? static_cast<long>(length) - C - place
+                    : static_cast<long>(place);
+  };
+  auto above = [&](int row) { return from_end ? C - 1 - row : row; };
 
-  // The state: tile i, values 16 j: the lane's column of it is its value lane % 16,
-  // its rows the keys key_of(i) + 0 ... 3.
+  // The state: tile i's column of the lane is its value lane % 16, its rows are the keys
+  // key_of(i) + 0 ... 3.
   float4v state[D / 16];
   auto key_of = [&](int i) {
     return i / HALVES * KB + group * (KB / 4) + i % HALVES * 4;
@@ -322,38 +346,45 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
   const long state_size = static_cast<long>(w.keys) * w.values;
   const long state_at =
       (static_cast<long>(part.bh) * p.pieces + part.piece) * state_size;
-  {
-    const float* from = nullptr;
-    bool transposed = false;
-    if (OUTPUT) {
-      if (p.pieces > 1)
-        from = w.states + state_at;
-      else if (w.initial != nullptr)
-        from = w.initial + part.bh * state_size;
-      transposed = w.transposed != 0;
-    }
-    const int value = col0 + c16;
+  const int my_value = col0 + c16;
+  // (through a buffer of the state's size: keys behind its own are out of range)
+  auto state_buffer = [&](const float* at) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(at), 0,
+                                             static_cast<int>(state_size * 4),
+                                             0x00020000);
+  };
+  auto start = [&] {
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-      state[i] = float4v{0.f, 0.f, 0.f, 0.f};
-      if (from != nullptr && value < w.values) {
+  for (int i = 0; i < D / 16; ++i) state[i] = float4v{0.f, 0.f, 0.f, 0.f};
+  if constexpr (OUTPUT) {
+    const float* const from = p.pieces > 1           ? w.states + state_at
+                              : w.initial != nullptr ? w.initial + part.bh * state_size
+                                                     : nullptr;
+    if (from != nullptr) {
+      const __amdgpu_buffer_rsrc_t rsrc = state_buffer(from);
+      const unsigned of_key = w.transposed ? 4 : 4 * w.values;
+      const unsigned of_value = w.transposed ? 4 * w.keys : 4;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int key = key_of(i) + r;
-          if (key < w.keys)
-            state[i][r] =
-                from[transposed ? static_cast<long>(value) * w.keys + key
-                                : static_cast<long>(key) * w.values + value];
+          const bool in = my_value < w.values && key < w.keys;
+          state[i][r] = __builtin_bit_cast(
+              float, __builtin_amdgcn_raw_buffer_load_b32(
+                         rsrc, in ? key * of_key + my_value * of_value : epi::kOob,
+                         0, 0));
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
+  };
 
-  // A block's rows on their way, in pieces of 16 bytes.  Rows behind the last are that
-  // one again and pieces that would reach behind a head's channels begin before, so
-  // that every load is of values that exist; on their way into LDS the one become
-  // zeros and the others are shifted to where the piece begins.
-  constexpr int kPer = 16 / E;
+  // A block's rows on their way, where they pass through registers.  Rows behind the
+  // last are that one again and pieces that would reach behind a head's channels begin
+  // before, so that every load is of values that exist; on their way into LDS the one
+  // become zeros and the others are shifted to where the piece begins.
   auto load_piece = [&](const T* base, long stride, int row, int place, int col,
                         int cols) {
     const T* const at = base + step_of(min(place + row, last - 1)) * stride;
@@ -369,6 +400,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
     return f;
   };
   auto whole_piece = [&](uint4v f, int row, int n, int col, int cols) {
+    if (n >= C && cols >= col + kPer) return f;
     if (row >= n || col >= cols) return uint4v{0u, 0u, 0u, 0u};
     if (cols >= kPer)
       return epi::shifted_down(f, max(0, col + kPer - cols) * E);
@@ -379,28 +411,112 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
       if (i >= cols) some[i] = T(0);
     return __builtin_bit_cast(uint4v, some);
   };
-  const int value0 = part.slice * BV;
-  const bool whole_keys = w.keys == D, whole_values = w.values - value0 >= BV;
-  uint4v held_q[OUTPUT ? kLoadsK : 1], held_k[kLoadsK], held_v[kLoadsV];
+  const int there = w.values - value0;  // values from the slice's first on
+  uint4v held_q[OUTPUT && !DIRECT ? kLoadsK : 1], held_k[DIRECT ? 1 : kLoadsK],
+      held_v[DIRECT ? 1 : kLoadsV];
   unsigned held_reset = 0;
   auto load = [&](int place) {
+    if constexpr (!DIRECT) {
 #pragma unroll
-    for (int l = 0; l < kLoadsK; ++l) {
-      const int at = tid + kThreads * l, row = at / Keys::kPieces;
-      const int col = at % Keys::kPieces * kPer;
-      held_k[l] = load_piece(k, w.k_row, row, place, col, w.keys);
-      if (OUTPUT) held_q[l] = load_piece(q, w.q_row, row, place, col, w.keys);
-    }
+      for (int l = 0; l < kLoadsK; ++l) {
+        const int at = tid + kThreads * l, row = at / Keys::kPieces;
+        const int col = at % Keys::kPieces * kPer;
+        held_k[l] = load_piece(k, w.k_row, row, place, col, w.keys);
+        if (OUTPUT) held_q[l] = load_piece(q, w.q_row, row, place, col, w.keys);
+      }
 #pragma unroll
-    for (int l = 0; l < kLoadsV; ++l) {
-      const int at = tid + kThreads * l, row = at / Values::kPieces;
-      const int col = at % Values::kPieces * kPer;
-      held_v[l] = load_piece(v, w.v_row, row, place, value0 + col, w.values);
+      for (int l = 0; l < kLoadsV; ++l) {
+        const int at = tid + kThreads * l, row = at / Values::kPieces;
+        const int col = at % Values::kPieces * kPer;
+        held_v[l] = load_piece(v, w.v_row, row, place, col, there);
+      }
     }
+  };
+  auto put = [&](int place, char* to) {
+    if constexpr (!DIRECT) {
+      const int n = min(C, last - place);
+#pragma unroll
+      for (int l = 0; l < kLoadsK; ++l) {
+        const int at = tid + kThreads * l, row = at / Keys::kPieces;
+        const int piece = at % Keys::kPieces;
+        const unsigned where = Keys::at(row, piece);
+        *reinterpret_cast<uint4v*>(to + where) =
+            whole_piece(held_k[l], row, n, piece * kPer, w.keys);
+        if (OUTPUT)
+          *reinterpret_cast<uint4v*>(to + kQAt + where) =
+              whole_piece(held_q[l], row, n, piece * kPer, w.keys);
+      }
+#pragma unroll
+      for (int l = 0; l < kLoadsV; ++l) {
+        const int at = tid + kThreads * l, row = at / Values::kPieces;
+        const int piece = at % Values::kPieces;
+        *reinterpret_cast<uint4v*>(to + kVAt + Values::at(row, piece)) =
+            whole_piece(held_v[l], row, n, piece * kPer, there);
+      }
+    }
+  };
+  // (every lane loads a byte that exists)
+  auto load_reset = [&](int place) {
     if (p.resets != nullptr)
-      held_reset = lane < C && place + lane < last
-                       ? p.resets[row_base + step_of(place + lane)]
-                       : 0u;
+      held_reset = p.resets[row_base + step_of(min(place + lane % C, last - 1))];
+  };
+
+  // ... and straight to LDS, a KiB of neighbouring places for each load: the row and
+  // the piece that belong there.
+  // (a load of all threads is a number of rows; every sixteen rows, where the swizzle
+  // comes again, the base moves)
+  constexpr int kTurnsK =
+      16 * Keys::kPieces > kThreads ? 16 * Keys::kPieces / kThreads : 1;
+  constexpr int kTurnsV =
+      16 * Values::kPieces > kThreads ? 16 * Values::kPieces / kThreads : 1;
+  unsigned from_k[kTurnsK], from_q[kTurnsK], from_v[kTurnsV];
+  if constexpr (DIRECT) {
+    auto places_of = [&](auto tile, long stride, int cols, auto& from) {
+      typedef decltype(tile) Of;
+      constexpr int kTurns = sizeof(from) / sizeof(unsigned);
+#pragma unroll
+      for (int u = 0; u < kTurns; ++u) {
+        const int row = (tid + kThreads * u) / Of::kPieces;
+        const int col = static_cast<int>(
+            (tid % Of::kPieces ^ swizzle<E, Of::kPitch>(row)) * kPer);
+        from[u] = col < cols
+                      ? static_cast<unsigned>((above(row) * stride + col) * E)
+                      : epi::kOob;
+      }
+    };
+    places_of(Keys(), w.k_row, w.keys, from_k);
+    if (OUTPUT) places_of(Keys(), w.q_row, w.keys, from_q);
+    places_of(Values(), w.v_row, there, from_v);
+  }
+  auto issue = [&](int place, char* to) {
+    if constexpr (DIRECT) {
+      if (place >= last) return;
+      const long low = lowest(place);
+      const int n = last - place;
+      auto some = [&](const T* base, long stride, const auto& from, auto tile,
+                      char* at) {
+        typedef decltype(tile) Of;
+        constexpr int kLoads = C * Of::kPieces / kThreads;
+        constexpr int kRows = kThreads / Of::kPieces;
+        constexpr int kTurns = sizeof(from) / sizeof(unsigned);
+        base += low * stride;
+#pragma unroll
+        for (int l = 0; l < kLoads; ++l) {
+          const int up = kRows * (l / kTurns * kTurns);
+          const __amdgpu_buffer_rsrc_t rsrc =
+              epi::make_rsrc(base + (from_end ? -up : up) * stride);
+          const unsigned offset = n < C && tid / Of::kPieces + kRows * l >= n
+                                      ? epi::kOob
+                                      : from[l % kTurns];
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(
+              rsrc, (lds_ptr)(at + (kThreads * l + 64 * wave) * 16), 16, offset, 0,
+              0, 0);
+        }
+      };
+      some(k, w.k_row, from_k, Keys(), to);
+      some(v, w.v_row, from_v, Values(), to + kVAt);
+      if (OUTPUT) some(q, w.q_row, from_q, Keys(), to + kQAt);
+    }
   };
 
   // The weights of the wave's tiles of q k: of row (column of the tile) 16 t + c16
@@ -426,95 +542,96 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
   Weights::start_rows(along_p, lane);
   Keys::start_columns(down_k, lane);
   Values::start_columns(down_v, wave * 16, lane);
+  // Where the lane's row c16 of the result goes, from the block's lowest step on.
+  const int out_size = w.out_float ? 4 : E;
+  const unsigned out_at =
+      my_value - c16 + 4 * group < w.values
+          ? static_cast<unsigned>((above(c16) * w.out_row + col0 + 4 * group) *
+                                  out_size)
+          : epi::kOob;
+  const int out_turn = static_cast<int>((from_end ? -16 : 16) * w.out_row * out_size);
 
-  if (first < last) load(first);
-  for (int place = first; place < last; place += C) {
+  // One block, whose rows are in `tile`.
+  // CAREFUL: rows that do not count are left out one by one; otherwise by weights of
+  // zero, after which `clean` tells whether that was enough.
+  float4v clean = {0.f, 0.f, 0.f, 0.f};  // stays zero while every v is finite
+  bool clean_k = true;
+  auto walk = [&](const char* tile, int place, auto careful, auto next) {
+    constexpr bool CAREFUL = decltype(careful)::value;
+    // (two tables in turn: waves may still read the ones of the block before)
+    const int turn = (place - first) / C % 2 * C;
+    int* const resets_to = all_resets_to + turn;
+    float* const into_part = into + C + turn;
     const int n = min(C, last - place);
-    if (n < C || !whole_keys) {
-#pragma unroll
-      for (int l = 0; l < kLoadsK; ++l) {
-        const int at = tid + kThreads * l, row = at / Keys::kPieces;
-        const int col = at % Keys::kPieces * kPer;
-        held_k[l] = whole_piece(held_k[l], row, n, col, w.keys);
-        if (OUTPUT) held_q[l] = whole_piece(held_q[l], row, n, col, w.keys);
-      }
-    }
-    if (n < C || !whole_values) {
-#pragma unroll
-      for (int l = 0; l < kLoadsV; ++l) {
-        const int at = tid + kThreads * l, row = at / Values::kPieces;
-        const int col = value0 + at % Values::kPieces * kPer;
-        held_v[l] = whole_piece(held_v[l], row, n, col, w.values);
-      }
-    }
-#pragma unroll
-    for (int l = 0; l < kLoadsK; ++l) {
-      const int at = tid + kThreads * l;
-      const unsigned to = Keys::at(at / Keys::kPieces, at % Keys::kPieces);
-      *reinterpret_cast<uint4v*>(k_tile + to) = held_k[l];
-      if (OUTPUT) *reinterpret_cast<uint4v*>(q_tile + to) = held_q[l];
-    }
-#pragma unroll
-    for (int l = 0; l < kLoadsV; ++l) {
-      const int at = tid + kThreads * l;
-      *reinterpret_cast<uint4v*>(
-          v_tile + Values::at(at / Values::kPieces, at % Values::kPieces)) =
-          held_v[l];
-    }
+    const char *const k_tile = tile, *const v_tile = tile + kVAt,
+                      *const q_tile = tile + kQAt;
     // Which of the block's rows are resets.  Rows s < r (in the walk's order) count
     // for one another where none is among s + 1 ... r, or s ... r - 1 from the end:
     // where as many are in front of both.
-    const unsigned long long resets = __ballot(held_reset != 0);
-    if (p.resets != nullptr && wave == 0 && lane < C) {
-      const unsigned long long before = (1ull << lane) - 1;
-      resets_to[lane] = static_cast<int>(__popcll(
-          resets & (from_end ? before : before | 1ull << lane)));
-    }
+    unsigned long long resets = 0;
+    if (p.resets != nullptr)
+      resets = __ballot(held_reset != 0 && lane < C && place + lane < last);
     const int all_resets = static_cast<int>(__popcll(resets));
-    __syncthreads();
-    if (place + C < last) load(place + C);
+    const int to_end = from_end ? n : n - 1;
+    const bool whole = n == C && resets == 0;
+    if (!whole && wave == 0 && lane < C) {
+      const unsigned long long before = (1ull << lane) - 1;
+      const int mine = static_cast<int>(
+          __popcll(resets & (from_end ? before : before | 1ull << lane)));
+      resets_to[lane] = mine;
+      into_part[lane] = lane < n && mine == all_resets
+                           ? w.state_weight * power[to_end - lane]
+                           : 0.f;
+    }
+    const float* const into_state = whole ? into : into_part;
+    __builtin_amdgcn_s_waitcnt(epi::kLgkm0 & epi::vmcnt_imm(63));
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    next();
 
     if constexpr (OUTPUT) {
+      // (tiles of later s are worked out as well and left out: no branches)
+      float4v acc[PT];
+#pragma unroll
+      for (int x = 0; x < PT; ++x) acc[x] = float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+        for (int x = 0; x < PT; ++x) {
+          const int t = (wave * PT + x) / TT % TT, s = (wave * PT + x) % TT;
+          acc[x] = epi::multiply<T>(Keys::rows(k_tile, along, s, b),
+                                    Keys::rows(q_tile, along, t, b), acc[x]);
+        }
 #pragma unroll
       for (int x = 0; x < PT; ++x) {
         const int t = (wave * PT + x) / TT, s = (wave * PT + x) % TT;
         if (t >= TT) continue;  // (blocks of fewer tiles than waves)
-        float4v acc = {0.f, 0.f, 0.f, 0.f};
-        if (s <= t) {
-#pragma unroll
-          for (int b = 0; b < BLOCKS; ++b)
-            acc = epi::multiply<T>(Keys::rows(k_tile, along, s, b),
-                                   Keys::rows(q_tile, along, t, b), acc);
-        }
+        const int row = 16 * t + c16, col = 16 * s + 4 * group;
         typedef T Four __attribute__((ext_vector_type(4)));
         Four to;
-        const int row = 16 * t + c16, col = 16 * s + 4 * group;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           bool on = col + r <= row;
           if (resets != 0) on = on && resets_to[col + r] == resets_to[row];
-          to[r] = static_cast<T>(on ? acc[r] * weight[x][r] : 0.f);
+          to[r] = static_cast<T>(on ? acc[x][r] * weight[x][r] : 0.f);
         }
-        *reinterpret_cast<Four*>(p_tile +
-                                 Weights::at(row, col / Weights::kPer) +
-                                 col % Weights::kPer * E) = to;
+        *reinterpret_cast<Four*>(p_tile + Weights::at(row, col / kPer) +
+                                 col % kPer * E) = to;
       }
-      __syncthreads();
+      __builtin_amdgcn_s_waitcnt(epi::kLgkm0 & epi::vmcnt_imm(63));
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
     }
 
     uint4v v_part[SB];
-    bool finite = true;
-    {
-      float4v zero = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int b = 0; b < SB; ++b) {
-        v_part[b] = Values::fragment(v_tile, down_v, b);
-        zero = epi::multiply<T>(v_part[b], uint4v{0u, 0u, 0u, 0u}, zero);
-      }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) finite = finite && zero[r] == 0.f;
+    for (int b = 0; b < SB; ++b) {
+      v_part[b] = Values::fragment(v_tile, down_v, b);
+      if (!CAREFUL)
+        clean = epi::multiply<T>(v_part[b], uint4v{0u, 0u, 0u, 0u}, clean);
     }
-    finite = __all(finite);
 
     if constexpr (OUTPUT) {
       // q X of all rows, and the sums over the block's v
@@ -552,141 +669,264 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
           x[i] = state[b * HALVES + i / 4][i % 4] * scale;
         uint4v high, low;
         Split<T>::split(x, &high, &low);
+        uint4v of_q[TT];
 #pragma unroll
-        for (int t = 0; t < TT; ++t) {
-          const uint4v of_q = Keys::rows(q_tile, along, t, b);
-          acc[t] = epi::multiply<T>(high, of_q, acc[t]);
-          if constexpr (E == 2) acc[t] = epi::multiply<T>(low, of_q, acc[t]);
+        for (int t = 0; t < TT; ++t) of_q[t] = Keys::rows(q_tile, along, t, b);
+#pragma unroll
+        for (int t = 0; t < TT; ++t)
+          acc[t] = epi::multiply<T>(high, of_q[t], acc[t]);
+        if constexpr (E == 2) {
+#pragma unroll
+          for (int t = 0; t < TT; ++t)
+            acc[t] = epi::multiply<T>(low, of_q[t], acc[t]);
         }
       }
 #pragma unroll
       for (int t = 0; t < TT; ++t) {
-        const int row = 16 * t + c16;
-        const bool reached = resets == 0 || resets_to[row] == 0;
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          acc[t][r] = reached ? acc[t][r] * reach[t] * unscale[r] : 0.f;
-        if (finite) {
+        for (int r = 0; r < 4; ++r) acc[t][r] *= reach[t] * unscale[r];
+        if (resets != 0) {
+          const bool reached = resets_to[16 * t + c16] == 0;
 #pragma unroll
-          for (int b = 0; b < SB; ++b) {
+          for (int r = 0; r < 4; ++r) acc[t][r] = reached ? acc[t][r] : 0.f;
+        }
+      }
+      if constexpr (!CAREFUL) {
+#pragma unroll
+        for (int b = 0; b < SB; ++b)
+#pragma unroll
+          for (int t = 0; t < TT; ++t) {
             if (b * KB > 16 * t + 15) continue;
             acc[t] = epi::multiply<T>(
                 v_part[b], Weights::rows(p_tile, along_p, t, b), acc[t]);
           }
-        } else {
-          int to = row, first_value = wave * 16 + 4 * group;
-          // (not worked out in front of the blocks, where it would take registers)
-          asm volatile("" : "+v"(to), "+v"(first_value));
-          for (int s = 0; s <= to; ++s) {
-            if (resets != 0 && resets_to[s] != resets_to[to]) continue;
-            const float x = Weights::value(p_tile, to, s);
+      } else {
+        const int first_value = wave * 16 + 4 * group;
+        for (int r = 0; r < n; ++r) {
+          typedef T Four __attribute__((ext_vector_type(4)));
+          const Four x = *reinterpret_cast<const Four*>(
+              v_tile + Values::at(r, first_value / kPer) + first_value % kPer * E);
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              acc[t][r] += x * Values::value(v_tile, s, first_value + r);
+          for (int t = 0; t < TT; ++t) {
+            const int to = 16 * t + c16;
+            if (r > to || (resets != 0 && resets_to[r] != resets_to[to])) continue;
+            const float by = Weights::value(p_tile, to, r);
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              acc[t][c] += by * static_cast<float>(x[c]);
           }
         }
-        if (w.out != nullptr && row < n) {
-          const long at =
-              (row_base + step_of(place + row)) * w.out_row +
-              static_cast<long>(part.h) * w.values;
-          const int col = col0 + 4 * group;
-          auto store = [&](auto* out) {
-            typedef std::remove_pointer_t<decltype(out)> O;
-            out += at + col;
-            if (col + 4 <= w.values) {
-              float x[4] = {acc[t][0], acc[t][1], acc[t][2], acc[t][3]};
-              *reinterpret_cast<typename seq::Pack<O, 4>::type*>(out) =
-                  seq::pack<O, 4>(x);
-            } else {
+      }
+      if (w.out != nullptr) {
+        char* const base =
+            static_cast<char*>(w.out) +
+            ((row_base + lowest(place)) * w.out_row +
+             static_cast<long>(part.h) * w.values) * out_size;
+        if constexpr (DIRECT) {
+          // (as many stores of every wave in every block, whether its rows and values
+          // exist or not: the waits for loads count them)
+          const __amdgpu_buffer_rsrc_t rsrc = epi::make_rsrc(base);
 #pragma unroll
-              for (int r = 0; r < 4; ++r)
-                if (col + r < w.values) out[r] = static_cast<O>(acc[t][r]);
+          for (int t = 0; t < TT; ++t) {
+            const unsigned at =
+                16 * t + c16 < n && out_at != epi::kOob
+                    ? out_at + static_cast<unsigned>(t * out_turn)
+                    : epi::kOob;
+            if (w.out_float) {
+              __builtin_amdgcn_raw_buffer_store_b128(
+                  __builtin_bit_cast(uint4v, acc[t]), rsrc, at, 0, 0);
+            } else if constexpr (E == 4) {
+              __builtin_amdgcn_raw_buffer_store_b128(
+                  __builtin_bit_cast(uint4v, acc[t]), rsrc, at, 0, 0);
+            } else {
+              float x[4] = {acc[t][0], acc[t][1], acc[t][2], acc[t][3]};
+              typedef unsigned int uint2v __attribute__((ext_vector_type(2)));
+              __builtin_amdgcn_raw_buffer_store_b64(
+                  __builtin_bit_cast(uint2v, seq::pack<T, 4>(x)), rsrc, at, 0, 0);
             }
-          };
-          if (w.out_float)
-            store(static_cast<float*>(w.out));
-          else
-            store(static_cast<T*>(w.out));
+          }
+        } else {
+#pragma unroll
+          for (int t = 0; t < TT; ++t) {
+            if (16 * t + c16 >= n) continue;
+            const int col = col0 + 4 * group;
+            auto store = [&](auto* out) {
+              typedef std::remove_pointer_t<decltype(out)> O;
+              if (col + 4 <= w.values) {
+                float x[4] = {acc[t][0], acc[t][1], acc[t][2], acc[t][3]};
+                *reinterpret_cast<typename seq::Pack<O, 4>::type*>(out) =
+                    seq::pack<O, 4>(x);
+              } else {
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                  if (col + r < w.values) out[r] = static_cast<O>(acc[t][r]);
+              }
+            };
+            char* const at =
+                base + (static_cast<long>(above(16 * t + c16)) * w.out_row + col) *
+                           out_size;
+            if (w.out_float)
+              store(reinterpret_cast<float*>(at));
+            else
+              store(reinterpret_cast<T*>(at));
+          }
         }
       }
     }
 
     // The state behind the block.
-    const float carry = power[n];
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        state[i][r] = all_resets == 0 ? state[i][r] * carry : 0.f;
     carried = carried && all_resets == 0;
-    const int to_end = from_end ? n : n - 1;
-    // (rows in front of a reset may hold a k that a weight of zero leaves infinite)
-    bool by_products = finite;
-    if (finite && resets != 0) {
+    if (all_resets == 0) {
+      const float carry = power[n];
 #pragma unroll
-      for (int b = 0; b < SB; ++b)
+      for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          const float4v zero = epi::multiply<T>(
-              Keys::columns(k_tile, down_k, i / HALVES, i % HALVES, b),
-              uint4v{0u, 0u, 0u, 0u}, float4v{0.f, 0.f, 0.f, 0.f});
+        for (int r = 0; r < 4; ++r) state[i][r] *= carry;
+    } else {
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            by_products = by_products && zero[r] == 0.f;
-        }
-      by_products = __all(by_products);
+      for (int i = 0; i < D / 16; ++i) state[i] = float4v{0.f, 0.f, 0.f, 0.f};
     }
-    if (by_products) {
+    if constexpr (!CAREFUL) {
+      // (rows in front of a reset may hold a k that a weight of zero leaves infinite)
+      if (resets != 0) {
+#pragma unroll 1
+        for (int piece = 0; piece < Keys::kPieces; ++piece) {
+          float x[kPer];
+          Split<T>::floats(*reinterpret_cast<const uint4v*>(
+                               k_tile + Keys::at(lane % C, piece)),
+                           x);
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) clean_k = clean_k && x[i] * 0.f == 0.f;
+        }
+      }
+      uint4v high[SB], low[SB];
 #pragma unroll
       for (int b = 0; b < SB; ++b) {
-        float by[16 / E];
-#pragma unroll
-        for (int i = 0; i < 16 / E; ++i)
-        {
-          const int row = b * KB + group * (KB / 4) + i;
-          by[i] = w.state_weight * power[max(0, to_end - row)];
-          if (resets != 0 && resets_to[row] != all_resets) by[i] = 0.f;
-        }
-        float x[16 / E];
+        float x[kPer];
         Split<T>::floats(v_part[b], x);
 #pragma unroll
-        for (int i = 0; i < 16 / E; ++i) x[i] *= by[i];
-        uint4v high, low;
-        Split<T>::split(x, &high, &low);
+        for (int i = 0; i < kPer; ++i)
+          x[i] *= into_state[b * KB + group * (KB / 4) + i];
+        Split<T>::split(x, &high[b], &low[b]);
+      }
+      // (two tiles' fragments are read while those before are multiplied, and no more of
+      // them: they would take the registers that the loads' and sums' need)
+      uint4v of_k[2][2][SB];
+      auto fetch = [&](int i) {
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          const uint4v of_k =
-              Keys::columns(k_tile, down_k, i / HALVES, i % HALVES, b);
-          state[i] = epi::multiply<T>(of_k, high, state[i]);
-          if constexpr (E == 2) state[i] = epi::multiply<T>(of_k, low, state[i]);
-        }
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int b = 0; b < SB; ++b)
+            of_k[i / 2 % 2][u][b] = Keys::columns(k_tile, down_k, (i + u) / HALVES,
+                                                  (i + u) % HALVES, b);
+      };
+      fetch(0);
+#pragma unroll
+      for (int i = 0; i < D / 16; i += 2) {
+        if (i + 2 < D / 16) fetch(i + 2);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int b = 0; b < SB; ++b)
+#pragma unroll
+          for (int part = 0; part < (E == 2 ? 2 : 1); ++part)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+              state[i + u] =
+                  epi::multiply<T>(of_k[i / 2 % 2][u][b],
+                                   part == 0 ? high[b] : low[b], state[i + u]);
+        __builtin_amdgcn_sched_barrier(0);
       }
     } else {
-      int value = wave * 16 + c16, key = group * (KB / 4);
-      asm volatile("" : "+v"(value), "+v"(key));
-      for (int s = 0; s < n; ++s) {
-        if (resets != 0 && resets_to[s] != all_resets) continue;
-        const float x =
-            w.state_weight * power[to_end - s] * Values::value(v_tile, s, value);
+      const int value = wave * 16 + c16;
+      for (int r = 0; r < n; ++r) {
+        if (resets != 0 && resets_to[r] != all_resets) continue;
+        const float x = into_state[r] * Values::value(v_tile, r, value);
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i)
+        for (int b = 0; b < BLOCKS; ++b) {
+          float of_k[kPer];  // the lane's keys of the block: a piece
+          Split<T>::floats(*reinterpret_cast<const uint4v*>(
+                               k_tile + Keys::at(r, 4 * b + group)),
+                           of_k);
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            state[i][r] += x * Keys::value(k_tile, s, key + i / HALVES * KB +
-                                                          i % HALVES * 4 + r);
+          for (int i = 0; i < kPer; ++i)
+            state[b * HALVES + i / 4][i % 4] += x * of_k[i];
+        }
       }
     }
-    __syncthreads();  // the tiles have been read
+  };
+
+  constexpr auto kFast = std::false_type();
+  constexpr auto kCareful = std::true_type();
+  start();
+  if constexpr (DIRECT) {
+    constexpr int kLoads = kLoadsV + kLoadsK * (OUTPUT ? 2 : 1);
+    if (first < last) load_reset(first);
+#pragma unroll
+    for (int u = 0; u < STAGES - 1; ++u) issue(first + u * C, ring(u));
+    auto step = [&](int place, int u) {
+      // (loads come in order: where no more accesses are under way than the loads of the
+      // blocks behind, the block's own have come, whatever has become of stores)
+      if (last - place <= (STAGES - 2) * C)
+        __builtin_amdgcn_s_waitcnt(epi::vmcnt_imm(0));
+      else
+        __builtin_amdgcn_s_waitcnt(epi::vmcnt_imm((STAGES - 2) * kLoads));
+      asm volatile("" ::: "memory");
+      walk(ring(u), place, kFast, [&] {
+        if (place + C < last) load_reset(place + C);
+        issue(place + (STAGES - 1) * C, ring((u + STAGES - 1) % STAGES));
+      });
+    };
+    for (int place = first; place < last; place += STAGES * C) {
+#pragma unroll
+      for (int u = 0; u < STAGES; ++u)
+        if (place + u * C < last) step(place + u * C, u);
+    }
+  } else {
+    if (first < last) {
+      load_reset(first);
+      load(first);
+    }
+    for (int place = first; place < last; place += C) {
+      put(place, ring0);
+      walk(ring0, place, kFast, [&] {
+        if (place + C < last) {
+          load_reset(place + C);
+          load(place + C);
+        }
+      });
+      __syncthreads();  // the tiles have been read
+    }
+  }
+  // Values that are not finite: once more, and with care.
+  const bool all_clean = clean_k && clean[0] == 0.f && clean[1] == 0.f &&
+                         clean[2] == 0.f && clean[3] == 0.f;
+  if (!__syncthreads_and(all_clean)) {
+    start();
+    carried = true;
+#pragma unroll 1
+    for (int place = first; place < last; place += C) {
+      load_reset(place);
+      if constexpr (DIRECT) {
+        issue(place, ring0);
+        __builtin_amdgcn_s_waitcnt(epi::vmcnt_imm(0));
+        asm volatile("" ::: "memory");
+      } else {
+        load(place);
+        put(place, ring0);
+      }
+      walk(ring0, place, kCareful, [] {});
+      __syncthreads();  // the tiles have been read
+    }
   }
 
   if (OUTPUT && w.out != nullptr) {  // rows behind the sequence's length
     const int end = min(first + p.piece_steps, p.steps);
-    const int columns = min(BV, w.values - part.slice * BV);
+    const int columns = min(BV, there);
     const long rows = end - max(first, length);
     for (long at = tid; at < rows * columns; at += kThreads) {
       const long to =
           (row_base + max(first, length) + at / columns) * w.out_row +
-          static_cast<long>(part.h) * w.values + part.slice * BV + at % columns;
+          static_cast<long>(part.h) * w.values + value0 + at % columns;
       if (w.out_float)
         static_cast<float*>(w.out)[to] = 0.f;
       else
@@ -704,46 +944,97 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
     to = w.final + part.bh * state_size;
   }
   if (to == nullptr) return;
-  const int value = col0 + c16;
-  if (value >= w.values) return;
+  const __amdgpu_buffer_rsrc_t rsrc = state_buffer(to);
 #pragma unroll
-  for (int i = 0; i < D / 16; ++i)
+  for (int i = 0; i < D / 16; ++i) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int key = key_of(i) + r;
-      if (key < w.keys)
-        to[static_cast<long>(key) * w.values + value] = state[i][r];
+      const bool in = my_value < w.values && key < w.keys;
+      __builtin_amdgcn_raw_buffer_store_b32(
+          __float_as_uint(state[i][r]), rsrc,
+          in ? static_cast<unsigned>((key * w.values + my_value) * 4) : epi::kOob, 0,
+          0);
     }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+template <typename T, int D, int WAVES, bool OUTPUT, bool DIRECT>
+__global__ void __launch_bounds__(64 * WAVES, (kWavesOfSimd<D, WAVES, OUTPUT>))
+    walk_kernel(Problem p) {
+#ifdef __HIP_DEVICE_COMPILE__
+  constexpr int E = sizeof(T), C = kBlock<T>;
+  constexpr int kStage = C * E * ((OUTPUT ? 2 : 1) * D + 16 * WAVES);
+  // (an array of its own for each block)
+  __shared__ __align__(1024) char ring0[kStage];
+  char *r1 = nullptr, *r2 = nullptr;
+  if constexpr (DIRECT) {
+    __shared__ __align__(1024) char ring1[kStage];
+    r1 = ring1;
+  }
+  if constexpr (DIRECT && kStages<D, OUTPUT> > 2) {
+    __shared__ __align__(1024) char ring2[kStage];
+    r2 = ring2;
+  }
+  __shared__ __align__(1024) char p_tile[OUTPUT ? C * C * E : 16];
+  __shared__ __align__(16) float power[4 * C + 4];
+  __shared__ int resets_to[2 * C];  // in front of a row that count against it
+  walk_body<T, D, WAVES, OUTPUT, DIRECT>(p, ring0, r1, r2, p_tile, power,
+                                         resets_to);
 #endif
 }
 
-template <typename T, int D, int WAVES>
+template <typename T, int D, int WAVES, bool DIRECT>
 int launch_walk(const Problem& p, bool outputs, hipStream_t stream) {
   const dim3 grid(static_cast<unsigned>(p.units) * p.batch * p.heads * p.pieces);
   if (outputs)
-    hipLaunchKernelGGL((walk_kernel<T, D, WAVES, true>), grid,
+    hipLaunchKernelGGL((walk_kernel<T, D, WAVES, true, DIRECT>), grid,
                        dim3(64 * WAVES), 0, stream, p);
   else
-    hipLaunchKernelGGL((walk_kernel<T, D, WAVES, false>), grid,
+    hipLaunchKernelGGL((walk_kernel<T, D, WAVES, false, DIRECT>), grid,
                        dim3(64 * WAVES), 0, stream, p);
   SNN_HIP_CHECK_LAUNCH();
   return SNN_HIP_OK;
 }
 
+// Whether all walks' rows go straight to LDS and from registers in whole pieces.
 template <typename T>
-int run_walks(const Problem& p, int keys_class, int waves, bool outputs,
+bool is_direct(const Problem& p, bool outputs) {
+  constexpr int kPer = 16 / sizeof(T);
+  auto ok = [](const void* at, long stride) {
+    return seq::aligned(static_cast<const char*>(at), 16) && stride % kPer == 0;
+  };
+  for (int i = 0; i < p.walks; ++i) {
+    const Walk& w = p.walk[i];
+    if (w.keys % kPer != 0 || w.values % kPer != 0 || !ok(w.k, w.k_row) ||
+        !ok(w.v, w.v_row))
+      return false;
+    if (outputs && (!ok(w.q, w.q_row) || !ok(w.out, w.out_row))) return false;
+  }
+  return true;
+}
+
+template <typename T, bool DIRECT>
+int run_class(const Problem& p, int keys_class, int waves, bool outputs,
               hipStream_t stream) {
   switch (keys_class) {
     case 64:
-      return waves == 8 ? launch_walk<T, 64, 8>(p, outputs, stream)
-                        : launch_walk<T, 64, 4>(p, outputs, stream);
+      return waves == 8 ? launch_walk<T, 64, 8, DIRECT>(p, outputs, stream)
+                        : launch_walk<T, 64, 4, DIRECT>(p, outputs, stream);
     case 128:
-      return waves == 8 ? launch_walk<T, 128, 8>(p, outputs, stream)
-                        : launch_walk<T, 128, 4>(p, outputs, stream);
+      return waves == 8 ? launch_walk<T, 128, 8, DIRECT>(p, outputs, stream)
+                        : launch_walk<T, 128, 4, DIRECT>(p, outputs, stream);
     default:
-      return waves == 8 ? launch_walk<T, 256, 8>(p, outputs, stream)
-                        : launch_walk<T, 256, 4>(p, outputs, stream);
+      return launch_walk<T, 256, 4, DIRECT>(p, outputs, stream);
   }
+}
+template <typename T>
+int run_walks(const Problem& p, int keys_class, int waves, bool outputs,
+              hipStream_t stream) {
+  return is_direct<T>(p, outputs)
+             ? run_class<T, true>(p, keys_class, waves, outputs, stream)
+             : run_class<T, false>(p, keys_class, waves, outputs, stream);
 }
 
 }  // namespace att

@@ -242,9 +242,15 @@ int check(const snn_hip_linear_attention_params* p, const void* workspace) {
               stride_ok(p->grad_k_stride, of_keys) &&
               stride_ok(p->grad_v_stride, of_values));
   SNN_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15u) == 0);
-  // (steps and places of pieces are counted in 31 bits, heads in a grid's y)
+  // (steps and places of pieces are counted in 31 bits, a block's rows in 31 bits of
+  // bytes)
   const size_t heads = static_cast<size_t>(p->batch) * p->heads;
-  if (p->steps > (1 << 30) || heads > (1u << 20)) return SNN_HIP_INDEX_EXCEEDED;
+  constexpr int kStride = 1 << 22;
+  if (p->steps > (1 << 30) || heads > (1u << 20) || of_keys > kStride ||
+      of_values > kStride || p->q_stride > kStride || p->k_stride > kStride ||
+      p->v_stride > kStride || p->grad_q_stride > kStride ||
+      p->grad_k_stride > kStride || p->grad_v_stride > kStride)
+    return SNN_HIP_INDEX_EXCEEDED;
   return SNN_HIP_OK;
 }
 
@@ -253,8 +259,12 @@ size_t round16(size_t bytes) { return (bytes + 15) / 16 * 16; }
 int class_of(int keys) { return keys <= 64 ? 64 : keys <= 128 ? 128 : 256; }
 
 // Waves of a work-group, and the work-groups that share the values.
-int waves_of(int values) { return values > 64 ? 8 : 4; }
-int slices_of(int values) { return ceil_div(values, 16 * waves_of(values)); }
+int waves_of(int keys, int values) {
+  return values > 64 && class_of(keys) <= 128 ? 8 : 4;
+}
+int slices_of(int keys, int values) {
+  return ceil_div(values, 16 * waves_of(keys, values));
+}
 
 // How a sequence is divided: enough work-groups for the GPU, pieces that are long
 // beside their states.
@@ -290,10 +300,10 @@ size_t division_bytes(const snn_hip_linear_attention_params& p,
 }
 
 int forward_units(const snn_hip_linear_attention_params& p) {
-  return slices_of(p.values);
+  return slices_of(p.keys, p.values);
 }
 int grad_units(const snn_hip_linear_attention_params& p) {
-  return 2 * slices_of(p.keys) + slices_of(p.values);
+  return 2 * slices_of(p.values, p.keys) + slices_of(p.keys, p.values);
 }
 int block_of(int elem_size) { return elem_size == 2 ? 64 : 32; }
 
@@ -334,7 +344,7 @@ Problem problem_of(const snn_hip_linear_attention_params& p, const Division& d,
 }
 void add(Problem* g, const Walk& w) {
   g->walk[g->walks] = w;
-  g->walk[g->walks].slices = slices_of(w.values);
+  g->walk[g->walks].slices = slices_of(w.keys, w.values);
   g->units += g->walk[g->walks].slices;
   ++g->walks;
 }
@@ -346,11 +356,11 @@ int run_all(const Problem& base, const Walk* walks, int n, bool outputs,
   for (int i = 0; i < n; ++i) {
     if (done[i]) continue;
     const int keys = class_of(walks[i].keys);
-    const int waves = waves_of(walks[i].values);
+    const int waves = waves_of(walks[i].keys, walks[i].values);
     Problem g = base;
     for (int j = i; j < n; ++j) {
       if (done[j] || class_of(walks[j].keys) != keys ||
-          waves_of(walks[j].values) != waves)
+          waves_of(walks[j].keys, walks[j].values) != waves)
         continue;
       add(&g, walks[j]);
       done[j] = true;
