@@ -246,11 +246,15 @@ __device__ __forceinline__ Part part_of(const Problem& p) {
   // read the same rows)
   const unsigned at = gemm::xcd_remap(blockIdx.x, gridDim.x);
   Part r;
-  unsigned unit = at % p.units;
-  const unsigned rest = at / p.units, heads = p.batch * p.heads;
-  r.bh = static_cast<int>(rest % heads);
-  r.piece = static_cast<int>(rest / heads);
-  r.b = r.bh / p.heads;
+  // (divisions are the vector unit's, their results the same for all lanes)
+  auto same = [](unsigned x) {
+    return static_cast<int>(__builtin_amdgcn_readfirstlane(static_cast<int>(x)));
+  };
+  unsigned unit = same(at % p.units);
+  const unsigned rest = same(at / p.units), heads = p.batch * p.heads;
+  r.bh = same(rest % heads);
+  r.piece = same(rest / heads);
+  r.b = same(r.bh / p.heads);
   r.h = r.bh - r.b * p.heads;
   r.walk = 0;
   while (unit >= static_cast<unsigned>(p.walk[r.walk].slices)) {
@@ -268,11 +272,9 @@ __device__ __forceinline__ Part part_of(const Problem& p) {
 // LDS holds three blocks of 128 keys, q and 128 values, or two work-groups of a CU
 // with two blocks each.
 template <int D, bool OUTPUT>
-constexpr int kStages = OUTPUT && D == 128 ? 3 : 2;
+constexpr int kStages = 1;
 template <int D, int WAVES, bool OUTPUT>
-constexpr int kWavesOfSimd = D == 256                ? 1
-                             : OUTPUT && D == 128 ? WAVES / 4
-                                                    : WAVES / 2;
+constexpr int kWavesOfSimd = D == 256 ? 1 : OUTPUT ? 3 : 4;
 
 template <typename T, int D, int WAVES, bool OUTPUT, bool DIRECT>
 __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* ring1,
@@ -283,7 +285,7 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
   constexpr int KB = 64 / E;       // reductions of a fragment
   constexpr int HALVES = KB / 16;  // state tiles of a block of KB keys
   constexpr int BLOCKS = D / KB, TT = C / 16, SB = C / KB;
-  constexpr int PT = (TT * TT + WAVES - 1) / WAVES;  // tiles of q k of a wave
+  constexpr int PT = TT * TT / WAVES;  // tiles of q k of a wave
   constexpr int kPer = 16 / E;
   constexpr int STAGES = DIRECT ? kStages<D, OUTPUT> : 1;
   typedef Tile<T, D> Keys;
@@ -300,34 +302,53 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
   const int c16 = lane & 15, group = lane >> 4;
   const Part part = part_of(p);
   const Walk& w = p.walk[part.walk];
-  const int length = length_of(p, part.b);
+  const int length = __builtin_amdgcn_readfirstlane(length_of(p, part.b));
   const int first = part.piece * p.piece_steps;  // in the walk's order
   const int last = min(first + p.piece_steps, length);
   const bool from_end = w.from_end != 0;
   // (the last piece's state is the second pass's to find)
   if (!OUTPUT && first + p.piece_steps >= length) return;
+  // (what the blocks need stays in scalar registers: read anew from the arguments it
+  // would hold up every block)
+  auto pin = [](auto x) {
+    asm volatile("" : "+s"(x));
+    return x;
+  };
+  auto same = [](unsigned x) {
+    return static_cast<unsigned>(
+        __builtin_amdgcn_readfirstlane(static_cast<int>(x)));
+  };
   const float log_a = log_decay(p.decay, part.h);
-  if (tid <= C) power[tid] = tid == 0 ? 1.f : expf(tid * log_a);
+  // (above zero: an infinite state stays infinite behind decays that fp32 has no value
+  // for)
+  if (tid <= C) power[tid] = tid == 0 ? 1.f : expf(tid * log_a) + 0x1p-126f;
   __syncthreads();
-  // The weights of v in the state behind the block, for a whole one and behind that for
-  // the one at hand.
-  float* const into = power + C + 4;
-  if (tid < C) into[tid] = w.state_weight * power[C - (from_end ? 0 : 1) - tid];
+  // Tables by row: what a block's v and the state in front of it enter with, and the v of
+  // a block that is not whole, two in turn.
+  float *const into = power + C + 4, *const reach = into + C,
+               *const into_parts = reach + C;
+  if (tid < C) {
+    into[tid] = w.state_weight * power[C - (from_end ? 0 : 1) - tid];
+    reach[tid] = w.reach_weight * power[tid + (from_end ? 0 : 1)];
+  }
+  const float state_weight = pin(w.state_weight);
   __syncthreads();
 
   const int value0 = part.slice * BV, col0 = value0 + wave * 16;
   const long row_base = static_cast<long>(part.b) * p.steps;
+  auto share_of = [&](int heads) {
+    return __builtin_amdgcn_readfirstlane(part.h / heads);
+  };
   const T* const q = OUTPUT ? static_cast<const T*>(w.q) +
                                   row_base * w.q_row +
-                                  static_cast<long>(part.h / w.q_share) * w.keys
+                                  static_cast<long>(share_of(w.q_share)) * w.keys
                             : nullptr;
   const T* const k = static_cast<const T*>(w.k) + row_base * w.k_row +
-                     static_cast<long>(part.h / w.k_share) * w.keys;
+                     static_cast<long>(share_of(w.k_share)) * w.keys;
   const T* const v = static_cast<const T*>(w.v) + row_base * w.v_row +
-                     static_cast<long>(part.h / w.v_share) * w.values + value0;
+                     static_cast<long>(share_of(w.v_share)) * w.values + value0;
   // The step of a place in the walk's order; a block's lowest step (which may be in
-  // front of the sequence, where the block's rows do not exist) and a row's distance
-  // from it.
+  // front of the sequence, where the block's rows do not exist).
   auto step_of = [&](int place) {
     return from_end ? length - 1 - place : place;
   };
@@ -335,7 +356,6 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
     return from_end ? static_cast<long>(length) - C - place
                     : static_cast<long>(place);
   };
-  auto above = [&](int row) { return from_end ? C - 1 - row : row; };
 
   // The state: tile i's column of the lane is its value lane % 16, its rows are the keys
   // key_of(i) + 0 ... 3.
@@ -347,38 +367,38 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
   const long state_at =
       (static_cast<long>(part.bh) * p.pieces + part.piece) * state_size;
   const int my_value = col0 + c16;
-  // (through a buffer of the state's size: keys behind its own are out of range)
+  // (through a buffer of the state's size, keys and values behind its own out of range:
+  // as bits and not as a choice, which would be a branch around every access, and a wait)
   auto state_buffer = [&](const float* at) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(at), 0,
                                              static_cast<int>(state_size * 4),
                                              0x00020000);
   };
+  auto state_offset = [&](int key, int of_key, int of_value) {
+    const int out = (w.keys - 1 - key) | (w.values - 1 - my_value);
+    return static_cast<unsigned>(key * of_key + my_value * of_value) |
+           (static_cast<unsigned>(out >> 31) & epi::kOob);
+  };
   auto start = [&] {
+    const float* from = nullptr;
+    if (OUTPUT)
+      from = p.pieces > 1           ? w.states + state_at
+             : w.initial != nullptr ? w.initial + part.bh * state_size
+                                    : nullptr;
+    if (from == nullptr) {
 #pragma unroll
-  for (int i = 0; i < D / 16; ++i) state[i] = float4v{0.f, 0.f, 0.f, 0.f};
-  if constexpr (OUTPUT) {
-    const float* const from = p.pieces > 1           ? w.states + state_at
-                              : w.initial != nullptr ? w.initial + part.bh * state_size
-                                                     : nullptr;
-    if (from != nullptr) {
-      const __amdgpu_buffer_rsrc_t rsrc = state_buffer(from);
-      const unsigned of_key = w.transposed ? 4 : 4 * w.values;
-      const unsigned of_value = w.transposed ? 4 * w.keys : 4;
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int key = key_of(i) + r;
-          const bool in = my_value < w.values && key < w.keys;
-          state[i][r] = __builtin_bit_cast(
-              float, __builtin_amdgcn_raw_buffer_load_b32(
-                         rsrc, in ? key * of_key + my_value * of_value : epi::kOob,
-                         0, 0));
-        }
-        __builtin_amdgcn_sched_barrier(0);
-      }
+      for (int i = 0; i < D / 16; ++i) state[i] = float4v{0.f, 0.f, 0.f, 0.f};
+      return;
     }
-  }
+    const __amdgpu_buffer_rsrc_t rsrc = state_buffer(from);
+    const int of_key = w.transposed ? 4 : 4 * w.values;
+    const int of_value = w.transposed ? 4 * w.keys : 4;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        state[i][r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
+            rsrc, state_offset(key_of(i) + r, of_key, of_value), 0, 0));
   };
 
   // A block's rows on their way, where they pass through registers.  Rows behind the
@@ -456,22 +476,41 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
     }
   };
   // (every lane loads a byte that exists)
+  const unsigned char* const resets_of =
+      p.resets == nullptr ? nullptr : p.resets + row_base;
   auto load_reset = [&](int place) {
-    if (p.resets != nullptr)
-      held_reset = p.resets[row_base + step_of(min(place + lane % C, last - 1))];
+    if (resets_of != nullptr)
+      held_reset = resets_of[step_of(min(place + lane % C, last - 1))];
   };
 
   // ... and straight to LDS, a KiB of neighbouring places for each load: the row and
   // the piece that belong there.
   // (a load of all threads is a number of rows; every sixteen rows, where the swizzle
-  // comes again, the base moves)
+  // comes again, a scalar offset moves: from the lowest step on)
   constexpr int kTurnsK =
       16 * Keys::kPieces > kThreads ? 16 * Keys::kPieces / kThreads : 1;
   constexpr int kTurnsV =
       16 * Values::kPieces > kThreads ? 16 * Values::kPieces / kThreads : 1;
   unsigned from_k[kTurnsK], from_q[kTurnsK], from_v[kTurnsV];
+  auto moves = [&](auto tile) {  // rows of such a move, and how many there are
+    typedef decltype(tile) Of;
+    constexpr int kTurns =
+        16 * Of::kPieces > kThreads ? 16 * Of::kPieces / kThreads : 1;
+    constexpr int kRows = kThreads * kTurns / Of::kPieces;
+    return std::integral_constant<int, kRows>();
+  };
+  constexpr int kMoveK = decltype(moves(Keys()))::value,
+                kMoveV = decltype(moves(Values()))::value;
+  const unsigned move_k = pin(static_cast<unsigned>(kMoveK * w.k_row * E)),
+                 move_q = pin(static_cast<unsigned>(kMoveK * w.q_row * E)),
+                 move_v = pin(static_cast<unsigned>(kMoveV * w.v_row * E));
+  // the block that is issued next, and from block to block
+  const char *at_k = nullptr, *at_q = nullptr, *at_v = nullptr;
+  const long step_k = pin((from_end ? -C : C) * w.k_row * E),
+             step_q = pin((from_end ? -C : C) * w.q_row * E),
+             step_v = pin((from_end ? -C : C) * w.v_row * E);
   if constexpr (DIRECT) {
-    auto places_of = [&](auto tile, long stride, int cols, auto& from) {
+    auto places_of = [&](auto tile, long stride, int cols, int move, auto& from) {
       typedef decltype(tile) Of;
       constexpr int kTurns = sizeof(from) / sizeof(unsigned);
 #pragma unroll
@@ -479,62 +518,88 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
         const int row = (tid + kThreads * u) / Of::kPieces;
         const int col = static_cast<int>(
             (tid % Of::kPieces ^ swizzle<E, Of::kPitch>(row)) * kPer);
-        from[u] = col < cols
-                      ? static_cast<unsigned>((above(row) * stride + col) * E)
-                      : epi::kOob;
+        const int up = from_end ? move - 1 - row : row;
+        from[u] = col < cols ? static_cast<unsigned>((up * stride + col) * E)
+                             : epi::kOob;
       }
     };
-    places_of(Keys(), w.k_row, w.keys, from_k);
-    if (OUTPUT) places_of(Keys(), w.q_row, w.keys, from_q);
-    places_of(Values(), w.v_row, there, from_v);
+    places_of(Keys(), w.k_row, w.keys, kMoveK, from_k);
+    if (OUTPUT) places_of(Keys(), w.q_row, w.keys, kMoveK, from_q);
+    places_of(Values(), w.v_row, there, kMoveV, from_v);
   }
   auto issue = [&](int place, char* to) {
     if constexpr (DIRECT) {
       if (place >= last) return;
-      const long low = lowest(place);
       const int n = last - place;
-      auto some = [&](const T* base, long stride, const auto& from, auto tile,
+      auto some = [&](const char* base, const auto& from, unsigned move, auto tile,
                       char* at) {
         typedef decltype(tile) Of;
         constexpr int kLoads = C * Of::kPieces / kThreads;
         constexpr int kRows = kThreads / Of::kPieces;
         constexpr int kTurns = sizeof(from) / sizeof(unsigned);
-        base += low * stride;
+        constexpr int kMoves = kLoads / kTurns;
+        const __amdgpu_buffer_rsrc_t rsrc = epi::make_rsrc(base);
+        auto all = [&](auto offset_of) {
 #pragma unroll
-        for (int l = 0; l < kLoads; ++l) {
-          const int up = kRows * (l / kTurns * kTurns);
-          const __amdgpu_buffer_rsrc_t rsrc =
-              epi::make_rsrc(base + (from_end ? -up : up) * stride);
-          const unsigned offset = n < C && tid / Of::kPieces + kRows * l >= n
-                                      ? epi::kOob
-                                      : from[l % kTurns];
-          __builtin_amdgcn_raw_ptr_buffer_load_lds(
-              rsrc, (lds_ptr)(at + (kThreads * l + 64 * wave) * 16), 16, offset, 0,
-              0, 0);
-        }
+          for (int l = 0; l < kLoads; ++l)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                rsrc, (lds_ptr)(at + (kThreads * l + 64 * wave) * 16), 16,
+                offset_of(l),
+                same((from_end ? kMoves - 1 - l / kTurns : l / kTurns) * move), 0,
+                0);
+        };
+        if (n >= C)
+          all([&](int l) { return from[l % kTurns]; });
+        else
+          all([&](int l) {
+            return tid / Of::kPieces + kRows * l >= n ? epi::kOob
+                                                      : from[l % kTurns];
+          });
       };
-      some(k, w.k_row, from_k, Keys(), to);
-      some(v, w.v_row, from_v, Values(), to + kVAt);
-      if (OUTPUT) some(q, w.q_row, from_q, Keys(), to + kQAt);
+      some(at_k, from_k, move_k, Keys(), to);
+      some(at_v, from_v, move_v, Values(), to + kVAt);
+      if (OUTPUT) some(at_q, from_q, move_q, Keys(), to + kQAt);
+      at_k += step_k;
+      at_v += step_v;
+      at_q += step_q;
     }
   };
 
-  // The weights of the wave's tiles of q k: of row (column of the tile) 16 t + c16
-  // and the four s from 16 x + 4 group on.
-  float weight[PT][4], reach[TT];
+  // The wave's tiles of q k: rows 16 t, s from 16 (t + x) % TT on.  Their weights: a power
+  // of the decay for the tile's distance from the diagonal, times the lane's four within
+  // a tile.
+  const int t_tile = wave * PT / TT;
+  auto s_tile = [&](int x) { return (t_tile + wave * PT % TT + x) % TT; };
+  // (the first of them is on the diagonal where a wave has all of a row)
+  constexpr int kWords = E;  // of four weights
+  float within[4], diagonal[4], beyond[PT];
+  unsigned counts[PT][kWords];  // bits of the weights that count
   if constexpr (OUTPUT) {
+    const int apart = c16 - 4 * group;
 #pragma unroll
-    for (int x = 0; x < PT; ++x) {
-      const int t = (wave * PT + x) / TT % TT, s = (wave * PT + x) % TT;
-      const int apart = 16 * (t - s) + c16 - 4 * group;
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        weight[x][r] = apart >= r ? w.weight * power[apart - r] : 0.f;
+    for (int r = 0; r < 4; ++r) {
+      within[r] = power[16 + apart - r];
+      diagonal[r] = w.weight * power[max(0, apart - r)];
     }
 #pragma unroll
-    for (int t = 0; t < TT; ++t)
-      reach[t] = w.reach_weight * power[16 * t + c16 + (from_end ? 0 : 1)];
+    for (int x = 0; x < PT; ++x) {
+      const int rows = 16 * (t_tile - s_tile(x));
+      beyond[x] = rows < 0 ? 0.f : w.weight * power[max(0, rows - 16)];
+#pragma unroll
+      for (int u = 0; u < kWords; ++u) {
+        counts[x][u] = 0;
+#pragma unroll
+        for (int r = u * 4 / kWords; r < (u + 1) * 4 / kWords; ++r)
+          if (rows + apart >= r)
+            counts[x][u] |= E == 4 ? ~0u : 0xFFFFu << 16 * (r % 2);
+      }
+    }
   }
+  auto weight_of = [&](int x, int r) {
+    const int rows = 16 * (t_tile - s_tile(x));
+    return rows > 0 ? within[r] * beyond[x]
+                    : diagonal[r];
+  };
   bool carried = true;  // no reset so far
   unsigned along[Keys::kAlong], along_p[Weights::kAlong];
   unsigned down_k[Keys::kAcross][Keys::kDown], down_v[Values::kDown];
@@ -542,14 +607,30 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
   Weights::start_rows(along_p, lane);
   Keys::start_columns(down_k, lane);
   Values::start_columns(down_v, wave * 16, lane);
-  // Where the lane's row c16 of the result goes, from the block's lowest step on.
-  const int out_size = w.out_float ? 4 : E;
+  // Where the lane's row c16 of the result goes, and its other rows 16 further, from the
+  // lowest step on.
+  const bool out_float = pin(w.out_float) != 0;
+  const int out_size = out_float ? 4 : E;
   const unsigned out_at =
-      my_value - c16 + 4 * group < w.values
-          ? static_cast<unsigned>((above(c16) * w.out_row + col0 + 4 * group) *
-                                  out_size)
+      w.out != nullptr && my_value - c16 + 4 * group < w.values
+          ? static_cast<unsigned>(
+                ((from_end ? 15 - c16 : c16) * w.out_row + col0 + 4 * group) *
+                out_size)
           : epi::kOob;
-  const int out_turn = static_cast<int>((from_end ? -16 : 16) * w.out_row * out_size);
+  const unsigned out_move = pin(static_cast<unsigned>(16 * w.out_row * out_size));
+  char* at_out = nullptr;
+  const long out_step = pin((from_end ? -C : C) * w.out_row * out_size);
+  auto rewind = [&] {
+    at_k = pin(reinterpret_cast<const char*>(k + lowest(first) * w.k_row));
+    at_v = pin(reinterpret_cast<const char*>(v + lowest(first) * w.v_row));
+    if (OUTPUT) {
+      at_q = pin(reinterpret_cast<const char*>(q + lowest(first) * w.q_row));
+      at_out = pin(static_cast<char*>(w.out) +
+                   ((row_base + lowest(first)) * w.out_row +
+                    static_cast<long>(part.h) * w.values) *
+                       out_size);
+    }
+  };
 
   // One block, whose rows are in `tile`.
   // CAREFUL: rows that do not count are left out one by one; otherwise by weights of
@@ -561,7 +642,7 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
     // (two tables in turn: waves may still read the ones of the block before)
     const int turn = (place - first) / C % 2 * C;
     int* const resets_to = all_resets_to + turn;
-    float* const into_part = into + C + turn;
+    float* const into_part = into_parts + turn;
     const int n = min(C, last - place);
     const char *const k_tile = tile, *const v_tile = tile + kVAt,
                       *const q_tile = tile + kQAt;
@@ -569,7 +650,7 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
     // for one another where none is among s + 1 ... r, or s ... r - 1 from the end:
     // where as many are in front of both.
     unsigned long long resets = 0;
-    if (p.resets != nullptr)
+    if (resets_of != nullptr)
       resets = __ballot(held_reset != 0 && lane < C && place + lane < last);
     const int all_resets = static_cast<int>(__popcll(resets));
     const int to_end = from_end ? n : n - 1;
@@ -580,7 +661,7 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
           __popcll(resets & (from_end ? before : before | 1ull << lane)));
       resets_to[lane] = mine;
       into_part[lane] = lane < n && mine == all_resets
-                           ? w.state_weight * power[to_end - lane]
+                           ? state_weight * power[to_end - lane]
                            : 0.f;
     }
     const float* const into_state = whole ? into : into_part;
@@ -593,31 +674,54 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
     if constexpr (OUTPUT) {
       // (tiles of later s are worked out as well and left out: no branches)
       float4v acc[PT];
+      uint4v of_q[2], of_k[2][PT];
+      auto fetch = [&](int b) {
+        of_q[b % 2] = Keys::rows(q_tile, along, t_tile, b);
+#pragma unroll
+        for (int x = 0; x < PT; ++x)
+          of_k[b % 2][x] = Keys::rows(k_tile, along, s_tile(x), b);
+      };
+      fetch(0);
 #pragma unroll
       for (int x = 0; x < PT; ++x) acc[x] = float4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int b = 0; b < BLOCKS; ++b)
+      for (int b = 0; b < BLOCKS; ++b) {
+        if (b + 1 < BLOCKS) fetch(b + 1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int x = 0; x < PT; ++x)
+          acc[x] = epi::multiply<T>(of_k[b % 2][x], of_q[b % 2], acc[x]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      typedef unsigned int Words __attribute__((ext_vector_type(kWords)));
+      const int row = 16 * t_tile + c16;
+      auto put = [&](auto also) {
 #pragma unroll
         for (int x = 0; x < PT; ++x) {
-          const int t = (wave * PT + x) / TT % TT, s = (wave * PT + x) % TT;
-          acc[x] = epi::multiply<T>(Keys::rows(k_tile, along, s, b),
-                                    Keys::rows(q_tile, along, t, b), acc[x]);
-        }
+          const int col = 16 * s_tile(x) + 4 * group;
+          float to[4];
 #pragma unroll
-      for (int x = 0; x < PT; ++x) {
-        const int t = (wave * PT + x) / TT, s = (wave * PT + x) % TT;
-        if (t >= TT) continue;  // (blocks of fewer tiles than waves)
-        const int row = 16 * t + c16, col = 16 * s + 4 * group;
-        typedef T Four __attribute__((ext_vector_type(4)));
-        Four to;
+          for (int r = 0; r < 4; ++r) to[r] = acc[x][r] * weight_of(x, r);
+          Words words = __builtin_bit_cast(Words, seq::pack<T, 4>(to));
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          bool on = col + r <= row;
-          if (resets != 0) on = on && resets_to[col + r] == resets_to[row];
-          to[r] = static_cast<T>(on ? acc[x][r] * weight[x][r] : 0.f);
+          for (int u = 0; u < kWords; ++u) words[u] &= counts[x][u] & also(col, u);
+          *reinterpret_cast<Words*>(p_tile + Weights::at(row, col / kPer) +
+                                    col % kPer * E) = words;
         }
-        *reinterpret_cast<Four*>(p_tile + Weights::at(row, col / kPer) +
-                                 col % kPer * E) = to;
+      };
+      if (resets == 0) {
+        put([](int, int) { return ~0u; });
+      } else {
+        const int mine = resets_to[row];
+        put([&](int col, int u) {
+          unsigned bits = 0;
+#pragma unroll
+          for (int r = u * 4 / kWords; r < (u + 1) * 4 / kWords; ++r)
+            bits |= resets_to[col + r] == mine
+                        ? (E == 4 ? ~0u : 0xFFFFu << 16 * (r % 2))
+                        : 0u;
+          return bits;
+        });
       }
       __builtin_amdgcn_s_waitcnt(epi::kLgkm0 & epi::vmcnt_imm(63));
       asm volatile("" ::: "memory");
@@ -626,13 +730,15 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
     }
 
     uint4v v_part[SB];
+    auto fetch_v = [&] {
 #pragma unroll
-    for (int b = 0; b < SB; ++b) {
-      v_part[b] = Values::fragment(v_tile, down_v, b);
-      if (!CAREFUL)
-        clean = epi::multiply<T>(v_part[b], uint4v{0u, 0u, 0u, 0u}, clean);
-    }
-
+      for (int b = 0; b < SB; ++b) {
+        v_part[b] = Values::fragment(v_tile, down_v, b);
+        if (!CAREFUL)
+          clean = epi::multiply<T>(v_part[b], uint4v{0u, 0u, 0u, 0u}, clean);
+      }
+    };
+    if constexpr (!OUTPUT) fetch_v();
     if constexpr (OUTPUT) {
       // q X of all rows, and the sums over the block's v
       float scale = 1.f, unscale[4] = {1.f, 1.f, 1.f, 1.f};
@@ -661,36 +767,45 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
       float4v acc[TT];
 #pragma unroll
       for (int t = 0; t < TT; ++t) acc[t] = float4v{0.f, 0.f, 0.f, 0.f};
+      uint4v of_q[2][TT];
+      auto fetch = [&](int b) {
+#pragma unroll
+        for (int t = 0; t < TT; ++t)
+          of_q[b % 2][t] = Keys::rows(q_tile, along, t, b);
+      };
+      fetch(0);
 #pragma unroll
       for (int b = 0; b < BLOCKS; ++b) {
+        if (b + 1 < BLOCKS) fetch(b + 1);
         float x[4 * HALVES];
 #pragma unroll
         for (int i = 0; i < 4 * HALVES; ++i)
           x[i] = state[b * HALVES + i / 4][i % 4] * scale;
         uint4v high, low;
         Split<T>::split(x, &high, &low);
-        uint4v of_q[TT];
-#pragma unroll
-        for (int t = 0; t < TT; ++t) of_q[t] = Keys::rows(q_tile, along, t, b);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int t = 0; t < TT; ++t)
-          acc[t] = epi::multiply<T>(high, of_q[t], acc[t]);
+          acc[t] = epi::multiply<T>(high, of_q[b % 2][t], acc[t]);
         if constexpr (E == 2) {
 #pragma unroll
           for (int t = 0; t < TT; ++t)
-            acc[t] = epi::multiply<T>(low, of_q[t], acc[t]);
+            acc[t] = epi::multiply<T>(low, of_q[b % 2][t], acc[t]);
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
       for (int t = 0; t < TT; ++t) {
+        const float by = reach[16 * t + c16];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) acc[t][r] *= reach[t] * unscale[r];
+        for (int r = 0; r < 4; ++r) acc[t][r] *= by * unscale[r];
         if (resets != 0) {
           const bool reached = resets_to[16 * t + c16] == 0;
 #pragma unroll
           for (int r = 0; r < 4; ++r) acc[t][r] = reached ? acc[t][r] : 0.f;
         }
       }
+      fetch_v();
       if constexpr (!CAREFUL) {
 #pragma unroll
         for (int b = 0; b < SB; ++b)
@@ -717,74 +832,76 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
           }
         }
       }
-      if (w.out != nullptr) {
-        char* const base =
-            static_cast<char*>(w.out) +
-            ((row_base + lowest(place)) * w.out_row +
-             static_cast<long>(part.h) * w.values) * out_size;
-        if constexpr (DIRECT) {
-          // (as many stores of every wave in every block, whether its rows and values
-          // exist or not: the waits for loads count them)
-          const __amdgpu_buffer_rsrc_t rsrc = epi::make_rsrc(base);
+      if constexpr (DIRECT) {
+        const __amdgpu_buffer_rsrc_t rsrc = epi::make_rsrc(at_out);
+        auto all = [&](auto store) {
 #pragma unroll
-          for (int t = 0; t < TT; ++t) {
-            const unsigned at =
-                16 * t + c16 < n && out_at != epi::kOob
-                    ? out_at + static_cast<unsigned>(t * out_turn)
-                    : epi::kOob;
-            if (w.out_float) {
-              __builtin_amdgcn_raw_buffer_store_b128(
-                  __builtin_bit_cast(uint4v, acc[t]), rsrc, at, 0, 0);
-            } else if constexpr (E == 4) {
-              __builtin_amdgcn_raw_buffer_store_b128(
-                  __builtin_bit_cast(uint4v, acc[t]), rsrc, at, 0, 0);
-            } else {
-              float x[4] = {acc[t][0], acc[t][1], acc[t][2], acc[t][3]};
-              typedef unsigned int uint2v __attribute__((ext_vector_type(2)));
-              __builtin_amdgcn_raw_buffer_store_b64(
-                  __builtin_bit_cast(uint2v, seq::pack<T, 4>(x)), rsrc, at, 0, 0);
-            }
-          }
+          for (int t = 0; t < TT; ++t)
+            store(acc[t], 16 * t + c16 < n ? out_at : epi::kOob,
+                  same((from_end ? TT - 1 - t : t) * out_move));
+        };
+        // (16-byte stores without a scalar offset: with one, registers were written anew
+        // before the store had read them, and no wait is put between the two)
+        auto floats = [&](float4v x, unsigned at, unsigned up) {
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uint4v, x), rsrc,
+                                                 at + up, 0, 0);
+        };
+        if constexpr (E == 4) {
+          all(floats);
+        } else if (out_float) {
+          all(floats);
         } else {
+          all([&](float4v x, unsigned at, unsigned up) {
+            const float v[4] = {x[0], x[1], x[2], x[3]};
+            typedef unsigned int uint2v __attribute__((ext_vector_type(2)));
+            __builtin_amdgcn_raw_buffer_store_b64(
+                __builtin_bit_cast(uint2v, seq::pack<T, 4>(v)), rsrc, at, up, 0);
+          });
+        }
+      } else if (out_at != epi::kOob) {
 #pragma unroll
-          for (int t = 0; t < TT; ++t) {
-            if (16 * t + c16 >= n) continue;
-            const int col = col0 + 4 * group;
-            auto store = [&](auto* out) {
-              typedef std::remove_pointer_t<decltype(out)> O;
-              if (col + 4 <= w.values) {
-                float x[4] = {acc[t][0], acc[t][1], acc[t][2], acc[t][3]};
-                *reinterpret_cast<typename seq::Pack<O, 4>::type*>(out) =
-                    seq::pack<O, 4>(x);
-              } else {
+        for (int t = 0; t < TT; ++t) {
+          if (16 * t + c16 >= n) continue;
+          auto store = [&](auto* out) {
+            typedef std::remove_pointer_t<decltype(out)> O;
+            if (col0 + 4 * group + 4 <= w.values) {
+              float x[4] = {acc[t][0], acc[t][1], acc[t][2], acc[t][3]};
+              *reinterpret_cast<typename seq::Pack<O, 4>::type*>(out) =
+                  seq::pack<O, 4>(x);
+            } else {
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                  if (col + r < w.values) out[r] = static_cast<O>(acc[t][r]);
-              }
-            };
-            char* const at =
-                base + (static_cast<long>(above(16 * t + c16)) * w.out_row + col) *
-                           out_size;
-            if (w.out_float)
-              store(reinterpret_cast<float*>(at));
-            else
-              store(reinterpret_cast<T*>(at));
-          }
+              for (int r = 0; r < 4; ++r)
+                if (col0 + 4 * group + r < w.values)
+                  out[r] = static_cast<O>(acc[t][r]);
+            }
+          };
+          char* const at =
+              at_out + ((from_end ? TT - 1 - t : t) * static_cast<long>(out_move) +
+                        out_at);
+          if (out_float)
+            store(reinterpret_cast<float*>(at));
+          else
+            store(reinterpret_cast<T*>(at));
         }
       }
+      at_out += out_step;
     }
 
     // The state behind the block.
     carried = carried && all_resets == 0;
-    if (all_resets == 0) {
-      const float carry = power[n];
+    const float carry = power[n];
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) state[i][r] *= carry;
+    if (all_resets != 0) {  // by selection: no infinity passes a reset
+      unsigned none = 0;
+      asm volatile("" : "+s"(none));  // (or zeros for this would be made in every block)
 #pragma unroll
       for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) state[i][r] *= carry;
-    } else {
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) state[i] = float4v{0.f, 0.f, 0.f, 0.f};
+        for (int r = 0; r < 4; ++r)
+          state[i][r] = __uint_as_float(__float_as_uint(state[i][r]) & none);
     }
     if constexpr (!CAREFUL) {
       // (rows in front of a reset may hold a k that a weight of zero leaves infinite)
@@ -858,7 +975,17 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
   constexpr auto kFast = std::false_type();
   constexpr auto kCareful = std::true_type();
   start();
-  if constexpr (DIRECT) {
+  rewind();
+  if constexpr (DIRECT && STAGES == 1) {
+    for (int place = first; place < last; place += C) {
+      load_reset(place);
+      issue(place, ring0);
+      __builtin_amdgcn_s_waitcnt(epi::vmcnt_imm(0));
+      asm volatile("" ::: "memory");
+      walk(ring0, place, kFast, [] {});
+      __syncthreads();  // the tiles have been read
+    }
+  } else if constexpr (DIRECT) {
     constexpr int kLoads = kLoadsV + kLoadsK * (OUTPUT ? 2 : 1);
     if (first < last) load_reset(first);
 #pragma unroll
@@ -869,7 +996,7 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
       if (last - place <= (STAGES - 2) * C)
         __builtin_amdgcn_s_waitcnt(epi::vmcnt_imm(0));
       else
-        __builtin_amdgcn_s_waitcnt(epi::vmcnt_imm((STAGES - 2) * kLoads));
+        __builtin_amdgcn_s_waitcnt(epi::vmcnt_imm(STAGES > 1 ? (STAGES - 2) * kLoads : 0));
       asm volatile("" ::: "memory");
       walk(ring(u), place, kFast, [&] {
         if (place + C < last) load_reset(place + C);
@@ -900,8 +1027,9 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
   // Values that are not finite: once more, and with care.
   const bool all_clean = clean_k && clean[0] == 0.f && clean[1] == 0.f &&
                          clean[2] == 0.f && clean[3] == 0.f;
-  if (!__syncthreads_and(all_clean)) {
+  if (__builtin_amdgcn_readfirstlane(__syncthreads_and(all_clean)) == 0) {
     start();
+    rewind();
     carried = true;
 #pragma unroll 1
     for (int place = first; place < last; place += C) {
@@ -948,14 +1076,10 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int key = key_of(i) + r;
-      const bool in = my_value < w.values && key < w.keys;
+    for (int r = 0; r < 4; ++r)
       __builtin_amdgcn_raw_buffer_store_b32(
           __float_as_uint(state[i][r]), rsrc,
-          in ? static_cast<unsigned>((key * w.values + my_value) * 4) : epi::kOob, 0,
-          0);
-    }
+          state_offset(key_of(i) + r, 4 * w.values, 4), 0, 0);
     __builtin_amdgcn_sched_barrier(0);
   }
 }
@@ -969,7 +1093,7 @@ __global__ void __launch_bounds__(64 * WAVES, (kWavesOfSimd<D, WAVES, OUTPUT>))
   // (an array of its own for each block)
   __shared__ __align__(1024) char ring0[kStage];
   char *r1 = nullptr, *r2 = nullptr;
-  if constexpr (DIRECT) {
+  if constexpr (DIRECT && kStages<D, OUTPUT> > 1) {
     __shared__ __align__(1024) char ring1[kStage];
     r1 = ring1;
   }
@@ -978,7 +1102,7 @@ __global__ void __launch_bounds__(64 * WAVES, (kWavesOfSimd<D, WAVES, OUTPUT>))
     r2 = ring2;
   }
   __shared__ __align__(1024) char p_tile[OUTPUT ? C * C * E : 16];
-  __shared__ __align__(16) float power[4 * C + 4];
+  __shared__ __align__(16) float power[5 * C + 4];
   __shared__ int resets_to[2 * C];  // in front of a row that count against it
   walk_body<T, D, WAVES, OUTPUT, DIRECT>(p, ring0, r1, r2, p_tile, power,
                                          resets_to);
@@ -1020,11 +1144,9 @@ int run_class(const Problem& p, int keys_class, int waves, bool outputs,
               hipStream_t stream) {
   switch (keys_class) {
     case 64:
-      return waves == 8 ? launch_walk<T, 64, 8, DIRECT>(p, outputs, stream)
-                        : launch_walk<T, 64, 4, DIRECT>(p, outputs, stream);
+      return launch_walk<T, 64, 4, DIRECT>(p, outputs, stream);
     case 128:
-      return waves == 8 ? launch_walk<T, 128, 8, DIRECT>(p, outputs, stream)
-                        : launch_walk<T, 128, 4, DIRECT>(p, outputs, stream);
+      return launch_walk<T, 128, 4, DIRECT>(p, outputs, stream);
     default:
       return launch_walk<T, 256, 4, DIRECT>(p, outputs, stream);
   }

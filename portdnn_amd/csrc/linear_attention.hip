@@ -260,7 +260,7 @@ int class_of(int keys) { return keys <= 64 ? 64 : keys <= 128 ? 128 : 256; }
 
 // Waves of a work-group, and the work-groups that share the values.
 int waves_of(int keys, int values) {
-  return values > 64 && class_of(keys) <= 128 ? 8 : 4;
+  return 4;
 }
 int slices_of(int keys, int values) {
   return ceil_div(values, 16 * waves_of(keys, values));
@@ -271,12 +271,13 @@ int slices_of(int keys, int values) {
 struct Division {
   int pieces, piece_steps;
 };
+constexpr size_t kGroups = 768;
 Division divide(const snn_hip_linear_attention_params& p, int units, int block,
                 size_t bytes, int states) {
   const int blocks = ceil_div(p.steps, block);
   const size_t groups = static_cast<size_t>(p.batch) * p.heads * units;
   int pieces = static_cast<int>(
-      std::min<size_t>(512 / std::min<size_t>(groups, 512), blocks / 4));
+      std::min<size_t>(kGroups / std::min<size_t>(groups, kGroups), blocks / 4));
 #ifdef SNN_HIP_TUNING
   if (const char* want = std::getenv("SNN_HIP_ATT_PIECES"))
     pieces = std::min(std::atoi(want), blocks);
