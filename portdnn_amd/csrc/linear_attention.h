@@ -271,10 +271,13 @@ __device__ __forceinline__ Part part_of(const Problem& p) {
 //
 // LDS holds three blocks of 128 keys, q and 128 values, or two work-groups of a CU
 // with two blocks each.
-template <int D, bool OUTPUT>
-constexpr int kStages = 1;
 template <int D, int WAVES, bool OUTPUT>
-constexpr int kWavesOfSimd = D == 256 ? 1 : OUTPUT ? 3 : 4;
+constexpr int kStages = WAVES == 8 ? (OUTPUT ? 3 : 2) : 1;
+template <int D, int WAVES, bool OUTPUT>
+constexpr int kWavesOfSimd = D == 256     ? 1
+                             : WAVES == 8 ? (OUTPUT ? 2 : 4)
+                             : OUTPUT     ? 3
+                                          : 4;
 
 template <typename T, int D, int WAVES, bool OUTPUT, bool DIRECT>
 __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* ring1,
@@ -287,7 +290,7 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
   constexpr int BLOCKS = D / KB, TT = C / 16, SB = C / KB;
   constexpr int PT = TT * TT / WAVES;  // tiles of q k of a wave
   constexpr int kPer = 16 / E;
-  constexpr int STAGES = DIRECT ? kStages<D, OUTPUT> : 1;
+  constexpr int STAGES = DIRECT ? kStages<D, WAVES, OUTPUT> : 1;
   typedef Tile<T, D> Keys;
   typedef Tile<T, BV> Values;
   typedef Tile<T, C> Weights;
@@ -529,8 +532,7 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
   }
   auto issue = [&](int place, char* to) {
     if constexpr (DIRECT) {
-      if (place >= last) return;
-      const int n = last - place;
+      const int n = last - place;  // (none: nothing but zeros comes)
       auto some = [&](const char* base, const auto& from, unsigned move, auto tile,
                       char* at) {
         typedef decltype(tile) Of;
@@ -695,33 +697,37 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
       }
       typedef unsigned int Words __attribute__((ext_vector_type(kWords)));
       const int row = 16 * t_tile + c16;
-      auto put = [&](auto also) {
+      unsigned bits[PT][kWords];
 #pragma unroll
-        for (int x = 0; x < PT; ++x) {
-          const int col = 16 * s_tile(x) + 4 * group;
-          float to[4];
+      for (int x = 0; x < PT; ++x)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) to[r] = acc[x][r] * weight_of(x, r);
-          Words words = __builtin_bit_cast(Words, seq::pack<T, 4>(to));
-#pragma unroll
-          for (int u = 0; u < kWords; ++u) words[u] &= counts[x][u] & also(col, u);
-          *reinterpret_cast<Words*>(p_tile + Weights::at(row, col / kPer) +
-                                    col % kPer * E) = words;
-        }
-      };
-      if (resets == 0) {
-        put([](int, int) { return ~0u; });
-      } else {
+        for (int u = 0; u < kWords; ++u) bits[x][u] = counts[x][u];
+      if (resets != 0) {
         const int mine = resets_to[row];
-        put([&](int col, int u) {
-          unsigned bits = 0;
 #pragma unroll
-          for (int r = u * 4 / kWords; r < (u + 1) * 4 / kWords; ++r)
-            bits |= resets_to[col + r] == mine
-                        ? (E == 4 ? ~0u : 0xFFFFu << 16 * (r % 2))
-                        : 0u;
-          return bits;
-        });
+        for (int x = 0; x < PT; ++x)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (resets_to[16 * s_tile(x) + 4 * group + r] != mine)
+              bits[x][r * kWords / 4] &= E == 4 ? 0u : ~(0xFFFFu << 16 * (r % 2));
+      }
+#pragma unroll
+      for (int x = 0; x < PT; ++x) {
+        const int col = 16 * s_tile(x) + 4 * group;
+        float to[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) to[r] = acc[x][r] * weight_of(x, r);
+        Words words = __builtin_bit_cast(Words, seq::pack<T, 4>(to));
+#pragma unroll
+        for (int u = 0; u < kWords; ++u) words[u] &= bits[x][u];
+        // (in assembly, as in front of a store that it knows the compiler waits for all
+        // loads into LDS, those of the blocks under way too; the wait is below)
+        const lds_ptr to_at = (lds_ptr)(p_tile + Weights::at(row, col / kPer) +
+                                        col % kPer * E);
+        if constexpr (E == 4)
+          asm volatile("ds_write_b128 %0, %1" ::"v"(to_at), "v"(words) : "memory");
+        else
+          asm volatile("ds_write_b64 %0, %1" ::"v"(to_at), "v"(words) : "memory");
       }
       __builtin_amdgcn_s_waitcnt(epi::kLgkm0 & epi::vmcnt_imm(63));
       asm volatile("" ::: "memory");
@@ -990,16 +996,16 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
     if (first < last) load_reset(first);
 #pragma unroll
     for (int u = 0; u < STAGES - 1; ++u) issue(first + u * C, ring(u));
+    // (the state has come: the compiler would wait for it inside of the loop, in every
+    // block, and so for the blocks under way)
+    __builtin_amdgcn_s_waitcnt(epi::vmcnt_imm(0));
     auto step = [&](int place, int u) {
       // (loads come in order: where no more accesses are under way than the loads of the
       // blocks behind, the block's own have come, whatever has become of stores)
-      if (last - place <= (STAGES - 2) * C)
-        __builtin_amdgcn_s_waitcnt(epi::vmcnt_imm(0));
-      else
-        __builtin_amdgcn_s_waitcnt(epi::vmcnt_imm(STAGES > 1 ? (STAGES - 2) * kLoads : 0));
+      __builtin_amdgcn_s_waitcnt(epi::vmcnt_imm((STAGES - 2) * kLoads));
       asm volatile("" ::: "memory");
       walk(ring(u), place, kFast, [&] {
-        if (place + C < last) load_reset(place + C);
+        load_reset(place + C);
         issue(place + (STAGES - 1) * C, ring((u + STAGES - 1) % STAGES));
       });
     };
@@ -1093,11 +1099,11 @@ __global__ void __launch_bounds__(64 * WAVES, (kWavesOfSimd<D, WAVES, OUTPUT>))
   // (an array of its own for each block)
   __shared__ __align__(1024) char ring0[kStage];
   char *r1 = nullptr, *r2 = nullptr;
-  if constexpr (DIRECT && kStages<D, OUTPUT> > 1) {
+  if constexpr (DIRECT && kStages<D, WAVES, OUTPUT> > 1) {
     __shared__ __align__(1024) char ring1[kStage];
     r1 = ring1;
   }
-  if constexpr (DIRECT && kStages<D, OUTPUT> > 2) {
+  if constexpr (DIRECT && kStages<D, WAVES, OUTPUT> > 2) {
     __shared__ __align__(1024) char ring2[kStage];
     r2 = ring2;
   }
@@ -1144,8 +1150,12 @@ int run_class(const Problem& p, int keys_class, int waves, bool outputs,
               hipStream_t stream) {
   switch (keys_class) {
     case 64:
+      if constexpr (sizeof(T) == 2)
+        if (waves == 8) return launch_walk<T, 64, 8, DIRECT>(p, outputs, stream);
       return launch_walk<T, 64, 4, DIRECT>(p, outputs, stream);
     case 128:
+      if constexpr (sizeof(T) == 2)
+        if (waves == 8) return launch_walk<T, 128, 8, DIRECT>(p, outputs, stream);
       return launch_walk<T, 128, 4, DIRECT>(p, outputs, stream);
     default:
       return launch_walk<T, 256, 4, DIRECT>(p, outputs, stream);

@@ -177,6 +177,7 @@ struct Chains {
   const float* decay;
   const int* lengths;
 };
+constexpr int kChained = 8;  // pieces under way at once
 __global__ void __launch_bounds__(256) chain_kernel(Chains p) {
   const Chain& c = p.chain[blockIdx.z];
   const int bh = blockIdx.y;
@@ -187,17 +188,27 @@ __global__ void __launch_bounds__(256) chain_kernel(Chains p) {
                          ? p.steps
                          : max(0, min(p.steps, p.lengths[b]));
   const float log_a = att::log_decay(p.decay, h);
-  const float whole = expf(p.piece_steps * log_a);
+  const float whole = expf(p.piece_steps * log_a) + 0x1p-126f;
   float state = c.initial == nullptr ? 0.f : c.initial[bh * p.size + at];
   float* to = c.states + static_cast<long>(bh) * p.pieces * p.size + at;
   const int* const carries = c.carries + static_cast<long>(bh) * p.pieces;
-  for (int i = 0; i < p.pieces; ++i, to += p.size) {
-    // (the last piece has left no state of its own, and those behind it none at all)
-    const bool on = static_cast<long>(i + 1) * p.piece_steps < length;
-    const float own = on ? *to : 0.f;
-    *to = state;
-    if (!on) break;
-    state = (carries[i] != 0 ? whole * state : 0.f) + own;
+  // (the last piece has left no state of its own, and those behind it none at all)
+  const int on = length == 0 ? 0 : (length - 1) / p.piece_steps;
+  for (int first = 0; first <= on; first += kChained, to += kChained * p.size) {
+    float own[kChained];
+    bool carried[kChained];
+#pragma unroll
+    for (int i = 0; i < kChained; ++i) {
+      const int piece = min(first + i, on);
+      own[i] = piece < on ? to[(piece - first) * p.size] : 0.f;
+      carried[i] = piece < on && carries[piece] != 0;
+    }
+#pragma unroll
+    for (int i = 0; i < kChained; ++i) {
+      if (first + i > on) break;
+      to[i * p.size] = state;
+      state = (carried[i] ? whole * state : 0.f) + own[i];
+    }
   }
 }
 
@@ -256,41 +267,67 @@ int check(const snn_hip_linear_attention_params* p, const void* workspace) {
 
 long or_else(int stride, long row) { return stride == 0 ? row : stride; }
 size_t round16(size_t bytes) { return (bytes + 15) / 16 * 16; }
+int block_of(int elem_size) { return elem_size == 2 ? 64 : 32; }
 int class_of(int keys) { return keys <= 64 ? 64 : keys <= 128 ? 128 : 256; }
 
 // Waves of a work-group, and the work-groups that share the values.
-int waves_of(int keys, int values) {
-  return 4;
+int waves_of(int size, int keys, int values) {
+  return size == 2 && values > 64 && class_of(keys) <= 128 ? 8 : 4;
 }
-int slices_of(int keys, int values) {
-  return ceil_div(values, 16 * waves_of(keys, values));
+int slices_of(int size, int keys, int values) {
+  return ceil_div(values, 16 * waves_of(size, keys, values));
 }
 
-// How a sequence is divided: enough work-groups for the GPU, pieces that are long
-// beside their states.
+// How a sequence is divided into pieces that are walked beside one another: as this
+// estimate says, in times of a block, where the work-groups of a CU wait for one another.
+// A piece costs four blocks for its states.  Work-groups of eight waves, or with states
+// of more than 128 keys, have a CU to themselves; of the others up to three share one,
+// and each further one takes 0.4 of the first's time.  The walk that leaves only states
+// takes 0.4 of one with outputs; it and the chain behind it cost their launches.
+// (bfloat16, us for 1, 2, 4, 8, 16, 32 pieces; * is what is taken.  1 x 32768 steps of 16
+// heads of 128 x 128: 1696, 1210, 630, 350, 217*, 235.  Gradients of 4 x 4096 steps of 16
+// such heads: 290*, 390, 345, 405, 500.  1 x 16384 steps of 16 heads of 64 x 64: 602, 458,
+// 236, 126, 75, 57*.  8 x 1000 steps of 8 such heads: 44, 44, 32, 29*, 38)
 struct Division {
   int pieces, piece_steps;
 };
-constexpr size_t kGroups = 768;
+constexpr int kCus = 256, kMostPieces = 128;
+double rounds_of(size_t groups, int of_cu) {
+  const size_t each = (groups + kCus - 1) / kCus;  // for the CU that has most
+  const size_t rest = each % of_cu;
+  return each / of_cu * (0.6 + 0.4 * of_cu) + (rest == 0 ? 0. : 0.6 + 0.4 * rest);
+}
 Division divide(const snn_hip_linear_attention_params& p, int units, int block,
-                size_t bytes, int states) {
+                int of_cu, size_t bytes, int states) {
   const int blocks = ceil_div(p.steps, block);
-  const size_t groups = static_cast<size_t>(p.batch) * p.heads * units;
-  int pieces = static_cast<int>(
-      std::min<size_t>(kGroups / std::min<size_t>(groups, kGroups), blocks / 4));
+  const size_t heads = static_cast<size_t>(p.batch) * p.heads;
+  auto need = [&](int pieces) {
+    return states * (round16(heads * pieces * p.keys * p.values * sizeof(float)) +
+                     round16(heads * pieces * sizeof(int)));
+  };
+  Division best = {1, blocks * block};
+  double least = rounds_of(heads * units, of_cu) * (blocks + 4);
+  for (int want = 2; want <= std::min(blocks, kMostPieces); ++want) {
+    const int each = ceil_div(blocks, want), pieces = ceil_div(blocks, each);
+    if (pieces != want || need(pieces) > bytes) continue;
+    // (of the gradients' three walks two leave states)
+    const size_t all = heads * units * pieces;
+    const double time =
+        (rounds_of(all, of_cu) + 0.4 * rounds_of(states == 1 ? all : all * 2 / 3, of_cu)) *
+            (each + 4) + 2 + pieces / 16.;
+    if (time < least) {
+      least = time;
+      best = {pieces, each * block};
+    }
+  }
 #ifdef SNN_HIP_TUNING
-  if (const char* want = std::getenv("SNN_HIP_ATT_PIECES"))
-    pieces = std::min(std::atoi(want), blocks);
+  if (const char* want = std::getenv("SNN_HIP_ATT_PIECES")) {
+    const int each = ceil_div(blocks, std::max(1, std::min(std::atoi(want), blocks)));
+    best = {ceil_div(blocks, each), each * block};
+    if (best.pieces == 1 || need(best.pieces) > bytes) best = {1, blocks * block};
+  }
 #endif
-  pieces = std::max(pieces, 1);
-  const int each = ceil_div(blocks, pieces);
-  pieces = ceil_div(blocks, each);
-  const size_t heads = static_cast<size_t>(p.batch) * p.heads * pieces;
-  const size_t need =
-      states * (round16(heads * p.keys * p.values * sizeof(float)) +
-                round16(heads * sizeof(int)));
-  if (pieces == 1 || need > bytes) return {1, blocks * block};
-  return {pieces, each * block};
+  return best;
 }
 size_t division_bytes(const snn_hip_linear_attention_params& p,
                       const Division& d, int states) {
@@ -300,13 +337,26 @@ size_t division_bytes(const snn_hip_linear_attention_params& p,
                    round16(heads * sizeof(int)));
 }
 
-int forward_units(const snn_hip_linear_attention_params& p) {
-  return slices_of(p.keys, p.values);
+// Work-groups of a pass over the whole sequence, and how many of them share a CU.
+int forward_units(const snn_hip_linear_attention_params& p, int size) {
+  return slices_of(size, p.keys, p.values);
 }
-int grad_units(const snn_hip_linear_attention_params& p) {
-  return 2 * slices_of(p.values, p.keys) + slices_of(p.keys, p.values);
+int grad_units(const snn_hip_linear_attention_params& p, int size) {
+  return 2 * slices_of(size, p.values, p.keys) + slices_of(size, p.keys, p.values);
 }
-int block_of(int elem_size) { return elem_size == 2 ? 64 : 32; }
+Division forward_division(const snn_hip_linear_attention_params& p, int size,
+                          size_t bytes) {
+  const bool alone =
+      class_of(p.keys) == 256 || waves_of(size, p.keys, p.values) == 8;
+  return divide(p, forward_units(p, size), block_of(size), alone ? 1 : 3, bytes, 1);
+}
+Division grad_division(const snn_hip_linear_attention_params& p, int size,
+                       size_t bytes) {
+  const bool alone =
+      class_of(std::max(p.keys, p.values)) == 256 ||
+      waves_of(size, p.keys, p.values) == 8 || waves_of(size, p.values, p.keys) == 8;
+  return divide(p, grad_units(p, size), block_of(size), alone ? 1 : 3, bytes, 2);
+}
 
 // fp32 gradients of q and k by heads, where heads share them.
 size_t shared_bytes(const snn_hip_linear_attention_params& p) {
@@ -343,9 +393,9 @@ Problem problem_of(const snn_hip_linear_attention_params& p, const Division& d,
   g.lengths = lengths;
   return g;
 }
-void add(Problem* g, const Walk& w) {
+void add(Problem* g, const Walk& w, int size) {
   g->walk[g->walks] = w;
-  g->walk[g->walks].slices = slices_of(w.keys, w.values);
+  g->walk[g->walks].slices = slices_of(size, w.keys, w.values);
   g->units += g->walk[g->walks].slices;
   ++g->walks;
 }
@@ -357,13 +407,13 @@ int run_all(const Problem& base, const Walk* walks, int n, bool outputs,
   for (int i = 0; i < n; ++i) {
     if (done[i]) continue;
     const int keys = class_of(walks[i].keys);
-    const int waves = waves_of(walks[i].keys, walks[i].values);
+    const int waves = waves_of(sizeof(T), walks[i].keys, walks[i].values);
     Problem g = base;
     for (int j = i; j < n; ++j) {
       if (done[j] || class_of(walks[j].keys) != keys ||
-          waves_of(walks[j].keys, walks[j].values) != waves)
+          waves_of(sizeof(T), walks[j].keys, walks[j].values) != waves)
         continue;
-      add(&g, walks[j]);
+      add(&g, walks[j], sizeof(T));
       done[j] = true;
     }
     const int s = run_class<T>(g, keys, waves, outputs, stream);
@@ -463,8 +513,7 @@ int forward(const void* q, const void* k, const void* v, const float* decay,
   w.reach_weight = p.scale;
   w.state_weight = 1.f;
   const Division d =
-      divide(p, forward_units(p), block_of(sizeof(T)),
-             workspace == nullptr ? 0 : elems * sizeof(T), 1);
+      forward_division(p, sizeof(T), workspace == nullptr ? 0 : elems * sizeof(T));
   const Problem base = problem_of(p, d, decay, resets, lengths);
   if (d.pieces > 1) {
     place_states(p, d.pieces, static_cast<char*>(workspace), &w);
@@ -587,8 +636,7 @@ int backward(const void* grad, const float* grad_final, const void* q,
   output(&of_k, grad_k, p.grad_k_stride, k_sums);
 
   KernelTimer timer(stream);
-  const Division d =
-      divide(p, grad_units(p), block_of(sizeof(T)), bytes - shared, 2);
+  const Division d = grad_division(p, sizeof(T), bytes - shared);
   const Problem base = problem_of(p, d, decay, resets, lengths);
   if (d.pieces > 1) {
     // the states from the front, as the forward pass has them, and from the end
@@ -671,24 +719,17 @@ int snn_hip_linear_attention_workspace_size(
     return SNN_HIP_INVALID_PARAMETER;
   const int valid = snn::check(params, nullptr);
   if (valid != SNN_HIP_OK) return valid;
-  const size_t size = dtype == SNN_HIP_DTYPE_F32 ? 4 : 2;
-  const int block = snn::block_of(static_cast<int>(size));
+  const int size = dtype == SNN_HIP_DTYPE_F32 ? 4 : 2;
+  size_t all = 0;
+  *required_elems = 0;
   if (grad != 0) {
-    const size_t shared = 2 * snn::shared_bytes(*params);
-    const snn::Division d = snn::divide(*params, snn::grad_units(*params), block,
-                                        ~size_t{0}, 2);
-    *required_elems = shared / size;
-    *recommended_elems =
-        (shared + snn::division_bytes(*params, d, 2)) / size;
-  } else {
-    *required_elems = 0;
-    *recommended_elems = 0;
-    if (params->steps > snn::kFewSteps) {
-      const snn::Division d = snn::divide(
-          *params, snn::forward_units(*params), block, ~size_t{0}, 1);
-      *recommended_elems = snn::division_bytes(*params, d, 1) / size;
-    }
+    all = 2 * snn::shared_bytes(*params);
+    *required_elems = all / size;
+    all += snn::division_bytes(*params, snn::grad_division(*params, size, ~size_t{0}), 2);
+  } else if (params->steps > snn::kFewSteps) {
+    all = snn::division_bytes(*params, snn::forward_division(*params, size, ~size_t{0}), 1);
   }
+  *recommended_elems = all / size;
   return SNN_HIP_OK;
 }
 
