@@ -985,8 +985,9 @@ SNN_HIP_API int snn_hip_rotary_frequencies(int turned, double base, int scaling,
  * strides of their own, elements from step to step (steps times that from sequence
  * to sequence), so that they may be slices of one projection's rows; output has
  * none.  decay holds `heads` floats, logarithms: 0 for a state that keeps
- * everything; values above 0 are taken as 0, values below -10000 as -10000.  Decays
- * are constants of the model and have no gradient here.
+ * everything; values above 0 are taken as 0, values below -10000 as -10000.  Powers
+ * of a decay are held above zero, by 2^-126, so that what is infinite stays so.
+ * Decays are constants of the model and have no gradient here.
  *
  * initial_state and final_state are [batch][heads][keys][values] floats (NULL: zero,
  * not wanted) and may be one buffer: a single token is a call with one step that
@@ -999,12 +1000,14 @@ SNN_HIP_API int snn_hip_rotary_frequencies(int turned, double base, int scaling,
  *
  * A few steps are taken one after the other, more in blocks: of each block of steps
  * the products q_t k_s, weighted by their decays, and the states come from the
- * matrix instructions.  These take scale q_t k_s rounded to the data type (in
- * binary16: infinite beyond 65504), the states and the weighted values as two
- * values of the data type each; sums and states are fp32.  Long sequences are
+ * matrix instructions.  These take scale q_t k_s rounded to the data type, the
+ * states and the weighted values as two values of the data type each (in binary16
+ * none of them is finite beyond 65504); sums and states are fp32.  Long sequences are
  * divided into pieces that run beside one another, given a workspace of the
  * recommended size.  The order of operations is fixed by the sizes and the
- * workspace.  At most 256 channels of a key or a value. */
+ * workspace.  At most 256 channels of a key or a value; more than 2^30 steps, 2^20
+ * heads of all sequences or 2^22 elements from step to step are
+ * SNN_HIP_INDEX_EXCEEDED. */
 typedef struct snn_hip_linear_attention_params {
   int batch;
   int steps;
