@@ -1,0 +1,5 @@
+// Not a portDNN include path: in the form of those of its operators.
+#ifndef SNN_FWD_ROTARY_LAUNCH_H
+#define SNN_FWD_ROTARY_LAUNCH_H
+#include "portdnn/hip/linear_attention_block.h"
+#endif
