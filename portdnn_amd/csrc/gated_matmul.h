@@ -557,7 +557,9 @@ __global__ void __launch_bounds__(256) join_kernel(Pair g) {
 // operands at any address.
 enum Kernel {
   kFew16x32,
+  kFew16x64,
   kFew32x32,
+  kFew32x64,
   kFew64x32,
   kTile64x128,
   kTile128,
@@ -567,11 +569,16 @@ enum Kernel {
   kAny16x32 = kDirectKernels,
 };
 inline epi::Shape shape_of(int elem_size, int kernel) {
-  constexpr int kSame[] = {epi::kFew16x32,   epi::kFew32x32, epi::kFew64x32,
+  constexpr int kSame[] = {epi::kFew16x32, -1, epi::kFew32x32, -1, epi::kFew64x32,
                            epi::kTile64x128, epi::kTile128,  epi::kTile128Pair,
                            epi::kTile256};
   if (kernel == kAny16x32)
     return {16, 32, 4, 512, 4, 3.0f, 1.2f, 2.4f};
+  const bool f32 = elem_size == 4;
+  if (kernel == kFew16x64)
+    return {16, 64, 4, 256, 4, 2.6f, f32 ? 0.8f : 0.6f, f32 ? 1.1f : 0.9f};
+  if (kernel == kFew32x64)
+    return {32, 64, 4, 256, 4, 2.8f, f32 ? 1.3f : 0.7f, f32 ? 1.6f : 1.1f};
   return epi::shape_of(elem_size, kSame[kernel]);
 }
 
@@ -600,7 +607,7 @@ inline float choose(const Pair& g, int elem_size, bool direct, size_t bytes,
   const double values = (g.gated ? g.m + 2.0 * g.n : 2.0 * g.m + 2.0 * g.n) * g.k;
   const bool cached = values * elem_size < 4e6;
   const float share_mb = static_cast<float>(g.m) * g.n * factors * 4e-6f;
-  const float memory = 1.f + static_cast<float>(values * elem_size / 4.2e6);
+  const double weights = 2.0 * g.n * g.k * elem_size;
   float best = -1.f;
   for (int kernel = direct ? 0 : kAny16x32;
        kernel < (direct ? kDirectKernels : kAny16x32 + 1); ++kernel) {
@@ -613,6 +620,15 @@ inline float choose(const Pair& g, int elem_size, bool direct, size_t bytes,
     const int tiles_m = ceil_div(g.m, s.bm);
     const int tiles_n = ceil_div(g.n, s.bn / factors);
     const double tiles = static_cast<double>(tiles_m) * tiles_n;
+    // Reading from memory: pieces of 16 columns cost a sixth more, weights that are
+    // read once more a quarter of a time, or a tenth where their rows are the
+    // reduction's.  (bfloat16, k 2048, n 8192, us beside a cold cache: 1 row 16x32 38.4,
+    // 16x64 33.2; 32 rows 16x64 41.6, 32x32 41.6, 32x64 33.8; transposed, 1 row
+    // 30.8, 31.2, 32 rows 34.4, 31.0, 32.0)
+    const bool narrow = !g.q_k_inner && s.bn / factors == 16;
+    const float memory = 1.f + static_cast<float>(
+        (values * elem_size * (narrow ? 1.17 : 1.0) +
+         weights * std::min(tiles_m - 1, 4) * (g.q_k_inner ? 0.1 : 0.25)) / 4.2e6);
     const int chunks = g.gated ? each : 2 * each;
     for (int want = 1; want <= 32; want *= 2) {
 #ifdef SNN_HIP_TUNING

@@ -83,9 +83,13 @@ template <typename T, bool GATED, bool QK>
 int launch_tile(const Pair& g, int kernel, hipStream_t stream) {
   switch (kernel) {
     case kFew16x32:
-      return launch_few<T, GATED, QK, 16, 32, 4, 4, true>(g, stream);
+      return launch_few<T, GATED, QK, 16, 32, 4, 3, true>(g, stream);
+    case kFew16x64:
+      return launch_few<T, GATED, QK, 16, 64, 4, 3, true>(g, stream);
     case kFew32x32:
       return launch_few<T, GATED, QK, 32, 32, 4, 2, true>(g, stream);
+    case kFew32x64:
+      return launch_few<T, GATED, QK, 32, 64, 4, 3, true>(g, stream);
     case kTile64x128:
       return launch_as<T, GATED, QK, 64, 128, 2, 4, 128, 5>(g, stream);
     case kAny16x32:

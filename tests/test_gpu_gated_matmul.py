@@ -119,6 +119,15 @@ def test_slices(dtype, m):
                       name)
 
 
+@pytest.mark.parametrize("size", [(3, 2048, 8192), (30, 1024, 16384)])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("trans_b", [False, True])
+def test_weights_larger_than_all_else(size, dtype, trans_b):
+    t, _ = _make(*size, dtype, trans_b)
+    got = ops.gated_matmul(*_cuda(t), trans_b=trans_b)
+    ref.check(got, plain.gated(*_wide(t, trans_b))[0], size[1] + 32)
+
+
 @pytest.mark.parametrize("size", [(2, 512, 64), (150, 513, 130), (64, 2048, 64)])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_without_a_workspace(size, dtype):
