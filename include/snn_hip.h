@@ -1000,11 +1000,11 @@ SNN_HIP_API int snn_hip_rotary_frequencies(int turned, double base, int scaling,
  *
  * A few steps are taken one after the other, more in blocks: of each block of steps
  * the products q_t k_s, weighted by their decays, and the states come from the
- * matrix instructions.  These take scale q_t k_s rounded to the data type, the
- * states and the weighted values as two values of the data type each (in binary16
- * none of them is finite beyond 65504); sums and states are fp32.  Long sequences are
- * divided into pieces that run beside one another, given a workspace of the
- * recommended size.  The order of operations is fixed by the sizes and the
+ * matrix instructions.  These take scale q_t k_s rounded to the data type (in
+ * binary16: infinite beyond 65504), states as sums of two values of the data type and
+ * weighted values as sums of two of binary16 or three of bfloat16; sums and states
+ * are fp32.  Long sequences are divided into pieces that run beside one another, given
+ * a workspace of the recommended size.  The order of operations is fixed by the sizes and the
  * workspace.  At most 256 channels of a key or a value; more than 2^30 steps, 2^20
  * heads of all sequences or 2^22 elements from step to step are
  * SNN_HIP_INDEX_EXCEEDED. */

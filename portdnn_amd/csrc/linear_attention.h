@@ -22,19 +22,31 @@
 //   X'    = a^n X + sum over s of a^(n - 1 - s) k_s^T v_s
 //
 // are four products of the matrix instructions.  All exponents are at least zero, so
-// that nothing overflows.  A work-group of four waves owns a piece of a head's
-// sequence and a slice of its values, which the waves divide.  The state stays in
-// registers: its accumulators' layout is that of the first operand of q X, as the
-// reduction's order is free as long as both operands agree.  The next block's rows
-// are on their way while one is multiplied.
+// that nothing overflows.  A work-group of four or eight waves owns a piece of a head's
+// sequence and a slice of its values, 16 for each wave.  The state stays in registers:
+// its accumulators' layout is that of the first operand of q X, as the reduction's order
+// is free as long as both operands agree.  The next blocks' rows are on their way while
+// one is multiplied.
+//
+// What bounds it: neither memory nor the matrix unit, but the chain of a block.  A block
+// of 64 steps and 128 channels takes a work-group 3.5 us alone on its CU: q k, its weights
+// by way of LDS, q X and the splits of X, the sums over v, the split of the weighted v,
+// its products; waits at two barriers lie between, and the vector unit is busy with
+// splits, weights and carries about half of the time.  bfloat16, 1 x 32768 steps of 16
+// heads of 128 channels: 224 us, of them 68 for the pass that leaves states, 10 for their
+// sums, 147 for the outputs (537 MB in all, 2.4 TB/s; 34 GFLOP by the formula of the steps,
+// 150 TFLOP/s).  Left out, of the 166 us that the outputs took before blocks
+// were asked for three ahead: loads 31, stores 44, the state's update 64, q X 90 us.
+// Gradients of 4 x 4096 steps, three walks of 64 heads in one launch: 279 us.
 //
 // Sequences that do not fill the GPU are divided into pieces: a first pass walks them
 // without outputs from a state of zero (k and v alone are read), the states are added
 // up along the sequence, and the second pass starts each piece from its own.
 //
-// The 16-bit types: q_r k_s and its decay are rounded to the type, as the softmax
-// weights of other attentions are; the state and the decayed v are held in two values
-// of the type (16 bits of a bfloat16 pair), as the state is an fp32 result.
+// The 16-bit types: q_r k_s and its decay are rounded to the type, once, as an output
+// is: a product of two more values would cost as much again.  The state is held in two
+// values of the type for q X (an output is rounded to 8 or 11 bits of the sum), and the
+// weighted v in as many as fp32 has bits, as the states are fp32 results.
 // Rows that may not count, those of later steps and those in front of a reset, are left
 // out by selection.  The matrix instructions would multiply their v by zero, which an
 // infinity or NaN survives: blocks that hold one (a product with zero tells) are
@@ -208,26 +220,28 @@ struct Tile {
   }
 };
 
-// Eight (four) floats as values of T, and what those leave of them; fp32 leaves none.
+// Eight (four) floats as a sum of values of T, each what those before leave of them:
+// three of bfloat16 and two of binary16 hold 24 and 22 bits, fp32 needs one.
 template <typename T>
 struct Split {
   static constexpr int N = 16 / sizeof(T);
+  static constexpr int kWhole = sizeof(T) == 4 ? 1 : std::is_same<T, _Float16>::value ? 2 : 3;
   typedef T V __attribute__((ext_vector_type(N)));
-  static __device__ __forceinline__ void split(const float (&v)[N], uint4v* high,
-                                               uint4v* low) {
-    V t;
+  template <int PARTS>
+  static __device__ __forceinline__ void split(float (&v)[N], uint4v (&parts)[PARTS]) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) t[i] = static_cast<T>(v[i]);
-    *high = __builtin_bit_cast(uint4v, t);
-    if constexpr (sizeof(T) == 2) {
+    for (int p = 0; p < PARTS; ++p) {
+      V t;
+#pragma unroll
+      for (int i = 0; i < N; ++i) t[i] = static_cast<T>(v[i]);
+      parts[p] = __builtin_bit_cast(uint4v, t);
+      if (p + 1 == PARTS) break;
       // (the rounded values themselves: worked out anew from a product, with one
       // rounding less, one in two thousand would be another than the one taken off)
-      asm volatile("" : "+v"(*high));
-      t = __builtin_bit_cast(V, *high);
+      asm volatile("" : "+v"(parts[p]));
+      t = __builtin_bit_cast(V, parts[p]);
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        t[i] = static_cast<T>(v[i] - static_cast<float>(t[i]));
-      *low = __builtin_bit_cast(uint4v, t);
+      for (int i = 0; i < N; ++i) v[i] -= static_cast<float>(t[i]);
     }
   }
   static __device__ __forceinline__ void floats(uint4v f, float (&v)[N]) {
@@ -270,11 +284,14 @@ __device__ __forceinline__ Part part_of(const Problem& p) {
 // in a ring; otherwise they pass through registers, where one block is under way.
 //
 // LDS holds three blocks of 128 keys, q and 128 values, or two work-groups of a CU
-// with two blocks each.
+// with two blocks each (outputs of 1 x 32768 steps of 16 heads: 166 us while every block
+// waited for the next as well, 149 with three under way).  Where four waves share a
+// CU's LDS with two others' work-groups, or states of 256 keys take the registers, one
+// block is loaded as the one before has been used.
 template <int D, int WAVES, bool OUTPUT>
-constexpr int kStages = WAVES == 8 ? (OUTPUT ? 3 : 2) : 1;
+constexpr int kStages = WAVES == 8 && D <= 128 ? (OUTPUT ? 3 : 2) : 1;
 template <int D, int WAVES, bool OUTPUT>
-constexpr int kWavesOfSimd = D == 256     ? 1
+constexpr int kWavesOfSimd = D == 256     ? WAVES / 4
                              : WAVES == 8 ? (OUTPUT ? 2 : 4)
                              : OUTPUT     ? 3
                                           : 4;
@@ -787,17 +804,14 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
 #pragma unroll
         for (int i = 0; i < 4 * HALVES; ++i)
           x[i] = state[b * HALVES + i / 4][i % 4] * scale;
-        uint4v high, low;
-        Split<T>::split(x, &high, &low);
+        uint4v parts[E == 4 ? 1 : 2];
+        Split<T>::split(x, parts);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int t = 0; t < TT; ++t)
-          acc[t] = epi::multiply<T>(high, of_q[b % 2][t], acc[t]);
-        if constexpr (E == 2) {
+        for (const uint4v& part : parts)
 #pragma unroll
           for (int t = 0; t < TT; ++t)
-            acc[t] = epi::multiply<T>(low, of_q[b % 2][t], acc[t]);
-        }
+            acc[t] = epi::multiply<T>(part, of_q[b % 2][t], acc[t]);
         __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
@@ -922,7 +936,11 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
           for (int i = 0; i < kPer; ++i) clean_k = clean_k && x[i] * 0.f == 0.f;
         }
       }
-      uint4v high[SB], low[SB];
+      // (weighted values in full, as the states that leave the kernel are fp32.  With two
+      // parts of bfloat16 these were off by 2.4e-6 instead of 2e-7, and 1 x 32768 steps of
+      // 16 heads of 128 channels took 215 us instead of 224)
+      constexpr int kParts = Split<T>::kWhole;
+      uint4v parts[SB][kParts];
 #pragma unroll
       for (int b = 0; b < SB; ++b) {
         float x[kPer];
@@ -930,7 +948,7 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
 #pragma unroll
         for (int i = 0; i < kPer; ++i)
           x[i] *= into_state[b * KB + group * (KB / 4) + i];
-        Split<T>::split(x, &high[b], &low[b]);
+        Split<T>::split(x, parts[b]);
       }
       // (two tiles' fragments are read while those before are multiplied, and no more of
       // them: they would take the registers that the loads' and sums' need)
@@ -951,12 +969,11 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
 #pragma unroll
         for (int b = 0; b < SB; ++b)
 #pragma unroll
-          for (int part = 0; part < (E == 2 ? 2 : 1); ++part)
+          for (int part = 0; part < kParts; ++part)
 #pragma unroll
             for (int u = 0; u < 2; ++u)
-              state[i + u] =
-                  epi::multiply<T>(of_k[i / 2 % 2][u][b],
-                                   part == 0 ? high[b] : low[b], state[i + u]);
+              state[i + u] = epi::multiply<T>(of_k[i / 2 % 2][u][b], parts[b][part],
+                                              state[i + u]);
         __builtin_amdgcn_sched_barrier(0);
       }
     } else {
@@ -1158,6 +1175,8 @@ int run_class(const Problem& p, int keys_class, int waves, bool outputs,
         if (waves == 8) return launch_walk<T, 128, 8, DIRECT>(p, outputs, stream);
       return launch_walk<T, 128, 4, DIRECT>(p, outputs, stream);
     default:
+      if constexpr (sizeof(T) == 2)
+        if (waves == 8) return launch_walk<T, 256, 8, DIRECT>(p, outputs, stream);
       return launch_walk<T, 256, 4, DIRECT>(p, outputs, stream);
   }
 }

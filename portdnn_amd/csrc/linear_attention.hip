@@ -31,7 +31,8 @@ struct Few {
 
 // One step after the other, all in fp32: a work-group owns 64 values of a head's
 // state, a lane four neighbouring values of every sixteenth key.  Bound by the state,
-// which is read and written once.
+// which is read and written once: one step of 64 sequences of 16 heads of 128 x 128 in
+// 28 us, 135 MB, 4.8 TB/s.
 template <typename T, int R>
 __global__ void __launch_bounds__(256) few_steps_kernel(Few p) {
   __shared__ float q_of[kFewSteps][16 * R], k_of[kFewSteps][16 * R];
@@ -164,7 +165,10 @@ int run_few(const Few& f, hipStream_t stream) {
 
 // ---- along the pieces ------------------------------------------------------------
 
-// The pieces' own states become the states in front of them, in the walk's order.
+// The pieces' own states become the states in front of them, in the walk's order: each
+// lane has one of a state's values and adds the pieces up, eight under way at once.  It
+// waits for memory: 10 us for 16 pieces of 16 heads of 128 x 128, 34 MB read and
+// written; 18 us with one under way.
 struct Chain {
   float* states;
   const int* carries;
@@ -270,9 +274,13 @@ size_t round16(size_t bytes) { return (bytes + 15) / 16 * 16; }
 int block_of(int elem_size) { return elem_size == 2 ? 64 : 32; }
 int class_of(int keys) { return keys <= 64 ? 64 : keys <= 128 ? 128 : 256; }
 
-// Waves of a work-group, and the work-groups that share the values.
+// Waves of a work-group, 16 values each, and the work-groups that share the values.
+// With eight, q, k and their products serve twice as many values.  (us, four and eight:
+// bfloat16, 1 x 32768 steps of 16 heads of 128 x 128 258, 219, gradients of 4 x 4096
+// steps 339, 256; 1 x 8192 steps of 16 heads of 256 x 256 266, 199, gradients 634, 510.
+// In fp32 a block of 32 steps has four tiles of q k, one for each of four waves.)
 int waves_of(int size, int keys, int values) {
-  return size == 2 && values > 64 && class_of(keys) <= 128 ? 8 : 4;
+  return size == 2 && values > 64 ? 8 : 4;
 }
 int slices_of(int size, int keys, int values) {
   return ceil_div(values, 16 * waves_of(size, keys, values));
@@ -284,10 +292,12 @@ int slices_of(int size, int keys, int values) {
 // of more than 128 keys, have a CU to themselves; of the others up to three share one,
 // and each further one takes 0.4 of the first's time.  The walk that leaves only states
 // takes 0.4 of one with outputs; it and the chain behind it cost their launches.
-// (bfloat16, us for 1, 2, 4, 8, 16, 32 pieces; * is what is taken.  1 x 32768 steps of 16
-// heads of 128 x 128: 1696, 1210, 630, 350, 217*, 235.  Gradients of 4 x 4096 steps of 16
-// such heads: 290*, 390, 345, 405, 500.  1 x 16384 steps of 16 heads of 64 x 64: 602, 458,
-// 236, 126, 75, 57*.  8 x 1000 steps of 8 such heads: 44, 44, 32, 29*, 38)
+// (us for 1, 2, 4, 8, 16, 32 pieces; * is what is taken.  bfloat16, 1 x 32768 steps of
+// 16 heads of 128 x 128: 1787, 1311, 663, 349, 222*, 248; gradients of 4 x 4096 steps
+// of such heads: 237*, 325, 304, 349, 461, 643; 1 x 16384 steps of 16 heads of 64 x 64:
+// 638, 490, 253, 134, 79, 60*; 1 x 8192 steps of 16 heads of 256 x 256: 759, 603, 335,
+// 202*, 221, 275.  fp32, 1 x 8192 steps of 8 heads of 128 x 128: 1007, 774, 396, 208,
+// 121, 103*)
 struct Division {
   int pieces, piece_steps;
 };

@@ -9,7 +9,12 @@
 // token's heads.  p f_i is taken in 64 bits and only its fraction, below half a turn,
 // goes on in fp32: at position 10^6 an angle that was held in fp32 throughout would
 // be off by 0.06.  A lane holds the sines and cosines of VEC pairs of a token and
-// walks its heads, kSlices at a time beside one another.
+// walks every `slices`-th of its heads.
+//
+// bfloat16, 4 x 4096 tokens of 32 heads of 128 channels: 54 us, 268 MB, 5.0 TB/s; fp32,
+// 2 x 5001 tokens of 12 heads of 100 channels, 64 of them turned as neighbours: 28.6 us,
+// 96 MB, 3.4 TB/s, with angles that memory waits for (31.2 us while the first heads were
+// asked for behind them).  A token of 16 sequences is the time of a launch.
 #include <algorithm>
 #include <cmath>
 
@@ -83,18 +88,42 @@ __global__ void __launch_bounds__(256) rotary_kernel(Rotary r) {
     const int first = r.turned + (unit - r.turns) * VEC;
     const int stay = r.channels - r.turned;
     const int c = stay >= VEC ? min(first, r.channels - VEC) : first;
-    for (int h = slice; h < r.heads; h += r.slices, in += step, out += step) {
+    constexpr int kAhead = 4;  // heads under way at once
+    for (int h = slice; h < r.heads; h += kAhead * r.slices) {
       if (stay >= VEC) {
-        *reinterpret_cast<V*>(out + c) = *reinterpret_cast<const V*>(in + c);
+        V some[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+          if (h + u * r.slices < r.heads)
+            some[u] = *reinterpret_cast<const V*>(in + u * step + c);
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+          if (h + u * r.slices < r.heads)
+            *reinterpret_cast<V*>(out + u * step + c) = some[u];
       } else {
-        for (int k = c; k < r.channels; ++k) out[k] = in[k];
+        for (int u = 0; u < kAhead && h + u * r.slices < r.heads; ++u)
+          for (int k = c; k < r.channels; ++k)
+            out[u * step + k] = in[u * step + k];
       }
+      in += kAhead * step;
+      out += kAhead * step;
     }
     return;
   }
 
   const int half = r.turned / 2;
   const Group<VEC> at(static_cast<int>(unit) * VEC, half);
+  const int c0 = PAIRS ? 2 * at.c : at.c;
+  const int c1 = PAIRS ? c0 + VEC : c0 + half;
+  // (two heads' values are on their way while the angles are worked out, and then while
+  // the ones before are turned)
+  V ahead[2][2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+    if (slice + u * r.slices < static_cast<unsigned>(r.heads)) {
+      ahead[u][0] = *reinterpret_cast<const V*>(in + u * step + c0);
+      ahead[u][1] = *reinterpret_cast<const V*>(in + u * step + c1);
+    }
   const unsigned b = row / r.steps, t = row - b * r.steps;
   const int kind = r.kind;
   const long p = kind == SNN_HIP_ROTARY_POSITIONS_NONE ? static_cast<long>(t)
@@ -110,13 +139,14 @@ __global__ void __launch_bounds__(256) rotary_kernel(Rotary r) {
     sine[i] *= r.inverse ? -r.magnitude : r.magnitude;
     cosine[i] *= r.magnitude;
   }
-  const int c0 = PAIRS ? 2 * at.c : at.c;
-  const int c1 = PAIRS ? c0 + VEC : c0 + half;
-#pragma unroll 2
-  for (int h = slice; h < r.heads; h += r.slices, in += step, out += step) {
+  auto turn = [&](V (&held)[2], bool more) {
     float x[2][VEC], y[2][VEC];
-    unpack<T, VEC>(*reinterpret_cast<const V*>(in + c0), x[0]);
-    unpack<T, VEC>(*reinterpret_cast<const V*>(in + c1), x[1]);
+    unpack<T, VEC>(held[0], x[0]);
+    unpack<T, VEC>(held[1], x[1]);
+    if (more) {
+      held[0] = *reinterpret_cast<const V*>(in + 2 * step + c0);
+      held[1] = *reinterpret_cast<const V*>(in + 2 * step + c1);
+    }
     if constexpr (PAIRS) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
@@ -136,6 +166,12 @@ __global__ void __launch_bounds__(256) rotary_kernel(Rotary r) {
       put<T, VEC>(out + c0, y[0], at.skip);
       put<T, VEC>(out + c1, y[1], at.skip);
     }
+    in += step;
+    out += step;
+  };
+  for (int h = slice; h < r.heads; h += 2 * r.slices) {
+    turn(ahead[0], h + 2 * r.slices < r.heads);
+    if (h + r.slices < r.heads) turn(ahead[1], h + 3 * r.slices < r.heads);
   }
 }
 

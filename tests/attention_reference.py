@@ -219,18 +219,20 @@ def attention_grad(do, q, k, v, decay, resets=None, lengths=None,
 def operations(channels, dtype):
     """fp32 operations that bound what a linear attention's outputs are off by:
     sums over the channels and over 64 steps of a block, decays whose exponent is
-    at most 88 and that come block by block; in 16 bits the rounding of q_t k_s,
-    and half a step of the second of the two values of a state and of a weighted
-    value, twice."""
+    at most 88 and that come block by block; in 16 bits the rounding of q_t k_s and
+    half a step of the second of the two values of a state, and the states' own."""
     least = channels + 320
     if dtype is torch.float32:
         return least
-    return least + per_rounding(dtype) * (1.01 + 2 * ROUND[dtype])
+    return (state_operations(channels, dtype) +
+            per_rounding(dtype) * (1.01 + ROUND[dtype]))
 
 
 def state_operations(channels, dtype):
-    """... and its states: without q_t k_s."""
+    """... and its states: of weighted values as sums of three values of bfloat16 or
+    two of binary16, half a step of the last."""
     least = channels + 320
     if dtype is torch.float32:
         return least
-    return least + 2 * per_rounding(dtype) * ROUND[dtype]
+    parts = 2 if dtype is torch.float16 else 3
+    return least + 2 * per_rounding(dtype) * ROUND[dtype] ** (parts - 1)
