@@ -926,8 +926,8 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
     if constexpr (!CAREFUL) {
       // (rows in front of a reset may hold a k that a weight of zero leaves infinite)
       if (resets != 0) {
-#pragma unroll 1
-        for (int piece = 0; piece < Keys::kPieces; ++piece) {
+#pragma unroll
+        for (int piece = wave; piece < Keys::kPieces; piece += WAVES) {
           float x[kPer];
           Split<T>::floats(*reinterpret_cast<const uint4v*>(
                                k_tile + Keys::at(lane % C, piece)),
