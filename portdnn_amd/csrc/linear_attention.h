@@ -37,7 +37,7 @@
 // sums, 147 for the outputs (537 MB in all, 2.4 TB/s; 34 GFLOP by the formula of the steps,
 // 150 TFLOP/s).  Left out, of the 166 us that the outputs took before blocks
 // were asked for three ahead: loads 31, stores 44, the state's update 64, q X 90 us.
-// Gradients of 4 x 4096 steps, three walks of 64 heads in one launch: 279 us.
+// Gradients of 4 x 4096 steps, three walks of 64 heads in one launch: 251 us.
 //
 // Sequences that do not fill the GPU are divided into pieces: a first pass walks them
 // without outputs from a state of zero (k and v alone are read), the states are added
