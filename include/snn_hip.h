@@ -1045,7 +1045,9 @@ SNN_HIP_API int snn_hip_linear_attention_bf16(
  * strides of their own and are zero from a sequence's length on; each of the four
  * outputs may be NULL and is then not computed.  No output may overlap an input.
  * Where key_heads is not heads, the sums over the heads that share a query or key
- * take workspace: SNN_HIP_INSUFFICIENT_WORKSPACE without the required size. */
+ * take workspace: SNN_HIP_INSUFFICIENT_WORKSPACE without the required size.  (In
+ * binary16 scale times a query or a value of grad_output is infinite beyond 65504 on
+ * its way into the states.) */
 SNN_HIP_API int snn_hip_linear_attention_grad_f32(
     const void* grad_output, const float* grad_final_state, const void* q,
     const void* k, const void* v, const float* decay,

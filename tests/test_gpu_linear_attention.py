@@ -196,6 +196,58 @@ def test_what_is_not_finite_stays_where_it_counts(keys, values, dtype, room):
               plain.state_operations(most, dtype))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_what_is_not_finite_among_a_few_steps(dtype):
+    t, _ = _make((2, 12, 2, 1, 40, 72), dtype)
+    t["resets"] = torch.zeros(2, 12, dtype=torch.uint8)
+    t["resets"][:, 8] = 1
+    bad = {**t, "v": t["v"].clone(), "k": t["k"].clone(), "q": t["q"].clone()}
+    bad["v"][:, 5, :, 2] = float("inf")
+    bad["q"][:, 2] = float("nan")
+    bad["k"][1, 7] = float("nan")
+    o, last = ops.linear_attention(**_cuda(bad))
+    want = plain.attention(dtype=dtype, **_wide(t))
+    others = [c for c in range(72) if c != 2]
+    count = plain.operations(72, dtype)
+
+    def part(pair, f):
+        return tuple(f(x) for x in pair)
+
+    for f in (lambda x: x[:, :2], lambda x: x[:, 3:5], lambda x: x[:, 8:],
+              lambda x: x[:1, 3:][..., others]):
+        ref.check(f(o), part(want[0], f), count)
+    assert torch.isnan(o[:, 2].float()).all()
+    assert torch.isnan(o[1, 7].float()).all()
+    assert not torch.isfinite(o[:, 5:8, :, 2].float()).any()
+    ref.check(last, want[1], plain.state_operations(72, dtype))
+
+
+@pytest.mark.parametrize("steps", [12, 150])
+def test_lengths_beyond_the_sequence(steps):
+    """They are taken as 0 and as all steps."""
+    t, grads = _make((3, steps, 2, 1, 24, 40), torch.bfloat16,
+                     lengths=[-5, steps + 1, 2 ** 31 - 1])
+    _check(t, grads, 0.3)
+
+
+@pytest.mark.parametrize("steps", [5, 200])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_infinite_states_end_at_a_reset(steps, dtype):
+    t, _ = _make((1, steps, 2, 2, 24, 40), dtype)
+    t["resets"] = torch.zeros(1, steps, dtype=torch.uint8)
+    t["resets"][:, 3] = 1
+    bad = {**t, "initial_state": t["initial_state"].clone()}
+    bad["initial_state"][:, :, 7, 11] = float("inf")
+    bad["initial_state"][:, :, 2, 30] = float("nan")
+    o, last = ops.linear_attention(**_cuda(bad))
+    want = plain.attention(dtype=dtype, **_wide(t))
+    others = [c for c in range(40) if c not in (11, 30)]
+    for f in (lambda x: x[:, 3:], lambda x: x[..., others]):
+        ref.check(f(o), tuple(f(x) for x in want[0]), plain.operations(40, dtype))
+    assert not torch.isfinite(o[:, :3, :, [11, 30]].float()).any()
+    ref.check(last, want[1], plain.state_operations(40, dtype))
+
+
 @pytest.mark.parametrize("steps", [5, 200])
 def test_differences(steps):
     """Outputs are linear in q, k, v and the state: <gradient, e> is half the
