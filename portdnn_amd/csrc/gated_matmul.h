@@ -13,10 +13,11 @@
 // reduction, whose chunks change operands halfway: nothing is rounded in between.
 //
 // Many rows are bound by the matrix unit, few by reading the weights.  bfloat16, 8192
-// rows, k 2048, n 8192, both factors kept: 533 us, 1.03 PFLOP/s (256 x 256 tiles; a
+// rows, k 2048, n 8192, both factors kept: 530 us, 1.04 PFLOP/s (256 x 256 tiles; a
 // library's product of these sizes reaches 1.35); SUM of 4096 rows, 2 x 8192 to 2048
-// columns: 278 us, 0.99 PFLOP/s (128 x 128 tiles, 512 of them).  1 row, k 2048, n 8192:
-// 15.2 us, 67 MB, 4.4 TB/s; binary16, 32 rows, k 4096, n 8192: 29.4 us, 134 MB, 4.6 TB/s.
+// columns: 249 us, 1.1 PFLOP/s (128 tiles of 256 x 256 in two shares, and their join).
+// 1 row, k 2048, n 8192: 15.2 us, 67 MB, 4.4 TB/s; binary16, 32 rows, k 4096, n 8192,
+// weights by column: 29.4 us, 134 MB, 4.6 TB/s.
 #ifndef PORTDNN_AMD_CSRC_GATED_MATMUL_H_
 #define PORTDNN_AMD_CSRC_GATED_MATMUL_H_
 
@@ -585,7 +586,12 @@ inline epi::Shape shape_of(int elem_size, int kernel) {
     return {16, 64, 4, 256, 4, 2.6f, f32 ? 0.8f : 0.6f, f32 ? 1.1f : 0.9f};
   if (kernel == kFew32x64)
     return {32, 64, 4, 256, 4, 2.8f, f32 ? 1.3f : 0.7f, f32 ? 1.6f : 1.1f};
-  return epi::shape_of(elem_size, kSame[kernel]);
+  epi::Shape s = epi::shape_of(elem_size, kSame[kernel]);
+  // (sums of 2 x 8192 products in bfloat16, at the clocks of long calls: 4096 x 2048 in
+  // 512 tiles of 128 x 128 281 us; in 128 of 256 x 256, in two shares, 233 and 16 for
+  // their join)
+  if (kernel == kTile128 && elem_size == 2) s.step_k = s.step_row = 0.48f;
+  return s;
 }
 
 // Bytes of a row in one of a kernel's chunks.
