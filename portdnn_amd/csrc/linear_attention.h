@@ -279,24 +279,16 @@ __device__ __forceinline__ Part part_of(const Problem& p) {
   return r;
 }
 
-// D: the keys, rounded up; WAVES: of a work-group, with 16 values each.  DIRECT: rows of
-// whole 16-byte pieces at aligned addresses, which go straight to LDS, STAGES blocks
-// in a ring; otherwise they pass through registers, where one block is under way.
-//
-// LDS holds three blocks of 128 keys, q and 128 values, or two work-groups of a CU
-// with two blocks each (outputs of 1 x 32768 steps of 16 heads: 166 us while every block
-// waited for the next as well, 149 with three under way).  Where four waves share a
-// CU's LDS with two others' work-groups, or states of 256 keys take the registers, one
-// block is loaded as the one before has been used.
-template <int D, int WAVES, bool OUTPUT>
-constexpr int kStages = WAVES == 8 && D <= 128 ? (OUTPUT ? 3 : 2) : 1;
+// D: the keys, rounded up; WAVES: of a work-group, with 16 values each.  STAGES: blocks
+// in a ring of LDS, to which rows of whole 16-byte pieces at aligned addresses go
+// straight; 0: rows pass through registers, where one block is under way.
 template <int D, int WAVES, bool OUTPUT>
 constexpr int kWavesOfSimd = D == 256     ? WAVES / 4
                              : WAVES == 8 ? (OUTPUT ? 2 : 4)
                              : OUTPUT     ? 3
                                           : 4;
 
-template <typename T, int D, int WAVES, bool OUTPUT, bool DIRECT>
+template <typename T, int D, int WAVES, bool OUTPUT, int RING>
 __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* ring1,
                                           char* ring2, char* p_tile, float* power,
                                           int* all_resets_to) {
@@ -307,7 +299,8 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
   constexpr int BLOCKS = D / KB, TT = C / 16, SB = C / KB;
   constexpr int PT = TT * TT / WAVES;  // tiles of q k of a wave
   constexpr int kPer = 16 / E;
-  constexpr int STAGES = DIRECT ? kStages<D, WAVES, OUTPUT> : 1;
+  constexpr bool DIRECT = RING > 0;
+  constexpr int STAGES = DIRECT ? RING : 1;
   typedef Tile<T, D> Keys;
   typedef Tile<T, BV> Values;
   typedef Tile<T, C> Weights;
@@ -1107,7 +1100,7 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
   }
 }
 
-template <typename T, int D, int WAVES, bool OUTPUT, bool DIRECT>
+template <typename T, int D, int WAVES, bool OUTPUT, int RING>
 __global__ void __launch_bounds__(64 * WAVES, (kWavesOfSimd<D, WAVES, OUTPUT>))
     walk_kernel(Problem p) {
 #ifdef __HIP_DEVICE_COMPILE__
@@ -1116,33 +1109,56 @@ __global__ void __launch_bounds__(64 * WAVES, (kWavesOfSimd<D, WAVES, OUTPUT>))
   // (an array of its own for each block)
   __shared__ __align__(1024) char ring0[kStage];
   char *r1 = nullptr, *r2 = nullptr;
-  if constexpr (DIRECT && kStages<D, WAVES, OUTPUT> > 1) {
+  if constexpr (RING > 1) {
     __shared__ __align__(1024) char ring1[kStage];
     r1 = ring1;
   }
-  if constexpr (DIRECT && kStages<D, WAVES, OUTPUT> > 2) {
+  if constexpr (RING > 2) {
     __shared__ __align__(1024) char ring2[kStage];
     r2 = ring2;
   }
   __shared__ __align__(1024) char p_tile[OUTPUT ? C * C * E : 16];
   __shared__ __align__(16) float power[5 * C + 4];
   __shared__ int resets_to[2 * C];  // in front of a row that count against it
-  walk_body<T, D, WAVES, OUTPUT, DIRECT>(p, ring0, r1, r2, p_tile, power,
-                                         resets_to);
+  walk_body<T, D, WAVES, OUTPUT, RING>(p, ring0, r1, r2, p_tile, power, resets_to);
 #endif
 }
 
-template <typename T, int D, int WAVES, bool DIRECT>
-int launch_walk(const Problem& p, bool outputs, hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(p.units) * p.batch * p.heads * p.pieces);
-  if (outputs)
-    hipLaunchKernelGGL((walk_kernel<T, D, WAVES, true, DIRECT>), grid,
-                       dim3(64 * WAVES), 0, stream, p);
-  else
-    hipLaunchKernelGGL((walk_kernel<T, D, WAVES, false, DIRECT>), grid,
-                       dim3(64 * WAVES), 0, stream, p);
+template <typename T, int D, int WAVES, bool OUTPUT, int RING>
+int launch_ring(const Problem& p, unsigned groups, hipStream_t stream) {
+  hipLaunchKernelGGL((walk_kernel<T, D, WAVES, OUTPUT, RING>), dim3(groups),
+                     dim3(64 * WAVES), 0, stream, p);
   SNN_HIP_CHECK_LAUNCH();
   return SNN_HIP_OK;
+}
+// The blocks of the ring.  LDS holds three of 128 keys, q and 128 values, and for walks
+// without q two work-groups of a CU with two each (outputs of 1 x 32768 steps of 16 heads
+// of 128 channels in bfloat16: 166 us while every block waited for the next as well, 149
+// with three under way).  Work-groups of four waves have two where they do not fill the
+// CUs three deep, otherwise one, loaded when the one before has been used.  (Heads of 64
+// channels in bfloat16, one and two: 8 x 2048 steps of 32 heads, one work-group a CU, 98
+// and 77 us; gradients of 1 x 16384 steps of 16 heads, up to three, 112 and 127 us.  fp32
+// heads of 128 channels, one work-group a CU: 105 and 107 us.)
+template <typename T, int D, int WAVES, bool OUTPUT, bool DIRECT>
+int launch_as(const Problem& p, hipStream_t stream) {
+  const unsigned groups =
+      static_cast<unsigned>(p.units) * p.batch * p.heads * p.pieces;
+  if constexpr (!DIRECT) {
+    return launch_ring<T, D, WAVES, OUTPUT, 0>(p, groups, stream);
+  } else if constexpr (WAVES == 8 && D <= 128) {
+    return launch_ring<T, D, WAVES, OUTPUT, OUTPUT ? 3 : 2>(p, groups, stream);
+  } else if constexpr (D > 64) {
+    return launch_ring<T, D, WAVES, OUTPUT, 1>(p, groups, stream);
+  } else {
+    return groups <= 512
+               ? launch_ring<T, D, WAVES, OUTPUT, 2>(p, groups, stream)
+               : launch_ring<T, D, WAVES, OUTPUT, 1>(p, groups, stream);
+  }
+}
+template <typename T, int D, int WAVES, bool DIRECT>
+int launch_walk(const Problem& p, bool outputs, hipStream_t stream) {
+  return outputs ? launch_as<T, D, WAVES, true, DIRECT>(p, stream)
+                 : launch_as<T, D, WAVES, false, DIRECT>(p, stream);
 }
 
 // Whether all walks' rows go straight to LDS and from registers in whole pieces.
