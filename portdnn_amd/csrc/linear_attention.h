@@ -282,11 +282,19 @@ __device__ __forceinline__ Part part_of(const Problem& p) {
 // D: the keys, rounded up; WAVES: of a work-group, with 16 values each.  STAGES: blocks
 // in a ring of LDS, to which rows of whole 16-byte pieces at aligned addresses go
 // straight; 0: rows pass through registers, where one block is under way.
-template <int D, int WAVES, bool OUTPUT>
-constexpr int kWavesOfSimd = D == 256     ? WAVES / 4
-                             : WAVES == 8 ? (OUTPUT ? 2 : 4)
-                             : OUTPUT     ? 3
-                                          : 4;
+//
+// Waves that share a SIMD's registers: as many as need not put many of their own into
+// memory.  (2 x 4096 steps of 16 heads of 127 x 63 in bfloat16, three and two: 174 and 69
+// us, gradients 353 and 169; of 128 x 64 64 and 57, 147 and 137.  fp32 gradients of 1 x
+// 8192 steps of 8 heads of 128 x 128: 212 and 228.)
+template <typename T, int D, int WAVES, bool OUTPUT, int RING>
+constexpr int kWavesOfSimd =
+    D == 256     ? WAVES / 4
+    : WAVES == 8 ? (OUTPUT || (D == 128 && RING == 0) ? 2 : 4)
+    : !OUTPUT    ? (D == 128 ? 3 : 4)
+    : RING == 2  ? 2
+    : D == 128   ? (sizeof(T) == 4 && RING == 1 ? 3 : 2)
+                 : 3;
 
 template <typename T, int D, int WAVES, bool OUTPUT, int RING>
 __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* ring1,
@@ -920,10 +928,10 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
       // (rows in front of a reset may hold a k that a weight of zero leaves infinite)
       if (resets != 0) {
 #pragma unroll
-        for (int piece = wave; piece < Keys::kPieces; piece += WAVES) {
+        for (int u = 0; u < Keys::kPieces / WAVES; ++u) {
           float x[kPer];
           Split<T>::floats(*reinterpret_cast<const uint4v*>(
-                               k_tile + Keys::at(lane % C, piece)),
+                               k_tile + Keys::at(lane % C, wave + u * WAVES)),
                            x);
 #pragma unroll
           for (int i = 0; i < kPer; ++i) clean_k = clean_k && x[i] * 0.f == 0.f;
@@ -1101,7 +1109,7 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
 }
 
 template <typename T, int D, int WAVES, bool OUTPUT, int RING>
-__global__ void __launch_bounds__(64 * WAVES, (kWavesOfSimd<D, WAVES, OUTPUT>))
+__global__ void __launch_bounds__(64 * WAVES, (kWavesOfSimd<T, D, WAVES, OUTPUT, RING>))
     walk_kernel(Problem p) {
 #ifdef __HIP_DEVICE_COMPILE__
   constexpr int E = sizeof(T), C = kBlock<T>;
