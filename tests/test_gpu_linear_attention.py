@@ -13,7 +13,8 @@ TYPES = [torch.float32, torch.float16, torch.bfloat16]
 # batch, steps, heads, key_heads, keys, values
 SIZES = [
     (2, 1, 2, 2, 16, 16), (3, 1, 6, 2, 200, 130), (2, 2, 1, 1, 1, 1),
-    (2, 16, 4, 2, 24, 40), (2, 17, 4, 2, 24, 40), (3, 33, 3, 1, 13, 21),
+    (2, 12, 4, 2, 24, 40), (2, 13, 4, 2, 24, 40), (2, 16, 4, 2, 24, 40),
+    (2, 17, 4, 2, 24, 40), (3, 33, 3, 1, 13, 21),
     (1, 64, 2, 2, 64, 64), (2, 65, 2, 2, 64, 128), (2, 63, 4, 2, 72, 100),
     (2, 129, 2, 1, 128, 128), (1, 90, 2, 2, 255, 37), (1, 130, 1, 1, 256, 256),
     (2, 100, 2, 2, 37, 255), (3, 70, 2, 2, 8, 3), (1, 450, 2, 1, 32, 48),
