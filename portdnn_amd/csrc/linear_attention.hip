@@ -319,7 +319,9 @@ Division divide(const snn_hip_linear_attention_params& p, int units, int block,
   };
   Division best = {1, blocks * block};
   double least = rounds_of(heads * units, of_cu) * (blocks + 4);
-  for (int want = 2; want <= std::min(blocks, kMostPieces); ++want) {
+  // (many work-groups fill the GPU evenly enough)
+  const int most = heads * units >= 8 * kCus ? 1 : std::min(blocks, kMostPieces);
+  for (int want = 2; want <= most; ++want) {
     const int each = ceil_div(blocks, want), pieces = ceil_div(blocks, each);
     if (pieces != want || need(pieces) > bytes) continue;
     // (of the gradients' three walks two leave states)

@@ -1029,7 +1029,7 @@ def rotary(x, frequencies, positions=None, layout=ROTARY.HALVES, magnitude=1.0,
     batch, steps, heads, channels = shape = x.shape
     dtype = x.dtype
     assert frequencies.dtype is torch.float64 and frequencies.dim() == 1 and \
-        frequencies.is_contiguous()
+        frequencies.is_contiguous() and frequencies.is_cuda == x.is_cuda
     kind = ROTARY_POSITIONS.NONE
     if positions is not None:
         kind = ROTARY_POSITIONS.FIRST

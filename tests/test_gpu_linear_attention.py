@@ -1,11 +1,13 @@
 """Linear attention and its gradients against 64 bits, and against itself where
 calls differ in ways that may not change a result."""
+import ctypes
+
 import pytest
 import torch
 
 import attention_reference as plain
 import sequence_reference as ref
-from portdnn_amd import ops
+from portdnn_amd import capi, ops
 
 pytestmark = pytest.mark.gpu
 
@@ -415,27 +417,46 @@ def test_streams_and_graphs(steps, dtype):
         run(both[1 - turn])  # eager work in between
 
 
-def test_parts_that_are_not_wanted():
+@pytest.mark.parametrize("groups", [4, 2])
+@pytest.mark.parametrize("steps", [9, 200])
+def test_parts_that_are_not_wanted(groups, steps):
     """Each gradient alone is what it is among the others."""
-    from portdnn_amd import capi
-    for steps in (9, 200):
-        size = (2, steps, 2, 2, 40, 40)
-        t, (do, ds) = _make(size, torch.float32)
-        gpu, do, ds = _cuda(t), do.cuda(), ds.cuda()
-        want = ops.linear_attention_grad(do, grad_final_state=ds, **gpu)
-        p = capi.LinearAttentionParams(batch=2, steps=steps, heads=2, key_heads=2,
-                                       keys=40, values=40, scale=1.0)
-        import ctypes
-        room = torch.empty(1 << 20, device="cuda")
-        for name, w in want.items():
-            got = torch.empty_like(w)
-            at = {n: got.data_ptr() if n == name else None for n in want}
-            capi.check(capi.lib().snn_hip_linear_attention_grad_f32(
-                do.data_ptr(), ds.data_ptr(), gpu["q"].data_ptr(),
-                gpu["k"].data_ptr(), gpu["v"].data_ptr(),
-                gpu["decay"].data_ptr(), None, None,
-                gpu["initial_state"].data_ptr(), at["q"], at["k"], at["v"],
-                at["initial_state"], ctypes.byref(p), room.data_ptr(),
-                room.numel(), None))
-            torch.cuda.synchronize()
-            assert torch.equal(got, w), name
+    t, (do, ds) = _make((2, steps, 4, groups, 40, 40), torch.float32)
+    gpu, do, ds = _cuda(t), do.cuda(), ds.cuda()
+    want = ops.linear_attention_grad(do, grad_final_state=ds, **gpu)
+    p = capi.LinearAttentionParams(batch=2, steps=steps, heads=4,
+                                   key_heads=groups, keys=40, values=40,
+                                   scale=1.0)
+    room = torch.empty(1 << 20, device="cuda")
+    for name, w in want.items():
+        got = torch.empty_like(w)
+        at = {n: got.data_ptr() if n == name else None for n in want}
+        capi.check(capi.lib().snn_hip_linear_attention_grad_f32(
+            do.data_ptr(), ds.data_ptr(), gpu["q"].data_ptr(),
+            gpu["k"].data_ptr(), gpu["v"].data_ptr(), gpu["decay"].data_ptr(),
+            None, None, gpu["initial_state"].data_ptr(), at["q"], at["k"],
+            at["v"], at["initial_state"], ctypes.byref(p), room.data_ptr(),
+            room.numel(), None))
+        torch.cuda.synchronize()
+        assert torch.equal(got, w), name
+
+
+@pytest.mark.parametrize("steps", [3, 100])
+@pytest.mark.parametrize("values", [24, 13])
+def test_states_at_any_address(steps, values):
+    """States that begin four bytes behind a multiple of sixteen."""
+    size = (2, steps, 2, 2, 40, values)
+    t, (do, ds) = _make(size, torch.bfloat16)
+    gpu, do, ds = _cuda(t), do.cuda(), ds.cuda()
+    want = ops.linear_attention(**gpu)
+    want_d = ops.linear_attention_grad(do, grad_final_state=ds, **gpu)
+
+    def moved(x):
+        y = torch.empty(x.numel() + 1, device="cuda")[1:].view(x.shape)
+        return y.copy_(x)
+
+    gpu["initial_state"] = moved(gpu["initial_state"])
+    got = ops.linear_attention(final_state=moved(ds), **gpu)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    got = ops.linear_attention_grad(do, grad_final_state=moved(ds), **gpu)
+    assert all(torch.equal(got[n], w) for n, w in want_d.items())
