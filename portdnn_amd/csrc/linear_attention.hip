@@ -220,22 +220,54 @@ __global__ void __launch_bounds__(256) chain_kernel(Chains p) {
 
 // ---- gradients of shared heads ---------------------------------------------------
 
-// out[row][g][c] = sum over the group's heads of in[row][g * share + i][c].
-template <typename T>
-__global__ void __launch_bounds__(256)
-    share_kernel(const float* __restrict__ in, T* __restrict__ out, size_t rows,
-                 long out_row, int groups, int share, int keys) {
-  const size_t size = static_cast<size_t>(groups) * keys;
-  for (size_t at = (blockIdx.x + static_cast<size_t>(blockIdx.y) *
-                                     seq::kGroupsOfX) * 256 + threadIdx.x;
-       at < rows * size;
-       at += static_cast<size_t>(gridDim.x) * gridDim.y * 256) {
-    const size_t row = at / size, rest = at - row * size;
-    const size_t g = rest / keys, c = rest - g * keys;
-    const float* const from = in + ((row * groups + g) * share) * keys + c;
-    float s = 0.f;
-    for (int i = 0; i < share; ++i) s += from[static_cast<long>(i) * keys];
-    out[row * out_row + rest] = static_cast<T>(s);
+// out[row][g][c] = sum over the group's heads of in[row][g * share + i][c], VEC
+// neighbouring c at a time, for q's and k's gradients beside one another.  Bound by
+// memory: bfloat16, 4 x 4096 steps of 16 heads of 128 channels, four of which share: 51
+// us for both, 302 MB, partly from the last cache (51 for each, one value at a time).
+struct Shared {
+  const float* in[2];
+  void* out[2];
+  long out_row[2];
+  size_t rows;
+  int groups, share, keys;
+};
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256) share_kernel(Shared p) {
+  const bool second = blockIdx.y != 0;
+  const float* const in = p.in[second];
+  T* const out = static_cast<T*>(p.out[second]);
+  const long out_row = p.out_row[second];
+  const unsigned pieces = static_cast<unsigned>(p.keys) / VEC;
+  const unsigned units = static_cast<unsigned>(p.groups) * pieces;
+  // (a lane's place goes on by the same rows and units of a row each time)
+  const size_t first = blockIdx.x * size_t{256} + threadIdx.x;
+  const size_t all = gridDim.x * size_t{256};
+  size_t row = first / units;
+  unsigned unit = static_cast<unsigned>(first - row * units);
+  const size_t on_rows = all / units;
+  const unsigned on_units = static_cast<unsigned>(all - on_rows * units);
+  while (row < p.rows) {
+    const unsigned g = unit / pieces, c = (unit - g * pieces) * VEC;
+    const float* const from =
+        in + ((row * p.groups + g) * p.share) * p.keys + c;
+    float sum[VEC] = {};
+    for (int i = 0; i < p.share; ++i) {
+      float x[VEC];
+      seq::unpack<float, VEC>(*reinterpret_cast<const typename Pack<float, VEC>::type*>(
+                                  from + static_cast<long>(i) * p.keys),
+                              x);
+#pragma unroll
+      for (int u = 0; u < VEC; ++u) sum[u] += x[u];
+    }
+    *reinterpret_cast<typename Pack<T, VEC>::type*>(
+        out + row * out_row + static_cast<long>(g) * p.keys + c) =
+        seq::pack<T, VEC>(sum);
+    row += on_rows;
+    unit += on_units;
+    if (unit >= units) {
+      unit -= units;
+      ++row;
+    }
   }
 }
 
@@ -538,15 +570,34 @@ int forward(const void* q, const void* k, const void* v, const float* decay,
 }
 
 template <typename T>
-int share_sum(const snn_hip_linear_attention_params& p, const float* in,
-              void* out, int stride, hipStream_t stream) {
+int share_sums(const snn_hip_linear_attention_params& p, const float* q_sums,
+               void* grad_q, const float* k_sums, void* grad_k, hipStream_t stream) {
   const long width = static_cast<long>(p.key_heads) * p.keys;
-  const size_t rows = static_cast<size_t>(p.batch) * p.steps;
-  const size_t groups = std::min<size_t>(
-      ceil_div(rows * static_cast<size_t>(width), size_t{256}), 1u << 20);
-  hipLaunchKernelGGL(share_kernel<T>, seq::grid_of(groups), dim3(256), 0, stream,
-                     in, static_cast<T*>(out), rows, or_else(stride, width),
-                     p.key_heads, p.heads / p.key_heads, p.keys);
+  Shared g = {};
+  unsigned n = 0;
+  auto add = [&](const float* in, void* out, int stride) {
+    if (in == nullptr) return;
+    g.in[n] = in;
+    g.out[n] = out;
+    g.out_row[n++] = or_else(stride, width);
+  };
+  add(q_sums, grad_q, p.grad_q_stride);
+  add(k_sums, grad_k, p.grad_k_stride);
+  g.rows = static_cast<size_t>(p.batch) * p.steps;
+  g.groups = p.key_heads;
+  g.share = p.heads / p.key_heads;
+  g.keys = p.keys;
+  const int vec = p.keys % 4 == 0 ? 4 : 1;
+  const dim3 grid(static_cast<unsigned>(std::min<size_t>(
+                      ceil_div(g.rows * static_cast<size_t>(width) / vec,
+                               size_t{256}),
+                      4096)),
+                  n);
+  if (n == 0) return SNN_HIP_OK;
+  if (vec == 4)
+    hipLaunchKernelGGL((share_kernel<T, 4>), grid, dim3(256), 0, stream, g);
+  else
+    hipLaunchKernelGGL((share_kernel<T, 1>), grid, dim3(256), 0, stream, g);
   SNN_HIP_CHECK_LAUNCH();
   return SNN_HIP_OK;
 }
@@ -684,10 +735,7 @@ int backward(const void* grad, const float* grad_final, const void* q,
   if (grad_k != nullptr) walks[n++] = of_k;
   if (grad_v != nullptr || grad_initial != nullptr) walks[n++] = of_v;
   int s = run_all<T>(base, walks, n, true, stream);
-  if (s == SNN_HIP_OK && q_sums != nullptr)
-    s = share_sum<T>(p, q_sums, grad_q, p.grad_q_stride, stream);
-  if (s == SNN_HIP_OK && k_sums != nullptr)
-    s = share_sum<T>(p, k_sums, grad_k, p.grad_k_stride, stream);
+  if (s == SNN_HIP_OK) s = share_sums<T>(p, q_sums, grad_q, k_sums, grad_k, stream);
   return s;
 }
 
