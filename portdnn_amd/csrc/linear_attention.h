@@ -46,11 +46,11 @@
 // The 16-bit types: q_r k_s and its decay are rounded to the type, once, as an output
 // is: a product of two more values would cost as much again.  The state is held in two
 // values of the type for q X (an output is rounded to 8 or 11 bits of the sum), and the
-// weighted v in as many as fp32 has bits, as the states are fp32 results.
+// weighted v in three (binary16: two, of 22 bits together), as states are fp32 results.
 // Rows that may not count, those of later steps and those in front of a reset, are left
 // out by selection.  The matrix instructions would multiply their v by zero, which an
-// infinity or NaN survives: blocks that hold one (a product with zero tells) are
-// summed value by value instead.
+// infinity or NaN survives: where there is one (a product with zero tells) they are
+// summed value by value instead, in a second walk of the work-group's piece.
 #ifndef PORTDNN_AMD_CSRC_LINEAR_ATTENTION_H_
 #define PORTDNN_AMD_CSRC_LINEAR_ATTENTION_H_
 
