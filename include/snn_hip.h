@@ -1045,7 +1045,8 @@ SNN_HIP_API int snn_hip_linear_attention_bf16(
  * strides of their own and are zero from a sequence's length on; each of the four
  * outputs may be NULL and is then not computed.  No output may overlap an input.
  * Where key_heads is not heads, the sums over the heads that share a query or key
- * take workspace: SNN_HIP_INSUFFICIENT_WORKSPACE without the required size.  (In
+ * take workspace: SNN_HIP_INSUFFICIENT_WORKSPACE without the required size; more than
+ * 2^23 channels of all heads' keys are then SNN_HIP_INDEX_EXCEEDED.  (In
  * binary16 scale times a query or a value of grad_output is infinite beyond 65504 on
  * its way into the states.) */
 SNN_HIP_API int snn_hip_linear_attention_grad_f32(

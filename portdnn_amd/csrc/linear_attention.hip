@@ -302,6 +302,19 @@ int check(const snn_hip_linear_attention_params* p, const void* workspace) {
     return SNN_HIP_INDEX_EXCEEDED;
   return SNN_HIP_OK;
 }
+// ... and of the gradients: where heads share queries and keys, a row of their fp32
+// sums is that of all heads, and a block's rows of them are counted in 31 bits of
+// bytes as well.
+int check_grad(const snn_hip_linear_attention_params* p, const void* workspace) {
+  const int valid = check(p, workspace);
+  if (valid != SNN_HIP_OK) return valid;
+  constexpr long kMostSums = 1 << 23;
+  static_assert(63 * kMostSums * 4 + 1024 < 0x7FFFFFF0l, "beyond a buffer's range");
+  if (p->heads != p->key_heads &&
+      static_cast<long>(p->heads) * p->keys > kMostSums)
+    return SNN_HIP_INDEX_EXCEEDED;
+  return SNN_HIP_OK;
+}
 
 long or_else(int stride, long row) { return stride == 0 ? row : stride; }
 size_t round16(size_t bytes) { return (bytes + 15) / 16 * 16; }
@@ -609,7 +622,7 @@ int backward(const void* grad, const float* grad_final, const void* q,
              const float* initial, void* grad_q, void* grad_k, void* grad_v,
              float* grad_initial, const snn_hip_linear_attention_params* params,
              void* workspace, size_t elems, void* stream_arg) {
-  const int valid = check(params, workspace);
+  const int valid = check_grad(params, workspace);
   if (valid != SNN_HIP_OK) return valid;
   const snn_hip_linear_attention_params& p = *params;
   SNN_REQUIRE(grad != nullptr && q != nullptr && k != nullptr && v != nullptr &&
@@ -779,7 +792,8 @@ int snn_hip_linear_attention_workspace_size(
   if (dtype < SNN_HIP_DTYPE_F32 || dtype > SNN_HIP_DTYPE_BF16 ||
       required_elems == nullptr || recommended_elems == nullptr)
     return SNN_HIP_INVALID_PARAMETER;
-  const int valid = snn::check(params, nullptr);
+  const int valid = grad != 0 ? snn::check_grad(params, nullptr)
+                              : snn::check(params, nullptr);
   if (valid != SNN_HIP_OK) return valid;
   const int size = dtype == SNN_HIP_DTYPE_F32 ? 4 : 2;
   size_t all = 0;

@@ -231,6 +231,36 @@ def test_attention_refusals(suffix):
     assert _attention_grad(suffix, p) == STATUS.INSUFFICIENT_WORKSPACE
 
 
+@pytest.mark.parametrize("suffix", TYPES)
+@pytest.mark.parametrize("heads,key_heads,keys,values", [
+    (65536, 1, 256, 16), (65536, 16384, 256, 8), (32769, 1, 256, 16),
+    (1 << 20, 1, 9, 1)])
+def test_attention_sums_of_many_heads(suffix, heads, key_heads, keys, values):
+    """A row of the sums over heads that share queries and keys holds heads * keys
+    floats: beyond 2^23 of them a block's rows pass 31 bits of bytes."""
+    p = _attention_params(batch=1, heads=heads, key_heads=key_heads, keys=keys,
+                          values=values)
+    entry = capi.lib().snn_hip_linear_attention_workspace_size
+    code = getattr(DTYPE, suffix.upper())
+    size = ctypes.c_size_t()
+    out = ctypes.byref(size)
+
+    def required(grad):
+        return entry(ctypes.byref(p), grad, code, out, out)
+
+    assert _attention_grad(suffix, p) == STATUS.INDEX_EXCEEDED
+    assert required(1) == STATUS.INDEX_EXCEEDED
+    # the forward call has no such sums
+    assert required(0) == STATUS.OK
+    # the largest row that is counted in 31 bits: the workspace is what is missing
+    p.heads = (1 << 23) // keys // key_heads * key_heads
+    assert _attention_grad(suffix, p) == STATUS.INSUFFICIENT_WORKSPACE
+    assert required(1) == STATUS.OK
+    if key_heads == 1:  # heads that share nothing: none
+        p.heads = p.key_heads = (1 << 22) // keys
+        assert required(1) == STATUS.OK
+
+
 def test_attention_workspace():
     name = "snn_hip_linear_attention_workspace_size"
     entry = getattr(capi.lib(), name)
