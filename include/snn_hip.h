@@ -1001,9 +1001,10 @@ SNN_HIP_API int snn_hip_rotary_frequencies(int turned, double base, int scaling,
  * A few steps are taken one after the other, more in blocks: of each block of steps
  * the products q_t k_s, weighted by their decays, and the states come from the
  * matrix instructions.  These take scale q_t k_s rounded to the data type (in
- * binary16: infinite beyond 65504), states as sums of two values of the data type and
- * weighted values as sums of two of binary16 or three of bfloat16; sums and states
- * are fp32.  Long sequences are divided into pieces that run beside one another, given
+ * binary16: infinite beyond 65504, in steps of 2^-24 below 2^-14), states as sums of two
+ * values of the data type and weighted values as sums of two of binary16, at a range for
+ * each of the values' channels in a block, or three of bfloat16; sums and states are
+ * fp32.  Long sequences are divided into pieces that run beside one another, given
  * a workspace of the recommended size.  The order of operations is fixed by the sizes and the
  * workspace.  At most 256 channels of a key or a value; more than 2^30 steps, 2^20
  * heads of all sequences or 2^22 elements from step to step are
@@ -1046,9 +1047,7 @@ SNN_HIP_API int snn_hip_linear_attention_bf16(
  * outputs may be NULL and is then not computed.  No output may overlap an input.
  * Where key_heads is not heads, the sums over the heads that share a query or key
  * take workspace: SNN_HIP_INSUFFICIENT_WORKSPACE without the required size; more than
- * 2^23 channels of all heads' keys are then SNN_HIP_INDEX_EXCEEDED.  (In
- * binary16 scale times a query or a value of grad_output is infinite beyond 65504 on
- * its way into the states.) */
+ * 2^23 channels of all heads' keys are then SNN_HIP_INDEX_EXCEEDED. */
 SNN_HIP_API int snn_hip_linear_attention_grad_f32(
     const void* grad_output, const float* grad_final_state, const void* q,
     const void* k, const void* v, const float* decay,

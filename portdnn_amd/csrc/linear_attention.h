@@ -46,7 +46,8 @@
 // The 16-bit types: q_r k_s and its decay are rounded to the type, once, as an output
 // is: a product of two more values would cost as much again.  The state is held in two
 // values of the type for q X (an output is rounded to 8 or 11 bits of the sum), and the
-// weighted v in three (binary16: two, of 22 bits together), as states are fp32 results.
+// weighted v in three, as states are fp32 results (binary16: two, of 22 bits together,
+// where a value's column of the block takes a power of two into the type's range).
 // Rows that may not count, those of later steps and those in front of a reset, are left
 // out by selection.  The matrix instructions would multiply their v by zero, which an
 // infinity or NaN survives: where there is one (a product with zero tells) they are
@@ -662,6 +663,22 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
     }
   };
 
+  // The power of two that brings the largest value of a column of the wave's, of which
+  // each lane has seen a part, close to binary16's largest; returns its inverse.
+  auto range_of = [&](float most, float* scale) {
+    // (rows of 16 lanes change places with their neighbours', halves with each other)
+    const unsigned bits = __float_as_uint(most);
+    const auto rows = __builtin_amdgcn_permlane16_swap(bits, bits, false, false);
+    most = fmaxf(__uint_as_float(rows[0]), __uint_as_float(rows[1]));
+    const unsigned pair = __float_as_uint(most);
+    const auto halves = __builtin_amdgcn_permlane32_swap(pair, pair, false, false);
+    most = fmaxf(__uint_as_float(halves[0]), __uint_as_float(halves[1]));
+    const int exponent =
+        min(126, max(-100, static_cast<int>(__float_as_uint(most) >> 23) - 141));
+    *scale = __uint_as_float(static_cast<unsigned>(127 - exponent) << 23);
+    return __uint_as_float(static_cast<unsigned>(127 + exponent) << 23);
+  };
+
   // One block, whose rows are in `tile`.
   // CAREFUL: rows that do not count are left out one by one; otherwise by weights of
   // zero, after which `clean` tells whether that was enough.
@@ -764,12 +781,31 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
     }
 
     uint4v v_part[SB];
+    auto weighted = [&](int b, float (&x)[kPer]) {
+      Split<T>::floats(v_part[b], x);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        x[i] *= into_state[b * KB + group * (KB / 4) + i];
+    };
+    constexpr bool kScaled = std::is_same<T, _Float16>::value;
+    float range = 1.f, range_back = 1.f;  // of the weighted values
     auto fetch_v = [&] {
 #pragma unroll
       for (int b = 0; b < SB; ++b) {
         v_part[b] = Values::fragment(v_tile, down_v, b);
         if (!CAREFUL)
           clean = epi::multiply<T>(v_part[b], uint4v{0u, 0u, 0u, 0u}, clean);
+      }
+      if constexpr (kScaled && !CAREFUL) {
+        float most = 0.f;
+#pragma unroll
+        for (int b = 0; b < SB; ++b) {
+          float x[kPer];
+          weighted(b, x);
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) most = fmaxf(most, fabsf(x[i]));
+        }
+        range_back = range_of(most, &range);
       }
     };
     if constexpr (!OUTPUT) fetch_v();
@@ -787,14 +823,7 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
             const float x = fabsf(state[i][r]);
             most = x < INFINITY ? fmaxf(most, x) : most;
           }
-        most = fmaxf(most, __shfl_xor(most, 16));
-        most = fmaxf(most, __shfl_xor(most, 32));
-        const int exponent = min(
-            126,
-            max(-100, static_cast<int>(__float_as_uint(most) >> 23) - 141));
-        scale = __uint_as_float(static_cast<unsigned>(127 - exponent) << 23);
-        const float back =
-            __uint_as_float(static_cast<unsigned>(127 + exponent) << 23);
+        const float back = range_of(most, &scale);
 #pragma unroll
         for (int r = 0; r < 4; ++r) unscale[r] = __shfl(back, 4 * group + r);
       }
@@ -950,43 +979,70 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
       // (weighted values in full, as the states that leave the kernel are fp32.  With two
       // parts of bfloat16 these were off by 2.4e-6 instead of 2e-7, and 1 x 32768 steps of
       // 16 heads of 128 channels took 215 us instead of 224)
+      // (binary16: a value's column times a power of two, which its sums of the block
+      // lose again, as the second part of small values would be below the type's
+      // smallest: gradients of 1e-3 left states that were off by 4e-4.  1 x 32768 steps of
+      // 16 heads of 128 channels 270 us, 247 without; 64 x 512 of 64 channels 84 and 81)
       constexpr int kParts = Split<T>::kWhole;
       uint4v parts[SB][kParts];
 #pragma unroll
       for (int b = 0; b < SB; ++b) {
+        if (kScaled) asm volatile("" : "+v"(v_part[b]));  // (worked out again, not kept)
         float x[kPer];
-        Split<T>::floats(v_part[b], x);
+        weighted(b, x);
 #pragma unroll
         for (int i = 0; i < kPer; ++i)
-          x[i] *= into_state[b * KB + group * (KB / 4) + i];
+          if (kScaled) x[i] *= range;
         Split<T>::split(x, parts[b]);
       }
       // (two tiles' fragments are read while those before are multiplied, and no more of
-      // them: they would take the registers that the loads' and sums' need)
-      uint4v of_k[2][2][SB];
+      // them: they would take the registers that the loads' and sums' need.  Scaled sums
+      // join the state while the next are multiplied; without outputs, where twice as many
+      // waves share a SIMD's registers, a tile at a time and at once)
+      constexpr bool kFewer = kScaled && !OUTPUT;
+      constexpr int kStep = kFewer ? 1 : 2, kBehind = kFewer ? 0 : kStep;
+      uint4v of_k[2][kStep][SB];
+      float4v sums[2][kStep];
       auto fetch = [&](int i) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < kStep; ++u)
 #pragma unroll
           for (int b = 0; b < SB; ++b)
-            of_k[i / 2 % 2][u][b] = Keys::columns(k_tile, down_k, (i + u) / HALVES,
-                                                  (i + u) % HALVES, b);
+            of_k[i / kStep % 2][u][b] = Keys::columns(
+                k_tile, down_k, (i + u) / HALVES, (i + u) % HALVES, b);
+      };
+      auto join = [&](int i) {
+#pragma unroll
+        for (int u = 0; u < kStep; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            state[i + u][r] += range_back * sums[i / kStep % 2][u][r];
       };
       fetch(0);
 #pragma unroll
-      for (int i = 0; i < D / 16; i += 2) {
-        if (i + 2 < D / 16) fetch(i + 2);
+      for (int i = 0; i < D / 16; i += kStep) {
+        if (i + kStep < D / 16) fetch(i + kStep);
         __builtin_amdgcn_sched_barrier(0);
+        float4v (&to)[kStep] = sums[i / kStep % 2];
+#pragma unroll
+        for (int u = 0; u < kStep; ++u)
+          to[u] = kScaled ? float4v{0.f, 0.f, 0.f, 0.f} : state[i + u];
 #pragma unroll
         for (int b = 0; b < SB; ++b)
 #pragma unroll
           for (int part = 0; part < kParts; ++part)
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
-              state[i + u] = epi::multiply<T>(of_k[i / 2 % 2][u][b], parts[b][part],
-                                              state[i + u]);
+            for (int u = 0; u < kStep; ++u)
+              to[u] = epi::multiply<T>(of_k[i / kStep % 2][u][b], parts[b][part], to[u]);
+        if constexpr (kScaled) {
+          if (i >= kBehind) join(i - kBehind);
+        } else {
+#pragma unroll
+          for (int u = 0; u < kStep; ++u) state[i + u] = to[u];
+        }
         __builtin_amdgcn_sched_barrier(0);
       }
+      if constexpr (kScaled && kBehind > 0) join(D / 16 - kBehind);
     } else {
       const int value = wave * 16 + c16;
       for (int r = 0; r < n; ++r) {
