@@ -87,7 +87,8 @@ __global__ void __launch_bounds__(256) few_steps_kernel(Few p) {
     q_of[t][key] = in ? static_cast<float>(q[t * p.q_row + key]) : 0.f;
     k_of[t][key] = in ? static_cast<float>(k[t * p.k_row + key]) : 0.f;
   }
-  const float a = expf(att::log_decay(p.decay, h));
+  // (above zero, as in the walks over blocks)
+  const float a = expf(att::log_decay(p.decay, h)) + 0x1p-126f;
   __syncthreads();
   for (int t = 0; t < length; ++t) {
     float x[4] = {};
