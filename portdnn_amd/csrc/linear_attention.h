@@ -228,13 +228,21 @@ struct Split {
   static constexpr int N = 16 / sizeof(T);
   static constexpr int kWhole = sizeof(T) == 4 ? 1 : std::is_same<T, _Float16>::value ? 2 : 3;
   typedef T V __attribute__((ext_vector_type(N)));
-  template <int PARTS>
+  // ANY: values that are infinite, which leave nothing, and that would be when rounded.
+  template <bool ANY = false, int PARTS>
   static __device__ __forceinline__ void split(float (&v)[N], uint4v (&parts)[PARTS]) {
+    constexpr float kMost = std::is_same<T, _Float16>::value ? 65504.f : 0x1.fep127f;
 #pragma unroll
     for (int p = 0; p < PARTS; ++p) {
       V t;
 #pragma unroll
       for (int i = 0; i < N; ++i) t[i] = static_cast<T>(v[i]);
+      if constexpr (ANY && PARTS > 1) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (fabsf(v[i]) < INFINITY && fabsf(v[i]) > kMost)
+            t[i] = static_cast<T>(copysignf(kMost, v[i]));
+      }
       parts[p] = __builtin_bit_cast(uint4v, t);
       if (p + 1 == PARTS) break;
       // (the rounded values themselves: worked out anew from a product, with one
@@ -242,7 +250,10 @@ struct Split {
       asm volatile("" : "+v"(parts[p]));
       t = __builtin_bit_cast(V, parts[p]);
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] -= static_cast<float>(t[i]);
+      for (int i = 0; i < N; ++i) {
+        const float rest = v[i] - static_cast<float>(t[i]);
+        v[i] = ANY && fabsf(v[i]) == INFINITY ? 0.f : rest;
+      }
     }
   }
   static __device__ __forceinline__ void floats(uint4v f, float (&v)[N]) {
@@ -684,6 +695,24 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
   // zero, after which `clean` tells whether that was enough.
   float4v clean = {0.f, 0.f, 0.f, 0.f};  // stays zero while every v is finite
   bool clean_k = true;
+  // (... and while no state is infinite or would be when rounded: what the first of its
+  // two values leaves is no number then.  Looked at in front of a reset and behind the
+  // last block, as what is infinite stays so in between; bfloat16, which rounds the largest
+  // states to infinity, also in front of the first)
+  auto look = [&] {
+    if constexpr (OUTPUT && E == 2) {
+      unsigned most = 0;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          most = max(most, __float_as_uint(fabsf(state[i][r])));
+      if (most >= __float_as_uint(0x1.ffp127f)) clean[0] = NAN;
+    }
+  };
+  auto look_first = [&] {
+    if constexpr (std::is_same<T, __bf16>::value) look();
+  };
   auto walk = [&](const char* tile, int place, auto careful, auto next) {
     constexpr bool CAREFUL = decltype(careful)::value;
     // (two tables in turn: waves may still read the ones of the block before)
@@ -845,7 +874,7 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
         for (int i = 0; i < 4 * HALVES; ++i)
           x[i] = state[b * HALVES + i / 4][i % 4] * scale;
         uint4v parts[E == 4 ? 1 : 2];
-        Split<T>::split(x, parts);
+        Split<T>::template split<CAREFUL>(x, parts);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (const uint4v& part : parts)
@@ -950,6 +979,7 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
     // The state behind the block.
     carried = carried && all_resets == 0;
     const float carry = power[n];
+    if (!CAREFUL && all_resets != 0) look();
 #pragma unroll
     for (int i = 0; i < D / 16; ++i)
 #pragma unroll
@@ -1072,6 +1102,7 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
       issue(place, ring0);
       __builtin_amdgcn_s_waitcnt(epi::vmcnt_imm(0));
       asm volatile("" ::: "memory");
+      if (place == first) look_first();
       walk(ring0, place, kFast, [] {});
       __syncthreads();  // the tiles have been read
     }
@@ -1083,6 +1114,7 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
     // (the state has come: the compiler would wait for it inside of the loop, in every
     // block, and so for the blocks under way)
     __builtin_amdgcn_s_waitcnt(epi::vmcnt_imm(0));
+    look_first();
     auto step = [&](int place, int u) {
       // (loads come in order: where no more accesses are under way than the loads of the
       // blocks behind, the block's own have come, whatever has become of stores)
@@ -1104,6 +1136,7 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
       load(first);
     }
     for (int place = first; place < last; place += C) {
+      if (place == first) look_first();
       put(place, ring0);
       walk(ring0, place, kFast, [&] {
         if (place + C < last) {
@@ -1115,6 +1148,7 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
     }
   }
   // Values that are not finite: once more, and with care.
+  look();
   const bool all_clean = clean_k && clean[0] == 0.f && clean[1] == 0.f &&
                          clean[2] == 0.f && clean[3] == 0.f;
   if (__builtin_amdgcn_readfirstlane(__syncthreads_and(all_clean)) == 0) {

@@ -11,8 +11,11 @@ from test_gpu_linear_attention import TYPES, _cuda, _make, _wide
 pytestmark = pytest.mark.gpu
 
 INF = float("inf")
-# batch, steps, heads, key_heads, keys, values: up to 12 steps
-SIZES = [(1, 5, 2, 2, 24, 40), (2, 12, 2, 2, 100, 72)]
+# batch, steps, heads, key_heads, keys, values: up to 12 steps, blocks, pieces; each
+# way into LDS, four waves and eight
+SIZES = [(1, 5, 2, 2, 24, 40), (2, 12, 2, 2, 100, 72), (1, 200, 2, 2, 24, 40),
+         (2, 130, 2, 2, 37, 53), (1, 450, 1, 1, 64, 128), (1, 385, 1, 1, 128, 48),
+         (1, 130, 1, 1, 256, 256), (2, 90, 1, 1, 200, 40), (1, 450, 1, 1, 128, 128)]
 KEY, VALUE = 7, 11
 
 
@@ -56,3 +59,49 @@ def test_initial_states(size, dtype, decay, sign):
         else:
             ref.check(o[:, reset:], [x[:, reset:] for x in want[0]], count)
         ref.check(got, want[1], plain.state_operations(max(size[4:]), dtype))
+
+
+@pytest.mark.parametrize("size", SIZES)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gradients(size, dtype):
+    """A state in front that is infinite has it in a channel of q's gradient, the
+    gradient of the state behind in one of k's, one of v's and its own."""
+    t, (do, ds) = _make(size, dtype)
+    for x in (t["k"], t["v"], do):
+        x[x == 0] = 1.0
+    bad = {**t, "initial_state": t["initial_state"].clone()}
+    bad["initial_state"][:, :, KEY, VALUE] = INF
+    bad_ds = ds.clone()
+    bad_ds[:, :, KEY, VALUE] = -INF
+    got = ops.linear_attention_grad(do.cuda(), grad_final_state=bad_ds.cuda(),
+                                    **_cuda(bad))
+    want = plain.attention_grad(do.double(), grad_final_state=ds.double(),
+                                dtype=dtype, **_wide(t))
+    _signs(got["q"][..., KEY], do[..., VALUE], 1.0)
+    _signs(got["k"][..., KEY], t["v"][..., VALUE], -1.0)
+    _signs(got["v"][..., VALUE], t["k"][..., KEY], -1.0)
+    assert (got["initial_state"][:, :, KEY, VALUE] == -INF).all()
+    most = max(size[4:])
+    for name, at in (("q", KEY), ("k", KEY), ("v", VALUE)):
+        part = [c for c in range(got[name].shape[3]) if c != at]
+        ref.check(got[name][..., part], [x[..., part] for x in want[name]],
+                  plain.operations(most, dtype), name)
+    first = got["initial_state"].cpu()
+    first[:, :, KEY, VALUE] = want["initial_state"][0][:, :, KEY, VALUE].float()
+    ref.check(first, want["initial_state"], plain.state_operations(most, dtype))
+
+
+@pytest.mark.parametrize("size", SIZES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("value", [3.4e38, -3.3999e38])
+def test_states_that_rounding_would_make_infinite(size, dtype, value):
+    """fp32 values beyond the largest of bfloat16."""
+    t, _ = _make(size, dtype)
+    t["initial_state"][:, :, KEY, VALUE] = value
+    # (at most 1e34 of a state that large, in front of the scale)
+    t["q"][..., KEY] = (t["q"][..., KEY].float() * 1e-5).to(dtype)
+    o, last = ops.linear_attention(scale=0.5, **_cuda(t))
+    want = plain.attention(scale=0.5, dtype=dtype, **_wide(t))
+    most = max(size[4:])
+    ref.check(o, want[0], plain.operations(most, dtype))
+    ref.check(last, want[1], plain.state_operations(most, dtype))
