@@ -1085,8 +1085,9 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
                                k_tile + Keys::at(r, 4 * b + group)),
                            of_k);
 #pragma unroll
-          for (int i = 0; i < kPer; ++i)
-            state[b * HALVES + i / 4][i % 4] += x * of_k[i];
+          for (int i = 0; i < kPer; ++i)  // (keys that do not exist stay zero)
+            if (b * KB + group * kPer + i < w.keys)
+              state[b * HALVES + i / 4][i % 4] += x * of_k[i];
         }
       }
     }

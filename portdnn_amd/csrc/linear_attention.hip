@@ -107,10 +107,12 @@ __global__ void __launch_bounds__(256) few_steps_kernel(Few p) {
     for (int i = 0; i < R; ++i) {
       const float key = k_of[t][first_key + 16 * i];
       const float query = q_of[t][first_key + 16 * i];
+      // (keys that do not exist hold zeros, also beside an infinite v)
+      const bool in = first_key + 16 * i < p.keys;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        state[i][c] = key * x[c] + (fresh ? 0.f : a * state[i][c]);
-        // (keys that do not exist hold zeros)
+        const float now = key * x[c] + (fresh ? 0.f : a * state[i][c]);
+        state[i][c] = in ? now : 0.f;
         sum[c] += query * state[i][c];
       }
     }

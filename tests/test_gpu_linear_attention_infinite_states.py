@@ -91,6 +91,28 @@ def test_gradients(size, dtype):
     ref.check(first, want["initial_state"], plain.state_operations(most, dtype))
 
 
+@pytest.mark.parametrize("steps", [5, 12, 13, 70, 200, 900])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("keys,values", [(1, 5), (1, 64), (3, 72), (65, 9), (130, 130)])
+def test_values(steps, dtype, keys, values):
+    """Queries and keys above zero and an infinite value: keys that pad a head take
+    nothing from it."""
+    g = torch.Generator().manual_seed(steps + keys)
+    q = (0.5 + torch.rand(1, steps, 1, keys, generator=g)).to(dtype)
+    k = (0.5 + torch.rand(1, steps, 1, keys, generator=g)).to(dtype)
+    v = torch.randn(1, steps, 1, values, generator=g).to(dtype)
+    at = steps // 2
+    v[0, at, 0, 2] = -INF
+    o, last = ops.linear_attention(q.cuda(), k.cuda(), v.cuda(),
+                                   torch.tensor([-0.02]).cuda())
+    o, last = o.float().cpu(), last.cpu()
+    assert (o[0, at:, 0, 2] == -INF).all()
+    assert (last[0, 0, :, 2] == -INF).all()
+    o[0, at:, 0, 2] = 0.0
+    last[0, 0, :, 2] = 0.0
+    assert torch.isfinite(o).all() and torch.isfinite(last).all()
+
+
 @pytest.mark.parametrize("size", SIZES)
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("value", [3.4e38, -3.3999e38])
