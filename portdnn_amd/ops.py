@@ -1035,8 +1035,10 @@ def rotary(x, frequencies, positions=None, layout=ROTARY.HALVES, magnitude=1.0,
         kind = ROTARY_POSITIONS.FIRST
         if positions.dim() != 1:
             kind = ROTARY_POSITIONS.EACH
-        assert positions.dtype is torch.int32 and positions.is_contiguous() and \
+        assert positions.dim() in (1, 2) and \
             positions.shape == shape[:positions.dim()]
+        assert positions.dtype is torch.int32 and positions.is_contiguous() and \
+            positions.is_cuda == x.is_cuda
     stride = _head_stride(x)
     if out is None:
         out = x.new_empty(shape)

@@ -316,3 +316,12 @@ def test_python_refusals():
                 dict(w_up=normal(4, 10)[:, :5])):
         with pytest.raises(AssertionError):
             ops.gated_matmul(**{**dict(a=a, w_gate=w, w_up=w), **bad})
+
+
+@pytest.mark.parametrize("size", [(), (2, 5, 2), (2, 5, 2, 8), (2, 5, 2, 8, 1)])
+def test_positions_of_anything_but_sequences_or_tokens(size):
+    """They would be read as the tokens', which one number for all is too short for."""
+    x = torch.zeros(2, 5, 2, 8)
+    table = torch.zeros(4, dtype=torch.float64)
+    with pytest.raises(AssertionError):
+        ops.rotary(x, table, positions=torch.zeros(size, dtype=torch.int32))
