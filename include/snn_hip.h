@@ -869,7 +869,8 @@ SNN_HIP_API int snn_hip_gated_matmul_bf16(
  * weights' gradients are stored as those are, without a stride; each of the five
  * may be NULL and is then not computed.  lhs is needed for the weights' gradients
  * and both weights for grad_lhs only.  The gradients of the two factors, rounded to
- * the data type, and the biases' sums take workspace:
+ * the data type (in binary16: infinite beyond 65504, in steps of 2^-24 below 2^-14),
+ * and the biases' sums take workspace:
  * SNN_HIP_INSUFFICIENT_WORKSPACE without the required size. */
 SNN_HIP_API int snn_hip_gated_matmul_grad_f32(
     const void* grad_output, const void* lhs, const void* gate_weight,
@@ -894,6 +895,13 @@ SNN_HIP_API int snn_hip_gated_matmul_grad_bf16(
 SNN_HIP_API int snn_hip_gated_matmul_workspace_size(
     const snn_hip_gated_matmul_params* params, int grad, int dtype,
     size_t* required_elems, size_t* recommended_elems);
+/* Diagnostics for tests of the kernels, as snn_hip_matmul_bias_act_planned: `product`
+ * is 0 for the forward call, 1 for grad_lhs and 2 for a weight's gradient of a call for
+ * all five gradients.  tile_cols are those of both weights together (0), and both
+ * weights or both factors are copied or neither is. */
+SNN_HIP_API int snn_hip_gated_matmul_planned(
+    const snn_hip_gated_matmul_params* params, int product, int dtype,
+    int aligned, size_t workspace_elems, snn_hip_matmul_bias_act_plan* plan);
 
 /* Positions by rotation.  Of each head's `channels` the first `turned` form pairs
  * (a, b), channel i with i + turned / 2 (HALVES) or 2 i with 2 i + 1 (PAIRS), and

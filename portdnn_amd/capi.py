@@ -277,6 +277,7 @@ SIGNATURES = {
         _P, _I, ctypes.POINTER(_SZ), ctypes.POINTER(_SZ)],
     "snn_hip_gated_matmul_workspace_size": [
         _P, _I, _I, ctypes.POINTER(_SZ), ctypes.POINTER(_SZ)],
+    "snn_hip_gated_matmul_planned": [_P, _I, _I, _I, _SZ, _P],
     "snn_hip_rotary_frequencies": [
         _I, ctypes.c_double, _I] + [ctypes.c_double] * 4 + [_P],
     "snn_hip_linear_attention_workspace_size": [

@@ -380,4 +380,60 @@ int snn_hip_gated_matmul_workspace_size(
   return SNN_HIP_OK;
 }
 
+int snn_hip_gated_matmul_planned(
+    const snn_hip_gated_matmul_params* params, int product, int dtype,
+    int aligned, size_t workspace_elems, snn_hip_matmul_bias_act_plan* plan) {
+  if (dtype < SNN_HIP_DTYPE_F32 || dtype > SNN_HIP_DTYPE_BF16 || product < 0 ||
+      product > 2 || plan == nullptr)
+    return SNN_HIP_INVALID_PARAMETER;
+  const int size = snn::elem_size(dtype);
+  const int v = snn::check(params, size, nullptr);
+  if (v != SNN_HIP_OK) return v;
+  const bool at16 = aligned != 0;
+  size_t bytes = workspace_elems * size;
+  if (product > 0) {
+    const snn::GradSpace s = snn::grad_space(*params, size);
+    if (bytes < 2 * s.factor + s.sums) return SNN_HIP_INSUFFICIENT_WORKSPACE;
+    bytes -= 2 * s.factor + s.sums;
+  }
+  if (product == 2) {
+    const snn::epi::Product g =
+        snn::weight_product(*params, size, nullptr, nullptr);
+    // (the factor's gradient is in the workspace)
+    const bool first = params->transpose_rhs != 0;
+    const snn::epi::Plan p =
+        snn::epi::make_plan(g, size, bytes, first || at16, !first || at16);
+    if (p.splits == 0) return SNN_HIP_INDEX_EXCEEDED;
+    const snn::epi::Shape& shape = snn::epi::shape_of(size, p.kernel);
+    *plan = {shape.bm,
+             shape.bn,
+             shape.chunks > 1,
+             p.kernel >= snn::epi::kAny16x16,
+             p.kernel == snn::epi::kTile128Pair,
+             g.p_k_inner,
+             g.q_k_inner,
+             p.copy_p,
+             p.copy_q,
+             p.splits};
+    return SNN_HIP_OK;
+  }
+  const snn::gated::Pair g = product == 0 ? snn::forward_pair(*params)
+                                          : snn::lhs_pair(*params, size);
+  const snn::gated::Plan p =
+      snn::gated::make_plan(g, size, bytes, product == 1 || at16, at16);
+  if (p.splits == 0) return SNN_HIP_INDEX_EXCEEDED;
+  const snn::epi::Shape shape = snn::gated::shape_of(size, p.kernel);
+  *plan = {shape.bm,
+           shape.bn,
+           shape.chunks > 1,
+           p.kernel >= snn::gated::kDirectKernels,
+           p.kernel == snn::gated::kTile128Pair,
+           1,
+           g.q_k_inner,
+           p.copy_p,
+           p.copy_q,
+           p.splits};
+  return SNN_HIP_OK;
+}
+
 }  // extern "C"

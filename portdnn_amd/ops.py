@@ -921,6 +921,24 @@ def _gated_plan(key, a, w_gate, w_up, grad, activation, trans_b):
                        out_stride, elems))
 
 
+def gated_matmul_plan(m, k, n, dtype, product=0, activation=ACTIVATION.SILU,
+                      trans_b=False, aligned=True, workspace_elems=None,
+                      **strides):
+    """What a gated product runs on (snn_hip_gated_matmul_planned), a dict by the
+    names of capi.MATMUL_PLAN; by default with the recommended workspace."""
+    p = GatedMatmulParams(m=m, k=k, n=n, transpose_rhs=int(trans_b),
+                          activation=activation, **strides)
+    code = _TYPES[dtype][1]
+    if workspace_elems is None:
+        workspace_elems = _workspace("snn_hip_gated_matmul_workspace_size", p,
+                                     int(product > 0), code)
+    plan = capi.MatmulBiasActPlan()
+    capi.check(capi.lib().snn_hip_gated_matmul_planned(
+        ctypes.byref(p), product, code, int(aligned), workspace_elems,
+        ctypes.byref(plan)))
+    return {name: getattr(plan, name) for name in capi.MATMUL_PLAN}
+
+
 def gated_matmul(a, w_gate, w_up, bias_gate=None, bias_up=None,
                  activation=ACTIVATION.SILU, trans_b=False,
                  keep_pre_activation=False, out=None, workspace=None):
@@ -1177,7 +1195,7 @@ __all__ = [
     "conv2d_raw", "conv_flops", "conv_params", "conv_sizes",
     "default_algorithm",
     "depthwise_conv2d", "depthwise_params", "depthwise_sizes",
-    "gated_matmul", "gated_matmul_grad", "linear_attention",
+    "gated_matmul", "gated_matmul_grad", "gated_matmul_plan", "linear_attention",
     "linear_attention_grad",
     "linear_recurrence", "linear_recurrence_grad", "matmul", "matmul_bias_act",
     "matmul_bias_act_grad", "matmul_plan",
