@@ -1082,6 +1082,25 @@ SNN_HIP_API int snn_hip_linear_attention_grad_bf16(
 SNN_HIP_API int snn_hip_linear_attention_workspace_size(
     const snn_hip_linear_attention_params* params, int grad, int dtype,
     size_t* required_elems, size_t* recommended_elems);
+/* Diagnostics for tests of the kernels: how a call, or one for all four gradients, goes
+ * over its sequences in blocks, given a workspace of `workspace_elems` and operands that
+ * start at multiples of 16 bytes or do not.  No launches: step by step. */
+typedef struct snn_hip_linear_attention_launch {
+  int outputs;     /* 1: outputs, 0: the states of pieces */
+  int keys;        /* channels of the states' first side, rounded up to 64, 128, 256 */
+  int waves;       /* of a work-group */
+  int ring;        /* blocks in a ring that rows go to straight; 0: by registers */
+  int work_groups;
+} snn_hip_linear_attention_launch;
+typedef struct snn_hip_linear_attention_plan {
+  int pieces;      /* of a sequence */
+  int piece_steps;
+  int launches;
+  snn_hip_linear_attention_launch launch[4];
+} snn_hip_linear_attention_plan;
+SNN_HIP_API int snn_hip_linear_attention_planned(
+    const snn_hip_linear_attention_params* params, int grad, int dtype,
+    int aligned, size_t workspace_elems, snn_hip_linear_attention_plan* plan);
 
 #ifdef __cplusplus
 }

@@ -201,6 +201,15 @@ LinearAttentionParams = _struct(
      "grad_v_stride", "scale"],
     {"scale": 1.0}, {"scale": ctypes.c_float})
 
+LINEAR_ATTENTION_LAUNCH = ["outputs", "keys", "waves", "ring", "work_groups"]
+LinearAttentionLaunch = _struct("LinearAttentionLaunch", LINEAR_ATTENTION_LAUNCH, {})
+
+
+class LinearAttentionPlan(ctypes.Structure):
+    _fields_ = [("pieces", ctypes.c_int), ("piece_steps", ctypes.c_int),
+                ("launches", ctypes.c_int), ("launch", LinearAttentionLaunch * 4)]
+
+
 _P = ctypes.c_void_p
 _SZ = ctypes.c_size_t
 _I = ctypes.c_int
@@ -282,6 +291,7 @@ SIGNATURES = {
         _I, ctypes.c_double, _I] + [ctypes.c_double] * 4 + [_P],
     "snn_hip_linear_attention_workspace_size": [
         _P, _I, _I, ctypes.POINTER(_SZ), ctypes.POINTER(_SZ)],
+    "snn_hip_linear_attention_planned": [_P, _I, _I, _I, _SZ, _P],
 }
 for _type in ("f32", "f16", "bf16"):
     SIGNATURES["snn_hip_matmul_bias_act_" + _type] = [_P] * 8 + [_SZ, _P]

@@ -1248,6 +1248,12 @@ int launch_ring(const Problem& p, unsigned groups, hipStream_t stream) {
 // channels in bfloat16, one and two: 8 x 2048 steps of 32 heads, one work-group a CU, 98
 // and 77 us; gradients of 1 x 16384 steps of 16 heads, up to three, 112 and 127 us.  fp32
 // heads of 128 channels, one work-group a CU: 105 and 107 us.)
+inline int ring_of(int keys_class, int waves, bool outputs, bool direct,
+                   unsigned groups) {
+  if (!direct) return 0;
+  if (waves == 8 && keys_class <= 128) return outputs ? 3 : 2;
+  return keys_class > 64 || groups > 512 ? 1 : 2;
+}
 template <typename T, int D, int WAVES, bool OUTPUT, bool DIRECT>
 int launch_as(const Problem& p, hipStream_t stream) {
   const unsigned groups =
@@ -1259,7 +1265,7 @@ int launch_as(const Problem& p, hipStream_t stream) {
   } else if constexpr (D > 64) {
     return launch_ring<T, D, WAVES, OUTPUT, 1>(p, groups, stream);
   } else {
-    return groups <= 512
+    return ring_of(D, WAVES, OUTPUT, DIRECT, groups) == 2
                ? launch_ring<T, D, WAVES, OUTPUT, 2>(p, groups, stream)
                : launch_ring<T, D, WAVES, OUTPUT, 1>(p, groups, stream);
   }

@@ -758,6 +758,40 @@ int backward(const void* grad, const float* grad_final, const void* q,
 }  // namespace
 }  // namespace snn
 
+namespace snn {
+namespace {
+
+// The launches that run_all makes of walks over these keys and values.
+struct Sizes {
+  int keys, values;
+};
+void add_launches(const snn_hip_linear_attention_params& p, const Sizes* walks, int n,
+                  bool outputs, bool direct, int size,
+                  snn_hip_linear_attention_plan* plan) {
+  bool done[att::kMostWalks] = {};
+  for (int i = 0; i < n; ++i) {
+    if (done[i]) continue;
+    const int keys = class_of(walks[i].keys);
+    const int waves = waves_of(size, walks[i].keys, walks[i].values);
+    size_t units = 0;
+    for (int j = i; j < n; ++j) {
+      if (done[j] || class_of(walks[j].keys) != keys ||
+          waves_of(size, walks[j].keys, walks[j].values) != waves)
+        continue;
+      units += slices_of(size, walks[j].keys, walks[j].values);
+      done[j] = true;
+    }
+    const unsigned groups = static_cast<unsigned>(
+        units * p.batch * p.heads * static_cast<size_t>(plan->pieces));
+    plan->launch[plan->launches++] = {
+        outputs, keys, waves, att::ring_of(keys, waves, outputs, direct, groups),
+        static_cast<int>(groups)};
+  }
+}
+
+}  // namespace
+}  // namespace snn
+
 #define SNN_LINEAR_ATTENTION(suffix, T)                                        \
   int snn_hip_linear_attention_##suffix(                                       \
       const void* q, const void* k, const void* v, const float* decay,         \
@@ -809,6 +843,45 @@ int snn_hip_linear_attention_workspace_size(
     all = snn::division_bytes(*params, snn::forward_division(*params, size, ~size_t{0}), 1);
   }
   *recommended_elems = all / size;
+  return SNN_HIP_OK;
+}
+
+int snn_hip_linear_attention_planned(
+    const snn_hip_linear_attention_params* params, int grad, int dtype,
+    int aligned, size_t workspace_elems, snn_hip_linear_attention_plan* plan) {
+  if (dtype < SNN_HIP_DTYPE_F32 || dtype > SNN_HIP_DTYPE_BF16 || plan == nullptr)
+    return SNN_HIP_INVALID_PARAMETER;
+  const int valid = grad != 0 ? snn::check_grad(params, nullptr)
+                              : snn::check(params, nullptr);
+  if (valid != SNN_HIP_OK) return valid;
+  const snn_hip_linear_attention_params& p = *params;
+  const int size = dtype == SNN_HIP_DTYPE_F32 ? 4 : 2, piece = 16 / size;
+  *plan = {};
+  plan->pieces = 1;
+  if (grad == 0 && p.steps <= snn::kFewSteps) return SNN_HIP_OK;
+  bool direct = aligned != 0;
+  for (const int n : {p.keys, p.values, p.q_stride, p.k_stride, p.v_stride,
+                      p.grad_q_stride, p.grad_k_stride, p.grad_v_stride})
+    direct = direct && n % piece == 0;
+  size_t bytes = workspace_elems * size;
+  snn::Division d;
+  if (grad != 0) {
+    const size_t shared = 2 * snn::shared_bytes(p);
+    if (bytes < shared) return SNN_HIP_INSUFFICIENT_WORKSPACE;
+    d = snn::grad_division(p, size, bytes - shared);
+  } else {
+    d = snn::forward_division(p, size, bytes);
+  }
+  plan->pieces = d.pieces;
+  plan->piece_steps = d.piece_steps;
+  const snn::Sizes across = {p.keys, p.values}, back = {p.values, p.keys};
+  const snn::Sizes states[] = {across, across}, walks[] = {back, back, across};
+  if (d.pieces > 1)
+    snn::add_launches(p, states, grad != 0 ? 2 : 1, false, direct, size, plan);
+  if (grad != 0)
+    snn::add_launches(p, walks, 3, true, direct, size, plan);
+  else
+    snn::add_launches(p, &across, 1, true, direct, size, plan);
   return SNN_HIP_OK;
 }
 

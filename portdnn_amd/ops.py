@@ -1101,6 +1101,28 @@ def _attention_operands(q, k, v, decay, resets, lengths, grad):
         _vector(lengths, sizes[0], torch.int32)
 
 
+def linear_attention_plan(batch, steps, heads, key_heads, keys, values, dtype,
+                          grad=False, aligned=True, workspace_elems=None,
+                          **strides):
+    """How a call goes over its sequences (snn_hip_linear_attention_planned): pieces,
+    steps of a piece, and a list of launches, dicts by the names of
+    capi.LINEAR_ATTENTION_LAUNCH; by default with the recommended workspace."""
+    p = LinearAttentionParams(batch=batch, steps=steps, heads=heads,
+                              key_heads=key_heads, keys=keys, values=values,
+                              **strides)
+    code = _TYPES[dtype][1]
+    if workspace_elems is None:
+        workspace_elems = _workspace("snn_hip_linear_attention_workspace_size", p,
+                                     int(grad), code)
+    plan = capi.LinearAttentionPlan()
+    capi.check(capi.lib().snn_hip_linear_attention_planned(
+        ctypes.byref(p), int(grad), code, int(aligned), workspace_elems,
+        ctypes.byref(plan)))
+    return plan.pieces, plan.piece_steps, [
+        {name: getattr(l, name) for name in capi.LINEAR_ATTENTION_LAUNCH}
+        for l in plan.launch[:plan.launches]]
+
+
 def linear_attention(q, k, v, decay, resets=None, lengths=None,
                      initial_state=None, scale=1.0, out=None, final_state=None,
                      workspace=None):
@@ -1196,7 +1218,7 @@ __all__ = [
     "default_algorithm",
     "depthwise_conv2d", "depthwise_params", "depthwise_sizes",
     "gated_matmul", "gated_matmul_grad", "gated_matmul_plan", "linear_attention",
-    "linear_attention_grad",
+    "linear_attention_grad", "linear_attention_plan",
     "linear_recurrence", "linear_recurrence_grad", "matmul", "matmul_bias_act",
     "matmul_bias_act_grad", "matmul_plan",
     "pointwise_forward", "pointwise_grad", "pool_params", "pooling_avg_grad",
