@@ -20,8 +20,7 @@ using gated::Pair;
 using seq::Pack;
 
 // dg and du of a block of 32 VEC columns and `rows` rows: 8 rows at a time, and their
-// sums at the end.  Rows of the two are `stride` values with zeros behind the last
-// column.  Bound by memory: bfloat16, 4096 x 8192, 70 us, 336 MB, 4.8 TB/s.
+// sums at the end.  Rows of the two are `stride` values apart.  Bound by memory: bfloat16, 4096 x 8192, 70 us, 336 MB, 4.8 TB/s.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256)
     gated_grad_kernel(const T* __restrict__ grad, long grad_stride,
@@ -59,12 +58,6 @@ __global__ void __launch_bounds__(256)
         const long to = row * stride + at.c;
         *reinterpret_cast<V*>(dg + to) = seq::pack<T, VEC>(g);
         *reinterpret_cast<V*>(du + to) = seq::pack<T, VEC>(u);
-        if (first + VEC >= n) {
-          for (long c = n; c < stride; ++c) {
-            dg[row * stride + c] = T(0);
-            du[row * stride + c] = T(0);
-          }
-        }
       }
     }
   }
