@@ -329,11 +329,11 @@ int class_of(int keys) { return keys <= 64 ? 64 : keys <= 128 ? 128 : 256; }
 // bfloat16, 1 x 32768 steps of 16 heads of 128 x 128 258, 219, gradients of 4 x 4096
 // steps 339, 256; 1 x 8192 steps of 16 heads of 256 x 256 266, 199, gradients 634, 510.
 // In fp32 a block of 32 steps has four tiles of q k, one for each of four waves.)
-int waves_of(int size, int keys, int values) {
+int waves_of(int size, int values) {
   return size == 2 && values > 64 ? 8 : 4;
 }
-int slices_of(int size, int keys, int values) {
-  return ceil_div(values, 16 * waves_of(size, keys, values));
+int slices_of(int size, int values) {
+  return ceil_div(values, 16 * waves_of(size, values));
 }
 
 // How a sequence is divided into pieces that are walked beside one another: as this
@@ -401,22 +401,22 @@ size_t division_bytes(const snn_hip_linear_attention_params& p,
 
 // Work-groups of a pass over the whole sequence, and how many of them share a CU.
 int forward_units(const snn_hip_linear_attention_params& p, int size) {
-  return slices_of(size, p.keys, p.values);
+  return slices_of(size, p.values);
 }
 int grad_units(const snn_hip_linear_attention_params& p, int size) {
-  return 2 * slices_of(size, p.values, p.keys) + slices_of(size, p.keys, p.values);
+  return 2 * slices_of(size, p.keys) + slices_of(size, p.values);
 }
 Division forward_division(const snn_hip_linear_attention_params& p, int size,
                           size_t bytes) {
   const bool alone =
-      class_of(p.keys) == 256 || waves_of(size, p.keys, p.values) == 8;
+      class_of(p.keys) == 256 || waves_of(size, p.values) == 8;
   return divide(p, forward_units(p, size), block_of(size), alone ? 1 : 3, bytes, 1);
 }
 Division grad_division(const snn_hip_linear_attention_params& p, int size,
                        size_t bytes) {
   const bool alone =
       class_of(std::max(p.keys, p.values)) == 256 ||
-      waves_of(size, p.keys, p.values) == 8 || waves_of(size, p.values, p.keys) == 8;
+      waves_of(size, p.values) == 8 || waves_of(size, p.keys) == 8;
   return divide(p, grad_units(p, size), block_of(size), alone ? 1 : 3, bytes, 2);
 }
 
@@ -457,7 +457,7 @@ Problem problem_of(const snn_hip_linear_attention_params& p, const Division& d,
 }
 void add(Problem* g, const Walk& w, int size) {
   g->walk[g->walks] = w;
-  g->walk[g->walks].slices = slices_of(size, w.keys, w.values);
+  g->walk[g->walks].slices = slices_of(size, w.values);
   g->units += g->walk[g->walks].slices;
   ++g->walks;
 }
@@ -469,11 +469,11 @@ int run_all(const Problem& base, const Walk* walks, int n, bool outputs,
   for (int i = 0; i < n; ++i) {
     if (done[i]) continue;
     const int keys = class_of(walks[i].keys);
-    const int waves = waves_of(sizeof(T), walks[i].keys, walks[i].values);
+    const int waves = waves_of(sizeof(T), walks[i].values);
     Problem g = base;
     for (int j = i; j < n; ++j) {
       if (done[j] || class_of(walks[j].keys) != keys ||
-          waves_of(sizeof(T), walks[j].keys, walks[j].values) != waves)
+          waves_of(sizeof(T), walks[j].values) != waves)
         continue;
       add(&g, walks[j], sizeof(T));
       done[j] = true;
@@ -772,13 +772,13 @@ void add_launches(const snn_hip_linear_attention_params& p, const Sizes* walks, 
   for (int i = 0; i < n; ++i) {
     if (done[i]) continue;
     const int keys = class_of(walks[i].keys);
-    const int waves = waves_of(size, walks[i].keys, walks[i].values);
+    const int waves = waves_of(size, walks[i].values);
     size_t units = 0;
     for (int j = i; j < n; ++j) {
       if (done[j] || class_of(walks[j].keys) != keys ||
-          waves_of(size, walks[j].keys, walks[j].values) != waves)
+          waves_of(size, walks[j].values) != waves)
         continue;
-      units += slices_of(size, walks[j].keys, walks[j].values);
+      units += slices_of(size, walks[j].values);
       done[j] = true;
     }
     const unsigned groups = static_cast<unsigned>(
