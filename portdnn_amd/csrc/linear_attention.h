@@ -887,7 +887,13 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
       for (int t = 0; t < TT; ++t) {
         const float by = reach[16 * t + c16];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) acc[t][r] *= by * unscale[r];
+        for (int r = 0; r < 4; ++r) {
+          // (the two factors together may be zero, which no infinity survives)
+          if (CAREFUL)
+            acc[t][r] = acc[t][r] * unscale[r] * by;
+          else
+            acc[t][r] *= by * unscale[r];
+        }
         if (resets != 0) {
           const bool reached = resets_to[16 * t + c16] == 0;
 #pragma unroll

@@ -127,3 +127,21 @@ def test_states_that_rounding_would_make_infinite(size, dtype, value):
     most = max(size[4:])
     ref.check(o, want[0], plain.operations(most, dtype))
     ref.check(last, want[1], plain.state_operations(most, dtype))
+
+
+@pytest.mark.parametrize("size", SIZES)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_states_of_nothing_else(size, dtype):
+    """All of a column but one key is zero, and decays take what there was from all
+    others: a range that small times a decay may be no number above zero."""
+    t, _ = _make(size, dtype)
+    t["decay"][:] = -2.0
+    t["q"][..., KEY] = 1.0
+    t["initial_state"].zero_()
+    t["initial_state"][:, :, KEY, VALUE] = INF
+    t["v"][..., VALUE] = 0.0
+    o, last = ops.linear_attention(scale=1e-3, **_cuda(t))
+    o = o.float().cpu()
+    assert (o[..., VALUE] == INF).all()
+    assert torch.isfinite(o[..., _others(size[5])]).all()
+    assert (last[:, :, KEY, VALUE] == INF).all()
