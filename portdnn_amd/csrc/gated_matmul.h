@@ -17,7 +17,8 @@
 // library's product of these sizes reaches 1.35); SUM of 4096 rows, 2 x 8192 to 2048
 // columns: 249 us, 1.1 PFLOP/s (128 tiles of 256 x 256 in two shares, and their join).
 // 1 row, k 2048, n 8192: 15.2 us, 67 MB, 4.4 TB/s; binary16, 32 rows, k 4096, n 8192,
-// weights by column: 29.4 us, 134 MB, 4.6 TB/s.
+// weights by column: 29.4 us, 134 MB, 4.6 TB/s; fp32, 1 row or 16, k 2048, n 8192: 30.8
+// us, 134 MB, 4.4 TB/s.
 #ifndef PORTDNN_AMD_CSRC_GATED_MATMUL_H_
 #define PORTDNN_AMD_CSRC_GATED_MATMUL_H_
 
@@ -589,7 +590,12 @@ inline epi::Shape shape_of(int elem_size, int kernel) {
   epi::Shape s = epi::shape_of(elem_size, kSame[kernel]);
   // (sums of 2 x 8192 products in bfloat16, at the clocks of long calls: 4096 x 2048 in
   // 512 tiles of 128 x 128 281 us; in 128 of 256 x 256, in two shares, 233 and 16 for
-  // their join)
+  // their join.  GATED has hardly a use for them; us in tiles of 128 x 128, two such to a
+  // CU, 256 x 256, * is what is taken: 2048 x 2048 x 8192 158, 149, 119*; 4096 x 1024 x 4096
+  // 100, 85, 74*; 1024 x 4096 x 4096 74, 68*, 79; 512 x 2048 x 8192 42, 42*, 46.  SUM, with
+  // the pass over the factors: 155*, 205, 165; 94*, 126, 108; 77*, 109, 90; 56, 71, 68 (64 x
+  // 128: 59*).  6000 x 2000 x 3000 takes two of 128 x 128 to a CU, 197, SUM 238, where 256 x
+  // 256 would take 170 and 195)
   if (kernel == kTile128 && elem_size == 2) s.step_k = s.step_row = 0.48f;
   return s;
 }

@@ -20,7 +20,8 @@ using gated::Pair;
 using seq::Pack;
 
 // dg and du of a block of 32 VEC columns and `rows` rows: 8 rows at a time, and their
-// sums at the end.  Rows of the two are `stride` values apart.  Bound by memory: bfloat16, 4096 x 8192, 70 us, 336 MB, 4.8 TB/s.
+// sums at the end.  Rows of the two are `stride` values apart.  Bound by memory:
+// bfloat16, 4096 x 8192, 72 us, 336 MB, 4.7 TB/s.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256)
     gated_grad_kernel(const T* __restrict__ grad, long grad_stride,

@@ -33,11 +33,12 @@
 // by way of LDS, q X and the splits of X, the sums over v, the split of the weighted v,
 // its products; waits at two barriers lie between, and the vector unit is busy with
 // splits, weights and carries about half of the time.  bfloat16, 1 x 32768 steps of 16
-// heads of 128 channels: 224 us, of them 68 for the pass that leaves states, 10 for their
-// sums, 147 for the outputs (537 MB in all, 2.4 TB/s; 34 GFLOP by the formula of the steps,
-// 150 TFLOP/s).  Left out, of the 166 us that the outputs took before blocks
+// heads of 128 channels: 228 us, of them 70 for the pass that leaves states, 10 for their
+// sums, 151 for the outputs (537 MB in all, 2.4 TB/s; 34 GFLOP by the formula of the steps,
+// 150 TFLOP/s); binary16 249.  Left out, of the 166 us that the outputs took before blocks
 // were asked for three ahead: loads 31, stores 44, the state's update 64, q X 90 us.
-// Gradients of 4 x 4096 steps, three walks of 64 heads in one launch: 251 us.
+// Gradients of 4 x 4096 steps, three walks of 64 heads in one launch: 254 us.  fp32, 1 x
+// 8192 steps of 8 heads: 98 us, gradients 206.
 //
 // Sequences that do not fill the GPU are divided into pieces: a first pass walks them
 // without outputs from a state of zero (k and v alone are read), the states are added
@@ -51,7 +52,10 @@
 // Rows that may not count, those of later steps and those in front of a reset, are left
 // out by selection.  The matrix instructions would multiply their v by zero, which an
 // infinity or NaN survives: where there is one (a product with zero tells) they are
-// summed value by value instead, in a second walk of the work-group's piece.
+// summed value by value instead, in a second walk of the work-group's piece, and so they
+// are where a state of a 16-bit walk is infinite.  That walk is slow: with one such value in
+// a sequence, or in all, bfloat16 calls of 228 us (above) take 2990, gradients of 240 3760,
+// 64 x 512 steps of 16 heads of 64 channels 679 for 80; fp32 calls of 98 us 331.
 #ifndef PORTDNN_AMD_CSRC_LINEAR_ATTENTION_H_
 #define PORTDNN_AMD_CSRC_LINEAR_ATTENTION_H_
 
@@ -1250,10 +1254,12 @@ int launch_ring(const Problem& p, unsigned groups, hipStream_t stream) {
 // without q two work-groups of a CU with two each (outputs of 1 x 32768 steps of 16 heads
 // of 128 channels in bfloat16: 166 us while every block waited for the next as well, 149
 // with three under way).  Work-groups of four waves have two where they do not fill the
-// CUs three deep, otherwise one, loaded when the one before has been used.  (Heads of 64
-// channels in bfloat16, one and two: 8 x 2048 steps of 32 heads, one work-group a CU, 98
-// and 77 us; gradients of 1 x 16384 steps of 16 heads, up to three, 112 and 127 us.  fp32
-// heads of 128 channels, one work-group a CU: 105 and 107 us.)
+// CUs three deep, otherwise one, loaded when the one before has been used.  (us for 256,
+// 512, 640, 768, 1024, 2048 work-groups with 1024 steps of 64 channels, one and two:
+// bfloat16 46 and 40, 65 and 58, 86 and 102, 97 and 107, 149 and 125, 250 and 239; gradients
+// 44 and 40, 53 and 51, 65 and 82, 74 and 85, 120 and 106, 217 and 214; fp32 101 and 81, 145
+// and 137, 187 and 198, 203 and 209, 286 and 273, 529 and 535.  The rule leaves a sixth of
+// the time around 1024.  fp32 heads of 128 channels, one work-group a CU: 105 and 107.)
 inline int ring_of(int keys_class, int waves, bool outputs, bool direct,
                    unsigned groups) {
   if (!direct) return 0;

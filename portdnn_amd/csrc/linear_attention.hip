@@ -14,8 +14,9 @@ using seq::Pack;
 
 // ---- a few steps ---------------------------------------------------------------
 
-// (bfloat16, 64 sequences of 16 heads of 128 x 128: 1 step 24 us, 4 31, 16 59; 17 steps in
-// a block 50)
+// (bfloat16, 64 sequences of 16 heads of 128 x 128, call after call on the same states,
+// which are partly in the last cache: 1 step 22 us, 4 29, 12 48, 16 59; 17 steps in a block
+// 50)
 constexpr int kFewSteps = 12;
 
 struct Few {
@@ -33,8 +34,8 @@ struct Few {
 
 // One step after the other, all in fp32: a work-group owns 64 values of a head's
 // state, a lane four neighbouring values of every sixteenth key.  Bound by the state,
-// which is read and written once: one step of 64 sequences of 16 heads of 128 x 128 in
-// 28 us, 135 MB, 4.8 TB/s.
+// which is read and written once: one step of 64 sequences of 16 heads of 128 x 128, among
+// other calls, in 27.5 us, 135 MB, 4.9 TB/s.
 template <typename T, int R>
 __global__ void __launch_bounds__(256) few_steps_kernel(Few p) {
   __shared__ float q_of[kFewSteps][16 * R], k_of[kFewSteps][16 * R];
@@ -226,7 +227,8 @@ __global__ void __launch_bounds__(256) chain_kernel(Chains p) {
 // out[row][g][c] = sum over the group's heads of in[row][g * share + i][c], VEC
 // neighbouring c at a time, for q's and k's gradients beside one another.  Bound by
 // memory: bfloat16, 4 x 4096 steps of 16 heads of 128 channels, four of which share: 51
-// us for both, 302 MB, partly from the last cache (51 for each, one value at a time).
+// us for both, 302 MB, partly from the last cache (51 for each, one value at a time), of
+// 309 for the call; 240 where no heads share.
 struct Shared {
   const float* in[2];
   void* out[2];
@@ -367,7 +369,10 @@ Division divide(const snn_hip_linear_attention_params& p, int units, int block,
   };
   Division best = {1, blocks * block};
   double least = rounds_of(heads * units, of_cu) * (blocks + 4);
-  // (many work-groups fill the GPU evenly enough)
+  // (many work-groups fill the GPU evenly enough, and pieces would take half as long again
+  // and more.  us for 1, 2, 4 pieces: bfloat16, 64 x 1024 steps of 32 heads of 64 x 64 263,
+  // 418, 474; 128 x 1024 of 16 heads of 128 x 128 630, 1148, 1409, gradients of 48 x 512
+  // 346, 709, 906; fp32, 64 x 256 of 16 heads of 128 x 128 227, 493, 574)
   const int most = heads * units >= 8 * kCus ? 1 : std::min(blocks, kMostPieces);
   for (int want = 2; want <= most; ++want) {
     const int each = ceil_div(blocks, want), pieces = ceil_div(blocks, each);
