@@ -1022,7 +1022,8 @@ __device__ __forceinline__ void walk_body(const Problem& p, char* ring0, char* r
       // (binary16: a value's column times a power of two, which its sums of the block
       // lose again, as the second part of small values would be below the type's
       // smallest: gradients of 1e-3 left states that were off by 4e-4.  1 x 32768 steps of
-      // 16 heads of 128 channels 270 us, 247 without; 64 x 512 of 64 channels 84 and 81)
+      // 16 heads of 128 channels 247 us, 229 without, gradients of 4 x 4096 294 and 270; 64 x
+      // 512 of 64 channels 84 and 81, gradients 181 and 172)
       constexpr int kParts = Split<T>::kWhole;
       uint4v parts[SB][kParts];
 #pragma unroll
